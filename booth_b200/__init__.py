@@ -20,7 +20,7 @@ INCLUDE_DIR = os.path.join(os.path.dirname(_HERE), "include")
 
 OK, ERR_DL, ERR_SYM, ERR_CUDA, ERR_NO_GPU, ERR_IO, ERR_KERN, ERR_ARG, ERR_NCCL = 0, -1, -2, -3, -4, -5, -6, -7, -8
 FILL_F32_PM1, FILL_F32_01, FILL_I32_1000, FILL_U32_RAW = 0, 1, 2, 3
-I32, F32, F64 = 0, 1, 2
+I32, F32, F64, BF16, F16 = 0, 1, 2, 3, 4
 GEMM_B_UNCHANGED, GEMM_TEST_SILENT_PRODUCER = 1, 0x80000000
 COMM_ID_BYTES = 128
 
@@ -106,6 +106,11 @@ _SIGNATURES = {
     "booth_sm100_gemm_wait_limit": (C.c_int, [_dev, C.c_uint]),
     "booth_sm100_asian": (C.c_int, [_dev, C.POINTER(AsianParams), C.c_longlong, C.c_longlong, _ptr]),
     "booth_sm100_asian_paths": (C.c_int, [_dev, C.POINTER(AsianParams), C.c_longlong, C.c_longlong, _ptr, _ptr]),
+    # training operators
+    "booth_sm100_layernorm": (C.c_int, [_dev] + [_ptr] * 6 + [C.c_longlong, C.c_int, C.c_longlong, C.c_longlong, C.c_float, C.c_int, C.c_int]),
+    "booth_sm100_layernorm_backward": (C.c_int, [_dev] + [_ptr] * 8 + [C.c_longlong, C.c_int] + [C.c_longlong] * 3 +
+                                       [C.c_int, C.c_int, _ptr, C.c_size_t]),
+    "booth_sm100_layernorm_backward_workspace": (C.c_size_t, [_dev, C.c_longlong, C.c_int, C.c_int, C.c_int]),
     # layer 3
     "sm100_comm_unique_id": (C.c_int, [C.c_void_p]),
     "sm100_comm_init_rank": (C.c_int, [C.POINTER(C.c_void_p), _dev, C.c_int, C.c_int, C.c_void_p]),
@@ -305,6 +310,27 @@ class Device:
     def asian_paths(self, params, path0, npaths, arith, geom):
         self._ck("booth_sm100_asian_paths",
                  lib().booth_sm100_asian_paths(self._h, C.byref(params), path0, npaths, arith, geom))
+
+    # -- training operators (addresses of device memory; 0 for an operand that is not there) --
+    def layernorm(self, y, x, w, b, rows, cols, eps=1e-5, dtype=F32, wdtype=None, mean=0, rstd=0, ldx=None, ldy=None):
+        """y = (x - mean) rstd w + b over each row; also writes mean and rstd where they are given."""
+        self._ck("booth_sm100_layernorm", lib().booth_sm100_layernorm(
+            self._h, y, x, w, b, mean, rstd, rows, cols, cols if ldx is None else ldx, cols if ldy is None else ldy, eps,
+            dtype, dtype if wdtype is None else wdtype))
+
+    def layernorm_backward_workspace(self, rows, cols, dtype=F32, wdtype=None):
+        """Bytes of workspace that layernorm_backward needs for dw and db."""
+        n = lib().booth_sm100_layernorm_backward_workspace(self._h, rows, cols, dtype, dtype if wdtype is None else wdtype)
+        if n == 0:
+            self._ck("booth_sm100_layernorm_backward_workspace", ERR_ARG)
+        return n
+
+    def layernorm_backward(self, dx, dw, db, dy, x, w, mean, rstd, rows, cols, ws=0, ws_bytes=0, dtype=F32, wdtype=None,
+                           lddx=None, lddy=None, ldx=None):
+        """dx, dw, db (0: not wanted) from dy and the forward pass's x, mean and rstd."""
+        self._ck("booth_sm100_layernorm_backward", lib().booth_sm100_layernorm_backward(
+            self._h, dx, dw, db, dy, x, w, mean, rstd, rows, cols, cols if lddx is None else lddx,
+            cols if lddy is None else lddy, cols if ldx is None else ldx, dtype, dtype if wdtype is None else wdtype, ws, ws_bytes))
 
 
 class Comm:

@@ -26,7 +26,7 @@ SO = os.path.join(LIB, "libbooth_sm100.so")
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo",
               "-std=c++17", "--fmad=true", "-Xptxas", "-v"]
-C_SOURCES = ["sm100_shim.c", "bc_runtime.c", "sm100_ops.c", "sm100_comm.c", "rt_sm100.c", "lf_gpu_sm100.c", "nv_rt_sm100.c"]
+C_SOURCES = ["sm100_shim.c", "bc_runtime.c", "sm100_ops.c", "sm100_train.c", "sm100_comm.c", "rt_sm100.c", "lf_gpu_sm100.c", "nv_rt_sm100.c"]
 
 
 def _cuda_home():

@@ -7,6 +7,7 @@
 #include "tile.cu"
 #include "canonical.cu"
 #include "pipe_probe.cu"
+#include "layernorm.cu"
 #if __has_include("gemm_tf32x3.cu")
 #include "gemm_tf32x3.cu"
 #endif

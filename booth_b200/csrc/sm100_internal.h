@@ -68,6 +68,9 @@ typedef struct sm100_api {
 #define SM100_SCRATCH_GEMM_STATUS  128
 #define SM100_SCRATCH_PARTIALS     256
 
+/* Forms of the layer normalisation kernels, the same for both directions. */
+#define SM100_LN_FORMS 6
+
 /* Built-in kernels, resolved once per device from the embedded image. */
 enum {
     SM100_K_VADD, SM100_K_SAXPY, SM100_K_FILL,
@@ -75,7 +78,10 @@ enum {
     SM100_K_ASIAN_MC, SM100_K_ASIAN_MC_PRECISE,
     SM100_K_ASIAN_PATHS, SM100_K_ASIAN_PATHS_PRECISE,
     SM100_K_GEMM_PREPASS, SM100_K_GEMM_TF32X3, SM100_K_GEMM_TF32X3_N128, SM100_K_GEMM_TF32X3_2CTA, SM100_K_GEMM_TF32X3_2CTA_N128, SM100_K_GEMM_PERSIST,
-    SM100_K_COUNT
+    /* layer normalisation: five pairs of types, six forms each; per element type (f32, bf16, f16) the column sums */
+    SM100_K_LN_FWD, SM100_K_LN_BWD = SM100_K_LN_FWD + 5 * SM100_LN_FORMS,
+    SM100_K_LN_COLUMNS = SM100_K_LN_BWD + 5 * SM100_LN_FORMS, SM100_K_LN_PARAM_GRAD = SM100_K_LN_COLUMNS + 3,
+    SM100_K_COUNT = SM100_K_LN_PARAM_GRAD + 3
 };
 
 struct sm100_dev {

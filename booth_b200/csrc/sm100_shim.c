@@ -143,12 +143,19 @@ int sm100_enter(sm100_dev_t *dev)
 
 /* ---- init / shut ---- */
 
+#define LN_FORM_NAMES(k) k "_v8", k "_v16", k "_v32", k "_s8", k "_s16", k "_loop"
 static const char *const k_names[SM100_K_COUNT] = {
     "vadd_stream", "saxpy_stream", "fill_philox",
     "reduce_sum_i32", "reduce_sum_f32",
     "asian_mc", "asian_mc_precise",
     "asian_paths", "asian_paths_precise",
     "gemm_prepass", "gemm_tf32x3", "gemm_tf32x3_n128", "gemm_tf32x3_2cta", "gemm_tf32x3_2cta_n128", "gemm_tf32x3_persist",
+    LN_FORM_NAMES("layernorm_f32"), LN_FORM_NAMES("layernorm_bf16"), LN_FORM_NAMES("layernorm_bf16_f32"),
+    LN_FORM_NAMES("layernorm_f16"), LN_FORM_NAMES("layernorm_f16_f32"),
+    LN_FORM_NAMES("layernorm_bwd_f32"), LN_FORM_NAMES("layernorm_bwd_bf16"), LN_FORM_NAMES("layernorm_bwd_bf16_f32"),
+    LN_FORM_NAMES("layernorm_bwd_f16"), LN_FORM_NAMES("layernorm_bwd_f16_f32"),
+    "layernorm_bwd_columns_f32", "layernorm_bwd_columns_bf16", "layernorm_bwd_columns_f16",
+    "layernorm_param_grad_f32", "layernorm_param_grad_bf16", "layernorm_param_grad_f16",
 };
 
 int sm100_rt_device_count(void)

@@ -268,6 +268,42 @@ int  booth_sm100_asian_paths(sm100_dev_t *dev, const booth_asian_t *p,
                              sm100_ptr_t arith, sm100_ptr_t geom);
 
 /* ---------------------------------------------------------------------------
+ * Training operators (asynchronous on the device's stream; device pointers)
+ * Everything is checked on the host before any GPU work and refused with
+ * SM100_ERR_ARG. The calls allocate nothing and wait for nothing, so they can be
+ * captured into a graph; work memory is the caller's: one workspace serves any
+ * number of calls that follow one another on the stream, and calls or graphs that
+ * may run at the same time need one each. No counterpart in the reference.
+ * ------------------------------------------------------------------------- */
+/* Layer normalisation of each row of x [rows, cols], rows ldx elements apart:
+ *   mean = sum x / cols, rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps),
+ *   y = (x - mean) * rstd * w + b
+ * w and b [cols] may be NULL (ones, zeros); mean and rstd [rows], fp32, may be NULL
+ * and are what the backward pass wants. dtype is x's and y's type, wdtype w's and
+ * b's (SM100_F32, SM100_BF16 or SM100_F16): the same, or SM100_F32 beside 16-bit values. Statistics and products are
+ * fp32, y is rounded once. y may be x (same pitch); otherwise outputs must not
+ * overlap inputs. Rows beyond `rows` and columns beyond `cols` are neither read nor
+ * written. Any alignment of whole elements; rows that start on 16 bytes and are a
+ * multiple of 16 bytes long are read in 16-byte vectors. rows = 0 does nothing. */
+int  booth_sm100_layernorm(sm100_dev_t *dev, sm100_ptr_t y, sm100_ptr_t x, sm100_ptr_t w, sm100_ptr_t b,
+                           sm100_ptr_t mean, sm100_ptr_t rstd, long long rows, int cols,
+                           long long ldx, long long ldy, float eps, int dtype, int wdtype);
+/* Its gradient, from the saved mean and rstd: with xhat = (x - mean) rstd,
+ * p = mean over the row of w dy, q = mean over the row of w dy xhat,
+ *   dx = rstd (w dy - p - xhat q),  dw = sum over rows of dy xhat,  db = sum over rows of dy
+ * dx (x's type), dw and db (wdtype) are overwritten; any of them may be NULL. w may
+ * be NULL (ones). dx must not be dy or x, nor overlap any input. With rows = 0 dw and db
+ * become zero. The sums over rows are taken in a fixed order: the same call gives
+ * the same bits. ws: booth_sm100_layernorm_backward_workspace bytes, 16-byte
+ * aligned, any contents; NULL when neither dw nor db is asked for. */
+int  booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t dw, sm100_ptr_t db,
+                                    sm100_ptr_t dy, sm100_ptr_t x, sm100_ptr_t w, sm100_ptr_t mean, sm100_ptr_t rstd,
+                                    long long rows, int cols, long long lddx, long long lddy, long long ldx,
+                                    int dtype, int wdtype, sm100_ptr_t ws, size_t ws_bytes);
+/* Bytes of workspace the call above needs; 0 on a bad argument. */
+size_t booth_sm100_layernorm_backward_workspace(sm100_dev_t *dev, long long rows, int cols, int dtype, int wdtype);
+
+/* ---------------------------------------------------------------------------
  * Layer 3: the collective (NCCL over NVLink; libnccl.so.2 is dlopen'ed)
  * The reference has no counterpart: it drives one device only
  * (src/nvidia/nv_rt.c:132, src/runtime/bc_runtime.c:234-244).
@@ -277,6 +313,9 @@ typedef struct sm100_comm sm100_comm_t;
 #define SM100_I32 0
 #define SM100_F32 1
 #define SM100_F64 2
+/* Element types of the training operators beside SM100_F32 (the collective does not take them). */
+#define SM100_BF16 3   /* 8-bit exponent, 7-bit fraction */
+#define SM100_F16  4   /* IEEE half */
 /* One process per GPU: rank 0 makes an id, the host program hands it to every
  * rank (any transport), each rank calls init_rank with its own device. */
 int  sm100_comm_unique_id(void *id128);
