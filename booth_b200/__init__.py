@@ -42,6 +42,18 @@ class AsianParams(C.Structure):
                 ("nstep", C.c_int32), ("k0", C.c_uint32), ("k1", C.c_uint32), ("precise", C.c_int32)]
 
 
+class NewtonSchulz(C.Structure):
+    """booth_newton_schulz_t (include/booth_sm100.h)."""
+    _fields_ = [("steps", C.c_int32), ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float)]
+
+
+class Muon(C.Structure):
+    """booth_muon_t (include/booth_sm100.h)."""
+    _fields_ = ([(n, C.c_float) for n in ("lr", "scale", "momentum", "weight_decay")] +
+                [(n, C.c_int32) for n in ("nesterov", "wdtype", "mdtype", "gdtype")] +
+                [(n, C.c_longlong) for n in ("ld_w", "stride_w", "ld_m", "stride_m", "ld_g", "stride_g")])
+
+
 class Kern(C.Structure):
     """sm100_kern_t (include/booth_sm100.h)."""
     _fields_ = [("mod", C.c_void_p), ("func", C.c_void_p), ("param_bytes", C.c_uint32),
@@ -111,6 +123,11 @@ _SIGNATURES = {
     "booth_sm100_layernorm_backward": (C.c_int, [_dev] + [_ptr] * 8 + [C.c_longlong, C.c_int] + [C.c_longlong] * 3 +
                                        [C.c_int, C.c_int, _ptr, C.c_size_t]),
     "booth_sm100_layernorm_backward_workspace": (C.c_size_t, [_dev, C.c_longlong, C.c_int, C.c_int, C.c_int]),
+    "booth_sm100_orthogonalise": (C.c_int, [_dev, _ptr, _ptr, C.c_int, C.c_int, C.c_int] + [C.c_longlong] * 4 +
+                                  [C.c_int, C.POINTER(NewtonSchulz), _ptr, C.c_size_t]),
+    "booth_sm100_orthogonalise_workspace": (C.c_size_t, [_dev, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "booth_sm100_muon_step": (C.c_int, [_dev, _ptr, _ptr, _ptr, C.c_int, C.c_int, C.c_int, C.POINTER(Muon), C.POINTER(NewtonSchulz),
+                                        _ptr, C.c_size_t]),
     # layer 3
     "sm100_comm_unique_id": (C.c_int, [C.c_void_p]),
     "sm100_comm_init_rank": (C.c_int, [C.POINTER(C.c_void_p), _dev, C.c_int, C.c_int, C.c_void_p]),
@@ -331,6 +348,33 @@ class Device:
         self._ck("booth_sm100_layernorm_backward", lib().booth_sm100_layernorm_backward(
             self._h, dx, dw, db, dy, x, w, mean, rstd, rows, cols, cols if lddx is None else lddx,
             cols if lddy is None else lddy, cols if ldx is None else ldx, dtype, dtype if wdtype is None else wdtype, ws, ws_bytes))
+
+    def orthogonalise_workspace(self, batch, rows, cols, dtype=F32):
+        """Bytes of workspace for results of this type (a Muon step: the type of its weights)."""
+        n = lib().booth_sm100_orthogonalise_workspace(self._h, batch, rows, cols, dtype)
+        if n == 0:
+            self._ck("booth_sm100_orthogonalise_workspace", ERR_ARG)
+        return n
+
+    def orthogonalise(self, out, inp, batch, rows, cols, ws, ws_bytes, dtype=F32, steps=5, abc=(3.4445, -4.7750, 2.0315), eps=1e-7,
+                      ld_in=None, stride_in=None, ld_out=None, stride_out=None):
+        """out = Newton-Schulz iteration of each of `batch` matrices [rows, cols]."""
+        ld_in, ld_out = cols if ld_in is None else ld_in, cols if ld_out is None else ld_out
+        ns = NewtonSchulz(steps, *abc, eps)
+        self._ck("booth_sm100_orthogonalise", lib().booth_sm100_orthogonalise(
+            self._h, out, inp, batch, rows, cols, ld_in, rows * ld_in if stride_in is None else stride_in,
+            ld_out, rows * ld_out if stride_out is None else stride_out, dtype, C.byref(ns), ws, ws_bytes))
+
+    def muon_step(self, w, m, g, batch, rows, cols, ws, ws_bytes, lr, scale=1.0, momentum=0.95, weight_decay=0.0, nesterov=True,
+                  wdtype=F32, mdtype=F32, gdtype=F32, steps=5, abc=(3.4445, -4.7750, 2.0315), eps=1e-7,
+                  ld_w=None, stride_w=None, ld_m=None, stride_m=None, ld_g=None, stride_g=None):
+        """One Muon update of the weights w and the momentum m from the gradient g."""
+        ld_w, ld_m, ld_g = (cols if v is None else v for v in (ld_w, ld_m, ld_g))
+        p = Muon(lr, scale, momentum, weight_decay, 1 if nesterov else 0, wdtype, mdtype, gdtype,
+                 ld_w, rows * ld_w if stride_w is None else stride_w, ld_m, rows * ld_m if stride_m is None else stride_m,
+                 ld_g, rows * ld_g if stride_g is None else stride_g)
+        ns = NewtonSchulz(steps, *abc, eps)
+        self._ck("booth_sm100_muon_step", lib().booth_sm100_muon_step(self._h, w, m, g, batch, rows, cols, C.byref(p), C.byref(ns), ws, ws_bytes))
 
 
 class Comm:

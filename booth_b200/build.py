@@ -83,7 +83,7 @@ def build(force=False, verbose=False):
               '-DBOOTH_SM100_IMAGE="%s"' % CUBIN,
               "-o", SO] + csrc + [os.path.join(CSRC, "image.S"), noalloc_o] +
              ["-Wl,-Bsymbolic", "-Wl,-z,noexecstack", "-Wl,--exclude-libs,ALL", "-L", os.path.join(cuda, "lib64"), "-lcudart_static",
-              "-lstdc++", "-lrt", "-ldl", "-lpthread"], log)
+              "-lstdc++", "-lrt", "-ldl", "-lpthread", "-lm"], log)
     if verbose:
         sys.stdout.write("\n".join(log))
     return SO

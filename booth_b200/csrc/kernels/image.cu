@@ -11,3 +11,4 @@
 #if __has_include("gemm_tf32x3.cu")
 #include "gemm_tf32x3.cu"
 #endif
+#include "orthogonal.cu"

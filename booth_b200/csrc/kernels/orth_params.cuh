@@ -1,0 +1,50 @@
+// orth_params.cuh -- parameter blocks of the orthogonalisation kernels, shared by the
+// kernels (orthogonal.cu) and the C host code that fills them (sm100_train.c): plain C
+// layout, device addresses as typed pointers on the device and integers on the host.
+#ifndef ORTH_PARAMS_CUH
+#define ORTH_PARAMS_CUH
+#ifdef __CUDACC__
+#define ORTH_PTR(T) T *
+#else
+#define ORTH_PTR(T) unsigned long long
+#endif
+
+/* Element types inside the kernels. */
+#define ORTH_F32  0
+#define ORTH_BF16 1
+#define ORTH_F16  2
+
+/* The matrices a call reads: the gradient and, for Muon, the momentum beside it
+ * (m = 0: none). Element (r, c) of matrix k lies at k * stride + r * ld + c. */
+typedef struct orth_source {
+    ORTH_PTR(const void) g;
+    ORTH_PTR(void) m;
+    long long ld_g, stride_g, ld_m, stride_m;
+    int type_g, type_m, rows, cols, nesterov, vec;      /* vec: groups of four elements are aligned in g and m */
+    float mu;
+    int pad_;
+} orth_source_t;
+
+/* What a product kernel computes. */
+#define ORTH_GRAM   0       /* A = X X^t */
+#define ORTH_POLY   1       /* P = b A + c A A */
+#define ORTH_UPDATE 2       /* X = a X + P X */
+#define ORTH_RESULT 3       /* the same into the caller's matrix: w = keep w + value */
+
+typedef struct orth_product {
+    int mode, rows, cols, K, batch;                     /* of the product: rows x cols, square for GRAM and POLY */
+    float alpha, beta;                                  /* out = alpha * accumulator + beta * in */
+    int type_w, tall, vec_w;
+    ORTH_PTR(const void) in_hi;
+    ORTH_PTR(const void) in_lo;                         /* 0: hi alone */
+    ORTH_PTR(void) out_hi;
+    ORTH_PTR(void) out_lo;                              /* 0: hi alone */
+    long long pitch, plane;                             /* of in and out: equal shapes */
+    ORTH_PTR(void) w;                                   /* RESULT; transposed when tall */
+    long long ld_w, stride_w;
+    float keep;                                         /* 0: w is not read */
+    int pad_;
+    ORTH_PTR(int) status;
+    unsigned long long wait_ns;
+} orth_product_t;
+#endif

@@ -41,6 +41,7 @@ typedef struct sm100_api {
     CUresult (*StreamCreate)(CUstream *, unsigned);
     CUresult (*StreamDestroy)(CUstream);
     CUresult (*StreamSynchronize)(CUstream);
+    CUresult (*StreamIsCapturing)(CUstream, CUstreamCaptureStatus *);       /* optional */
     CUresult (*StreamWaitEvent)(CUstream, CUevent, unsigned);
     CUresult (*EventCreate)(CUevent *, unsigned);
     CUresult (*EventDestroy)(CUevent);
@@ -66,6 +67,7 @@ typedef struct sm100_api {
 /* Byte offsets inside the device scratch buffer. */
 #define SM100_SCRATCH_TICKET       0
 #define SM100_SCRATCH_GEMM_STATUS  128
+#define SM100_SCRATCH_ORTH_STATUS  160
 #define SM100_SCRATCH_PARTIALS     256
 
 /* Forms of the layer normalisation kernels, the same for both directions. */
@@ -81,7 +83,9 @@ enum {
     /* layer normalisation: five pairs of types, six forms each; per element type (f32, bf16, f16) the column sums */
     SM100_K_LN_FWD, SM100_K_LN_BWD = SM100_K_LN_FWD + 5 * SM100_LN_FORMS,
     SM100_K_LN_COLUMNS = SM100_K_LN_BWD + 5 * SM100_LN_FORMS, SM100_K_LN_PARAM_GRAD = SM100_K_LN_COLUMNS + 3,
-    SM100_K_COUNT = SM100_K_LN_PARAM_GRAD + 3
+    /* orthogonalisation: the products by form (single, pair) and planes (1, 2) */
+    SM100_K_ORTH_NORM = SM100_K_LN_PARAM_GRAD + 3, SM100_K_ORTH_SPLIT, SM100_K_ORTH_PRODUCT,
+    SM100_K_COUNT = SM100_K_ORTH_PRODUCT + 4
 };
 
 struct sm100_dev {
@@ -113,6 +117,9 @@ struct sm100_dev {
     int         gemm_pending;          /* a GEMM was enqueued since the last status check */
     int         gemm_smem_set;         /* dynamic shared memory limit raised on the GEMM kernels */
     unsigned    gemm_wait_ms;          /* limit of the GEMM kernel's barrier waits */
+    int         orth_pending;          /* an orthogonalisation was enqueued since the last status check */
+    int         orth_captured;         /* one was captured into a graph: its replays are not seen here */
+    int         orth_smem_set;         /* dynamic shared memory limit raised on the product kernels */
     unsigned    gemm_epoch;            /* tag of the latest persistent GEMM call (never zero once used) */
     int         gemm_clusters;         /* CTA pairs of the persistent GEMM kernel this GPU holds at once (0 = not asked yet) */
     /* The GEMM's four tensor maps (64-byte aligned, allocated on first use) and what they were encoded for. */
@@ -153,7 +160,7 @@ void sm100_func_name(sm100_dev_t *dev, void *func, char *out, size_t n);
 CUdeviceptr sm100_scratch(sm100_dev_t *dev, size_t bytes);
 CUdeviceptr sm100_gemm_ws(sm100_dev_t *dev, size_t bytes);
 
-/* Reads the status word of a GEMM enqueued since the last check (the stream must
+/* Reads the status words of a GEMM and of an orthogonalisation enqueued since the last check (the stream must
  * be idle): SM100_OK, or SM100_ERR_CUDA with the text recorded and printed. */
 int  sm100_gemm_outcome(sm100_dev_t *dev);
 

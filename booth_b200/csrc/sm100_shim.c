@@ -87,6 +87,7 @@ static int api_load(void)
     SYM(EventSynchronize, "cuEventSynchronize");
     SYM(EventElapsedTime, "cuEventElapsedTime");
     SYM(LaunchKernel, "cuLaunchKernel");
+    OPT(StreamIsCapturing, "cuStreamIsCapturing");
     OPT(LaunchKernelEx, "cuLaunchKernelEx");
     OPT(OccupancyMaxActiveClusters, "cuOccupancyMaxActiveClusters");
     SYM(GetErrorString, "cuGetErrorString");
@@ -156,6 +157,7 @@ static const char *const k_names[SM100_K_COUNT] = {
     LN_FORM_NAMES("layernorm_bwd_f16"), LN_FORM_NAMES("layernorm_bwd_f16_f32"),
     "layernorm_bwd_columns_f32", "layernorm_bwd_columns_bf16", "layernorm_bwd_columns_f16",
     "layernorm_param_grad_f32", "layernorm_param_grad_bf16", "layernorm_param_grad_f16",
+    "orth_norm", "orth_split", "orth_product_1_single", "orth_product_2_single", "orth_product_1_pair", "orth_product_2_pair",
 };
 
 int sm100_rt_device_count(void)
@@ -439,9 +441,28 @@ void sm100_rt_unload(sm100_dev_t *dev, sm100_kern_t *kern)
  * (sync, the synchronous copies, toc, free) calls this, so a caller that goes from
  * booth_sm100_gemm straight to a copy back learns of it too. The stream must be
  * idle when this is called. */
+static int orth_outcome(sm100_dev_t *dev)
+{
+    if (!dev->orth_pending && !dev->orth_captured) return SM100_OK;
+    int st = 0;
+    dev->orth_pending = 0;
+    const CUdeviceptr word = dev->scratch + SM100_SCRATCH_ORTH_STATUS;
+    CUresult cr = dev->api->MemcpyDtoH(&st, word, sizeof st);
+    if (cr != CUDA_SUCCESS) return sm100_fail(dev, "reading the orthogonalisation's status", cr);
+    if (st != 0) {
+        (void)dev->api->MemsetD8Async(word, 0, sizeof st, dev->stream);
+        snprintf(dev->err, sizeof dev->err, "orth_product gave up waiting on a barrier (code %d: "
+                 "1 = producer, 2 = MMA issuer on operands, 3 = epilogue, 4 = MMA issuer on a free accumulator)", st);
+        fprintf(stderr, "sm100_rt: %s\n", dev->err);
+        return SM100_ERR_CUDA;
+    }
+    return SM100_OK;
+}
+
 int sm100_gemm_outcome(sm100_dev_t *dev)
 {
-    if (!dev->gemm_pending) return SM100_OK;
+    const int orth = orth_outcome(dev);
+    if (!dev->gemm_pending) return orth;
     int st = 0;
     dev->gemm_pending = 0;
     CUresult cr = dev->api->MemcpyDtoH(&st, dev->scratch + SM100_SCRATCH_GEMM_STATUS, sizeof st);
@@ -452,7 +473,7 @@ int sm100_gemm_outcome(sm100_dev_t *dev)
         fprintf(stderr, "sm100_rt: %s\n", dev->err);
         return SM100_ERR_CUDA;
     }
-    return SM100_OK;
+    return orth;
 }
 
 /* ---- memory ---- */
@@ -477,7 +498,7 @@ void sm100_rt_free(sm100_dev_t *dev, sm100_ptr_t ptr)
     /* cuMemFree itself waits for the work that may still use the block. Only a
      * GEMM whose outcome nobody has asked for yet needs a wait of our own: its
      * status is read (and a failure printed) before the memory goes away. */
-    if (dev->gemm_pending && dev->api->StreamSynchronize(dev->stream) == CUDA_SUCCESS)
+    if ((dev->gemm_pending || dev->orth_pending) && dev->api->StreamSynchronize(dev->stream) == CUDA_SUCCESS)
         (void)sm100_gemm_outcome(dev);
     dev->api->MemFree((CUdeviceptr)ptr);
 }

@@ -1,4 +1,5 @@
-/* sm100_train.c -- the training operators: layer normalisation and its gradient.
+/* sm100_train.c -- the training operators: layer normalisation and its gradient,
+ * Newton-Schulz orthogonalisation and the Muon update.
  *
  * Like the workloads in sm100_ops.c each call checks its arguments on the host,
  * enqueues its kernels on the device's stream and returns. Nothing is allocated
@@ -7,10 +8,12 @@
  * two streams that the caller orders, share one only where the caller says so. */
 #define _POSIX_C_SOURCE 200809L
 #include <limits.h>
+#include <math.h>
 #include <stdio.h>
 #include <string.h>
 
 #include "sm100_internal.h"
+#include "kernels/orth_params.cuh"
 
 static int bad_arg(sm100_dev_t *dev, const char *what)
 {
@@ -157,4 +160,265 @@ int booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t
         rc = sm100_launch_k3_overlapped(dev, SM100_K_LN_PARAM_GRAD + type_index(wdtype), (unsigned)(((long long)cols + 31) / 32), 2, 1, 256, 1, 1, 0, pa);
     }
     return rc;
+}
+
+/* ---- orthogonalisation and Muon ---- */
+
+#define ORTH_MAX_SIDE (1 << 20)
+#define ORTH_SMEM 197632u               /* 6 x 32 KB or 3 x 64 KB of operand stages, and 1 KB to align them */
+
+static size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+/* Where things lie in the workspace: the norms' partial sums, then fp16 planes. X is
+ * short x long, A and P short x short; rows of a plane are a multiple of 64 elements
+ * apart. X exists twice, the products read one copy and write the other. One-plane
+ * results (bf16) keep lo planes of X only. */
+typedef struct orth_layout {
+    long long s, l, x_pitch, a_pitch;
+    int parts;
+    size_t x_hi[2], x_lo[2], a_hi, a_lo, p_hi, p_lo, bytes;
+} orth_layout_t;
+
+static int orth_layout(orth_layout_t *o, int batch, int rows, int cols, int two_planes)
+{
+    if (batch < 1 || batch > 65535 || rows < 1 || cols < 1 || rows > ORTH_MAX_SIDE || cols > ORTH_MAX_SIDE) return 0;
+    o->s = rows < cols ? rows : cols;
+    o->l = rows < cols ? cols : rows;
+    o->x_pitch = (long long)up((size_t)o->l, 64);
+    o->a_pitch = (long long)up((size_t)o->s, 64);
+    /* the norm: a few thousand elements a block, some four blocks an SM over the batch */
+    long long parts = ((long long)rows * cols + 4095) / 4096, most = 592 / batch > 8 ? 592 / batch : 8;
+    o->parts = (int)(parts < most ? parts : most);
+    const size_t x = up((size_t)batch * o->s * o->x_pitch * 2, 128), a = up((size_t)batch * o->s * o->a_pitch * 2, 128);
+    size_t at = up((size_t)batch * o->parts * sizeof(double), 128);
+    for (int i = 0; i < 2; i++) { o->x_hi[i] = at; at += x; o->x_lo[i] = at; at += x; }
+    o->a_hi = at; at += a;
+    o->a_lo = at; if (two_planes) at += a;
+    o->p_hi = at; at += a;
+    o->p_lo = at; if (two_planes) at += a;
+    o->bytes = at;
+    const long long t = (o->l + 127) / 128;
+    return t * ((o->s + 127) / 128) <= INT_MAX / batch;
+}
+
+size_t booth_sm100_orthogonalise_workspace(sm100_dev_t *dev, int batch, int rows, int cols, int dtype)
+{
+    orth_layout_t o;
+    if (!dev || type_index(dtype) < 0 || !orth_layout(&o, batch, rows, cols, dtype != SM100_BF16)) {
+        bad_arg(dev, "booth_sm100_orthogonalise_workspace: bad argument");
+        return 0;
+    }
+    return o.bytes;
+}
+
+/* Map of one plane: batch matrices of rows x cols, rows `pitch` apart, in boxes of 64 x 64
+ * (128 bytes a row, 128-byte swizzle). What lies outside a matrix reads as zero. */
+static int plane_map(sm100_dev_t *dev, CUtensorMap *map, CUdeviceptr p, long long rows, long long cols, long long pitch, int batch)
+{
+    cuuint64_t dims[3] = { (cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch };
+    cuuint64_t strides[2] = { (cuuint64_t)pitch * 2, (cuuint64_t)pitch * rows * 2 };
+    cuuint32_t box[3] = { 64, 64, 1 }, step[3] = { 1, 1, 1 };
+    CUresult cr = dev->api->TensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void *)(size_t)p, dims, strides, box, step,
+                                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return cr == CUDA_SUCCESS ? SM100_OK : sm100_fail(dev, "cuTensorMapEncodeTiled", cr);
+}
+
+/* cuTensorMapEncodeTiled wants its maps on 64-byte boundaries. */
+typedef struct { CUtensorMap hi __attribute__((aligned(64))), lo __attribute__((aligned(64))); } plane_maps_t;
+
+/* Pairs of CTAs on 256 x 256 tiles, or single CTAs on 128 x 128. A pair tile takes
+ * twice as long as a single one at full rate, and the narrow tile, which reads its
+ * operands from shared memory twice as often, runs at about 3/4 of it: the form with the
+ * shorter list of waves wins. */
+static int orth_pairs(const sm100_dev_t *dev, long long rows, long long cols, int batch, int sym)
+{
+    const long long pm = (rows + 255) / 256, pn = (cols + 255) / 256, sm = (rows + 127) / 128, sn = (cols + 127) / 128;
+    const long long pt = batch * (sym ? pm * (pm + 1) / 2 : pm * pn), st = batch * (sym ? sm * (sm + 1) / 2 : sm * sn);
+    const long long slots = dev->sm_count / 2 > 0 ? dev->sm_count / 2 : 1;
+    const long long pw = (pt + slots - 1) / slots, sw = (st + 2 * slots - 1) / (2 * slots);
+    return 6 * pw <= 4 * sw;
+}
+
+static int orth_launch(sm100_dev_t *dev, const plane_maps_t *a, const plane_maps_t *b, orth_product_t *p, int two_planes)
+{
+    const int sym = p->mode <= ORTH_POLY, pairs = orth_pairs(dev, p->rows, p->cols, p->batch, sym);
+    const long long side = pairs ? 256 : 128, tm = (p->rows + side - 1) / side, tn = (p->cols + side - 1) / side;
+    const long long tiles = p->batch * (sym ? tm * (tm + 1) / 2 : tm * tn), slots = pairs ? dev->sm_count / 2 : dev->sm_count;
+    const unsigned grid = (unsigned)((tiles < slots ? tiles : slots) * (pairs ? 2 : 1));
+    void *args[] = { (void *)&a->hi, (void *)&a->lo, (void *)&b->hi, (void *)&b->lo, p };
+    return sm100_launch_k3_overlapped(dev, SM100_K_ORTH_PRODUCT + (pairs ? 2 : 0) + (two_planes ? 1 : 0), grid, 1, 1, 384, 1, 1, ORTH_SMEM, args);
+}
+
+static int orth_status_ready(sm100_dev_t *dev)
+{
+    if (!dev->orth_smem_set) {
+        for (int i = 0; i < 4; i++) {
+            CUresult cr = dev->api->FuncSetAttribute(dev->k[SM100_K_ORTH_PRODUCT + i], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)ORTH_SMEM);
+            if (cr != CUDA_SUCCESS) return sm100_fail(dev, "raising the product kernels' shared memory limit", cr);
+        }
+        dev->orth_smem_set = 1;
+    }
+    /* A captured call runs when its graph is replayed, which this library does not see: from then on the
+     * status word is read at every wait. */
+    CUstreamCaptureStatus capturing = CU_STREAM_CAPTURE_STATUS_NONE;
+    if (dev->api->StreamIsCapturing && dev->api->StreamIsCapturing(dev->stream, &capturing) == CUDA_SUCCESS &&
+        capturing != CU_STREAM_CAPTURE_STATUS_NONE)
+        dev->orth_captured = 1;
+    dev->orth_pending = 1;
+    return SM100_OK;
+}
+
+/* src -> normalise -> ns->steps x (gram, polynomial, update); the last update goes to w. */
+static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_product_t *last, int batch, int two_planes,
+                         const booth_newton_schulz_t *ns, float factor, sm100_ptr_t ws, const orth_layout_t *o)
+{
+    int rc = orth_status_ready(dev);
+    if (rc != SM100_OK) return rc;
+    const int tall = src->rows > src->cols;
+    CUdeviceptr partial = ws;
+    int parts = o->parts;
+    void *na[] = { src, &partial };
+    rc = sm100_launch_k3_overlapped(dev, SM100_K_ORTH_NORM, (unsigned)parts, (unsigned)batch, 1, 256, 1, 1, 0, na);
+    if (rc != SM100_OK) return rc;
+    CUdeviceptr hi = ws + o->x_hi[0], lo = ws + o->x_lo[0];
+    float eps = ns->eps;
+    long long pitch = o->x_pitch, plane = o->x_pitch * o->s;
+    int t = tall;
+    void *sa[] = { src, &partial, &parts, &eps, &hi, &lo, &pitch, &plane, &t };
+    rc = sm100_launch_k3_overlapped(dev, SM100_K_ORTH_SPLIT, (unsigned)((src->cols + 63) / 64), (unsigned)((src->rows + 63) / 64), (unsigned)batch,
+                                    256, 1, 1, 0, sa);
+    if (rc != SM100_OK) return rc;
+
+    plane_maps_t x[2], a, p;
+    for (int i = 0; i < 2; i++) {
+        if ((rc = plane_map(dev, &x[i].hi, ws + o->x_hi[i], o->s, o->l, o->x_pitch, batch)) != SM100_OK) return rc;
+        if ((rc = plane_map(dev, &x[i].lo, ws + o->x_lo[i], o->s, o->l, o->x_pitch, batch)) != SM100_OK) return rc;
+    }
+    if ((rc = plane_map(dev, &a.hi, ws + o->a_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+    if ((rc = plane_map(dev, &p.hi, ws + o->p_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+    a.lo = a.hi; p.lo = p.hi;           /* not read by the one-plane kernels */
+    if (two_planes) {
+        if ((rc = plane_map(dev, &a.lo, ws + o->a_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+        if ((rc = plane_map(dev, &p.lo, ws + o->p_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+    }
+    /* P's scale: with singular values below 2, |P| <= 4 |b| + 16 |c| has to stay below fp16's 65504. */
+    const double bound = 4.0 * fabs(ns->b) + 16.0 * fabs(ns->c);
+    double p_scale = 16384.0;
+    while (p_scale * bound > 65000.0) p_scale *= 0.5;
+    const double inv = 1.0 / 16384.0;
+
+    orth_product_t q = *last;
+    q.batch = batch;
+    q.status = dev->scratch + SM100_SCRATCH_ORTH_STATUS;
+    q.wait_ns = (unsigned long long)dev->gemm_wait_ms * 1000000ull;
+    for (int i = 0; i < ns->steps; i++) {
+        const int from = i & 1, to = from ^ 1;
+        q.rows = q.cols = (int)o->s;
+        q.pitch = o->a_pitch; q.plane = o->a_pitch * o->s;
+        q.mode = ORTH_GRAM; q.K = (int)o->l;
+        q.alpha = (float)inv; q.beta = 0.0f;
+        q.in_hi = q.in_lo = 0;
+        q.out_hi = ws + o->a_hi; q.out_lo = two_planes ? ws + o->a_lo : 0;
+        if ((rc = orth_launch(dev, &x[from], &x[from], &q, two_planes)) != SM100_OK) return rc;
+        q.mode = ORTH_POLY; q.K = (int)o->s;
+        q.alpha = (float)(ns->c * p_scale * inv * inv); q.beta = (float)(ns->b * p_scale * inv);
+        q.in_hi = q.out_hi; q.in_lo = q.out_lo;
+        q.out_hi = ws + o->p_hi; q.out_lo = two_planes ? ws + o->p_lo : 0;
+        if ((rc = orth_launch(dev, &a, &a, &q, two_planes)) != SM100_OK) return rc;
+        const int end = i == ns->steps - 1;
+        q.mode = end ? ORTH_RESULT : ORTH_UPDATE;
+        q.cols = (int)o->l;
+        q.pitch = o->x_pitch; q.plane = plane;
+        q.alpha = (float)((end ? factor * inv : 1.0) / p_scale); q.beta = (float)(end ? factor * inv * ns->a : ns->a);
+        q.in_hi = ws + o->x_hi[from]; q.in_lo = ws + o->x_lo[from];
+        q.out_hi = ws + o->x_hi[to]; q.out_lo = ws + o->x_lo[to];
+        if ((rc = orth_launch(dev, &p, &x[from], &q, two_planes)) != SM100_OK) return rc;
+    }
+    return SM100_OK;
+}
+
+static const booth_newton_schulz_t ns_default = { 5, 3.4445f, -4.7750f, 2.0315f, 1e-7f };
+
+static int ns_ok(const booth_newton_schulz_t *ns)
+{
+    return ns->steps >= 1 && ns->steps <= 64 && isfinite(ns->a) && isfinite(ns->b) && isfinite(ns->c) && isfinite(ns->eps) && ns->eps > 0.0f;
+}
+
+/* batch matrices: the pitch no shorter than a row, the last element within 2^59 elements of the first. */
+static int matrices_ok(sm100_ptr_t p, int dtype, int batch, int rows, int cols, long long ld, long long stride)
+{
+    if (!matrix_ok(p, type_bytes(dtype), rows, cols, ld) || stride < 0) return 0;
+    return batch <= 1 || (stride >= cols && stride <= (1ll << 59) / batch);
+}
+
+/* Whether groups of four elements of every row are aligned to their size. */
+static int four_ok(sm100_ptr_t p, int dtype, int batch, int cols, long long ld, long long stride)
+{
+    return !(p & (4 * type_bytes(dtype) - 1)) && cols % 4 == 0 && ld % 4 == 0 && (batch == 1 || stride % 4 == 0);
+}
+
+int booth_sm100_orthogonalise(sm100_dev_t *dev, sm100_ptr_t out, sm100_ptr_t in, int batch, int rows, int cols,
+                              long long ld_in, long long stride_in, long long ld_out, long long stride_out,
+                              int dtype, const booth_newton_schulz_t *ns, sm100_ptr_t ws, size_t ws_bytes)
+{
+    int rc = sm100_enter(dev);
+    if (rc != SM100_OK) return rc;
+    orth_layout_t o;
+    if (!ns) ns = &ns_default;
+    if (type_index(dtype) < 0) return bad_arg(dev, "booth_sm100_orthogonalise: the type is f32, bf16 or f16");
+    if (!ns_ok(ns)) return bad_arg(dev, "booth_sm100_orthogonalise: need 1 to 64 steps, finite coefficients and eps > 0");
+    if (!orth_layout(&o, batch, rows, cols, dtype != SM100_BF16) || !matrices_ok(in, dtype, batch, rows, cols, ld_in, stride_in) ||
+        !matrices_ok(out, dtype, batch, rows, cols, ld_out, stride_out) || (in == out && (ld_in != ld_out || (batch > 1 && stride_in != stride_out))))
+        return bad_arg(dev, "booth_sm100_orthogonalise: need 1 to 65535 matrices of 1 to 2^20 rows and columns, operands non-NULL and aligned to "
+                            "their element, pitches >= cols, strides >= cols (equal ones when out is in)");
+    if (!ws || (ws & 127) || ws_bytes < o.bytes)
+        return bad_arg(dev, "booth_sm100_orthogonalise: workspace missing, not 128-byte aligned or too small");
+    orth_source_t src;
+    memset(&src, 0, sizeof src);
+    src.g = in; src.ld_g = ld_in; src.stride_g = stride_in; src.type_g = type_index(dtype);
+    src.rows = rows; src.cols = cols;
+    src.vec = four_ok(in, dtype, batch, cols, ld_in, stride_in);
+    orth_product_t last;
+    memset(&last, 0, sizeof last);
+    last.w = out; last.ld_w = ld_out; last.stride_w = stride_out; last.type_w = type_index(dtype);
+    last.tall = rows > cols;
+    last.vec_w = four_ok(out, dtype, batch, cols, ld_out, stride_out);
+    return newton_schulz(dev, &src, &last, batch, dtype != SM100_BF16, ns, 1.0f, ws, &o);
+}
+
+int booth_sm100_muon_step(sm100_dev_t *dev, sm100_ptr_t w, sm100_ptr_t m, sm100_ptr_t g, int batch, int rows, int cols,
+                          const booth_muon_t *p, const booth_newton_schulz_t *ns, sm100_ptr_t ws, size_t ws_bytes)
+{
+    int rc = sm100_enter(dev);
+    if (rc != SM100_OK) return rc;
+    orth_layout_t o;
+    if (!ns) ns = &ns_default;
+    if (!p || type_index(p->wdtype) < 0 || type_index(p->mdtype) < 0 || type_index(p->gdtype) < 0)
+        return bad_arg(dev, "booth_sm100_muon_step: the types are f32, bf16 or f16");
+    if (!ns_ok(ns)) return bad_arg(dev, "booth_sm100_muon_step: need 1 to 64 steps, finite coefficients and eps > 0");
+    if (!isfinite(p->lr) || !isfinite(p->scale) || !isfinite(p->weight_decay) || !(p->momentum >= 0.0f && p->momentum <= 1.0f))
+        return bad_arg(dev, "booth_sm100_muon_step: need a finite learning rate, scale and weight decay, and momentum in [0, 1]");
+    const int two_planes = p->wdtype != SM100_BF16;
+    if (!orth_layout(&o, batch, rows, cols, two_planes) || !matrices_ok(w, p->wdtype, batch, rows, cols, p->ld_w, p->stride_w) ||
+        !matrices_ok(m, p->mdtype, batch, rows, cols, p->ld_m, p->stride_m) || !matrices_ok(g, p->gdtype, batch, rows, cols, p->ld_g, p->stride_g) ||
+        w == m || w == g || m == g)
+        return bad_arg(dev, "booth_sm100_muon_step: need 1 to 65535 matrices of 1 to 2^20 rows and columns; w, m and g non-NULL, apart from one "
+                            "another and aligned to their element; pitches >= cols, strides >= cols");
+    if (!ws || (ws & 127) || ws_bytes < o.bytes)
+        return bad_arg(dev, "booth_sm100_muon_step: workspace missing, not 128-byte aligned or too small");
+    orth_source_t src;
+    memset(&src, 0, sizeof src);
+    src.g = g; src.ld_g = p->ld_g; src.stride_g = p->stride_g; src.type_g = type_index(p->gdtype);
+    src.m = m; src.ld_m = p->ld_m; src.stride_m = p->stride_m; src.type_m = type_index(p->mdtype);
+    src.rows = rows; src.cols = cols;
+    src.nesterov = p->nesterov != 0; src.mu = p->momentum;
+    src.vec = four_ok(g, p->gdtype, batch, cols, p->ld_g, p->stride_g) && four_ok(m, p->mdtype, batch, cols, p->ld_m, p->stride_m);
+    orth_product_t last;
+    memset(&last, 0, sizeof last);
+    last.w = w; last.ld_w = p->ld_w; last.stride_w = p->stride_w; last.type_w = type_index(p->wdtype);
+    last.tall = rows > cols;
+    last.vec_w = four_ok(w, p->wdtype, batch, cols, p->ld_w, p->stride_w);
+    last.keep = (float)(1.0 - (double)p->lr * p->weight_decay);
+    return newton_schulz(dev, &src, &last, batch, two_planes, ns, (float)(-(double)p->lr * p->scale), ws, &o);
 }

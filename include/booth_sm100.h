@@ -303,6 +303,48 @@ int  booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_
 /* Bytes of workspace the call above needs; 0 on a bad argument. */
 size_t booth_sm100_layernorm_backward_workspace(sm100_dev_t *dev, long long rows, int cols, int dtype, int wdtype);
 
+/* The Newton-Schulz iteration of the two calls below: steps of
+ *   A = X X^t,  X = a X + (b A + c A A) X,  from X = G / (|G|_F + eps)
+ * (for a matrix with more rows than columns X is its transpose, the result is the same
+ * polynomial). NULL where one is expected means five steps of the Muon optimiser's
+ * quintic, 3.4445, -4.7750, 2.0315, and eps = 1e-7. 1 to 64 steps; eps > 0. The
+ * coefficients must keep the singular values below 2, as every scheme that converges
+ * from [0, 1] does (the operands are fp16, scaled for that range): beyond, results are not finite. */
+typedef struct booth_newton_schulz {
+    int32_t steps;
+    float   a, b, c, eps;
+} booth_newton_schulz_t;
+/* out = the iteration's result for each of `batch` matrices [rows, cols]; element (r, c)
+ * of matrix k lies k * stride + r * ld + c elements from the operand's address (strides
+ * are not looked at when batch is 1). dtype (SM100_F32, SM100_BF16, SM100_F16) is the type
+ * of both. f32 and f16 results are computed from 22-bit operands (no less exact than
+ * fp32 products), bf16 results from 11-bit operands and a 22-bit X: off by less than a step
+ * of bf16, where the usual bf16 iteration is off by 1 to 50 percent. A matrix of zeros
+ * gives zeros; one that holds an infinity or NaN gives no finite result, without
+ * touching the others. out may be in (same pitch and stride); otherwise they must not
+ * overlap. ws: booth_sm100_orthogonalise_workspace bytes for the same batch, rows,
+ * cols and dtype, 128-byte aligned, any contents. */
+int  booth_sm100_orthogonalise(sm100_dev_t *dev, sm100_ptr_t out, sm100_ptr_t in, int batch, int rows, int cols,
+                               long long ld_in, long long stride_in, long long ld_out, long long stride_out,
+                               int dtype, const booth_newton_schulz_t *ns, sm100_ptr_t ws, size_t ws_bytes);
+/* Bytes of workspace for dtype results (of the weights, for a Muon step); 0 on a bad argument. */
+size_t booth_sm100_orthogonalise_workspace(sm100_dev_t *dev, int batch, int rows, int cols, int dtype);
+
+/* One Muon update of `batch` weights w with their momentum m and gradient g:
+ *   m = momentum m + (1 - momentum) g,  u = nesterov ? momentum m + (1 - momentum) g : m,
+ *   w = (1 - lr weight_decay) w - lr scale NS(u)
+ * w and m are updated in place, g is read only; u is formed from m as stored. The three
+ * may have different types; the products' precision goes by w's (see above). `scale`
+ * is the caller's choice of update size, for instance 0.2 sqrt(max(rows, cols)). The
+ * workspace is booth_sm100_orthogonalise_workspace(batch, rows, cols, wdtype). */
+typedef struct booth_muon {
+    float     lr, scale, momentum, weight_decay;
+    int32_t   nesterov, wdtype, mdtype, gdtype;
+    long long ld_w, stride_w, ld_m, stride_m, ld_g, stride_g;
+} booth_muon_t;
+int  booth_sm100_muon_step(sm100_dev_t *dev, sm100_ptr_t w, sm100_ptr_t m, sm100_ptr_t g, int batch, int rows, int cols,
+                           const booth_muon_t *p, const booth_newton_schulz_t *ns, sm100_ptr_t ws, size_t ws_bytes);
+
 /* ---------------------------------------------------------------------------
  * Layer 3: the collective (NCCL over NVLink; libnccl.so.2 is dlopen'ed)
  * The reference has no counterpart: it drives one device only

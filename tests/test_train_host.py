@@ -1,8 +1,12 @@
 """Host side of the training operators over the stand-in driver of tests/fake_driver: which kernels a call
 launches and with which shape, and what it refuses before any GPU work."""
+import os
+import subprocess
+
 import pytest
 
-from test_host_logic import fake, run  # noqa: F401  (fixture and helper)
+from conftest import ROOT
+from test_host_logic import CUDA_INC, FAKE_SRC, fake, run  # noqa: F401  (fixture and helper)
 
 
 def test_layernorm_forms_and_shapes(fake, tmp_path):  # noqa: F811
@@ -60,6 +64,119 @@ d.sync(); d.close()
 def test_layernorm_refusals(fake, tmp_path, call):  # noqa: F811
     res, L, _ = run(fake, tmp_path, """
 d = sm.Device(0); p = 1 << 20
+try:
+    %s
+except sm.Sm100Error as e:
+    assert e.code == sm.ERR_ARG, e
+else:
+    raise SystemExit("not refused")
+d.close()
+""" % call)
+    assert res.returncode == 0, res.stderr
+    assert not L
+
+
+KERNELS = os.path.join(ROOT, "booth_b200", "csrc", "kernels")
+
+
+@pytest.fixture(scope="module")
+def fake3(tmp_path_factory, sm):
+    if not os.path.exists(os.path.join(CUDA_INC, "cuda.h")):
+        pytest.skip("cuda.h not found")
+    out = tmp_path_factory.mktemp("fake_driver_train") / "libcuda_fake_train.so"
+    subprocess.run(["gcc", "-std=c99", "-O1", "-shared", "-fPIC", "-I", CUDA_INC, "-I", os.path.dirname(FAKE_SRC), "-I", KERNELS,
+                    os.path.join(os.path.dirname(FAKE_SRC), "fake_cuda_train.c"), "-o", str(out)], check=True)
+    return str(out)
+
+
+def products(lines):
+    return [dict(zip(ln.split()[1::2], map(float, ln.split()[2::2]))) for ln in lines if ln.startswith("product")]
+
+
+def test_orthogonalise_launches(fake3, tmp_path):
+    res, L, lines = run(fake3, tmp_path, """
+d = sm.Device(0); p = 1 << 20
+def go(b, r, c, dt, steps):
+    n = d.orthogonalise_workspace(b, r, c, dt)
+    d.orthogonalise(p, 2 * p, b, r, c, 4 * p, n, dtype=dt, steps=steps)
+go(1, 4096, 4096, sm.BF16, 2)
+go(3, 1000, 500, sm.F32, 1)
+d.sync(); d.close()
+""")
+    assert res.returncode == 0, res.stderr
+    assert [l["kernel"] for l in L] == ["orth_norm", "orth_split"] + ["orth_product_1_pair"] * 6 + ["orth_norm", "orth_split"] + ["orth_product_2_single"] * 3
+    assert all(l["overlap"] == 1 for l in L)
+    assert all(l["shmem"] == 197632 and l["block"] == (384, 1, 1) for l in L if l["kernel"].startswith("orth_product"))
+    P = products(lines)
+    assert [(p["mode"], p["rows"], p["cols"], p["K"], p["batch"], p["tall"]) for p in P] == [
+        (0, 4096, 4096, 4096, 1, 0), (1, 4096, 4096, 4096, 1, 0), (2, 4096, 4096, 4096, 1, 0),
+        (0, 4096, 4096, 4096, 1, 0), (1, 4096, 4096, 4096, 1, 0), (3, 4096, 4096, 4096, 1, 0),
+        (0, 500, 500, 1000, 3, 1), (1, 500, 500, 500, 3, 1), (3, 500, 1000, 500, 3, 1)]
+    # X and A are kept times 2^14, P times 2^10 with the default coefficients
+    want = [(2.0 ** -14, 0), (2.0315 * 2.0 ** -18, -4.7750 * 2.0 ** -4), (2.0 ** -10, 3.4445), (2.0 ** -24, 3.4445 * 2.0 ** -14)]
+    for p, k in zip(P, (0, 1, 2, 0, 1, 3, 0, 1, 3)):
+        assert (p["alpha"], p["beta"]) == pytest.approx(want[k], rel=1e-6)
+    maps = [ln for ln in lines if ln.startswith("tensormap3")]
+    # one plane: hi and lo of both copies of X, A and P; rows a multiple of 64 apart
+    assert maps[:6] == ["tensormap3 dims 4096 4096 1 strides 8192 33554432 box 64 64 1"] * 6
+    assert maps[6:] == ["tensormap3 dims 1000 500 3 strides 2048 1024000 box 64 64 1"] * 4 + ["tensormap3 dims 500 500 3 strides 1024 512000 box 64 64 1"] * 4
+
+
+def test_muon_parameters(fake3, tmp_path):
+    res, L, lines = run(fake3, tmp_path, """
+d = sm.Device(0); p = 1 << 20
+n = d.orthogonalise_workspace(1, 300, 200, sm.F32)
+d.muon_step(p, 2 * p, 3 * p, 1, 300, 200, 4 * p, n, lr=0.1, scale=4.0, weight_decay=0.5, gdtype=sm.BF16, steps=1)
+d.sync(); d.close()
+""")
+    assert res.returncode == 0, res.stderr
+    last = products(lines)[-1]
+    assert last["mode"] == 3 and last["keep"] == pytest.approx(0.95) and last["alpha"] == pytest.approx(-0.4 * 2.0 ** -24) and last["beta"] == pytest.approx(-0.4 * 3.4445 * 2.0 ** -14)
+
+
+def test_a_wait_that_ran_out_is_reported_once(fake3, tmp_path):
+    res, _, _ = run(fake3, tmp_path, """
+import os
+d = sm.Device(0); p = 1 << 20
+n = d.orthogonalise_workspace(1, 64, 64)
+os.environ["FAKE_CUDA_ORTH_STATUS"] = "2"
+import ctypes; ctypes.CDLL(None).setenv(b"FAKE_CUDA_ORTH_STATUS", b"2", 1)
+d.orthogonalise(p, 2 * p, 1, 64, 64, 4 * p, n)
+try:
+    d.sync()
+except sm.Sm100Error as e:
+    assert e.code == sm.ERR_CUDA and "orth_product gave up" in str(e) and "code 2" in str(e), e
+else:
+    raise SystemExit("not reported")
+d.sync()
+ctypes.CDLL(None).unsetenv(b"FAKE_CUDA_ORTH_STATUS")
+d.orthogonalise(p, 2 * p, 1, 64, 64, 4 * p, n)
+d.sync(); d.close()
+""")
+    assert res.returncode == 0, res.stderr
+
+
+@pytest.mark.parametrize("call", [
+    "d.orthogonalise(0, p, 1, 8, 8, p, big)", "d.orthogonalise(p, 0, 1, 8, 8, p, big)", "d.orthogonalise(p, 2 * p, 0, 8, 8, p, big)",
+    "d.orthogonalise(p, 2 * p, 1, 0, 8, p, big)", "d.orthogonalise(p, 2 * p, 1, 8, 0, p, big)", "d.orthogonalise(p, 2 * p, 1, (1 << 20) + 1, 8, p, big)",
+    "d.orthogonalise(p, 2 * p, 65536, 8, 8, p, big)", "d.orthogonalise(p, 2 * p, 1, 8, 8, 0, big)", "d.orthogonalise(p, 2 * p, 1, 8, 8, p + 64, big)",
+    "d.orthogonalise(p, 2 * p, 1, 8, 8, p, d.orthogonalise_workspace(1, 8, 8) - 1)", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, steps=0)",
+    "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, steps=65)", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, eps=0.0)",
+    "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, abc=(1.0, float('nan'), 0.0))", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, abc=(float('inf'), 1.0, 0.0))",
+    "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, ld_in=7)", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, ld_out=7)",
+    "d.orthogonalise(p, 2 * p, 2, 8, 8, p, big, stride_in=7)", "d.orthogonalise(p, 2 * p, 2, 8, 8, p, big, stride_out=-64)",
+    "d.orthogonalise(p, p, 1, 8, 8, p, big, ld_out=9)", "d.orthogonalise(p, p, 2, 8, 8, p, big, stride_out=65)", "d.orthogonalise(p + 2, 2 * p, 1, 8, 8, p, big)",
+    "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, dtype=sm.F64)", "d.orthogonalise(p, 2 * p, 2, 8, 8, p, big, stride_in=1 << 60)",
+    "d.orthogonalise_workspace(0, 8, 8)", "d.orthogonalise_workspace(1, 8, 8, sm.I32)",
+    "d.muon_step(0, p, 2 * p, 1, 8, 8, p, big, lr=0.1)", "d.muon_step(p, p, 2 * p, 1, 8, 8, p, big, lr=0.1)", "d.muon_step(p, 2 * p, p, 1, 8, 8, p, big, lr=0.1)",
+    "d.muon_step(3 * p, 2 * p, 2 * p, 1, 8, 8, p, big, lr=0.1)", "d.muon_step(p, 2 * p, 3 * p, 1, 8, 8, p, big, lr=float('nan'))",
+    "d.muon_step(p, 2 * p, 3 * p, 1, 8, 8, p, big, lr=0.1, momentum=1.5)", "d.muon_step(p, 2 * p, 3 * p, 1, 8, 8, p, big, lr=0.1, weight_decay=float('inf'))",
+    "d.muon_step(p, 2 * p, 3 * p, 1, 8, 8, p, 100, lr=0.1)", "d.muon_step(p, 2 * p, 3 * p, 1, 8, 8, p, big, lr=0.1, mdtype=sm.F64)",
+    "d.muon_step(p, 2 * p, 3 * p, 1, 8, 8, p, big, lr=0.1, ld_m=4)", "d.muon_step(p, 2 * p, 3 * p, 1, 8, 8, p, big, lr=0.1, steps=0)",
+])
+def test_orthogonalise_and_muon_refusals(fake3, tmp_path, call):
+    res, L, _ = run(fake3, tmp_path, """
+d = sm.Device(0); p = 1 << 20; big = 1 << 30
 try:
     %s
 except sm.Sm100Error as e:
