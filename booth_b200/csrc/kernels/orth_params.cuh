@@ -35,6 +35,8 @@ typedef struct orth_product {
     int mode, rows, cols, K, batch;                     /* of the product: rows x cols, square for GRAM and POLY */
     float alpha, beta;                                  /* out = alpha * accumulator + beta * in */
     int type_w, tall, vec_w;
+    int tri;                                            /* tile side of the stored triangle of the symmetric operand (GRAM: of the output) */
+    int pad0_;
     ORTH_PTR(const void) in_hi;
     ORTH_PTR(const void) in_lo;                         /* 0: hi alone */
     ORTH_PTR(void) out_hi;

@@ -20,8 +20,11 @@
 //     values lose by up to a^steps = 485, so rounding X to 11 bits each step showed as 2 to
 //     4 % on matrices of low rank, while rounding only the products' operands leaves 1e-3.
 //
-// A and P are symmetric: only tiles on and below the diagonal are computed, each
-// stored twice (the second time transposed).
+// A and P are symmetric: only tiles on and below the diagonal are computed and stored.
+// Where a product needs a block above the diagonal it loads the mirrored block and has the
+// tensor core take it transposed (an operand may have either index contiguous), so nothing
+// is stored twice: with 2-byte transposed stores the epilogue of a 1024 x 1024
+// product took 12 of its 27 us.
 //
 // Launches per call: orth_norm (sums of squares; Muon: also the momentum), orth_split (planes of
 // the normalised, possibly transposed matrix), then steps x 3 products. A product kernel
@@ -220,17 +223,20 @@ __device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap *map
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
-// fp16 x fp16 -> fp32; bit 16: the second operand's tile has its columns, not K, contiguous.
-__host__ __device__ constexpr uint32_t instr_desc(int m, int n, int b_cols_contiguous)
+// fp16 x fp16 -> fp32; bits 15 and 16: the first or second operand's tile has its rows (columns), not K, contiguous.
+__device__ __forceinline__ uint32_t instr_desc(int m, int n, bool a_t, bool b_t)
 {
-    return (1u << 4) | ((uint32_t)b_cols_contiguous << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+    return (1u << 4) | ((uint32_t)a_t << 15) | ((uint32_t)b_t << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// Tile with 64 columns contiguous (128 bytes a row of K, 128-byte swizzle): 8 rows of K
-// are 1024 bytes, the next 64 columns lie 8192 bytes on.
-__device__ __forceinline__ uint64_t smem_desc_cols(uint32_t addr)
+// A tile of two 64 x 64 boxes, 128 bytes a box row, 128-byte swizzle, 8 rows 1024 bytes. K
+// contiguous (`t` false): rows of the operand, the boxes one below the other. Else rows of K, each with 64
+// rows of the operand; the next 64 lie 8192 bytes on.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, bool t)
 {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(8192u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+    return gemm::smem_desc(addr) | (t ? (uint64_t)(8192u >> 4) << 16 : 0ull);
 }
+// Sixteen of K further: 32 bytes along a row, or sixteen rows.
+__device__ __forceinline__ uint64_t k_advance(int kk, bool t) { return (uint64_t)(kk * (t ? 2048 >> 4 : 32 >> 4)); }
 
 template <bool PAIR>
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
@@ -247,7 +253,9 @@ template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar)
     if constexpr (PAIR) gemm::umma_commit_pair(bar); else gemm::umma_commit(bar);
 }
 
-// Tile number -> matrix, tile row and tile column. Symmetric products number the tiles on and below the diagonal row by row.
+// Tile number -> matrix, tile row and tile column. Tiles that run at the same time should share
+// operand panels through L2: eight tile rows at a time, column by column; symmetric products
+// number the tiles on and below the diagonal that way.
 struct Tiles {
     int tm, tn, each;
     bool sym;
@@ -260,96 +268,177 @@ struct Tiles {
     __device__ __forceinline__ void at(int item, int &k, int &i, int &j) const
     {
         k = item / each;
-        const int t = item - k * each;
+        int t = item - k * each;
         if (!sym) { gemm::pair_tile_coords(t, tm, tn, i, j); return; }
-        i = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-        while ((i + 1) * (i + 2) / 2 <= t) i++;
-        while (i * (i + 1) / 2 > t) i--;
-        j = t - i * (i + 1) / 2;
+        int r0 = 0, h;
+        for (;; r0 += 8) {                      // the group of eight rows: r0 .. r0 + h - 1
+            h = min(tm - r0, 8);
+            const int n = h * r0 + h * (h + 1) / 2;
+            if (t < n) break;
+            t -= n;
+        }
+        if (t < h * (r0 + 1)) { j = t / h; i = r0 + t % h; return; }
+        t -= h * (r0 + 1);
+        for (j = r0 + 1, h--; t >= h; j++, h--) t -= h;
+        i = j + t;
     }
 };
 
-// Thirty-two consecutive columns of one row of the product, from the accumulator: epilogue and stores.
-template <int PLANES>
-__device__ __forceinline__ void emit(const Product &p, float (&v)[32], int k, int row, int col0, bool mirror)
+// One warp's 32 x 32 piece of the product, a row a lane in v, goes out through 4 KB of shared
+// memory of the warp's own, so that global accesses run along rows: a piece's row is 64 bytes of a plane
+// (two sectors), where a store straight from the registers touched 32 lines at once.
+// Shared layout: 16-byte units, swizzled so that neither the lane-a-row nor the along-the-row access conflicts.
+struct Stage {
+    uint32_t base;
+    int lane;
+    // 16-byte unit u of row r: planes (hi, then lo 2048 bytes on) have 4 units a row, fp32 pieces 8
+    __device__ __forceinline__ uint32_t half_at(int r, int u) const { return base + (uint32_t)(r * 64 + ((u ^ (r >> 1)) & 3) * 16); }
+    __device__ __forceinline__ uint32_t f32_at(int r, int u) const { return base + (uint32_t)(r * 128 + ((u ^ r) & 7) * 16); }
+};
+__device__ __forceinline__ void sts(uint32_t a, uint4 v) { asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
+__device__ __forceinline__ uint4 lds(uint32_t a)
 {
-    if (row >= p.rows || col0 >= p.cols) return;
-    const long long at = k * p.plane + row * p.pitch + col0;
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+
+// The piece of `in` (A or X) at rows row0.., columns col0.., read along rows into registers; zero outside the matrix.
+struct Piece { uint4 hi[4], lo[4]; };
+__device__ __forceinline__ void fetch(const Product &p, Piece &x, int k, int row0, int col0, int lane)
+{
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int r = row0 + q * 8 + (lane >> 2), c = col0 + (lane & 3) * 8;
+        x.hi[q] = x.lo[q] = make_uint4(0, 0, 0, 0);
+        if (r < p.rows && c < p.cols) {
+            const long long at = k * p.plane + r * p.pitch + c;
+            x.hi[q] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.in_hi) + at));
+            if (p.in_lo) x.lo[q] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.in_lo) + at));
+        }
+    }
+}
+
+__device__ __forceinline__ void put(const Piece &in, const Stage &st)
+{
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const uint32_t a = st.half_at(q * 8 + (st.lane >> 2), st.lane & 3);
+        sts(a, in.hi[q]);
+        sts(a + 2048, in.lo[q]);
+    }
+}
+
+// v (32 columns of this lane's row of the accumulator) -> epilogue -> memory. The piece of `in` is in the stage.
+__device__ __forceinline__ void emit(const Product &p, float (&v)[32], const Stage &st, int k, int row0, int col0)
+{
+    const int lane = st.lane, row = row0 + lane;
 #pragma unroll
     for (int j = 0; j < 32; j++) v[j] *= p.alpha;
     if (p.mode != ORTH_GRAM) {
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-            if (col0 + j >= p.cols) break;
-            const uint4 h = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.in_hi) + at + j));
-            const __half2 *h2 = reinterpret_cast<const __half2 *>(&h);
-            float2 x[4];
+        for (int q = 0; q < 4; q++) {
+            const uint32_t a = st.half_at(lane, q);
+            const uint4 h = lds(a), l = lds(a + 2048);
+            const __half2 *h2 = reinterpret_cast<const __half2 *>(&h), *l2 = reinterpret_cast<const __half2 *>(&l);
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = __half22float2(h2[e]);
-            if (p.in_lo) {
-                const uint4 l = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.in_lo) + at + j));
-                const __half2 *l2 = reinterpret_cast<const __half2 *>(&l);
-#pragma unroll
-                for (int e = 0; e < 4; e++) { const float2 y = __half22float2(l2[e]); x[e].x += y.x; x[e].y += y.y; }
+            for (int e = 0; e < 4; e++) {
+                const float2 x = __half22float2(h2[e]), y = __half22float2(l2[e]);
+                v[8 * q + 2 * e] = fmaf(p.beta, x.x + y.x, v[8 * q + 2 * e]);
+                v[8 * q + 2 * e + 1] = fmaf(p.beta, x.y + y.y, v[8 * q + 2 * e + 1]);
             }
-#pragma unroll
-            for (int e = 0; e < 4; e++) { v[j + 2 * e] = fmaf(p.beta, x[e].x, v[j + 2 * e]); v[j + 2 * e + 1] = fmaf(p.beta, x[e].y, v[j + 2 * e + 1]); }
         }
+        __syncwarp();
     }
-    if (p.mode == ORTH_RESULT) {
-        if (p.tall) {
-            // neighbouring lanes hold neighbouring rows: one column is a contiguous run of the caller's row
+    if (p.mode != ORTH_RESULT) {
+        // planes: the pitch is a multiple of 64 columns, so a unit of eight that begins inside the matrix lies inside the plane
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-                if (col0 + j < p.cols) {
-                    const long long o = k * p.stride_w + (long long)(col0 + j) * p.ld_w + row;
-                    store1(p.w, p.type_w, o, p.keep != 0.f ? fmaf(p.keep, load1(p.w, p.type_w, o), v[j]) : v[j]);
-                }
-        } else {
-            const long long o = k * p.stride_w + row * p.ld_w + col0;
+        for (int q = 0; q < 4; q++) {
+            __half2 h[4], l[4];
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-                if (p.vec_w) {
-                    if (col0 + j >= p.cols) break;
-                    float4 x = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                    if (p.keep != 0.f) {
-                        const float4 w = load4(p.w, p.type_w, o + j);
-                        x = make_float4(fmaf(p.keep, w.x, x.x), fmaf(p.keep, w.y, x.y), fmaf(p.keep, w.z, x.z), fmaf(p.keep, w.w, x.w));
-                    }
-                    store4(p.w, p.type_w, o + j, x);
-                } else {
-#pragma unroll
-                    for (int e = j; e < j + 4; e++)
-                        if (col0 + e < p.cols) store1(p.w, p.type_w, o + e, p.keep != 0.f ? fmaf(p.keep, load1(p.w, p.type_w, o + e), v[e]) : v[e]);
-                }
+            for (int e = 0; e < 4; e++) {
+                h[e] = __floats2half2_rn(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
+                const float2 f = __half22float2(h[e]);
+                l[e] = __floats2half2_rn(v[8 * q + 2 * e] - f.x, v[8 * q + 2 * e + 1] - f.y);
             }
+            const uint32_t a = st.half_at(lane, q);
+            sts(a, *reinterpret_cast<const uint4 *>(h));
+            sts(a + 2048, *reinterpret_cast<const uint4 *>(l));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int r = q * 8 + (lane >> 2), u = lane & 3;
+            if (row0 + r < p.rows && col0 + u * 8 < p.cols) {
+                const long long at = k * p.plane + (row0 + r) * p.pitch + col0 + u * 8;
+                const uint32_t a = st.half_at(r, u);
+                *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out_hi) + at) = lds(a);
+                if (p.out_lo) *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out_lo) + at) = lds(a + 2048);
+            }
+        }
+        __syncwarp();
+        return;
+    }
+    if (p.tall) {
+        // neighbouring lanes hold neighbouring rows: a column is a contiguous run of the caller's row. Loads ahead of stores.
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 8) {
+            const long long o = k * p.stride_w + (long long)(col0 + j0) * p.ld_w + row;
+            if (p.keep != 0.f) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) w[j] = row < p.rows && col0 + j0 + j < p.cols ? load1(p.w, p.type_w, o + j * p.ld_w) : 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j0 + j] = fmaf(p.keep, w[j], v[j0 + j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (row < p.rows && col0 + j0 + j < p.cols) store1(p.w, p.type_w, o + j * p.ld_w, v[j0 + j]);
         }
         return;
     }
-    __half *const out_hi = static_cast<__half *>(p.out_hi), *const out_lo = static_cast<__half *>(p.out_lo);
-    // planes: the pitch is a multiple of 64 columns, so a group of eight that begins inside the matrix lies inside the plane
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-        if (col0 + j >= p.cols) break;
-        __half2 h[4], l[4];
+    for (int u = 0; u < 8; u++)
+        sts(st.f32_at(lane, u), make_uint4(__float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3])));
+    __syncwarp();
+    if (p.vec_w) {
+        const int u = lane & 7, r0 = lane >> 3, c = col0 + 4 * u;
+#pragma unroll 1
+        for (int q0 = 0; q0 < 8; q0 += 4) {
+            const long long o = k * p.stride_w + (row0 + r0 + 4 * q0) * p.ld_w + c;
+            float4 w[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            h[e] = __floats2half2_rn(v[j + 2 * e], v[j + 2 * e + 1]);
-            const float2 f = __half22float2(h[e]);
-            l[e] = __floats2half2_rn(v[j + 2 * e] - f.x, v[j + 2 * e + 1] - f.y);
+            for (int q = 0; q < 4; q++) {
+                w[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p.keep != 0.f && row0 + r0 + 4 * (q0 + q) < p.rows && c < p.cols) w[q] = load4(p.w, p.type_w, o + 4 * q * p.ld_w);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                if (row0 + r0 + 4 * (q0 + q) < p.rows && c < p.cols) {
+                    const uint4 x = lds(st.f32_at(r0 + 4 * (q0 + q), u));
+                    store4(p.w, p.type_w, o + 4 * q * p.ld_w, make_float4(fmaf(p.keep, w[q].x, __uint_as_float(x.x)), fmaf(p.keep, w[q].y, __uint_as_float(x.y)),
+                                                                         fmaf(p.keep, w[q].z, __uint_as_float(x.z)), fmaf(p.keep, w[q].w, __uint_as_float(x.w))));
+                }
         }
-        *reinterpret_cast<uint4 *>(out_hi + at + j) = *reinterpret_cast<const uint4 *>(h);
-        if (out_lo) *reinterpret_cast<uint4 *>(out_lo + at + j) = *reinterpret_cast<const uint4 *>(l);
-        if (mirror) {
+    } else {
+        // a column a lane, eight rows at a time
+        const int c = col0 + lane;
+#pragma unroll 1
+        for (int q0 = 0; q0 < 32; q0 += 8) {
+            const long long o = k * p.stride_w + (row0 + q0) * p.ld_w + c;
+            float w[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if (col0 + j + e >= p.cols) break;
-                const long long m = k * p.plane + (long long)(col0 + j + e) * p.pitch + row;
-                out_hi[m] = (e & 1) ? __high2half(h[e >> 1]) : __low2half(h[e >> 1]);
-                if (out_lo) out_lo[m] = (e & 1) ? __high2half(l[e >> 1]) : __low2half(l[e >> 1]);
+            for (int q = 0; q < 8; q++) w[q] = p.keep != 0.f && row0 + q0 + q < p.rows && c < p.cols ? load1(p.w, p.type_w, o + q * p.ld_w) : 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                float x;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(st.f32_at(q0 + q, lane >> 2) + (uint32_t)(lane & 3) * 4) : "memory");
+                if (row0 + q0 + q < p.rows && c < p.cols) store1(p.w, p.type_w, o + q * p.ld_w, fmaf(p.keep, w[q], x));
             }
         }
     }
+    __syncwarp();
 }
 
 // 384 threads; grid: any number of CTAs (pairs), each takes every grid-th tile.
@@ -380,7 +469,12 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     const Tiles tiles(p, SIDE);
     const int items = tiles.each * p.batch;
     const int nkb = (p.K + BK - 1) / BK;
-    const bool b_cols = p.mode >= ORTH_UPDATE;                           // P X: X has its columns contiguous
+    // Which operand blocks come transposed. X as the second operand of P X has its columns contiguous. Of a
+    // symmetric operand the block at K block kb is above the stored triangle when kb's tile lies beyond the tile
+    // of the rows. (A pair whose triangle was stored in 128-tiles takes the rule of its upper half: for the
+    // lower half that differs only inside its own diagonal tile, which is stored whole.)
+    const bool a_sym = p.mode != ORTH_GRAM, b_sym = p.mode == ORTH_POLY, b_cols = p.mode >= ORTH_UPDATE;
+    const int tri_shift = p.tri == 256 ? 8 : 7;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
@@ -415,6 +509,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                 int k, i, j;
                 tiles.at(item, k, i, j);
                 const int m0 = i * SIDE + (int)rank * 128, n0 = j * SIDE + (int)rank * 128;
+                const int ti = (i * SIDE) >> tri_shift, tj = (j * SIDE) >> tri_shift;
                 for (int kb = 0; kb < nkb; kb++, it++) {
                     const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
                     if (!mbar_wait(empty0 + 8 * s, ph ^ 1u, status, 1)) { ok = false; break; }
@@ -422,22 +517,25 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     uint32_t bar = full0 + 8 * s;
                     if (leader) mbar_expect_tx(bar, (PAIR ? 2 : 1) * STAGE);
                     if constexpr (PAIR) bar = map_to_cta(bar, 0);
+                    const int tk = (kb * BK) >> tri_shift;
+                    const bool a_t = a_sym && tk > ti, b_t = b_cols || (b_sym && tk > tj);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {                   // 64 rows (or columns) at a time
+                    for (int h = 0; h < 2; h++) {                   // 64 rows of an operand at a time
                         const uint32_t d = st + (uint32_t)h * (TILE / 2);
-                        const int ay = m0 + 64 * h, bx = b_cols ? n0 + 64 * h : kb * BK, by = b_cols ? kb * BK : n0 + 64 * h;
+                        const int ax = a_t ? m0 + 64 * h : kb * BK, ay = a_t ? kb * BK : m0 + 64 * h;
+                        const int bx = b_t ? n0 + 64 * h : kb * BK, by = b_t ? kb * BK : n0 + 64 * h;
                         if constexpr (PAIR) {
-                            tma_3d_pair(d, &a_hi, bar, kb * BK, ay, k);
+                            tma_3d_pair(d, &a_hi, bar, ax, ay, k);
                             tma_3d_pair(d + PLANES * TILE, &b_hi, bar, bx, by, k);
                             if constexpr (PLANES == 2) {
-                                tma_3d_pair(d + TILE, &a_lo, bar, kb * BK, ay, k);
+                                tma_3d_pair(d + TILE, &a_lo, bar, ax, ay, k);
                                 tma_3d_pair(d + 3 * TILE, &b_lo, bar, bx, by, k);
                             }
                         } else {
-                            tma_3d(d, &a_hi, bar, kb * BK, ay, k);
+                            tma_3d(d, &a_hi, bar, ax, ay, k);
                             tma_3d(d + PLANES * TILE, &b_hi, bar, bx, by, k);
                             if constexpr (PLANES == 2) {
-                                tma_3d(d + TILE, &a_lo, bar, kb * BK, ay, k);
+                                tma_3d(d + TILE, &a_lo, bar, ax, ay, k);
                                 tma_3d(d + 3 * TILE, &b_lo, bar, bx, by, k);
                             }
                         }
@@ -448,11 +546,12 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
         __syncwarp();
       } else if (warp == 1) {
         if (leader && lane == 0) {
-            const uint32_t idesc = instr_desc(SIDE, SIDE, b_cols ? 1 : 0);
-            const uint32_t b_adv = b_cols ? 2048u >> 4 : 32u >> 4;  // sixteen of K: two groups of eight rows, or 32 bytes along a row
             uint32_t it = 0, g = 0;
             bool ok = true;
             for (int item = cl; ok && item < items; item += C) {
+                int k, i, j;
+                tiles.at(item, k, i, j);
+                const int ti = (i * SIDE) >> tri_shift, tj = (j * SIDE) >> tri_shift;
                 for (int kb = 0; kb < nkb && ok; g++) {
                     const uint32_t buf = g & 1u;
                     ok = mbar_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1u) ^ 1u, status, 4);
@@ -467,24 +566,23 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t st = smem0 + s * STAGE;
-                        const uint64_t ah = smem_desc(st), al = smem_desc(st + TILE);
-                        const uint32_t bt = st + PLANES * TILE;
-                        const uint64_t bh = b_cols ? smem_desc_cols(bt) : smem_desc(bt);
-                        const uint64_t bl = b_cols ? smem_desc_cols(bt + TILE) : smem_desc(bt + TILE);
+                        const int tk = (kb * BK) >> tri_shift;
+                        const bool a_t = a_sym && tk > ti, b_t = b_cols || (b_sym && tk > tj);
+                        const uint32_t idesc = instr_desc(SIDE, SIDE, a_t, b_t), bt = st + PLANES * TILE;
+                        const uint64_t ah = tile_desc(st, a_t), al = tile_desc(st + TILE, a_t), bh = tile_desc(bt, b_t), bl = tile_desc(bt + TILE, b_t);
                         // two planes: the small products first. The tensor core truncates what it adds to a sum
                         // to the sum's last bit, so adds to a sum that is still small cost less.
                         if constexpr (PLANES == 2) {
 #pragma unroll
                             for (int kk = 0; kk < BK / 16; kk++) {
-                                const uint64_t ad = (uint64_t)(kk * (32 >> 4)), bd = (uint64_t)(kk * b_adv);
-                                umma<PAIR>(tacc, al + ad, bh + bd, idesc, acc);
-                                umma<PAIR>(tacc, ah + ad, bl + bd, idesc, 1u);
+                                umma<PAIR>(tacc, al + k_advance(kk, a_t), bh + k_advance(kk, b_t), idesc, acc);
+                                umma<PAIR>(tacc, ah + k_advance(kk, a_t), bl + k_advance(kk, b_t), idesc, 1u);
                                 acc = 1;
                             }
                         }
 #pragma unroll
                         for (int kk = 0; kk < BK / 16; kk++) {
-                            umma<PAIR>(tacc, ah + (uint64_t)(kk * (32 >> 4)), bh + (uint64_t)(kk * b_adv), idesc, acc);
+                            umma<PAIR>(tacc, ah + k_advance(kk, a_t), bh + k_advance(kk, b_t), idesc, acc);
                             acc = 1;
                         }
                         commit<PAIR>(empty0 + 8 * s);
@@ -499,64 +597,49 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int q = warp & 3, h = (warp - 4) >> 2;
         const uint32_t acc_empty = PAIR ? map_to_cta(acc_empty0, 0) : acc_empty0;
+        const Stage stage = { smem0 + STAGES * STAGE + (uint32_t)(warp - 4) * 4096u, lane };
         uint32_t g = 0;
         bool ok = true;
         for (int item = cl; ok && item < items; item += C) {
             int k, i, j;
             tiles.at(item, k, i, j);
-            const int row = i * SIDE + (int)rank * 128 + q * 32 + lane, col0 = j * SIDE + h * HALF;
-            const bool mirror = tiles.sym && i != j;
-            if constexpr (PLANES == 1) {
+            const int row0 = i * SIDE + (int)rank * 128 + q * 32, col0 = j * SIDE + h * HALF;
+            Piece in;
+            if (p.mode != ORTH_GRAM) fetch(p, in, k, row0, col0, lane);       // lands while the products run
+            float acc[HALF];
+#pragma unroll
+            for (int e = 0; e < HALF; e++) acc[e] = 0.f;
+            for (int kb = 0; kb < nkb; kb += PLANES == 2 ? CHUNK_KB : nkb, g++) {
                 const uint32_t buf = g & 1u;
-                ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
                 if (!ok) break;
-                g++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + buf * (uint32_t)SIDE + (uint32_t)(h * HALF);
-#pragma unroll 1
-                for (int cc = 0; cc < HALF / 32; cc++) {
-                    uint32_t r[32];
-                    tmem_ld32(src + (uint32_t)(cc * 32), r);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    float v[32];
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = __uint_as_float(r[e]);
-                    emit<PLANES>(p, v, k, row, col0 + cc * 32, mirror);
-                    __syncwarp();
+                for (int cc = 0; cc < HALF / 16; cc++) {
+                    uint32_t r[16];
+                    tmem_ld16(src + (uint32_t)(cc * 16), r);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int e = 0; e < 16; e++) acc[cc * 16 + e] = __fadd_rn(acc[cc * 16 + e], __uint_as_float(r[e]));
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
-            } else {
-                float acc[HALF];
-#pragma unroll
-                for (int e = 0; e < HALF; e++) acc[e] = 0.f;
-                for (int kb = 0; kb < nkb; kb += CHUNK_KB, g++) {
-                    const uint32_t buf = g & 1u;
-                    ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + buf * (uint32_t)SIDE + (uint32_t)(h * HALF);
-#pragma unroll
-                    for (int cc = 0; cc < HALF / 16; cc++) {
-                        uint32_t r[16];
-                        tmem_ld16(src + (uint32_t)(cc * 16), r);
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                        for (int e = 0; e < 16; e++) acc[cc * 16 + e] = __fadd_rn(acc[cc * 16 + e], __uint_as_float(r[e]));
-                    }
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
+            }
+            if (!ok) break;
+#pragma unroll 1
+            for (int cc = 0; cc < HALF / 32; cc++) {
+                if (row0 >= p.rows || col0 + cc * 32 >= p.cols) break;
+                if (p.mode != ORTH_GRAM) {
+                    put(in, stage);
+                    if (cc + 1 < HALF / 32) fetch(p, in, k, row0, col0 + (cc + 1) * 32, lane);
                 }
-                if (!ok) break;
+                float v[32];
 #pragma unroll
-                for (int cc = 0; cc < HALF / 32; cc++) {
-                    float v[32];
-#pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = acc[cc * 32 + e];
-                    emit<PLANES>(p, v, k, row, col0 + cc * 32, mirror);
-                }
+                for (int e = 0; e < 32; e++)
+                    v[e] = HALF == 64 ? (cc ? acc[32 + e] : acc[e]) : cc < 2 ? (cc ? acc[32 + e] : acc[e]) : cc == 2 ? acc[HALF / 2 + e] : acc[HALF - 32 + e];
+                emit(p, v, stage, k, row0, col0 + cc * 32);
             }
             __syncwarp();
         }

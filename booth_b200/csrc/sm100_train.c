@@ -165,7 +165,7 @@ int booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t
 /* ---- orthogonalisation and Muon ---- */
 
 #define ORTH_MAX_SIDE (1 << 20)
-#define ORTH_SMEM 197632u               /* 6 x 32 KB or 3 x 64 KB of operand stages, and 1 KB to align them */
+#define ORTH_SMEM (1024u + 6u * 32768u + 8u * 4096u)    /* 6 x 32 KB or 3 x 64 KB of operand stages, 4 KB for each epilogue warp, and 1 KB to align them */
 
 static size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
@@ -245,6 +245,7 @@ static int orth_launch(sm100_dev_t *dev, const plane_maps_t *a, const plane_maps
     const int sym = p->mode <= ORTH_POLY, pairs = orth_pairs(dev, p->rows, p->cols, p->batch, sym);
     const long long side = pairs ? 256 : 128, tm = (p->rows + side - 1) / side, tn = (p->cols + side - 1) / side;
     const long long tiles = p->batch * (sym ? tm * (tm + 1) / 2 : tm * tn), slots = pairs ? dev->sm_count / 2 : dev->sm_count;
+    if (sym) p->tri = (int)side;        /* A, then P: both are s x s, so both get the same tiles; the update reads P's */
     const unsigned grid = (unsigned)((tiles < slots ? tiles : slots) * (pairs ? 2 : 1));
     void *args[] = { (void *)&a->hi, (void *)&a->lo, (void *)&b->hi, (void *)&b->lo, p };
     return sm100_launch_k3_overlapped(dev, SM100_K_ORTH_PRODUCT + (pairs ? 2 : 0) + (two_planes ? 1 : 0), grid, 1, 1, 384, 1, 1, ORTH_SMEM, args);

@@ -106,7 +106,7 @@ d.sync(); d.close()
     assert res.returncode == 0, res.stderr
     assert [l["kernel"] for l in L] == ["orth_norm", "orth_split"] + ["orth_product_1_pair"] * 6 + ["orth_norm", "orth_split"] + ["orth_product_2_single"] * 3
     assert all(l["overlap"] == 1 for l in L)
-    assert all(l["shmem"] == 197632 and l["block"] == (384, 1, 1) for l in L if l["kernel"].startswith("orth_product"))
+    assert all(l["shmem"] == 230400 and l["block"] == (384, 1, 1) for l in L if l["kernel"].startswith("orth_product"))
     P = products(lines)
     assert [(p["mode"], p["rows"], p["cols"], p["K"], p["batch"], p["tall"]) for p in P] == [
         (0, 4096, 4096, 4096, 1, 0), (1, 4096, 4096, 4096, 1, 0), (2, 4096, 4096, 4096, 1, 0),
