@@ -248,6 +248,17 @@ __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a, uint64_t b, ui
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                      ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+                 ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
+                   "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]),
+                   "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]),
+                   "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]),
+                   "r"(taddr) : "memory");
+}
 template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar)
 {
     if constexpr (PAIR) gemm::umma_commit_pair(bar); else gemm::umma_commit(bar);
@@ -481,6 +492,14 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
         for (int b = 0; b < 2; b++) { mbar_init(acc_full0 + 8 * b, 1); mbar_init(acc_empty0 + 8 * b, PAIR ? 16 : 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (threadIdx.x == 32) {        // the descriptors, while the kernel before still runs
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a_hi) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&b_hi) : "memory");
+        if constexpr (PLANES == 2) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&a_lo) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&b_lo) : "memory");
+        }
+    }
     __syncwarp();
     if (warp == 1) {
         if constexpr (PAIR) {
@@ -606,28 +625,45 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
             const int row0 = i * SIDE + (int)rank * 128 + q * 32, col0 = j * SIDE + h * HALF;
             Piece in;
             if (p.mode != ORTH_GRAM) fetch(p, in, k, row0, col0, lane);       // lands while the products run
-            float acc[HALF];
-#pragma unroll
-            for (int e = 0; e < HALF; e++) acc[e] = 0.f;
-            for (int kb = 0; kb < nkb; kb += PLANES == 2 ? CHUNK_KB : nkb, g++) {
-                const uint32_t buf = g & 1u;
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
+            const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * HALF);
+            uint32_t buf = g & 1u;
+            if constexpr (PLANES == 1) {
+                ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
                 if (!ok) break;
+                g++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + buf * (uint32_t)SIDE + (uint32_t)(h * HALF);
+            } else {
+                // the chunks' sums in registers; the total goes back to tensor memory in place of the last chunk, so
+                // that the epilogue below holds 32 columns at a time (with all of them in registers it
+                // spilled, and beside 225 KB of shared memory there is no first-level cache to spill to)
+                float acc[HALF];
 #pragma unroll
-                for (int cc = 0; cc < HALF / 16; cc++) {
-                    uint32_t r[16];
-                    tmem_ld16(src + (uint32_t)(cc * 16), r);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                for (int e = 0; e < HALF; e++) acc[e] = 0.f;
+                for (int kb = 0; kb < nkb; kb += CHUNK_KB, g++) {
+                    buf = g & 1u;
+                    ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                    for (int e = 0; e < 16; e++) acc[cc * 16 + e] = __fadd_rn(acc[cc * 16 + e], __uint_as_float(r[e]));
+                    for (int cc = 0; cc < HALF / 16; cc++) {
+                        uint32_t r[16];
+                        tmem_ld16(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 16), r);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int e = 0; e < 16; e++) acc[cc * 16 + e] = __fadd_rn(acc[cc * 16 + e], __uint_as_float(r[e]));
+                    }
+                    if (kb + CHUNK_KB >= nkb) {
+#pragma unroll
+                        for (int cc = 0; cc < HALF / 32; cc++) tmem_st32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 32), acc + cc * 32);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    } else {
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
+                    }
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
+                if (!ok) break;
             }
-            if (!ok) break;
 #pragma unroll 1
             for (int cc = 0; cc < HALF / 32; cc++) {
                 if (row0 >= p.rows || col0 + cc * 32 >= p.cols) break;
@@ -636,12 +672,18 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     if (cc + 1 < HALF / 32) fetch(p, in, k, row0, col0 + (cc + 1) * 32, lane);
                 }
                 float v[32];
+                {
+                    uint32_t r[32];
+                    tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 32), r);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                for (int e = 0; e < 32; e++)
-                    v[e] = HALF == 64 ? (cc ? acc[32 + e] : acc[e]) : cc < 2 ? (cc ? acc[32 + e] : acc[e]) : cc == 2 ? acc[HALF / 2 + e] : acc[HALF - 32 + e];
+                    for (int e = 0; e < 32; e++) v[e] = __uint_as_float(r[e]);
+                }
                 emit(p, v, stage, k, row0, col0 + cc * 32);
             }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
         }
         if (!ok) {      // a wait ran out: copies that may still be in flight land before the shared memory is released
             for (int i = 0; i < 64; i++) __nanosleep(4000);
