@@ -20,32 +20,30 @@ typedef struct orth_source {
     ORTH_PTR(const void) g;
     ORTH_PTR(void) m;
     long long ld_g, stride_g, ld_m, stride_m;
-    int type_g, type_m, rows, cols, nesterov, vec;      /* vec: groups of four elements are aligned in g and m */
+    int type_g, type_m, rows, cols, nesterov;
+    int vec;                                            /* groups of four elements are aligned in g and m */
+    int flat;                                           /* no gaps between rows in g and m */
     float mu;
-    int pad_;
 } orth_source_t;
 
 /* What a product kernel computes. */
-#define ORTH_GRAM   0       /* A = X X^t */
-#define ORTH_POLY   1       /* P = b A + c A A */
-#define ORTH_UPDATE 2       /* X = a X + P X */
+#define ORTH_GRAM   0       /* S = X X^t + diag I */
+#define ORTH_POLY   1       /* Q = alpha S S + diag I */
+#define ORTH_UPDATE 2       /* X = Q X */
 #define ORTH_RESULT 3       /* the same into the caller's matrix: w = keep w + value */
 
 typedef struct orth_product {
     int mode, rows, cols, K, batch;                     /* of the product: rows x cols, square for GRAM and POLY */
-    float alpha, beta;                                  /* out = alpha * accumulator + beta * in */
+    float alpha, diag;                                  /* out = alpha * accumulator, + diag where row = column */
+    int tri;                                            /* tile side of the stored triangle of the symmetric operand */
+    int split;                                          /* parts of K, one CTA pair of a cluster each */
+    int lo;                                             /* whether out has a lo plane */
+    /* RESULT: element (r, c) of matrix k at k * stride_w + r * ld_w + c; transposed when tall */
     int type_w, tall, vec_w;
-    int tri;                                            /* tile side of the stored triangle of the symmetric operand (GRAM: of the output) */
-    int pad0_;
-    ORTH_PTR(const void) in_hi;
-    ORTH_PTR(const void) in_lo;                         /* 0: hi alone */
-    ORTH_PTR(void) out_hi;
-    ORTH_PTR(void) out_lo;                              /* 0: hi alone */
-    long long pitch, plane;                             /* of in and out: equal shapes */
-    ORTH_PTR(void) w;                                   /* RESULT; transposed when tall */
-    long long ld_w, stride_w;
     float keep;                                         /* 0: w is not read */
-    int pad_;
+    ORTH_PTR(void) w;
+    long long ld_w, stride_w;
+    ORTH_PTR(float) sums;                               /* where the parts of a tile meet: 32,768 floats a CTA */
     ORTH_PTR(int) status;
     unsigned long long wait_ns;
 } orth_product_t;

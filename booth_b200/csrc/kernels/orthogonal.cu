@@ -1,38 +1,44 @@
 // orthogonal.cu -- Newton-Schulz orthogonalisation of a matrix on the tensor cores.
 //
-//     X = G / (|G|_F + eps);   steps times:  A = X X^t,  P = b A + c A A,  X = a X + P X
+//     X = G / (|G|_F + eps);   steps times:  A = X X^t,  X = (a I + b A + c A A) X
 //
 // drives the singular values of X towards one (the Muon optimiser's update). X is
-// s x l with s <= l: a tall G is transposed on the way in and on the way out. All
-// three products run on fp16 operands with fp32 accumulation (tcgen05 kind::f16),
-// which hold 11 bits where bf16 holds 8 at the same rate. X and A are kept times 2^14
-// and P times a power of two that its coefficients allow: singular values stay
-// below 2, so the scaled entries fit fp16, and small entries stay above its
-// subnormal range.
+// s x l with s <= l: a tall G is transposed on the way in and on the way out. With the
+// square completed, beta = b / 2c and gamma = a - b^2 / 4c, a step is three plain products,
+//     S = X X^t + beta I,   Q = c S S + gamma I,   X = Q X
+// whose epilogues add at most a constant to the diagonal and read nothing. (The form P = b A + c A A,
+// X = a X + P X reads A and X again, tile by tile, in the epilogue; that took 1.5 to 2 us
+// per 32 columns of a tile and bound every product with K below 2000.) With c = 0: Q = b A + a I at once.
+//
+// All three run on fp16 operands with fp32 accumulation (tcgen05 kind::f16), which hold 11
+// bits where bf16 holds 8 at the same rate. X is kept times 2^14, S times 2^12 and Q times a
+// power of two that its coefficients allow: singular values stay below 2, so the scaled entries
+// fit fp16, and small entries stay above its subnormal range.
 //
 // Precision, by the type of the result:
 //   two planes (f32, f16 results): every operand is hi + lo = fp16(x) + fp16(x - hi), 22
-//     bits, and a product is lo.hi + hi.lo + hi.hi; K is cut into chunks of 128 whose sums
-//     leave the tensor core (it adds with truncation, so a long sum drifts) and are
-//     added round-to-nearest in registers. As exact as an fp32 iteration or better.
+//     bits, and a product is lo.hi + hi.lo + hi.hi. The tensor core adds with truncation, so a
+//     long sum drifts: K is cut into chunks of 128, of 64 where the large diagonal of S or Q comes
+//     in, whose sums are added round-to-nearest in registers. As exact as fp32 products.
 //   one plane (bf16 results): products use the hi parts only, a third of the work. X
-//     still keeps hi + lo for the term a X: the iteration multiplies what small singular
-//     values lose by up to a^steps = 485, so rounding X to 11 bits each step showed as 2 to
-//     4 % on matrices of low rank, while rounding only the products' operands leaves 1e-3.
+//     still has a lo plane, and Q X adds Q_hi X_lo for the K blocks around the diagonal, where a X
+//     comes from: the iteration multiplies what small singular values lose by up to
+//     a^steps = 485, so with X rounded to 11 bits each step matrices of low rank came out 2 to 4 %
+//     off, with the lo blocks 1e-3 to 3e-3.
 //
-// A and P are symmetric: only tiles on and below the diagonal are computed and stored.
+// S and Q are symmetric: only tiles on and below the diagonal are computed and stored.
 // Where a product needs a block above the diagonal it loads the mirrored block and has the
 // tensor core take it transposed (an operand may have either index contiguous), so nothing
-// is stored twice: with 2-byte transposed stores the epilogue of a 1024 x 1024
-// product took 12 of its 27 us.
+// is stored twice.
 //
 // Launches per call: orth_norm (sums of squares; Muon: also the momentum), orth_split (planes of
 // the normalised, possibly transposed matrix), then steps x 3 products. A product kernel
 // keeps one CTA or CTA pair per SM (pair) and walks over the tiles of all matrices of
 // the batch; the roles inside are those of the fp32 GEMM: warp 0 TMA, warp 1 MMA, warps 4-11
-// drain tensor memory and apply the epilogue.
-//   pair:   256 x 256 tile per two CTAs, tcgen05.mma.cta_group::2
-//   single: 128 x 128 tile per CTA, for matrices with too few tiles of the other size
+// drain tensor memory, apply the epilogue and store, planes by TMA from shared memory.
+//   pair:   256 x 256 tile per two CTAs, tcgen05.mma.cta_group::2; few tiles: the K of
+//           a tile shared by up to four pairs of a cluster
+//   single: 128 x 128 tile per CTA
 #include "common.cuh"
 #include "orth_params.cuh"
 #include <cuda.h>
@@ -59,6 +65,12 @@ __device__ __forceinline__ void store1(void *p, int type, long long i, float v)
     else if (type == ORTH_BF16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
     else static_cast<__half *>(p)[i] = __float2half_rn(v);
 }
+// The value that a store to this type and a load back would give.
+__device__ __forceinline__ float rounded(float v, int type)
+{
+    return type == ORTH_F32 ? v : type == ORTH_BF16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
+}
+__device__ __forceinline__ float4 rounded4(float4 v, int type) { return make_float4(rounded(v.x, type), rounded(v.y, type), rounded(v.z, type), rounded(v.w, type)); }
 // Four neighbouring elements; p + i is aligned to four elements.
 __device__ __forceinline__ float4 load4(const void *p, int type, long long i)
 {
@@ -115,30 +127,38 @@ orth_norm(const __grid_constant__ orth::Source s, double *__restrict__ partial)
     __shared__ double sh[8];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const int k = (int)blockIdx.y;
-    const int w = s.vec ? 4 : 1, per_row = s.cols / w;
-    const long long total = (long long)s.rows * per_row;
+    const int k = (int)blockIdx.y, W = s.vec ? 4 : 1;
+    // matrices without gaps are walked as one row, the others a row a block at a time
+    const long long rows = s.flat ? 1 : s.rows, cols = s.flat ? (long long)s.rows * s.cols : s.cols;
+    const long long r0 = s.flat ? 0 : blockIdx.x, r_step = s.flat ? 1 : gridDim.x;
+    const long long c0 = (long long)((s.flat ? blockIdx.x * 256u : 0u) + threadIdx.x) * W, c_step = (s.flat ? gridDim.x : 1u) * 256ll * W;
     double sum = 0.0;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * w;
+    for (long long r = r0; r < rows; r += r_step) {
+        const long long at_g = k * s.stride_g + r * s.ld_g, at_m = k * s.stride_m + r * s.ld_m;
         if (s.vec) {
-            float4 u = load4(s.g, s.type_g, k * s.stride_g + r * s.ld_g + c);
-            if (s.m) {
-                const long long at = k * s.stride_m + r * s.ld_m + c;
-                float4 m = load4(s.m, s.type_m, at);
-                m = make_float4(lerp(m.x, u.x, s.mu), lerp(m.y, u.y, s.mu), lerp(m.z, u.z, s.mu), lerp(m.w, u.w, s.mu));
-                store4(s.m, s.type_m, at, m);
-                u = source4(s, k, r, c);
+#pragma unroll 4
+            for (long long c = c0; c < cols; c += c_step) {
+                float4 u = load4(s.g, s.type_g, at_g + c);
+                if (s.m) {
+                    float4 m = load4(s.m, s.type_m, at_m + c);
+                    m = make_float4(lerp(m.x, u.x, s.mu), lerp(m.y, u.y, s.mu), lerp(m.z, u.z, s.mu), lerp(m.w, u.w, s.mu));
+                    m = rounded4(m, s.type_m);
+                    store4(s.m, s.type_m, at_m + c, m);
+                    u = make_float4(update_of(m.x, u.x, s), update_of(m.y, u.y, s), update_of(m.z, u.z, s), update_of(m.w, u.w, s));
+                }
+                sum += ((double)u.x * u.x + (double)u.y * u.y) + ((double)u.z * u.z + (double)u.w * u.w);
             }
-            sum += ((double)u.x * u.x + (double)u.y * u.y) + ((double)u.z * u.z + (double)u.w * u.w);
         } else {
-            float u = load1(s.g, s.type_g, k * s.stride_g + r * s.ld_g + c);
-            if (s.m) {
-                const long long at = k * s.stride_m + r * s.ld_m + c;
-                store1(s.m, s.type_m, at, lerp(load1(s.m, s.type_m, at), u, s.mu));
-                u = source1(s, k, r, c);
+#pragma unroll 4
+            for (long long c = c0; c < cols; c += c_step) {
+                float u = load1(s.g, s.type_g, at_g + c);
+                if (s.m) {
+                    const float m = rounded(lerp(load1(s.m, s.type_m, at_m + c), u, s.mu), s.type_m);
+                    store1(s.m, s.type_m, at_m + c, m);
+                    u = update_of(m, u, s);
+                }
+                sum += (double)u * u;
             }
-            sum += (double)u * u;
         }
     }
 #pragma unroll
@@ -259,9 +279,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *v)
                    "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]),
                    "r"(taddr) : "memory");
 }
-template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar)
+// Arrives on the barrier at this offset, for a pair in both of its CTAs (cluster ranks first, first + 1).
+template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar, uint32_t first)
 {
-    if constexpr (PAIR) gemm::umma_commit_pair(bar); else gemm::umma_commit(bar);
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"((uint16_t)(3u << first)) : "memory");
+    else gemm::umma_commit(bar);
 }
 
 // Tile number -> matrix, tile row and tile column. Tiles that run at the same time should share
@@ -295,17 +319,6 @@ struct Tiles {
     }
 };
 
-// One warp's 32 x 32 piece of the product, a row a lane in v, goes out through 4 KB of shared
-// memory of the warp's own, so that global accesses run along rows: a piece's row is 64 bytes of a plane
-// (two sectors), where a store straight from the registers touched 32 lines at once.
-// Shared layout: 16-byte units, swizzled so that neither the lane-a-row nor the along-the-row access conflicts.
-struct Stage {
-    uint32_t base;
-    int lane;
-    // 16-byte unit u of row r: planes (hi, then lo 2048 bytes on) have 4 units a row, fp32 pieces 8
-    __device__ __forceinline__ uint32_t half_at(int r, int u) const { return base + (uint32_t)(r * 64 + ((u ^ (r >> 1)) & 3) * 16); }
-    __device__ __forceinline__ uint32_t f32_at(int r, int u) const { return base + (uint32_t)(r * 128 + ((u ^ r) & 7) * 16); }
-};
 __device__ __forceinline__ void sts(uint32_t a, uint4 v) { asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
 __device__ __forceinline__ uint4 lds(uint32_t a)
 {
@@ -313,155 +326,131 @@ __device__ __forceinline__ uint4 lds(uint32_t a)
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
     return v;
 }
-
-// The piece of `in` (A or X) at rows row0.., columns col0.., read along rows into registers; zero outside the matrix.
-struct Piece { uint4 hi[4], lo[4]; };
-__device__ __forceinline__ void fetch(const Product &p, Piece &x, int k, int row0, int col0, int lane)
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, uint32_t src, int x, int y, int z)
 {
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-        const int r = row0 + q * 8 + (lane >> 2), c = col0 + (lane & 3) * 8;
-        x.hi[q] = x.lo[q] = make_uint4(0, 0, 0, 0);
-        if (r < p.rows && c < p.cols) {
-            const long long at = k * p.plane + r * p.pitch + c;
-            x.hi[q] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.in_hi) + at));
-            if (p.in_lo) x.lo[q] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.in_lo) + at));
-        }
-    }
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-__device__ __forceinline__ void put(const Piece &in, const Stage &st)
+// Two warps hold 64 rows x 64 columns, a row a lane: one plane of them goes through 8 KB of
+// shared memory, in the 128-byte-swizzled form of the tensor map's box, and out by TMA, which clips at
+// the matrix's edges. `packed`: this lane's 64 halves. Barrier `bar` joins the two warps; thread `issuer` of them issues.
+__device__ __forceinline__ void store_plane(const CUtensorMap *map, uint32_t buf, const uint32_t (&packed)[32], int r, int bar, bool issuer, int x, int y, int z)
 {
+    if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the buffer's last content has left
+    asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-        const uint32_t a = st.half_at(q * 8 + (st.lane >> 2), st.lane & 3);
-        sts(a, in.hi[q]);
-        sts(a + 2048, in.lo[q]);
-    }
+    for (int u = 0; u < 8; u++)
+        sts(buf + (uint32_t)(r * 128 + ((u ^ r) & 7) * 16), make_uint4(packed[4 * u], packed[4 * u + 1], packed[4 * u + 2], packed[4 * u + 3]));
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+    if (issuer) tma_store(map, buf, x, y, z);
 }
 
-// v (32 columns of this lane's row of the accumulator) -> epilogue -> memory. The piece of `in` is in the stage.
-__device__ __forceinline__ void emit(const Product &p, float (&v)[32], const Stage &st, int k, int row0, int col0)
+// Whether both warps of barrier `bar` say so.
+__device__ __forceinline__ bool both_ok(int bar, bool ok)
 {
-    const int lane = st.lane, row = row0 + lane;
-#pragma unroll
-    for (int j = 0; j < 32; j++) v[j] *= p.alpha;
-    if (p.mode != ORTH_GRAM) {
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint32_t a = st.half_at(lane, q);
-            const uint4 h = lds(a), l = lds(a + 2048);
-            const __half2 *h2 = reinterpret_cast<const __half2 *>(&h), *l2 = reinterpret_cast<const __half2 *>(&l);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float2 x = __half22float2(h2[e]), y = __half22float2(l2[e]);
-                v[8 * q + 2 * e] = fmaf(p.beta, x.x + y.x, v[8 * q + 2 * e]);
-                v[8 * q + 2 * e + 1] = fmaf(p.beta, x.y + y.y, v[8 * q + 2 * e + 1]);
-            }
-        }
-        __syncwarp();
-    }
-    if (p.mode != ORTH_RESULT) {
-        // planes: the pitch is a multiple of 64 columns, so a unit of eight that begins inside the matrix lies inside the plane
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            __half2 h[4], l[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                h[e] = __floats2half2_rn(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
-                const float2 f = __half22float2(h[e]);
-                l[e] = __floats2half2_rn(v[8 * q + 2 * e] - f.x, v[8 * q + 2 * e + 1] - f.y);
-            }
-            const uint32_t a = st.half_at(lane, q);
-            sts(a, *reinterpret_cast<const uint4 *>(h));
-            sts(a + 2048, *reinterpret_cast<const uint4 *>(l));
-        }
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const int r = q * 8 + (lane >> 2), u = lane & 3;
-            if (row0 + r < p.rows && col0 + u * 8 < p.cols) {
-                const long long at = k * p.plane + (row0 + r) * p.pitch + col0 + u * 8;
-                const uint32_t a = st.half_at(r, u);
-                *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out_hi) + at) = lds(a);
-                if (p.out_lo) *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out_lo) + at) = lds(a + 2048);
-            }
-        }
-        __syncwarp();
-        return;
-    }
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((uint32_t)ok), "r"(bar) : "memory");
+    return all != 0;
+}
+
+// One warp's 32 rows x 32 columns of the result, a row a lane, into the caller's matrix. Through 4 KB of the
+// warp's own shared memory, so that accesses run along the rows; loads ahead of stores.
+__device__ __forceinline__ void store_result(const Product &p, const float (&v)[32], uint32_t buf, int lane, int k, int row0, int col0)
+{
+    const int row = row0 + lane;
     if (p.tall) {
-        // neighbouring lanes hold neighbouring rows: a column is a contiguous run of the caller's row. Loads ahead of stores.
+        // neighbouring lanes hold neighbouring rows: a column is a contiguous run of the caller's row
 #pragma unroll
-        for (int j0 = 0; j0 < 32; j0 += 8) {
+        for (int j0 = 0; j0 < 32; j0 += 16) {
             const long long o = k * p.stride_w + (long long)(col0 + j0) * p.ld_w + row;
-            if (p.keep != 0.f) {
-                float w[8];
+            float w[16];
 #pragma unroll
-                for (int j = 0; j < 8; j++) w[j] = row < p.rows && col0 + j0 + j < p.cols ? load1(p.w, p.type_w, o + j * p.ld_w) : 0.f;
+            for (int j = 0; j < 16; j++) w[j] = p.keep != 0.f && row < p.rows && col0 + j0 + j < p.cols ? load1(p.w, p.type_w, o + j * p.ld_w) : 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j0 + j] = fmaf(p.keep, w[j], v[j0 + j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (row < p.rows && col0 + j0 + j < p.cols) store1(p.w, p.type_w, o + j * p.ld_w, v[j0 + j]);
+            for (int j = 0; j < 16; j++)
+                if (row < p.rows && col0 + j0 + j < p.cols) store1(p.w, p.type_w, o + j * p.ld_w, fmaf(p.keep, w[j], v[j0 + j]));
         }
         return;
     }
 #pragma unroll
     for (int u = 0; u < 8; u++)
-        sts(st.f32_at(lane, u), make_uint4(__float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3])));
+        sts(buf + (uint32_t)(lane * 128 + ((u ^ lane) & 7) * 16),
+            make_uint4(__float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3])));
     __syncwarp();
     if (p.vec_w) {
         const int u = lane & 7, r0 = lane >> 3, c = col0 + 4 * u;
-#pragma unroll 1
-        for (int q0 = 0; q0 < 8; q0 += 4) {
-            const long long o = k * p.stride_w + (row0 + r0 + 4 * q0) * p.ld_w + c;
-            float4 w[4];
+        const long long o = k * p.stride_w + (row0 + r0) * p.ld_w + c;
+        float4 w[8];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                w[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (p.keep != 0.f && row0 + r0 + 4 * (q0 + q) < p.rows && c < p.cols) w[q] = load4(p.w, p.type_w, o + 4 * q * p.ld_w);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                if (row0 + r0 + 4 * (q0 + q) < p.rows && c < p.cols) {
-                    const uint4 x = lds(st.f32_at(r0 + 4 * (q0 + q), u));
-                    store4(p.w, p.type_w, o + 4 * q * p.ld_w, make_float4(fmaf(p.keep, w[q].x, __uint_as_float(x.x)), fmaf(p.keep, w[q].y, __uint_as_float(x.y)),
-                                                                         fmaf(p.keep, w[q].z, __uint_as_float(x.z)), fmaf(p.keep, w[q].w, __uint_as_float(x.w))));
-                }
+        for (int q = 0; q < 8; q++) {
+            w[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p.keep != 0.f && row0 + r0 + 4 * q < p.rows && c < p.cols) w[q] = load4(p.w, p.type_w, o + 4 * q * p.ld_w);
         }
+#pragma unroll
+        for (int q = 0; q < 8; q++)
+            if (row0 + r0 + 4 * q < p.rows && c < p.cols) {
+                const int r = r0 + 4 * q;
+                const uint4 x = lds(buf + (uint32_t)(r * 128 + ((u ^ r) & 7) * 16));
+                store4(p.w, p.type_w, o + 4 * q * p.ld_w, make_float4(fmaf(p.keep, w[q].x, __uint_as_float(x.x)), fmaf(p.keep, w[q].y, __uint_as_float(x.y)),
+                                                                     fmaf(p.keep, w[q].z, __uint_as_float(x.z)), fmaf(p.keep, w[q].w, __uint_as_float(x.w))));
+            }
     } else {
-        // a column a lane, eight rows at a time
+        // a column a lane, sixteen rows at a time
         const int c = col0 + lane;
 #pragma unroll 1
-        for (int q0 = 0; q0 < 32; q0 += 8) {
+        for (int q0 = 0; q0 < 32; q0 += 16) {
             const long long o = k * p.stride_w + (row0 + q0) * p.ld_w + c;
-            float w[8];
+            float w[16];
 #pragma unroll
-            for (int q = 0; q < 8; q++) w[q] = p.keep != 0.f && row0 + q0 + q < p.rows && c < p.cols ? load1(p.w, p.type_w, o + q * p.ld_w) : 0.f;
+            for (int q = 0; q < 16; q++) w[q] = p.keep != 0.f && row0 + q0 + q < p.rows && c < p.cols ? load1(p.w, p.type_w, o + q * p.ld_w) : 0.f;
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
+            for (int q = 0; q < 16; q++) {
+                const int r = q0 + q;
                 float x;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(st.f32_at(q0 + q, lane >> 2) + (uint32_t)(lane & 3) * 4) : "memory");
-                if (row0 + q0 + q < p.rows && c < p.cols) store1(p.w, p.type_w, o + q * p.ld_w, fmaf(p.keep, w[q], x));
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buf + (uint32_t)(r * 128 + (((lane >> 2) ^ r) & 7) * 16 + (lane & 3) * 4)) : "memory");
+                if (row0 + r < p.rows && c < p.cols) store1(p.w, p.type_w, o + q * p.ld_w, fmaf(p.keep, w[q], x));
             }
         }
     }
     __syncwarp();
 }
 
-// 384 threads; grid: any number of CTAs (pairs), each takes every grid-th tile.
+// The K blocks of one tile, in the order they are multiplied, for the part of K a pair has. One plane, Q X: first
+// the blocks on the tile's diagonal with the lo plane of X. Two planes: the chunk ends, where the
+// accumulator is drained. All roles walk this list.
+__device__ __forceinline__ bool chunk_ends(int kb, int diag0, int diag, bool sym)
+{
+    return (kb & 1) || (sym && kb >= diag0 && kb < diag0 + diag);
+}
+struct Blocks {
+    int kb0, kb1, d0, n_lo, n;
+    __device__ __forceinline__ Blocks(int kb0_, int kb1_, int diag0, int diag1, bool lo) : kb0(kb0_), kb1(kb1_), d0(max(diag0, kb0_))
+    {
+        n_lo = lo ? max(0, min(diag1, kb1) - d0) : 0;
+        n = n_lo + kb1 - kb0;
+    }
+    __device__ __forceinline__ bool lo(int t) const { return t < n_lo; }
+    __device__ __forceinline__ int at(int t) const { return t < n_lo ? d0 + t : kb0 + t - n_lo; }
+};
+
+// 384 threads; grid: any number of CTAs (pairs), each takes every grid-th tile. PAIR with p.split > 1: a
+// cluster of that many pairs shares one tile, each takes a range of K, and the sums meet in the
+// workspace, 64 columns of the tile with each owner; the grid is then one cluster a tile. Few tiles
+// leave most of the GPU idle: the 10 tiles of a 1000 x 1000 symmetric product with K = 2049 took 33 us
+// on 36 single CTAs. (Through distributed shared memory instead of L2 the meeting alone took 10 us.)
 template <int PLANES, bool PAIR>
-__device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorMap &a_lo, const CUtensorMap &b_hi, const CUtensorMap &b_lo, const Product &p)
+__device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorMap &a_lo, const CUtensorMap &b_hi, const CUtensorMap &b_lo,
+                                        const CUtensorMap &o_hi, const CUtensorMap &o_lo, const Product &p)
 {
     using namespace gemm;
     constexpr int BK = 64, SIDE = PAIR ? 256 : 128;                 // K block; tile side
     constexpr uint32_t TILE = 128 * BK * 2;                         // one operand plane of one CTA: 16 KB
     constexpr uint32_t STAGE = 2 * PLANES * TILE;
     constexpr int STAGES = 6 / PLANES;
-    constexpr int CHUNK_KB = PLANES == 2 ? 2 : 1 << 30;             // K blocks per accumulation in tensor memory
     constexpr int HALF = SIDE / 2;                                  // columns per epilogue warp
     constexpr uint32_t TMEM_COLS = 2 * SIDE;                        // two accumulators
     const WaitCtl status = { p.status, p.wait_ns };
@@ -470,22 +459,27 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     __shared__ __align__(8) uint64_t bars[2 * STAGES + 4];
     __shared__ uint32_t s_tmem;
 
-    const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+    const uint32_t cta = PAIR ? cluster_ctarank() : 0, rank = cta & 1u, first = cta & ~1u;      // first: the pair's leader
     const bool leader = rank == 0;
+    const int split = PAIR ? p.split : 1, part = PAIR ? (int)(cta >> 1) : 0;
     const uint32_t smem0 = (smem_u32(smem_orth) + 1023u) & ~1023u;
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]);
     const uint32_t acc_full0 = smem_u32(&bars[2 * STAGES]), acc_empty0 = smem_u32(&bars[2 * STAGES + 2]);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int C = (int)(PAIR ? gridDim.x >> 1 : gridDim.x), cl = (int)(PAIR ? blockIdx.x >> 1 : blockIdx.x);
+    const int C = (int)(PAIR ? gridDim.x / (2u * split) : gridDim.x), cl = (int)(PAIR ? blockIdx.x / (2u * split) : blockIdx.x);
     const Tiles tiles(p, SIDE);
     const int items = tiles.each * p.batch;
-    const int nkb = (p.K + BK - 1) / BK;
-    // Which operand blocks come transposed. X as the second operand of P X has its columns contiguous. Of a
+    // K blocks of this pair: [kb0, kb1), an even number but for the last
+    const int all_kb = (p.K + BK - 1) / BK, all_ck = (all_kb + 1) / 2;
+    const int kb0 = 2 * (all_ck * part / split), kb1 = min(all_kb, 2 * (all_ck * (part + 1) / split));
+    // Which operand blocks come transposed. X as the second operand of Q X has its columns contiguous. Of a
     // symmetric operand the block at K block kb is above the stored triangle when kb's tile lies beyond the tile
     // of the rows. (A pair whose triangle was stored in 128-tiles takes the rule of its upper half: for the
     // lower half that differs only inside its own diagonal tile, which is stored whole.)
     const bool a_sym = p.mode != ORTH_GRAM, b_sym = p.mode == ORTH_POLY, b_cols = p.mode >= ORTH_UPDATE;
+    const bool lo_blocks = PLANES == 1 && b_cols;
     const int tri_shift = p.tri == 256 ? 8 : 7;
+    constexpr int DIAG = SIDE / BK;                                 // K blocks on a tile's diagonal
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
@@ -495,10 +489,10 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     if (threadIdx.x == 32) {        // the descriptors, while the kernel before still runs
         asm volatile("prefetch.tensormap [%0];" ::"l"(&a_hi) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&b_hi) : "memory");
-        if constexpr (PLANES == 2) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&a_lo) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&b_lo) : "memory");
-        }
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&b_lo) : "memory");
+        if constexpr (PLANES == 2) asm volatile("prefetch.tensormap [%0];" ::"l"(&a_lo) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&o_hi) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&o_lo) : "memory");
     }
     __syncwarp();
     if (warp == 1) {
@@ -529,14 +523,16 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                 tiles.at(item, k, i, j);
                 const int m0 = i * SIDE + (int)rank * 128, n0 = j * SIDE + (int)rank * 128;
                 const int ti = (i * SIDE) >> tri_shift, tj = (j * SIDE) >> tri_shift;
-                for (int kb = 0; kb < nkb; kb++, it++) {
+                const Blocks blocks(kb0, kb1, i * DIAG, i * DIAG + DIAG, lo_blocks);
+                for (int t = 0; t < blocks.n; t++, it++) {
                     const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
                     if (!mbar_wait(empty0 + 8 * s, ph ^ 1u, status, 1)) { ok = false; break; }
                     const uint32_t st = smem0 + s * STAGE;
                     uint32_t bar = full0 + 8 * s;
                     if (leader) mbar_expect_tx(bar, (PAIR ? 2 : 1) * STAGE);
-                    if constexpr (PAIR) bar = map_to_cta(bar, 0);
-                    const int tk = (kb * BK) >> tri_shift;
+                    if constexpr (PAIR) bar = map_to_cta(bar, first);
+                    const int kb = blocks.at(t), tk = (kb * BK) >> tri_shift;
+                    const CUtensorMap *const b1 = blocks.lo(t) ? &b_lo : &b_hi;
                     const bool a_t = a_sym && tk > ti, b_t = b_cols || (b_sym && tk > tj);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {                   // 64 rows of an operand at a time
@@ -545,14 +541,14 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         const int bx = b_t ? n0 + 64 * h : kb * BK, by = b_t ? kb * BK : n0 + 64 * h;
                         if constexpr (PAIR) {
                             tma_3d_pair(d, &a_hi, bar, ax, ay, k);
-                            tma_3d_pair(d + PLANES * TILE, &b_hi, bar, bx, by, k);
+                            tma_3d_pair(d + PLANES * TILE, b1, bar, bx, by, k);
                             if constexpr (PLANES == 2) {
                                 tma_3d_pair(d + TILE, &a_lo, bar, ax, ay, k);
                                 tma_3d_pair(d + 3 * TILE, &b_lo, bar, bx, by, k);
                             }
                         } else {
                             tma_3d(d, &a_hi, bar, ax, ay, k);
-                            tma_3d(d + PLANES * TILE, &b_hi, bar, bx, by, k);
+                            tma_3d(d + PLANES * TILE, b1, bar, bx, by, k);
                             if constexpr (PLANES == 2) {
                                 tma_3d(d + TILE, &a_lo, bar, ax, ay, k);
                                 tma_3d(d + 3 * TILE, &b_lo, bar, bx, by, k);
@@ -571,78 +567,86 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                 int k, i, j;
                 tiles.at(item, k, i, j);
                 const int ti = (i * SIDE) >> tri_shift, tj = (j * SIDE) >> tri_shift;
-                for (int kb = 0; kb < nkb && ok; g++) {
-                    const uint32_t buf = g & 1u;
-                    ok = mbar_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1u) ^ 1u, status, 4);
+                const Blocks blocks(kb0, kb1, i * DIAG, i * DIAG + DIAG, lo_blocks);
+                uint32_t acc = 0, buf = 0;
+                for (int t = 0; t < blocks.n; t++, it++) {
+                    const int kb = blocks.at(t), tk = (kb * BK) >> tri_shift;
+                    if (acc == 0) {                                 // a chunk begins
+                        buf = g & 1u;
+                        ok = mbar_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1u) ^ 1u, status, 4);
+                        if (!ok) break;
+                        g++;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    }
+                    const uint32_t tacc = tmem + buf * (uint32_t)SIDE;
+                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
+                    ok = mbar_wait(full0 + 8 * s, ph, status, 2);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t tacc = tmem + buf * (uint32_t)SIDE;
-                    const int kb_end = PLANES == 2 ? min(kb + CHUNK_KB, nkb) : nkb;
-                    uint32_t acc = 0;
-                    for (; kb < kb_end; kb++, it++) {
-                        const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
-                        ok = mbar_wait(full0 + 8 * s, ph, status, 2);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t st = smem0 + s * STAGE;
-                        const int tk = (kb * BK) >> tri_shift;
-                        const bool a_t = a_sym && tk > ti, b_t = b_cols || (b_sym && tk > tj);
-                        const uint32_t idesc = instr_desc(SIDE, SIDE, a_t, b_t), bt = st + PLANES * TILE;
-                        const uint64_t ah = tile_desc(st, a_t), al = tile_desc(st + TILE, a_t), bh = tile_desc(bt, b_t), bl = tile_desc(bt + TILE, b_t);
-                        // two planes: the small products first. The tensor core truncates what it adds to a sum
-                        // to the sum's last bit, so adds to a sum that is still small cost less.
-                        if constexpr (PLANES == 2) {
-#pragma unroll
-                            for (int kk = 0; kk < BK / 16; kk++) {
-                                umma<PAIR>(tacc, al + k_advance(kk, a_t), bh + k_advance(kk, b_t), idesc, acc);
-                                umma<PAIR>(tacc, ah + k_advance(kk, a_t), bl + k_advance(kk, b_t), idesc, 1u);
-                                acc = 1;
-                            }
-                        }
+                    const uint32_t st = smem0 + s * STAGE;
+                    const bool a_t = a_sym && tk > ti, b_t = b_cols || (b_sym && tk > tj);
+                    const uint32_t idesc = instr_desc(SIDE, SIDE, a_t, b_t), bt = st + PLANES * TILE;
+                    const uint64_t ah = tile_desc(st, a_t), al = tile_desc(st + TILE, a_t), bh = tile_desc(bt, b_t), bl = tile_desc(bt + TILE, b_t);
+                    // two planes: the small products first. The tensor core truncates what it adds to a sum
+                    // to the sum's last bit, so adds to a sum that is still small cost less.
+                    if constexpr (PLANES == 2) {
 #pragma unroll
                         for (int kk = 0; kk < BK / 16; kk++) {
-                            umma<PAIR>(tacc, ah + k_advance(kk, a_t), bh + k_advance(kk, b_t), idesc, acc);
+                            umma<PAIR>(tacc, al + k_advance(kk, a_t), bh + k_advance(kk, b_t), idesc, acc);
+                            umma<PAIR>(tacc, ah + k_advance(kk, a_t), bl + k_advance(kk, b_t), idesc, 1u);
                             acc = 1;
                         }
-                        commit<PAIR>(empty0 + 8 * s);
                     }
-                    if (ok) commit<PAIR>(acc_full0 + 8 * buf);
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; kk++) {
+                        umma<PAIR>(tacc, ah + k_advance(kk, a_t), bh + k_advance(kk, b_t), idesc, acc);
+                        acc = 1;
+                    }
+                    commit<PAIR>(empty0 + 8 * s, first);
+                    if (t + 1 == blocks.n || (PLANES == 2 && chunk_ends(kb, i * DIAG, DIAG, a_sym))) {
+                        commit<PAIR>(acc_full0 + 8 * buf, first);
+                        acc = 0;
+                    }
                 }
             }
         }
         __syncwarp();
       }
+      if (PAIR && split > 1) cluster_sync_all();                    // the meeting of the epilogue warps
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int q = warp & 3, h = (warp - 4) >> 2;
-        const uint32_t acc_empty = PAIR ? map_to_cta(acc_empty0, 0) : acc_empty0;
-        const Stage stage = { smem0 + STAGES * STAGE + (uint32_t)(warp - 4) * 4096u, lane };
+        const int e = warp - 4, q = warp & 3, h = e >> 2;
+        const uint32_t acc_empty = PAIR ? map_to_cta(acc_empty0, first) : acc_empty0;
+        const uint32_t staging = smem0 + STAGES * STAGE;
+        // two warps (q even and odd) store planes together
+        const uint32_t pair_buf = staging + (uint32_t)(h * 2 + (q >> 1)) * 8192u;
+        const int pair_bar = 1 + h * 2 + (q >> 1), pair_row = (q & 1) * 32 + lane;
+        const bool issuer = pair_row == 0;
         uint32_t g = 0;
         bool ok = true;
         for (int item = cl; ok && item < items; item += C) {
             int k, i, j;
             tiles.at(item, k, i, j);
             const int row0 = i * SIDE + (int)rank * 128 + q * 32, col0 = j * SIDE + h * HALF;
-            Piece in;
-            if (p.mode != ORTH_GRAM) fetch(p, in, k, row0, col0, lane);       // lands while the products run
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * HALF);
             uint32_t buf = g & 1u;
             if constexpr (PLANES == 1) {
                 ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
-                if (!ok) break;
                 g++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             } else {
                 // the chunks' sums in registers; the total goes back to tensor memory in place of the last chunk, so
-                // that the epilogue below holds 32 columns at a time (with all of them in registers it
+                // that the epilogue below holds 64 columns at a time (with all of them in registers it
                 // spilled, and beside 225 KB of shared memory there is no first-level cache to spill to)
                 float acc[HALF];
 #pragma unroll
-                for (int e = 0; e < HALF; e++) acc[e] = 0.f;
-                for (int kb = 0; kb < nkb; kb += CHUNK_KB, g++) {
+                for (int c = 0; c < HALF; c++) acc[c] = 0.f;
+                for (int kb = kb0; kb < kb1; kb++) {
+                    if (kb + 1 < kb1 && !chunk_ends(kb, i * DIAG, DIAG, a_sym)) continue;
                     buf = g & 1u;
                     ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
                     if (!ok) break;
+                    g++;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                     for (int cc = 0; cc < HALF / 16; cc++) {
@@ -650,9 +654,9 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         tmem_ld16(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 16), r);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                        for (int e = 0; e < 16; e++) acc[cc * 16 + e] = __fadd_rn(acc[cc * 16 + e], __uint_as_float(r[e]));
+                        for (int c = 0; c < 16; c++) acc[cc * 16 + c] = __fadd_rn(acc[cc * 16 + c], __uint_as_float(r[c]));
                     }
-                    if (kb + CHUNK_KB >= nkb) {
+                    if (kb + 1 == kb1) {
 #pragma unroll
                         for (int cc = 0; cc < HALF / 32; cc++) tmem_st32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 32), acc + cc * 32);
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -662,31 +666,82 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
                     }
                 }
-                if (!ok) break;
             }
+            // where this warp's sums of 64 columns lie when parts meet: [part][CTA][warp][piece][unit of 4 columns][lane]
+            const size_t sums_at = (((size_t)cl * split * 2 + rank) * 8 + e) * 4096 + lane * 4, part_step = 2 * 8 * 4096;
+            if (PAIR && split > 1) {
 #pragma unroll 1
-            for (int cc = 0; cc < HALF / 32; cc++) {
-                if (row0 >= p.rows || col0 + cc * 32 >= p.cols) break;
-                if (p.mode != ORTH_GRAM) {
-                    put(in, stage);
-                    if (cc + 1 < HALF / 32) fetch(p, in, k, row0, col0 + (cc + 1) * 32, lane);
-                }
-                float v[32];
-                {
+                for (int cc = 0; ok && cc < HALF / 32; cc++) {
+                    if ((2 * h + (cc >> 1)) % split == part) continue;
                     uint32_t r[32];
                     tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 32), r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    float *const to = p.sums + sums_at + part * part_step + cc * 1024;
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = __uint_as_float(r[e]);
+                    for (int u = 0; u < 8; u++)
+                        __stcg(reinterpret_cast<float4 *>(to + u * 128), make_float4(__uint_as_float(r[4 * u]), __uint_as_float(r[4 * u + 1]),
+                                                                                   __uint_as_float(r[4 * u + 2]), __uint_as_float(r[4 * u + 3])));
                 }
-                emit(p, v, stage, k, row0, col0 + cc * 32);
+                cluster_sync_all();
+            }
+            // the two warps of a store go on only if both may
+            ok = both_ok(pair_bar, ok);
+#pragma unroll 1
+            for (int cc = 0; ok && cc < HALF / 64; cc++) {
+                if (split > 1 && (2 * h + cc) % split != part) continue;
+                const int col = col0 + cc * 64;
+                // both warps of a store agree: the upper one's rows decide
+                if (row0 - (q & 1) * 32 >= p.rows || col >= p.cols) break;
+                uint32_t hi[32], lo[32];
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    uint32_t r[32];
+                    tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 64 + half * 32), r);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    float v[32];
+#pragma unroll
+                    for (int c = 0; c < 32; c++) v[c] = __uint_as_float(r[c]);
+                    if (PAIR)
+                        for (int from = 0; from < split; from++) {
+                            if (from == part) continue;
+                            const float *const at = p.sums + sums_at + from * part_step + (cc * 2 + half) * 1024;
+#pragma unroll
+                            for (int u = 0; u < 8; u++) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(at + u * 128));
+                                v[4 * u] += x.x; v[4 * u + 1] += x.y; v[4 * u + 2] += x.z; v[4 * u + 3] += x.w;
+                            }
+                        }
+#pragma unroll
+                    for (int c = 0; c < 32; c++) v[c] *= p.alpha;
+                    if (p.mode == ORTH_RESULT) {
+                        store_result(p, v, staging + (uint32_t)e * 4096u, lane, k, row0, col + half * 32);
+                        continue;
+                    }
+                    if (tiles.sym && i == j) {
+#pragma unroll
+                        for (int c = 0; c < 32; c++) v[c] += row0 + lane == col + half * 32 + c ? p.diag : 0.f;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 16; c++) {
+                        const __half2 x = __floats2half2_rn(v[2 * c], v[2 * c + 1]);
+                        const float2 f = __half22float2(x);
+                        const __half2 y = __floats2half2_rn(v[2 * c] - f.x, v[2 * c + 1] - f.y);
+                        hi[half * 16 + c] = *reinterpret_cast<const uint32_t *>(&x);
+                        lo[half * 16 + c] = *reinterpret_cast<const uint32_t *>(&y);
+                    }
+                }
+                if (p.mode != ORTH_RESULT) {
+                    store_plane(&o_hi, pair_buf, hi, pair_row, pair_bar, issuer, col, row0, k);
+                    if (p.lo) store_plane(&o_lo, pair_buf, lo, pair_row, pair_bar, issuer, col, row0, k);
+                }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
         }
+        if (issuer) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if (!ok) {      // a wait ran out: copies that may still be in flight land before the shared memory is released
-            for (int i = 0; i < 64; i++) __nanosleep(4000);
+            for (int n = 0; n < 64; n++) __nanosleep(4000);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -700,12 +755,14 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
 
 }  // namespace orth
 
-#define ORTH_PRODUCT(name, PLANES, PAIR, CLUSTER)                                                                                    \
-    extern "C" __global__ void CLUSTER __launch_bounds__(384, 1)                                                                     \
+// the pair forms are launched in clusters of 2 x split CTAs
+#define ORTH_PRODUCT(name, PLANES, PAIR)                                                                                             \
+    extern "C" __global__ void __launch_bounds__(384, 1)                                                                             \
     name(const __grid_constant__ CUtensorMap a_hi, const __grid_constant__ CUtensorMap a_lo, const __grid_constant__ CUtensorMap b_hi, \
-         const __grid_constant__ CUtensorMap b_lo, const __grid_constant__ orth::Product p)                                           \
-    { orth::product<PLANES, PAIR>(a_hi, a_lo, b_hi, b_lo, p); }
-ORTH_PRODUCT(orth_product_1_single, 1, false, )
-ORTH_PRODUCT(orth_product_2_single, 2, false, )
-ORTH_PRODUCT(orth_product_1_pair, 1, true, __cluster_dims__(2, 1, 1))
-ORTH_PRODUCT(orth_product_2_pair, 2, true, __cluster_dims__(2, 1, 1))
+         const __grid_constant__ CUtensorMap b_lo, const __grid_constant__ CUtensorMap o_hi, const __grid_constant__ CUtensorMap o_lo, \
+         const __grid_constant__ orth::Product p)                                                                                    \
+    { orth::product<PLANES, PAIR>(a_hi, a_lo, b_hi, b_lo, o_hi, o_lo, p); }
+ORTH_PRODUCT(orth_product_1_single, 1, false)
+ORTH_PRODUCT(orth_product_2_single, 2, false)
+ORTH_PRODUCT(orth_product_1_pair, 1, true)
+ORTH_PRODUCT(orth_product_2_pair, 2, true)

@@ -119,6 +119,7 @@ struct sm100_dev {
     unsigned    gemm_wait_ms;          /* limit of the GEMM kernel's barrier waits */
     int         orth_pending;          /* an orthogonalisation was enqueued since the last status check */
     int         orth_captured;         /* one was captured into a graph: its replays are not seen here */
+    int         orth_clusters[5];      /* clusters of 2 x split CTAs the GPU holds at once, by split (0 = not asked yet) */
     int         orth_smem_set;         /* dynamic shared memory limit raised on the product kernels */
     unsigned    gemm_epoch;            /* tag of the latest persistent GEMM call (never zero once used) */
     int         gemm_clusters;         /* CTA pairs of the persistent GEMM kernel this GPU holds at once (0 = not asked yet) */
@@ -153,6 +154,9 @@ int  sm100_launch_k_overlapped(sm100_dev_t *dev, int which, unsigned grid, unsig
                                unsigned shmem, void **args);
 int  sm100_launch_k3_overlapped(sm100_dev_t *dev, int which, unsigned gx, unsigned gy, unsigned gz,
                                 unsigned bx, unsigned by, unsigned bz, unsigned shmem, void **args);
+/* The same (one-dimensional) in clusters of `cluster` blocks. */
+int  sm100_launch_k_cluster(sm100_dev_t *dev, int which, unsigned grid, unsigned cluster, unsigned block,
+                            unsigned shmem, void **args);
 /* The kernel's name as the driver knows it, for messages; "kernel" when the driver
  * cannot say (cuFuncGetName is a CUDA 12.3 entry point). */
 void sm100_func_name(sm100_dev_t *dev, void *func, char *out, size_t n);

@@ -725,27 +725,36 @@ int sm100_launch_k(sm100_dev_t *dev, int which, unsigned grid, unsigned block,
     return sm100_launch_k3(dev, which, grid, 1, 1, block, 1, 1, shmem, args);
 }
 
-int sm100_launch_k3_overlapped(sm100_dev_t *dev, int which, unsigned gx, unsigned gy, unsigned gz,
-                               unsigned bx, unsigned by, unsigned bz, unsigned shmem, void **args)
+static int launch_overlapped(sm100_dev_t *dev, int which, unsigned gx, unsigned gy, unsigned gz,
+                             unsigned bx, unsigned by, unsigned bz, unsigned shmem, unsigned cluster, void **args)
 {
     static int enabled = -1;
     if (enabled < 0) {
         const char *e = getenv("BOOTH_SM100_PDL");
         enabled = !(e && e[0] == '0');
     }
-    if (!enabled || !dev->api->LaunchKernelEx) return sm100_launch_k3(dev, which, gx, gy, gz, bx, by, bz, shmem, args);
-    CUlaunchAttribute attr;
-    memset(&attr, 0, sizeof attr);
-    attr.id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
-    attr.value.programmaticStreamSerializationAllowed = 1;
+    if (cluster <= 1 && (!enabled || !dev->api->LaunchKernelEx)) return sm100_launch_k3(dev, which, gx, gy, gz, bx, by, bz, shmem, args);
+    if (!dev->api->LaunchKernelEx) return fail_arg(dev, "this driver has no cuLaunchKernelEx: clusters cannot be launched");
+    CUlaunchAttribute attr[2];
+    memset(attr, 0, sizeof attr);
+    unsigned n = 0;
+    if (enabled) {
+        attr[n].id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
+        attr[n++].value.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+        attr[n].value.clusterDim.x = cluster; attr[n].value.clusterDim.y = 1;
+        attr[n++].value.clusterDim.z = 1;
+    }
     CUlaunchConfig cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDimX = gx; cfg.gridDimY = gy; cfg.gridDimZ = gz;
     cfg.blockDimX = bx; cfg.blockDimY = by; cfg.blockDimZ = bz;
     cfg.sharedMemBytes = shmem;
     cfg.hStream = dev->stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
     CUresult cr = dev->api->LaunchKernelEx(&cfg, dev->k[which], args, NULL);
     if (cr != CUDA_SUCCESS) {
         char what[160];
@@ -755,6 +764,18 @@ int sm100_launch_k3_overlapped(sm100_dev_t *dev, int which, unsigned gx, unsigne
     }
     dev->launches++;
     return SM100_OK;
+}
+
+int sm100_launch_k3_overlapped(sm100_dev_t *dev, int which, unsigned gx, unsigned gy, unsigned gz,
+                               unsigned bx, unsigned by, unsigned bz, unsigned shmem, void **args)
+{
+    return launch_overlapped(dev, which, gx, gy, gz, bx, by, bz, shmem, 1, args);
+}
+
+int sm100_launch_k_cluster(sm100_dev_t *dev, int which, unsigned grid, unsigned cluster, unsigned block,
+                           unsigned shmem, void **args)
+{
+    return launch_overlapped(dev, which, grid, 1, 1, block, 1, 1, shmem, cluster, args);
 }
 
 int sm100_launch_k_overlapped(sm100_dev_t *dev, int which, unsigned grid, unsigned block,

@@ -169,17 +169,17 @@ int booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t
 
 static size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
-/* Where things lie in the workspace: the norms' partial sums, then fp16 planes. X is
- * short x long, A and P short x short; rows of a plane are a multiple of 64 elements
- * apart. X exists twice, the products read one copy and write the other. One-plane
- * results (bf16) keep lo planes of X only. */
+/* Where things lie in the workspace: the norms' partial sums, then fp16 planes, then the
+ * sums of tiles whose K is shared (128 KB a CTA). X is short x long, S and Q short x
+ * short; rows of a plane are a multiple of 64 elements apart. X exists twice, the products
+ * read one copy and write the other. One-plane results (bf16) keep lo planes of X only. */
 typedef struct orth_layout {
     long long s, l, x_pitch, a_pitch;
     int parts;
-    size_t x_hi[2], x_lo[2], a_hi, a_lo, p_hi, p_lo, bytes;
+    size_t x_hi[2], x_lo[2], s_hi, s_lo, q_hi, q_lo, sums, bytes;
 } orth_layout_t;
 
-static int orth_layout(orth_layout_t *o, int batch, int rows, int cols, int two_planes)
+static int orth_layout(const sm100_dev_t *dev, orth_layout_t *o, int batch, int rows, int cols, int two_planes)
 {
     if (batch < 1 || batch > 65535 || rows < 1 || cols < 1 || rows > ORTH_MAX_SIDE || cols > ORTH_MAX_SIDE) return 0;
     o->s = rows < cols ? rows : cols;
@@ -192,10 +192,13 @@ static int orth_layout(orth_layout_t *o, int batch, int rows, int cols, int two_
     const size_t x = up((size_t)batch * o->s * o->x_pitch * 2, 128), a = up((size_t)batch * o->s * o->a_pitch * 2, 128);
     size_t at = up((size_t)batch * o->parts * sizeof(double), 128);
     for (int i = 0; i < 2; i++) { o->x_hi[i] = at; at += x; o->x_lo[i] = at; at += x; }
-    o->a_hi = at; at += a;
-    o->a_lo = at; if (two_planes) at += a;
-    o->p_hi = at; at += a;
-    o->p_lo = at; if (two_planes) at += a;
+    o->s_hi = at; at += a;
+    o->s_lo = at; if (two_planes) at += a;
+    o->q_hi = at; at += a;
+    o->q_lo = at; if (two_planes) at += a;
+    /* K is shared only while all parts of all tiles run at once, so no more CTAs than SMs meet */
+    const long long pairs = batch * ((o->l + 255) / 256) * ((o->s + 255) / 256), ctas = 2 * 4 * pairs < dev->sm_count ? 2 * 4 * pairs : dev->sm_count;
+    o->sums = at; at += (size_t)ctas * 131072;
     o->bytes = at;
     const long long t = (o->l + 127) / 128;
     return t * ((o->s + 127) / 128) <= INT_MAX / batch;
@@ -204,7 +207,7 @@ static int orth_layout(orth_layout_t *o, int batch, int rows, int cols, int two_
 size_t booth_sm100_orthogonalise_workspace(sm100_dev_t *dev, int batch, int rows, int cols, int dtype)
 {
     orth_layout_t o;
-    if (!dev || type_index(dtype) < 0 || !orth_layout(&o, batch, rows, cols, dtype != SM100_BF16)) {
+    if (!dev || type_index(dtype) < 0 || !orth_layout(dev, &o, batch, rows, cols, dtype != SM100_BF16)) {
         bad_arg(dev, "booth_sm100_orthogonalise_workspace: bad argument");
         return 0;
     }
@@ -227,28 +230,70 @@ static int plane_map(sm100_dev_t *dev, CUtensorMap *map, CUdeviceptr p, long lon
 /* cuTensorMapEncodeTiled wants its maps on 64-byte boundaries. */
 typedef struct { CUtensorMap hi __attribute__((aligned(64))), lo __attribute__((aligned(64))); } plane_maps_t;
 
-/* Pairs of CTAs on 256 x 256 tiles, or single CTAs on 128 x 128. A pair tile takes
- * twice as long as a single one at full rate, and the narrow tile, which reads its
- * operands from shared memory twice as often, runs at about 3/4 of it: the form with the
- * shorter list of waves wins. */
-static int orth_pairs(const sm100_dev_t *dev, long long rows, long long cols, int batch, int sym)
+/* How many clusters of 2 x split CTAs of the product kernels the GPU holds at once
+ * (asked of the driver once; else SM pairs, less one in seven for clusters that have
+ * to fit inside a group of SMs). Only a measure for the choice below: no cluster waits for another. */
+static int orth_clusters(sm100_dev_t *dev, int split)
 {
-    const long long pm = (rows + 255) / 256, pn = (cols + 255) / 256, sm = (rows + 127) / 128, sn = (cols + 127) / 128;
-    const long long pt = batch * (sym ? pm * (pm + 1) / 2 : pm * pn), st = batch * (sym ? sm * (sm + 1) / 2 : sm * sn);
-    const long long slots = dev->sm_count / 2 > 0 ? dev->sm_count / 2 : 1;
-    const long long pw = (pt + slots - 1) / slots, sw = (st + 2 * slots - 1) / (2 * slots);
-    return 6 * pw <= 4 * sw;
+    if (dev->orth_clusters[split]) return dev->orth_clusters[split];
+    int n = dev->sm_count / (2 * split);
+    if (split > 1) n = n * 6 / 7;
+    if (dev->api->OccupancyMaxActiveClusters) {
+        CUlaunchAttribute attr;
+        memset(&attr, 0, sizeof attr);
+        attr.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+        attr.value.clusterDim.x = 2u * (unsigned)split; attr.value.clusterDim.y = 1; attr.value.clusterDim.z = 1;
+        CUlaunchConfig cfg;
+        memset(&cfg, 0, sizeof cfg);
+        cfg.gridDimX = 2u * (unsigned)split * 64u; cfg.gridDimY = 1; cfg.gridDimZ = 1;
+        cfg.blockDimX = 384; cfg.blockDimY = 1; cfg.blockDimZ = 1;
+        cfg.sharedMemBytes = ORTH_SMEM;
+        cfg.hStream = dev->stream;
+        cfg.attrs = &attr; cfg.numAttrs = 1;
+        int got = 0;
+        if (dev->api->OccupancyMaxActiveClusters(&got, dev->k[SM100_K_ORTH_PRODUCT + 2], &cfg) == CUDA_SUCCESS && got > 0) n = got;
+    }
+    dev->orth_clusters[split] = n > 0 ? n : 1;
+    return dev->orth_clusters[split];
 }
 
-static int orth_launch(sm100_dev_t *dev, const plane_maps_t *a, const plane_maps_t *b, orth_product_t *p, int two_planes)
+/* Form of a product: pairs of CTAs on 256 x 256 tiles, the K of a tile shared by up to
+ * four pairs, or single CTAs on 128 x 128 tiles; the one with the shortest estimate in
+ * tensor clocks. A K block of 64 takes a pair 512 clocks a plane product (one or three). A
+ * single CTA needs 256 of them, but its narrow tile reads shared memory faster than it
+ * delivers: 512 and 1250 measured. Beside that a wave costs its epilogue, some 3000
+ * clocks (2000 for the smaller tile), and meeting in the workspace some 3000. */
+static void orth_plan(sm100_dev_t *dev, const orth_product_t *p, int two_planes, int *pairs, int *split)
 {
-    const int sym = p->mode <= ORTH_POLY, pairs = orth_pairs(dev, p->rows, p->cols, p->batch, sym);
+    const int sym = p->mode <= ORTH_POLY;
+    const long long pm = (p->rows + 255) / 256, pn = (p->cols + 255) / 256, sm = (p->rows + 127) / 128, sn = (p->cols + 127) / 128;
+    const long long pt = p->batch * (sym ? pm * (pm + 1) / 2 : pm * pn), st = p->batch * (sym ? sm * (sm + 1) / 2 : sm * sn);
+    const long long kb = (p->K + 63) / 64, chunks = (kb + 1) / 2;
+    double best = (double)((st + dev->sm_count - 1) / dev->sm_count) * (2000.0 + kb * (two_planes ? 1250.0 : 512.0));
+    *pairs = 0; *split = 1;
+    for (int s = 1; s <= 4 && s <= chunks; s++) {
+        const long long slots = orth_clusters(dev, s), waves = (pt + slots - 1) / slots;
+        if (s > 1 && (waves > 1 || 2 * s * pt > dev->sm_count)) break;
+        const double cost = (double)waves * (3000.0 / s + (s > 1 ? 3000.0 : 0.0) + 2.0 * ((chunks + s - 1) / s) * (two_planes ? 1536.0 : 512.0));
+        if (cost < best) { best = cost; *pairs = 1; *split = s; }
+    }
+}
+
+static int orth_launch(sm100_dev_t *dev, const plane_maps_t *a, const plane_maps_t *b, const plane_maps_t *out, orth_product_t *p, int two_planes)
+{
+    int pairs, split;
+    orth_plan(dev, p, two_planes, &pairs, &split);
+    const int sym = p->mode <= ORTH_POLY;
     const long long side = pairs ? 256 : 128, tm = (p->rows + side - 1) / side, tn = (p->cols + side - 1) / side;
-    const long long tiles = p->batch * (sym ? tm * (tm + 1) / 2 : tm * tn), slots = pairs ? dev->sm_count / 2 : dev->sm_count;
-    if (sym) p->tri = (int)side;        /* A, then P: both are s x s, so both get the same tiles; the update reads P's */
-    const unsigned grid = (unsigned)((tiles < slots ? tiles : slots) * (pairs ? 2 : 1));
-    void *args[] = { (void *)&a->hi, (void *)&a->lo, (void *)&b->hi, (void *)&b->lo, p };
-    return sm100_launch_k3_overlapped(dev, SM100_K_ORTH_PRODUCT + (pairs ? 2 : 0) + (two_planes ? 1 : 0), grid, 1, 1, 384, 1, 1, ORTH_SMEM, args);
+    const long long tiles = p->batch * (sym ? tm * (tm + 1) / 2 : tm * tn), slots = pairs ? orth_clusters(dev, 1) : dev->sm_count;
+    /* a split tile's cluster takes that one tile: the parts meet a fixed number of times */
+    const long long groups = split > 1 || tiles < slots ? tiles : slots;
+    p->split = split;
+    void *args[] = { (void *)&a->hi, (void *)&a->lo, (void *)&b->hi, (void *)&b->lo, (void *)&out->hi, (void *)&out->lo, p };
+    const int rc = sm100_launch_k_cluster(dev, SM100_K_ORTH_PRODUCT + (pairs ? 2 : 0) + (two_planes ? 1 : 0), (unsigned)(groups * (pairs ? 2 * split : 1)),
+                                          pairs ? 2u * (unsigned)split : 1u, 384, ORTH_SMEM, args);
+    if (sym) p->tri = (int)side;        /* how the product that reads this one finds its triangle */
+    return rc;
 }
 
 static int orth_status_ready(sm100_dev_t *dev)
@@ -291,50 +336,50 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
                                     256, 1, 1, 0, sa);
     if (rc != SM100_OK) return rc;
 
-    plane_maps_t x[2], a, p;
+    plane_maps_t x[2], sm, qm;
     for (int i = 0; i < 2; i++) {
         if ((rc = plane_map(dev, &x[i].hi, ws + o->x_hi[i], o->s, o->l, o->x_pitch, batch)) != SM100_OK) return rc;
         if ((rc = plane_map(dev, &x[i].lo, ws + o->x_lo[i], o->s, o->l, o->x_pitch, batch)) != SM100_OK) return rc;
     }
-    if ((rc = plane_map(dev, &a.hi, ws + o->a_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
-    if ((rc = plane_map(dev, &p.hi, ws + o->p_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
-    a.lo = a.hi; p.lo = p.hi;           /* not read by the one-plane kernels */
+    if ((rc = plane_map(dev, &sm.hi, ws + o->s_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+    if ((rc = plane_map(dev, &qm.hi, ws + o->q_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+    sm.lo = sm.hi; qm.lo = qm.hi;       /* not read or written by the one-plane kernels */
     if (two_planes) {
-        if ((rc = plane_map(dev, &a.lo, ws + o->a_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
-        if ((rc = plane_map(dev, &p.lo, ws + o->p_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+        if ((rc = plane_map(dev, &sm.lo, ws + o->s_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+        if ((rc = plane_map(dev, &qm.lo, ws + o->q_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
     }
-    /* P's scale: with singular values below 2, |P| <= 4 |b| + 16 |c| has to stay below fp16's 65504. */
-    const double bound = 4.0 * fabs(ns->b) + 16.0 * fabs(ns->c);
-    double p_scale = 16384.0;
-    while (p_scale * bound > 65000.0) p_scale *= 0.5;
-    const double inv = 1.0 / 16384.0;
+    /* a I + b A + c A A = c (A + beta I)^2 + gamma I; without the square, b A + a I. X is held times 2^14, S times
+     * 2^12 (|A| < 4 and |beta| <= 4), Q times what its largest value over singular values below 2 allows. */
+    const double a = ns->a, b = ns->b, c = ns->c, xs = 16384.0, ss = 4096.0;
+    const double beta = c != 0.0 ? b / (2.0 * c) : 0.0, gamma = c != 0.0 ? a - b * b / (4.0 * c) : a;
+    double most = fmax(fabs(a), fabs(a + 4.0 * b + 16.0 * c));
+    if (beta < 0.0) most = fmax(most, fabs(gamma));         /* the polynomial's value at its vertex */
+    double qs = 16384.0;
+    while (qs * most > 60000.0) qs *= 0.5;
 
     orth_product_t q = *last;
     q.batch = batch;
+    q.sums = ws + o->sums;
     q.status = dev->scratch + SM100_SCRATCH_ORTH_STATUS;
     q.wait_ns = (unsigned long long)dev->gemm_wait_ms * 1000000ull;
     for (int i = 0; i < ns->steps; i++) {
-        const int from = i & 1, to = from ^ 1;
+        const int from = i & 1, to = from ^ 1, end = i == ns->steps - 1;
         q.rows = q.cols = (int)o->s;
-        q.pitch = o->a_pitch; q.plane = o->a_pitch * o->s;
-        q.mode = ORTH_GRAM; q.K = (int)o->l;
-        q.alpha = (float)inv; q.beta = 0.0f;
-        q.in_hi = q.in_lo = 0;
-        q.out_hi = ws + o->a_hi; q.out_lo = two_planes ? ws + o->a_lo : 0;
-        if ((rc = orth_launch(dev, &x[from], &x[from], &q, two_planes)) != SM100_OK) return rc;
-        q.mode = ORTH_POLY; q.K = (int)o->s;
-        q.alpha = (float)(ns->c * p_scale * inv * inv); q.beta = (float)(ns->b * p_scale * inv);
-        q.in_hi = q.out_hi; q.in_lo = q.out_lo;
-        q.out_hi = ws + o->p_hi; q.out_lo = two_planes ? ws + o->p_lo : 0;
-        if ((rc = orth_launch(dev, &a, &a, &q, two_planes)) != SM100_OK) return rc;
-        const int end = i == ns->steps - 1;
-        q.mode = end ? ORTH_RESULT : ORTH_UPDATE;
+        q.mode = ORTH_GRAM; q.K = (int)o->l; q.lo = two_planes;
+        if (c == 0.0) {
+            q.alpha = (float)(b * qs / (xs * xs)); q.diag = (float)(a * qs);
+            if ((rc = orth_launch(dev, &x[from], &x[from], &qm, &q, two_planes)) != SM100_OK) return rc;
+        } else {
+            q.alpha = (float)(ss / (xs * xs)); q.diag = (float)(beta * ss);
+            if ((rc = orth_launch(dev, &x[from], &x[from], &sm, &q, two_planes)) != SM100_OK) return rc;
+            q.mode = ORTH_POLY; q.K = (int)o->s;
+            q.alpha = (float)(c * qs / (ss * ss)); q.diag = (float)(gamma * qs);
+            if ((rc = orth_launch(dev, &sm, &sm, &qm, &q, two_planes)) != SM100_OK) return rc;
+        }
+        q.mode = end ? ORTH_RESULT : ORTH_UPDATE; q.K = (int)o->s; q.lo = 1;
         q.cols = (int)o->l;
-        q.pitch = o->x_pitch; q.plane = plane;
-        q.alpha = (float)((end ? factor * inv : 1.0) / p_scale); q.beta = (float)(end ? factor * inv * ns->a : ns->a);
-        q.in_hi = ws + o->x_hi[from]; q.in_lo = ws + o->x_lo[from];
-        q.out_hi = ws + o->x_hi[to]; q.out_lo = ws + o->x_lo[to];
-        if ((rc = orth_launch(dev, &p, &x[from], &q, two_planes)) != SM100_OK) return rc;
+        q.alpha = (float)(end ? factor / (qs * xs) : 1.0 / qs); q.diag = 0.0f;
+        if ((rc = orth_launch(dev, &qm, &x[from], &x[to], &q, two_planes)) != SM100_OK) return rc;
     }
     return SM100_OK;
 }
@@ -343,7 +388,8 @@ static const booth_newton_schulz_t ns_default = { 5, 3.4445f, -4.7750f, 2.0315f,
 
 static int ns_ok(const booth_newton_schulz_t *ns)
 {
-    return ns->steps >= 1 && ns->steps <= 64 && isfinite(ns->a) && isfinite(ns->b) && isfinite(ns->c) && isfinite(ns->eps) && ns->eps > 0.0f;
+    return ns->steps >= 1 && ns->steps <= 64 && isfinite(ns->a) && isfinite(ns->b) && isfinite(ns->c) && isfinite(ns->eps) && ns->eps > 0.0f &&
+           (ns->c == 0.0f || fabsf(ns->b) <= 8.0f * fabsf(ns->c));
 }
 
 /* batch matrices: the pitch no shorter than a row, the last element within 2^59 elements of the first. */
@@ -368,8 +414,8 @@ int booth_sm100_orthogonalise(sm100_dev_t *dev, sm100_ptr_t out, sm100_ptr_t in,
     orth_layout_t o;
     if (!ns) ns = &ns_default;
     if (type_index(dtype) < 0) return bad_arg(dev, "booth_sm100_orthogonalise: the type is f32, bf16 or f16");
-    if (!ns_ok(ns)) return bad_arg(dev, "booth_sm100_orthogonalise: need 1 to 64 steps, finite coefficients and eps > 0");
-    if (!orth_layout(&o, batch, rows, cols, dtype != SM100_BF16) || !matrices_ok(in, dtype, batch, rows, cols, ld_in, stride_in) ||
+    if (!ns_ok(ns)) return bad_arg(dev, "booth_sm100_orthogonalise: need 1 to 64 steps, finite coefficients with c = 0 or |b| <= 8 |c|, and eps > 0");
+    if (!orth_layout(dev, &o, batch, rows, cols, dtype != SM100_BF16) || !matrices_ok(in, dtype, batch, rows, cols, ld_in, stride_in) ||
         !matrices_ok(out, dtype, batch, rows, cols, ld_out, stride_out) || (in == out && (ld_in != ld_out || (batch > 1 && stride_in != stride_out))))
         return bad_arg(dev, "booth_sm100_orthogonalise: need 1 to 65535 matrices of 1 to 2^20 rows and columns, operands non-NULL and aligned to "
                             "their element, pitches >= cols, strides >= cols (equal ones when out is in)");
@@ -380,6 +426,7 @@ int booth_sm100_orthogonalise(sm100_dev_t *dev, sm100_ptr_t out, sm100_ptr_t in,
     src.g = in; src.ld_g = ld_in; src.stride_g = stride_in; src.type_g = type_index(dtype);
     src.rows = rows; src.cols = cols;
     src.vec = four_ok(in, dtype, batch, cols, ld_in, stride_in);
+    src.flat = ld_in == cols;
     orth_product_t last;
     memset(&last, 0, sizeof last);
     last.w = out; last.ld_w = ld_out; last.stride_w = stride_out; last.type_w = type_index(dtype);
@@ -397,11 +444,11 @@ int booth_sm100_muon_step(sm100_dev_t *dev, sm100_ptr_t w, sm100_ptr_t m, sm100_
     if (!ns) ns = &ns_default;
     if (!p || type_index(p->wdtype) < 0 || type_index(p->mdtype) < 0 || type_index(p->gdtype) < 0)
         return bad_arg(dev, "booth_sm100_muon_step: the types are f32, bf16 or f16");
-    if (!ns_ok(ns)) return bad_arg(dev, "booth_sm100_muon_step: need 1 to 64 steps, finite coefficients and eps > 0");
+    if (!ns_ok(ns)) return bad_arg(dev, "booth_sm100_muon_step: need 1 to 64 steps, finite coefficients with c = 0 or |b| <= 8 |c|, and eps > 0");
     if (!isfinite(p->lr) || !isfinite(p->scale) || !isfinite(p->weight_decay) || !(p->momentum >= 0.0f && p->momentum <= 1.0f))
         return bad_arg(dev, "booth_sm100_muon_step: need a finite learning rate, scale and weight decay, and momentum in [0, 1]");
     const int two_planes = p->wdtype != SM100_BF16;
-    if (!orth_layout(&o, batch, rows, cols, two_planes) || !matrices_ok(w, p->wdtype, batch, rows, cols, p->ld_w, p->stride_w) ||
+    if (!orth_layout(dev, &o, batch, rows, cols, two_planes) || !matrices_ok(w, p->wdtype, batch, rows, cols, p->ld_w, p->stride_w) ||
         !matrices_ok(m, p->mdtype, batch, rows, cols, p->ld_m, p->stride_m) || !matrices_ok(g, p->gdtype, batch, rows, cols, p->ld_g, p->stride_g) ||
         w == m || w == g || m == g)
         return bad_arg(dev, "booth_sm100_muon_step: need 1 to 65535 matrices of 1 to 2^20 rows and columns; w, m and g non-NULL, apart from one "
@@ -415,6 +462,7 @@ int booth_sm100_muon_step(sm100_dev_t *dev, sm100_ptr_t w, sm100_ptr_t m, sm100_
     src.rows = rows; src.cols = cols;
     src.nesterov = p->nesterov != 0; src.mu = p->momentum;
     src.vec = four_ok(g, p->gdtype, batch, cols, p->ld_g, p->stride_g) && four_ok(m, p->mdtype, batch, cols, p->ld_m, p->stride_m);
+    src.flat = p->ld_g == cols && p->ld_m == cols;
     orth_product_t last;
     memset(&last, 0, sizeof last);
     last.w = w; last.ld_w = p->ld_w; last.stride_w = p->stride_w; last.type_w = type_index(p->wdtype);

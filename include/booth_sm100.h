@@ -307,7 +307,8 @@ size_t booth_sm100_layernorm_backward_workspace(sm100_dev_t *dev, long long rows
  *   A = X X^t,  X = a X + (b A + c A A) X,  from X = G / (|G|_F + eps)
  * (for a matrix with more rows than columns X is its transpose, the result is the same
  * polynomial). NULL where one is expected means five steps of the Muon optimiser's
- * quintic, 3.4445, -4.7750, 2.0315, and eps = 1e-7. 1 to 64 steps; eps > 0. The
+ * quintic, 3.4445, -4.7750, 2.0315, and eps = 1e-7. 1 to 64 steps; eps > 0; c = 0 or
+ * |b| <= 8 |c| (the square is completed: b / 2c must be of the size of the rest). The
  * coefficients must keep the singular values below 2, as every scheme that converges
  * from [0, 1] does (the operands are fp16, scaled for that range): beyond, results are not finite. */
 typedef struct booth_newton_schulz {

@@ -1,13 +1,15 @@
 """Newton-Schulz orthogonalisation and the Muon update against the iteration in 64 bits.
 
-Tolerance. With r the relative rounding of an operand (2^-11 for one fp16 plane, 2^-21 for two: hi + lo, and lo.lo
+Tolerance. A step is computed as S = X Xt + beta I, Q = c S S + gamma I, X' = Q X (beta = b / 2c, gamma = a - b^2 / 4c; with
+c = 0, Q = b A + a I). With r the relative rounding of an operand (2^-11 for one fp16 plane, 2^-21 for two: hi + lo, and lo.lo
 left out of the products) and t the error of a product's sum relative to the product of the operands' magnitudes (the tensor
 core drops what lies below the last bit of its sum, 2^-23 an add; one plane: an add per 16 of K; two planes: 24 adds
-a chunk of 128, and one fp32 add, 2^-24, per chunk), one step X' = a X + P X, P = b A + c A A, A = X Xt makes, to first order
-in Frobenius norms (|.|_F, |.|_2 and |.| the element-wise magnitude),
-    dA = 2 r |X|_2 |X|_F + t | |X||Xt| |_F + r |A|_F
-    dP = (|b| + 2 |c| |A|_2) dA + |c| (2 r |A|_2 |A|_F + t | |A||A| |_F) + r |P|_F
-    dX' = |X|_2 dP + r |P|_2 |X|_F + t | |P||X| |_F + 2^-21 |X'|_F           (X is stored in two planes in both cases)
+a chunk of 128, and one fp32 add, 2^-24, per chunk), it makes, to first order in Frobenius norms (|.|_F, |.|_2 and |.| the
+element-wise magnitude),
+    dS  = 2 r |X|_2 |X|_F + t | |X||Xt| |_F + r |S|_F
+    dQ  = |c| (2 |S|_2 dS + r |S|_2 |S|_F + t | |S||S| |_F) + r |Q|_F
+    dX' = |X|_2 dQ + 2 r |Q|_2 |X|_F + t | |Q||X| |_F + 2^-21 |X'|_F
+(X is stored in two planes in both cases; one plane leaves out Q X_lo outside the diagonal blocks, whose norm is at most 2 |Q|_2)
 and later steps carry it on with the Lipschitz constant of x -> a x + b x^3 + c x^5, taken on singular value pairs from
 [0, s]: max over [0, s] of |f'(x)| and |f(x) / x|. The sum of these, with a tenth for second order, and half a step of the
 result's type on every element is the bound. The norms come from the 64-bit iteration itself."""
@@ -46,13 +48,20 @@ def iterate64(g, t, steps=5, abc=ABC, eps=1e-7):
         A = x @ x.mT
         P = b * A + c * A @ A
         y = a * x + P @ x
-        X2, P2 = sv.amax(1), (b * sv ** 2 + c * sv ** 4).abs().amax(1)
-        A2 = X2 ** 2
+        s0, X2 = sv, sv.amax(1)
         sv = (a * sv + b * sv ** 3 + c * sv ** 5).abs()
         k, l = x.shape[1], x.shape[2]
-        dA = 2 * r * X2 * fro(x) + adds(l) * fro(x.abs() @ x.abs().mT) + r * fro(A)
-        dP = (abs(b) + 2 * abs(c) * A2) * dA + abs(c) * (2 * r * A2 * fro(A) + adds(k) * fro(A.abs() @ A.abs())) + r * fro(P)
-        local = X2 * dP + r * P2 * fro(x) + adds(k) * fro(P.abs() @ x.abs()) + 2.0 ** -21 * fro(y)
+        eye = torch.eye(k, dtype=x.dtype, device=x.device)
+        S = A + (b / (2 * c) if c else 0.0) * eye
+        Q = P + a * eye
+        S2 = (s0 ** 2 + (b / (2 * c) if c else 0.0)).abs().amax(1)
+        Q2 = (a + b * s0 ** 2 + c * s0 ** 4).abs().amax(1)
+        dS = 2 * r * X2 * fro(x) + adds(l) * fro(x.abs() @ x.abs().mT) + r * fro(S)
+        if c:
+            dQ = abs(c) * (2 * S2 * dS + r * S2 * fro(S) + adds(k) * fro(S.abs() @ S.abs())) + r * fro(Q)
+        else:
+            dQ = abs(b) * dS + r * fro(Q)
+        local = X2 * dQ + 2 * r * Q2 * fro(x) + adds(k) * fro(Q.abs() @ x.abs()) + 2.0 ** -21 * fro(y)
         grid = torch.linspace(1e-4, 1, 200, dtype=torch.float64, device=x.device)[None] * X2[:, None]
         lip = torch.maximum((a + 3 * b * grid ** 2 + 5 * c * grid ** 4).abs(), (a + b * grid ** 2 + c * grid ** 4).abs()).amax(1)
         err = lip * err + local
@@ -166,9 +175,12 @@ def test_identity_follows_the_scalar_iteration(dev, sm, t):
         x = 1 / n ** 0.5
         for _ in range(5):
             x = ABC[0] * x + ABC[1] * x ** 3 + ABC[2] * x ** 5
-        got = run(dev, sm, (7.0 * torch.eye(n, device="cuda"))[None].to(TYPES[t]))[0].double()
-        assert bool((got - torch.diag(got.diagonal()) == 0).all())
-        assert bool(((got.diagonal() - x).abs() < (5e-6 if t == "f32" else 1e-2) * x).all())
+        g = (7.0 * torch.eye(n, device="cuda"))[None].to(TYPES[t])
+        got = run(dev, sm, g)
+        assert bool((got[0] - torch.diag(got[0].diagonal()) == 0).all())
+        want, err = iterate64(g, g.dtype)
+        assert bool(((want[0].diagonal() - x).abs() < 1e-5).all())          # 64 bits, but the coefficients as fp32 and eps
+        check(got, want, err)
 
 
 @pytest.mark.gpu

@@ -104,7 +104,7 @@ go(3, 1000, 500, sm.F32, 1)
 d.sync(); d.close()
 """)
     assert res.returncode == 0, res.stderr
-    assert [l["kernel"] for l in L] == ["orth_norm", "orth_split"] + ["orth_product_1_pair"] * 6 + ["orth_norm", "orth_split"] + ["orth_product_2_single"] * 3
+    assert [l["kernel"] for l in L] == ["orth_norm", "orth_split"] + ["orth_product_1_pair"] * 6 + ["orth_norm", "orth_split"] + ["orth_product_2_pair"] * 3
     assert all(l["overlap"] == 1 for l in L)
     assert all(l["shmem"] == 230400 and l["block"] == (384, 1, 1) for l in L if l["kernel"].startswith("orth_product"))
     P = products(lines)
@@ -112,14 +112,28 @@ d.sync(); d.close()
         (0, 4096, 4096, 4096, 1, 0), (1, 4096, 4096, 4096, 1, 0), (2, 4096, 4096, 4096, 1, 0),
         (0, 4096, 4096, 4096, 1, 0), (1, 4096, 4096, 4096, 1, 0), (3, 4096, 4096, 4096, 1, 0),
         (0, 500, 500, 1000, 3, 1), (1, 500, 500, 500, 3, 1), (3, 500, 1000, 500, 3, 1)]
-    # X and A are kept times 2^14, P times 2^10 with the default coefficients
-    want = [(2.0 ** -14, 0), (2.0315 * 2.0 ** -18, -4.7750 * 2.0 ** -4), (2.0 ** -10, 3.4445), (2.0 ** -24, 3.4445 * 2.0 ** -14)]
+    # X is kept times 2^14, S = A + b / 2c times 2^12, Q = c S S + (a - b^2 / 4c) times 2^11 with the default coefficients
+    a, b, c = 3.4445, -4.7750, 2.0315
+    want = [(2.0 ** -16, b / (2 * c) * 2 ** 12), (c * 2.0 ** -13, (a - b * b / (4 * c)) * 2 ** 11), (2.0 ** -11, 0), (2.0 ** -25, 0)]
     for p, k in zip(P, (0, 1, 2, 0, 1, 3, 0, 1, 3)):
-        assert (p["alpha"], p["beta"]) == pytest.approx(want[k], rel=1e-6)
+        assert (p["alpha"], p["diag"]) == pytest.approx(want[k], rel=1e-6)
     maps = [ln for ln in lines if ln.startswith("tensormap3")]
     # one plane: hi and lo of both copies of X, A and P; rows a multiple of 64 apart
     assert maps[:6] == ["tensormap3 dims 4096 4096 1 strides 8192 33554432 box 64 64 1"] * 6
     assert maps[6:] == ["tensormap3 dims 1000 500 3 strides 2048 1024000 box 64 64 1"] * 4 + ["tensormap3 dims 500 500 3 strides 1024 512000 box 64 64 1"] * 4
+
+
+def test_cubic_has_no_polynomial_product(fake3, tmp_path):
+    res, L, lines = run(fake3, tmp_path, """
+d = sm.Device(0); p = 1 << 20
+n = d.orthogonalise_workspace(1, 64, 64)
+d.orthogonalise(p, 2 * p, 1, 64, 64, 4 * p, n, steps=2, abc=(1.5, -0.5, 0.0))
+d.sync(); d.close()
+""")
+    assert res.returncode == 0, res.stderr
+    P = products(lines)
+    assert [p["mode"] for p in P] == [0, 2, 0, 3]
+    assert [P[0]["alpha"], P[0]["diag"], P[1]["alpha"]] == pytest.approx([-0.5 * 2.0 ** -15, 1.5 * 2 ** 13, 2.0 ** -13])
 
 
 def test_muon_parameters(fake3, tmp_path):
@@ -131,7 +145,7 @@ d.sync(); d.close()
 """)
     assert res.returncode == 0, res.stderr
     last = products(lines)[-1]
-    assert last["mode"] == 3 and last["keep"] == pytest.approx(0.95) and last["alpha"] == pytest.approx(-0.4 * 2.0 ** -24) and last["beta"] == pytest.approx(-0.4 * 3.4445 * 2.0 ** -14)
+    assert last["mode"] == 3 and last["keep"] == pytest.approx(0.95) and last["alpha"] == pytest.approx(-0.4 * 2.0 ** -25)
 
 
 def test_a_wait_that_ran_out_is_reported_once(fake3, tmp_path):
@@ -162,7 +176,7 @@ d.sync(); d.close()
     "d.orthogonalise(p, 2 * p, 65536, 8, 8, p, big)", "d.orthogonalise(p, 2 * p, 1, 8, 8, 0, big)", "d.orthogonalise(p, 2 * p, 1, 8, 8, p + 64, big)",
     "d.orthogonalise(p, 2 * p, 1, 8, 8, p, d.orthogonalise_workspace(1, 8, 8) - 1)", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, steps=0)",
     "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, steps=65)", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, eps=0.0)",
-    "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, abc=(1.0, float('nan'), 0.0))", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, abc=(float('inf'), 1.0, 0.0))",
+    "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, abc=(1.0, float('nan'), 0.0))", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, abc=(1.0, 1.0, 0.1))", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, abc=(float('inf'), 1.0, 0.0))",
     "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, ld_in=7)", "d.orthogonalise(p, 2 * p, 1, 8, 8, p, big, ld_out=7)",
     "d.orthogonalise(p, 2 * p, 2, 8, 8, p, big, stride_in=7)", "d.orthogonalise(p, 2 * p, 2, 8, 8, p, big, stride_out=-64)",
     "d.orthogonalise(p, p, 1, 8, 8, p, big, ld_out=9)", "d.orthogonalise(p, p, 2, 8, 8, p, big, stride_out=65)", "d.orthogonalise(p + 2, 2 * p, 1, 8, 8, p, big)",
