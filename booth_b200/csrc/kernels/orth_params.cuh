@@ -36,14 +36,14 @@ typedef struct orth_product {
     int mode, rows, cols, K, batch;                     /* of the product: rows x cols, square for GRAM and POLY */
     float alpha, diag;                                  /* out = alpha * accumulator, + diag where row = column */
     int tri;                                            /* tile side of the stored triangle of the symmetric operand */
-    int split;                                          /* parts of K, one CTA pair of a cluster each */
+    int split;                                          /* parts of K, one CTA (pair) of a cluster each */
     int lo;                                             /* whether out has a lo plane */
     /* RESULT: element (r, c) of matrix k at k * stride_w + r * ld_w + c; transposed when tall */
     int type_w, tall, vec_w;
     float keep;                                         /* 0: w is not read */
     ORTH_PTR(void) w;
     long long ld_w, stride_w;
-    ORTH_PTR(float) sums;                               /* where the parts of a tile meet: 32,768 floats a CTA */
+    ORTH_PTR(float) sums;                               /* where the parts of a tile meet */
     ORTH_PTR(int) status;
     unsigned long long wait_ns;
 } orth_product_t;

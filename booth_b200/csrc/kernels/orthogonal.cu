@@ -36,9 +36,10 @@
 // keeps one CTA or CTA pair per SM (pair) and walks over the tiles of all matrices of
 // the batch; the roles inside are those of the fp32 GEMM: warp 0 TMA, warp 1 MMA, warps 4-11
 // drain tensor memory, apply the epilogue and store, planes by TMA from shared memory.
-//   pair:   256 x 256 tile per two CTAs, tcgen05.mma.cta_group::2; few tiles: the K of
-//           a tile shared by up to four pairs of a cluster
-//   single: 128 x 128 tile per CTA
+//   256: 256 x 256 tile per two CTAs, tcgen05.mma.cta_group::2
+//   128: 128 x 128 tile per CTA
+//   64:  64 x 64 tile per CTA, for products so small that they are all latency
+// With few tiles the K of a tile is shared by up to four pairs or eight CTAs of a cluster.
 #include "common.cuh"
 #include "orth_params.cuh"
 #include <cuda.h>
@@ -232,15 +233,18 @@ orth_split(const __grid_constant__ orth::Source s, const double *__restrict__ pa
 
 namespace orth {
 
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z)
+// The completion is counted on `bar`, for a pair on the leader's barrier. One elected lane issues.
+template <bool PAIR>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z)
 {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
-}
-__device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z)
-{
-    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                     "@e cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                     "@e cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
 // fp16 x fp16 -> fp32; bits 15 and 16: the first or second operand's tile has its rows (columns), not K, contiguous.
@@ -248,24 +252,31 @@ __device__ __forceinline__ uint32_t instr_desc(int m, int n, bool a_t, bool b_t)
 {
     return (1u << 4) | ((uint32_t)a_t << 15) | ((uint32_t)b_t << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// A tile of two 64 x 64 boxes, 128 bytes a box row, 128-byte swizzle, 8 rows 1024 bytes. K
+// Shared-memory descriptor of an operand: 64 x 64 boxes, 128 bytes a box row, 128-byte swizzle, 8 rows 1024 bytes. K
 // contiguous (`t` false): rows of the operand, the boxes one below the other. Else rows of K, each with 64
-// rows of the operand; the next 64 lie 8192 bytes on.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, bool t)
+// rows of the operand; the next 64 lie 8192 bytes on. The address is the low word's low half, so a tile further on
+// is a 32-bit addition; the high word never changes.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, bool t) { return ((addr & 0x3FFFFu) >> 4) | (t ? (8192u >> 4) << 16 : 0u); }
+__device__ __forceinline__ uint64_t desc(uint32_t lo)
 {
-    return gemm::smem_desc(addr) | (t ? (uint64_t)(8192u >> 4) << 16 : 0ull);
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "n"((1024u >> 4) | (1u << 14) | (2u << 29)));
+    return d;
 }
-// Sixteen of K further: 32 bytes along a row, or sixteen rows.
-__device__ __forceinline__ uint64_t k_advance(int kk, bool t) { return (uint64_t)(kk * (t ? 2048 >> 4 : 32 >> 4)); }
 
+// The control warps run their loops with all lanes in step, so that addresses and descriptors stay in uniform
+// registers; one elected lane issues. (In a branch of a single lane every descriptor went through general
+// registers, and the issuer took 650 clocks for the four one-plane products of a K block, which take 512.)
 template <bool PAIR>
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
     if constexpr (PAIR)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+                     "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                      ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+                     "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                      ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *v)
@@ -279,13 +290,27 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *v)
                    "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]),
                    "r"(taddr) : "memory");
 }
-// Arrives on the barrier at this offset, for a pair in both of its CTAs (cluster ranks first, first + 1).
+// Arrives on the barrier at this offset, for a pair in both of its CTAs (cluster ranks first, first + 1), once the
+// products issued so far are complete.
 template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar, uint32_t first)
 {
     if constexpr (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                     "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
                      ::"r"(bar), "h"((uint16_t)(3u << first)) : "memory");
-    else gemm::umma_commit(bar);
+    else
+        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                     "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
+                 ::"r"(bar), "r"(bytes) : "memory");
+}
+// Bounded wait of a whole warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const WaitCtl &w, int code)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, w, code));
 }
 
 // Tile number -> matrix, tile row and tile column. Tiles that run at the same time should share
@@ -333,33 +358,42 @@ __device__ __forceinline__ void tma_store(const CUtensorMap *map, uint32_t src, 
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-// Two warps hold 64 rows x 64 columns, a row a lane: one plane of them goes through 8 KB of
-// shared memory, in the 128-byte-swizzled form of the tensor map's box, and out by TMA, which clips at
-// the matrix's edges. `packed`: this lane's 64 halves. Barrier `bar` joins the two warps; thread `issuer` of them issues.
-__device__ __forceinline__ void store_plane(const CUtensorMap *map, uint32_t buf, const uint32_t (&packed)[32], int r, int bar, bool issuer, int x, int y, int z)
+// Results go out by TMA in boxes of 64 x 64 of a plane, which clips them at the matrix's edges: a lane puts its
+// packed halves of row r, from 16-byte unit u0 on, into the box in the map's 128-byte swizzle.
+template <int N>
+__device__ __forceinline__ void put_box(uint32_t box, const uint32_t (&packed)[N], int r, int u0)
 {
-    if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the buffer's last content has left
-    asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
 #pragma unroll
-    for (int u = 0; u < 8; u++)
-        sts(buf + (uint32_t)(r * 128 + ((u ^ r) & 7) * 16), make_uint4(packed[4 * u], packed[4 * u + 1], packed[4 * u + 2], packed[4 * u + 3]));
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
-    if (issuer) tma_store(map, buf, x, y, z);
+    for (int u = 0; u < N / 4; u++)
+        sts(box + (uint32_t)(r * 128 + (((u0 + u) ^ r) & 7) * 16), make_uint4(packed[4 * u], packed[4 * u + 1], packed[4 * u + 2], packed[4 * u + 3]));
 }
-
-// Whether both warps of barrier `bar` say so.
-__device__ __forceinline__ bool both_ok(int bar, bool ok)
+template <int THREADS> __device__ __forceinline__ void team_sync(int bar) { asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(THREADS) : "memory"); }
+// Whether all warps of the team say so.
+template <int THREADS> __device__ __forceinline__ bool all_ok(int bar, bool ok)
 {
     uint32_t all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(all) : "r"((uint32_t)ok), "r"(bar) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((uint32_t)ok), "r"(bar), "n"(THREADS) : "memory");
     return all != 0;
 }
 
-// One warp's 32 rows x 32 columns of the result, a row a lane, into the caller's matrix. Through 4 KB of the
+// Brings the weights a warp's rows will read into L2 while the products run.
+__device__ __forceinline__ void prefetch_result(const Product &p, int lane, int k, int row0, int col0, int cols)
+{
+    const int bytes = p.type_w == ORTH_F32 ? 4 : 2;
+    const char *const w = static_cast<const char *>(p.w) + k * p.stride_w * bytes;
+    if (p.tall) {       // a column of the tile is a run of 32 elements of the caller's row
+        for (int c = lane; c < cols && col0 + c < p.cols; c += 32)
+            if (row0 < p.rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(w + ((col0 + c) * p.ld_w + row0) * bytes));
+    } else if (row0 + lane < p.rows) {
+        for (int c = 0; c < cols && col0 + c < p.cols; c += 128 / bytes)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(w + ((row0 + lane) * p.ld_w + col0 + c) * bytes));
+    }
+}
+
+// One warp's 32 columns of rows row0 .. rows_end (32 at most), a row a lane, into the caller's matrix. Through 4 KB of the
 // warp's own shared memory, so that accesses run along the rows; loads ahead of stores.
-__device__ __forceinline__ void store_result(const Product &p, const float (&v)[32], uint32_t buf, int lane, int k, int row0, int col0)
+__device__ __forceinline__ void store_result(const Product &p, const float (&v)[32], uint32_t buf, int lane, int k, int row0, int rows_end, int col0)
 {
     const int row = row0 + lane;
     if (p.tall) {
@@ -369,10 +403,10 @@ __device__ __forceinline__ void store_result(const Product &p, const float (&v)[
             const long long o = k * p.stride_w + (long long)(col0 + j0) * p.ld_w + row;
             float w[16];
 #pragma unroll
-            for (int j = 0; j < 16; j++) w[j] = p.keep != 0.f && row < p.rows && col0 + j0 + j < p.cols ? load1(p.w, p.type_w, o + j * p.ld_w) : 0.f;
+            for (int j = 0; j < 16; j++) w[j] = p.keep != 0.f && row < rows_end && col0 + j0 + j < p.cols ? load1(p.w, p.type_w, o + j * p.ld_w) : 0.f;
 #pragma unroll
             for (int j = 0; j < 16; j++)
-                if (row < p.rows && col0 + j0 + j < p.cols) store1(p.w, p.type_w, o + j * p.ld_w, fmaf(p.keep, w[j], v[j0 + j]));
+                if (row < rows_end && col0 + j0 + j < p.cols) store1(p.w, p.type_w, o + j * p.ld_w, fmaf(p.keep, w[j], v[j0 + j]));
         }
         return;
     }
@@ -388,11 +422,11 @@ __device__ __forceinline__ void store_result(const Product &p, const float (&v)[
 #pragma unroll
         for (int q = 0; q < 8; q++) {
             w[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (p.keep != 0.f && row0 + r0 + 4 * q < p.rows && c < p.cols) w[q] = load4(p.w, p.type_w, o + 4 * q * p.ld_w);
+            if (p.keep != 0.f && row0 + r0 + 4 * q < rows_end && c < p.cols) w[q] = load4(p.w, p.type_w, o + 4 * q * p.ld_w);
         }
 #pragma unroll
         for (int q = 0; q < 8; q++)
-            if (row0 + r0 + 4 * q < p.rows && c < p.cols) {
+            if (row0 + r0 + 4 * q < rows_end && c < p.cols) {
                 const int r = r0 + 4 * q;
                 const uint4 x = lds(buf + (uint32_t)(r * 128 + ((u ^ r) & 7) * 16));
                 store4(p.w, p.type_w, o + 4 * q * p.ld_w, make_float4(fmaf(p.keep, w[q].x, __uint_as_float(x.x)), fmaf(p.keep, w[q].y, __uint_as_float(x.y)),
@@ -406,51 +440,42 @@ __device__ __forceinline__ void store_result(const Product &p, const float (&v)[
             const long long o = k * p.stride_w + (row0 + q0) * p.ld_w + c;
             float w[16];
 #pragma unroll
-            for (int q = 0; q < 16; q++) w[q] = p.keep != 0.f && row0 + q0 + q < p.rows && c < p.cols ? load1(p.w, p.type_w, o + q * p.ld_w) : 0.f;
+            for (int q = 0; q < 16; q++) w[q] = p.keep != 0.f && row0 + q0 + q < rows_end && c < p.cols ? load1(p.w, p.type_w, o + q * p.ld_w) : 0.f;
 #pragma unroll
             for (int q = 0; q < 16; q++) {
                 const int r = q0 + q;
                 float x;
                 asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buf + (uint32_t)(r * 128 + (((lane >> 2) ^ r) & 7) * 16 + (lane & 3) * 4)) : "memory");
-                if (row0 + r < p.rows && c < p.cols) store1(p.w, p.type_w, o + q * p.ld_w, fmaf(p.keep, w[q], x));
+                if (row0 + r < rows_end && c < p.cols) store1(p.w, p.type_w, o + q * p.ld_w, fmaf(p.keep, w[q], x));
             }
         }
     }
     __syncwarp();
 }
 
-// The K blocks of one tile, in the order they are multiplied, for the part of K a pair has. One plane, Q X: first
-// the blocks on the tile's diagonal with the lo plane of X. Two planes: the chunk ends, where the
-// accumulator is drained. All roles walk this list.
+constexpr uint32_t OPERAND_BYTES = 196608;          // operand stages; behind them 32 KB in which results are staged
+
+// Two planes: where the accumulator is drained, every other K block and every one on the tile's diagonal.
 __device__ __forceinline__ bool chunk_ends(int kb, int diag0, int diag, bool sym)
 {
     return (kb & 1) || (sym && kb >= diag0 && kb < diag0 + diag);
 }
-struct Blocks {
-    int kb0, kb1, d0, n_lo, n;
-    __device__ __forceinline__ Blocks(int kb0_, int kb1_, int diag0, int diag1, bool lo) : kb0(kb0_), kb1(kb1_), d0(max(diag0, kb0_))
-    {
-        n_lo = lo ? max(0, min(diag1, kb1) - d0) : 0;
-        n = n_lo + kb1 - kb0;
-    }
-    __device__ __forceinline__ bool lo(int t) const { return t < n_lo; }
-    __device__ __forceinline__ int at(int t) const { return t < n_lo ? d0 + t : kb0 + t - n_lo; }
-};
 
-// 384 threads; grid: any number of CTAs (pairs), each takes every grid-th tile. PAIR with p.split > 1: a
-// cluster of that many pairs shares one tile, each takes a range of K, and the sums meet in the
+// 384 threads; grid: any number of CTAs (pairs), each takes every grid-th tile. p.split > 1: a
+// cluster of that many CTAs (pairs) shares one tile, each takes a range of K, and the sums meet in the
 // workspace, 64 columns of the tile with each owner; the grid is then one cluster a tile. Few tiles
 // leave most of the GPU idle: the 10 tiles of a 1000 x 1000 symmetric product with K = 2049 took 33 us
 // on 36 single CTAs. (Through distributed shared memory instead of L2 the meeting alone took 10 us.)
-template <int PLANES, bool PAIR>
+template <int PLANES, int SIDE>
 __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorMap &a_lo, const CUtensorMap &b_hi, const CUtensorMap &b_lo,
                                         const CUtensorMap &o_hi, const CUtensorMap &o_lo, const Product &p)
 {
     using namespace gemm;
-    constexpr int BK = 64, SIDE = PAIR ? 256 : 128;                 // K block; tile side
-    constexpr uint32_t TILE = 128 * BK * 2;                         // one operand plane of one CTA: 16 KB
+    constexpr bool PAIR = SIDE == 256;
+    constexpr int BK = 64, ROWS = SIDE == 64 ? 64 : 128;            // K block; rows of an operand that one CTA holds
+    constexpr uint32_t TILE = ROWS * BK * 2;                        // one operand plane of one CTA
     constexpr uint32_t STAGE = 2 * PLANES * TILE;
-    constexpr int STAGES = 6 / PLANES;
+    constexpr int STAGES = OPERAND_BYTES / STAGE;
     constexpr int HALF = SIDE / 2;                                  // columns per epilogue warp
     constexpr uint32_t TMEM_COLS = 2 * SIDE;                        // two accumulators
     const WaitCtl status = { p.status, p.wait_ns };
@@ -459,14 +484,15 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     __shared__ __align__(8) uint64_t bars[2 * STAGES + 4];
     __shared__ uint32_t s_tmem;
 
-    const uint32_t cta = PAIR ? cluster_ctarank() : 0, rank = cta & 1u, first = cta & ~1u;      // first: the pair's leader
+    constexpr int CTAS = PAIR ? 2 : 1;
+    const uint32_t cta = cluster_ctarank(), rank = PAIR ? cta & 1u : 0u, first = cta - rank;    // first: the pair's leader
     const bool leader = rank == 0;
-    const int split = PAIR ? p.split : 1, part = PAIR ? (int)(cta >> 1) : 0;
+    const int split = p.split, part = (int)cta / CTAS;
     const uint32_t smem0 = (smem_u32(smem_orth) + 1023u) & ~1023u;
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]);
     const uint32_t acc_full0 = smem_u32(&bars[2 * STAGES]), acc_empty0 = smem_u32(&bars[2 * STAGES + 2]);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int C = (int)(PAIR ? gridDim.x / (2u * split) : gridDim.x), cl = (int)(PAIR ? blockIdx.x / (2u * split) : blockIdx.x);
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int C = (int)(gridDim.x / (unsigned)(CTAS * split)), cl = (int)(blockIdx.x / (unsigned)(CTAS * split));
     const Tiles tiles(p, SIDE);
     const int items = tiles.each * p.batch;
     // K blocks of this pair: [kb0, kb1), an even number but for the last
@@ -474,12 +500,16 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     const int kb0 = 2 * (all_ck * part / split), kb1 = min(all_kb, 2 * (all_ck * (part + 1) / split));
     // Which operand blocks come transposed. X as the second operand of Q X has its columns contiguous. Of a
     // symmetric operand the block at K block kb is above the stored triangle when kb's tile lies beyond the tile
-    // of the rows. (A pair whose triangle was stored in 128-tiles takes the rule of its upper half: for the
-    // lower half that differs only inside its own diagonal tile, which is stored whole.)
+    // of the rows. (Rows that span two of the triangle's tiles take the rule of the upper one: for the
+    // lower one that differs only inside its own diagonal tile, which is stored whole.)
     const bool a_sym = p.mode != ORTH_GRAM, b_sym = p.mode == ORTH_POLY, b_cols = p.mode >= ORTH_UPDATE;
-    const bool lo_blocks = PLANES == 1 && b_cols;
-    const int tri_shift = p.tri == 256 ? 8 : 7;
-    constexpr int DIAG = SIDE / BK;                                 // K blocks on a tile's diagonal
+    const int tri_kb = p.tri / BK;
+    // first K block that comes transposed, of rows that begin at tile index x of SIDE
+    const auto turn = [&](int x, bool sym) { return sym ? (x * (SIDE / BK) / tri_kb + 1) * tri_kb : 0x7fffffff; };
+    // One plane, Q X: ahead of the K blocks, those on the tile's diagonal with the lo plane of X.
+    constexpr int DIAG = SIDE / BK;
+    const auto lo_from = [&](int x) { return max(x * DIAG, kb0); };
+    const auto lo_count = [&](int x) { return PLANES == 1 && b_cols ? max(0, min(x * DIAG + DIAG, kb1) - lo_from(x)) : 0; };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
@@ -515,119 +545,116 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     if (warp < 4) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
       if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
+        {
+            uint32_t st = smem0, full = full0, empty = empty0, ph = 1;      // stage and its barriers
             bool ok = true;
             for (int item = cl; ok && item < items; item += C) {
                 int k, i, j;
                 tiles.at(item, k, i, j);
                 const int m0 = i * SIDE + (int)rank * 128, n0 = j * SIDE + (int)rank * 128;
-                const int ti = (i * SIDE) >> tri_shift, tj = (j * SIDE) >> tri_shift;
-                const Blocks blocks(kb0, kb1, i * DIAG, i * DIAG + DIAG, lo_blocks);
-                for (int t = 0; t < blocks.n; t++, it++) {
-                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
-                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1u, status, 1)) { ok = false; break; }
-                    const uint32_t st = smem0 + s * STAGE;
-                    uint32_t bar = full0 + 8 * s;
-                    if (leader) mbar_expect_tx(bar, (PAIR ? 2 : 1) * STAGE);
-                    if constexpr (PAIR) bar = map_to_cta(bar, first);
-                    const int kb = blocks.at(t), tk = (kb * BK) >> tri_shift;
-                    const CUtensorMap *const b1 = blocks.lo(t) ? &b_lo : &b_hi;
-                    const bool a_t = a_sym && tk > ti, b_t = b_cols || (b_sym && tk > tj);
+                const int a_turn = turn(i, a_sym), b_turn = b_cols ? 0 : turn(j, b_sym);
+                int lo = lo_count(i);
+                for (int kb = lo ? lo_from(i) : kb0; kb < kb1;) {
+                    if (!warp_wait(empty, ph, status, 1)) { ok = false; break; }
+                    if (leader) expect_tx(full, CTAS * STAGE);
+                    const uint32_t bar = PAIR ? map_to_cta(full, first) : full;
+                    const CUtensorMap *const b1 = lo ? &b_lo : &b_hi;
+                    const bool a_t = kb >= a_turn, b_t = kb >= b_turn;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {                   // 64 rows of an operand at a time
-                        const uint32_t d = st + (uint32_t)h * (TILE / 2);
+                    for (int h = 0; h < ROWS / 64; h++) {           // 64 rows of an operand at a time
+                        const uint32_t d = st + (uint32_t)h * 8192u;
                         const int ax = a_t ? m0 + 64 * h : kb * BK, ay = a_t ? kb * BK : m0 + 64 * h;
                         const int bx = b_t ? n0 + 64 * h : kb * BK, by = b_t ? kb * BK : n0 + 64 * h;
-                        if constexpr (PAIR) {
-                            tma_3d_pair(d, &a_hi, bar, ax, ay, k);
-                            tma_3d_pair(d + PLANES * TILE, b1, bar, bx, by, k);
-                            if constexpr (PLANES == 2) {
-                                tma_3d_pair(d + TILE, &a_lo, bar, ax, ay, k);
-                                tma_3d_pair(d + 3 * TILE, &b_lo, bar, bx, by, k);
-                            }
-                        } else {
-                            tma_3d(d, &a_hi, bar, ax, ay, k);
-                            tma_3d(d + PLANES * TILE, b1, bar, bx, by, k);
-                            if constexpr (PLANES == 2) {
-                                tma_3d(d + TILE, &a_lo, bar, ax, ay, k);
-                                tma_3d(d + 3 * TILE, &b_lo, bar, bx, by, k);
-                            }
+                        load_box<PAIR>(d, &a_hi, bar, ax, ay, k);
+                        load_box<PAIR>(d + PLANES * TILE, b1, bar, bx, by, k);
+                        if constexpr (PLANES == 2) {
+                            load_box<PAIR>(d + TILE, &a_lo, bar, ax, ay, k);
+                            load_box<PAIR>(d + 3 * TILE, &b_lo, bar, bx, by, k);
                         }
                     }
+                    st += STAGE; full += 8; empty += 8;
+                    if (full == full0 + 8 * STAGES) { st = smem0; full = full0; empty = empty0; ph ^= 1u; }
+                    kb = lo && --lo == 0 ? kb0 : kb + 1;
                 }
             }
         }
         __syncwarp();
       } else if (warp == 1) {
-        if (leader && lane == 0) {
-            uint32_t it = 0, g = 0;
+        if (leader) {
+            uint32_t s_lo = desc_lo(smem0, false), full = full0, empty = empty0, ph = 0;
+            uint32_t g = 0, buf = 0;
             bool ok = true;
             for (int item = cl; ok && item < items; item += C) {
                 int k, i, j;
                 tiles.at(item, k, i, j);
-                const int ti = (i * SIDE) >> tri_shift, tj = (j * SIDE) >> tri_shift;
-                const Blocks blocks(kb0, kb1, i * DIAG, i * DIAG + DIAG, lo_blocks);
-                uint32_t acc = 0, buf = 0;
-                for (int t = 0; t < blocks.n; t++, it++) {
-                    const int kb = blocks.at(t), tk = (kb * BK) >> tri_shift;
+                const int a_turn = turn(i, a_sym), b_turn = b_cols ? 0 : turn(j, b_sym);
+                int lo = lo_count(i);
+                uint32_t acc = 0;
+                for (int kb = lo ? lo_from(i) : kb0; kb < kb1;) {
                     if (acc == 0) {                                 // a chunk begins
                         buf = g & 1u;
-                        ok = mbar_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1u) ^ 1u, status, 4);
+                        ok = warp_wait(acc_empty0 + 8 * buf, ((g >> 1) & 1u) ^ 1u, status, 4);
                         if (!ok) break;
                         g++;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     }
                     const uint32_t tacc = tmem + buf * (uint32_t)SIDE;
-                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1u;
-                    ok = mbar_wait(full0 + 8 * s, ph, status, 2);
+                    ok = warp_wait(full, ph, status, 2);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t st = smem0 + s * STAGE;
-                    const bool a_t = a_sym && tk > ti, b_t = b_cols || (b_sym && tk > tj);
-                    const uint32_t idesc = instr_desc(SIDE, SIDE, a_t, b_t), bt = st + PLANES * TILE;
-                    const uint64_t ah = tile_desc(st, a_t), al = tile_desc(st + TILE, a_t), bh = tile_desc(bt, b_t), bl = tile_desc(bt + TILE, b_t);
+                    const bool a_t = kb >= a_turn, b_t = kb >= b_turn;
+                    const uint32_t idesc = instr_desc(SIDE, SIDE, a_t, b_t);
+                    const uint32_t at = a_t ? (8192u >> 4) << 16 : 0u, bt = b_t ? (8192u >> 4) << 16 : 0u;
+                    const uint32_t ah = s_lo | at, bh = (s_lo + (PLANES * TILE >> 4)) | bt;
+                    // sixteen of K further: 32 bytes along a row, or sixteen rows
+                    const uint32_t ak = a_t ? 2048 >> 4 : 32 >> 4, bk = b_t ? 2048 >> 4 : 32 >> 4;
                     // two planes: the small products first. The tensor core truncates what it adds to a sum
                     // to the sum's last bit, so adds to a sum that is still small cost less.
                     if constexpr (PLANES == 2) {
+                        const uint32_t al = ah + (TILE >> 4), bl = bh + (TILE >> 4);
 #pragma unroll
                         for (int kk = 0; kk < BK / 16; kk++) {
-                            umma<PAIR>(tacc, al + k_advance(kk, a_t), bh + k_advance(kk, b_t), idesc, acc);
-                            umma<PAIR>(tacc, ah + k_advance(kk, a_t), bl + k_advance(kk, b_t), idesc, 1u);
+                            umma<PAIR>(tacc, desc(al + kk * ak), desc(bh + kk * bk), idesc, acc);
+                            umma<PAIR>(tacc, desc(ah + kk * ak), desc(bl + kk * bk), idesc, 1u);
                             acc = 1;
                         }
                     }
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; kk++) {
-                        umma<PAIR>(tacc, ah + k_advance(kk, a_t), bh + k_advance(kk, b_t), idesc, acc);
+                        umma<PAIR>(tacc, desc(ah + kk * ak), desc(bh + kk * bk), idesc, acc);
                         acc = 1;
                     }
-                    commit<PAIR>(empty0 + 8 * s, first);
-                    if (t + 1 == blocks.n || (PLANES == 2 && chunk_ends(kb, i * DIAG, DIAG, a_sym))) {
+                    commit<PAIR>(empty, first);
+                    const int next = lo && --lo == 0 ? kb0 : kb + 1;
+                    if (next == kb1 || (PLANES == 2 && chunk_ends(kb, i * DIAG, DIAG, a_sym))) {
                         commit<PAIR>(acc_full0 + 8 * buf, first);
                         acc = 0;
                     }
+                    kb = next;
+                    s_lo += STAGE >> 4; full += 8; empty += 8;
+                    if (full == full0 + 8 * STAGES) { s_lo = desc_lo(smem0, false); full = full0; empty = empty0; ph ^= 1u; }
                 }
             }
         }
         __syncwarp();
       }
-      if (PAIR && split > 1) cluster_sync_all();                    // the meeting of the epilogue warps
+      if (split > 1) cluster_sync_all();                            // the meeting of the epilogue warps
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int e = warp - 4, q = warp & 3, h = e >> 2;
         const uint32_t acc_empty = PAIR ? map_to_cta(acc_empty0, first) : acc_empty0;
-        const uint32_t staging = smem0 + STAGES * STAGE;
-        // two warps (q even and odd) store planes together
-        const uint32_t pair_buf = staging + (uint32_t)(h * 2 + (q >> 1)) * 8192u;
-        const int pair_bar = 1 + h * 2 + (q >> 1), pair_row = (q & 1) * 32 + lane;
-        const bool issuer = pair_row == 0;
+        const uint32_t staging = smem0 + OPERAND_BYTES;
+        // the warps that store a box of 64 x 64 together: two (q even and odd), each with 32 rows and all columns; with
+        // 64-tiles all eight, each with 16 rows (the lower half of its lanes) and half the columns
+        constexpr int TEAM = SIDE == 64 ? 256 : 64;
+        const int team = SIDE == 64 ? 0 : h * 2 + (q >> 1), team_row = SIDE == 64 ? q * 16 + lane : (q & 1) * 32 + lane;
+        const bool issuer = SIDE == 64 ? e == 0 && lane == 0 : team_row == 0;
         uint32_t g = 0;
         bool ok = true;
         for (int item = cl; ok && item < items; item += C) {
             int k, i, j;
             tiles.at(item, k, i, j);
-            const int row0 = i * SIDE + (int)rank * 128 + q * 32, col0 = j * SIDE + h * HALF;
+            const int row0 = i * SIDE + (int)rank * 128 + q * (SIDE == 64 ? 16 : 32), col0 = j * SIDE + h * HALF;
+            if (p.mode == ORTH_RESULT && p.keep != 0.f) prefetch_result(p, lane, k, row0, col0, HALF);
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * HALF);
             uint32_t buf = g & 1u;
             if constexpr (PLANES == 1) {
@@ -667,12 +694,15 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     }
                 }
             }
-            // where this warp's sums of 64 columns lie when parts meet: [part][CTA][warp][piece][unit of 4 columns][lane]
-            const size_t sums_at = (((size_t)cl * split * 2 + rank) * 8 + e) * 4096 + lane * 4, part_step = 2 * 8 * 4096;
-            if (PAIR && split > 1) {
+            // where this warp's sums lie when parts meet: [part][CTA][warp][4 columns][lane][4]
+            constexpr size_t WARP_SUMS = 32 * HALF, part_step = (size_t)CTAS * 8 * WARP_SUMS;
+            const size_t sums_at = (((size_t)cl * split * CTAS + rank) * 8 + e) * WARP_SUMS + lane * 4;
+            constexpr int PIECE = SIDE == 64 ? 32 : 64, PIECES = HALF / PIECE;         // columns that have one owner
+            const int piece0 = SIDE == 64 ? 0 : h * PIECES;
+            if (split > 1) {
 #pragma unroll 1
                 for (int cc = 0; ok && cc < HALF / 32; cc++) {
-                    if ((2 * h + (cc >> 1)) % split == part) continue;
+                    if ((piece0 + cc * 32 / PIECE) % split == part) continue;
                     uint32_t r[32];
                     tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 32), r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -684,37 +714,38 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                 }
                 cluster_sync_all();
             }
-            // the two warps of a store go on only if both may
-            ok = both_ok(pair_bar, ok);
+            // the warps of a store go on only if all of them may
+            ok = all_ok<TEAM>(1 + team, ok);
+            // behind the last tile the operand stages are free: every box has its own place there and none waits for another
+            const bool roomy = item + C >= items;
 #pragma unroll 1
-            for (int cc = 0; ok && cc < HALF / 64; cc++) {
-                if (split > 1 && (2 * h + cc) % split != part) continue;
-                const int col = col0 + cc * 64;
-                // both warps of a store agree: the upper one's rows decide
-                if (row0 - (q & 1) * 32 >= p.rows || col >= p.cols) break;
-                uint32_t hi[32], lo[32];
+            for (int cc = 0; ok && cc < PIECES; cc++) {
+                if (split > 1 && (piece0 + cc) % split != part) continue;
+                const int col = col0 + cc * PIECE;
+                // all warps of a store agree: its first row and column decide
+                if (row0 - (SIDE == 64 ? q * 16 : (q & 1) * 32) >= p.rows || (SIDE == 64 ? j * SIDE : col) >= p.cols) break;
+                uint32_t hi[PIECE / 2], lo[PIECE / 2];
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
+                for (int half = 0; half < PIECE / 32; half++) {
                     uint32_t r[32];
-                    tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 64 + half * 32), r);
+                    tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * PIECE + half * 32), r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     float v[32];
 #pragma unroll
                     for (int c = 0; c < 32; c++) v[c] = __uint_as_float(r[c]);
-                    if (PAIR)
-                        for (int from = 0; from < split; from++) {
-                            if (from == part) continue;
-                            const float *const at = p.sums + sums_at + from * part_step + (cc * 2 + half) * 1024;
+                    for (int from = 0; from < split; from++) {
+                        if (from == part) continue;
+                        const float *const at = p.sums + sums_at + from * part_step + (cc * PIECE + half * 32) * 32;
 #pragma unroll
-                            for (int u = 0; u < 8; u++) {
-                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(at + u * 128));
-                                v[4 * u] += x.x; v[4 * u + 1] += x.y; v[4 * u + 2] += x.z; v[4 * u + 3] += x.w;
-                            }
+                        for (int u = 0; u < 8; u++) {
+                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(at + u * 128));
+                            v[4 * u] += x.x; v[4 * u + 1] += x.y; v[4 * u + 2] += x.z; v[4 * u + 3] += x.w;
                         }
+                    }
 #pragma unroll
                     for (int c = 0; c < 32; c++) v[c] *= p.alpha;
                     if (p.mode == ORTH_RESULT) {
-                        store_result(p, v, staging + (uint32_t)e * 4096u, lane, k, row0, col + half * 32);
+                        store_result(p, v, staging + (uint32_t)e * 4096u, lane, k, row0, SIDE == 64 ? min(p.rows, row0 + 16) : p.rows, col + half * 32);
                         continue;
                     }
                     if (tiles.sym && i == j) {
@@ -724,15 +755,40 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
                         const __half2 x = __floats2half2_rn(v[2 * c], v[2 * c + 1]);
-                        const float2 f = __half22float2(x);
-                        const __half2 y = __floats2half2_rn(v[2 * c] - f.x, v[2 * c + 1] - f.y);
                         hi[half * 16 + c] = *reinterpret_cast<const uint32_t *>(&x);
-                        lo[half * 16 + c] = *reinterpret_cast<const uint32_t *>(&y);
+                    }
+                    if (p.lo) {
+#pragma unroll
+                        for (int c = 0; c < 16; c++) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[half * 16 + c]));
+                            const __half2 y = __floats2half2_rn(v[2 * c] - f.x, v[2 * c + 1] - f.y);
+                            lo[half * 16 + c] = *reinterpret_cast<const uint32_t *>(&y);
+                        }
                     }
                 }
                 if (p.mode != ORTH_RESULT) {
-                    store_plane(&o_hi, pair_buf, hi, pair_row, pair_bar, issuer, col, row0, k);
-                    if (p.lo) store_plane(&o_lo, pair_buf, lo, pair_row, pair_bar, issuer, col, row0, k);
+                    const uint32_t box = roomy ? smem0 + (uint32_t)(team * PIECES + cc) * 16384u : staging + (uint32_t)team * (SIDE == 64 ? 16384u : 8192u);
+                    const bool apart = roomy || SIDE == 64;         // hi and lo have a place each
+                    const int u0 = SIDE == 64 ? h * 4 : 0;
+                    if (issuer && !roomy) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the last content has left
+                    if (!roomy) team_sync<TEAM>(1 + team);
+                    if (SIDE != 64 || lane < 16) put_box(box, hi, team_row, u0);
+                    if (apart && p.lo && (SIDE != 64 || lane < 16)) put_box(box + 8192u, lo, team_row, u0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    team_sync<TEAM>(1 + team);
+                    const int x = SIDE == 64 ? j * SIDE : col;
+                    if (issuer) {
+                        tma_store(&o_hi, box, x, row0, k);
+                        if (apart && p.lo) tma_store(&o_lo, box + 8192u, x, row0, k);
+                    }
+                    if (!apart && p.lo) {
+                        if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        team_sync<TEAM>(1 + team);
+                        put_box(box, lo, team_row, u0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        team_sync<TEAM>(1 + team);
+                        if (issuer) tma_store(&o_lo, box, x, row0, k);
+                    }
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -755,14 +811,16 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
 
 }  // namespace orth
 
-// the pair forms are launched in clusters of 2 x split CTAs
-#define ORTH_PRODUCT(name, PLANES, PAIR)                                                                                             \
+// launched in clusters of split CTAs, the 256 forms of 2 x split
+#define ORTH_PRODUCT(name, PLANES, SIDE)                                                                                             \
     extern "C" __global__ void __launch_bounds__(384, 1)                                                                             \
     name(const __grid_constant__ CUtensorMap a_hi, const __grid_constant__ CUtensorMap a_lo, const __grid_constant__ CUtensorMap b_hi, \
          const __grid_constant__ CUtensorMap b_lo, const __grid_constant__ CUtensorMap o_hi, const __grid_constant__ CUtensorMap o_lo, \
          const __grid_constant__ orth::Product p)                                                                                    \
-    { orth::product<PLANES, PAIR>(a_hi, a_lo, b_hi, b_lo, o_hi, o_lo, p); }
-ORTH_PRODUCT(orth_product_1_single, 1, false)
-ORTH_PRODUCT(orth_product_2_single, 2, false)
-ORTH_PRODUCT(orth_product_1_pair, 1, true)
-ORTH_PRODUCT(orth_product_2_pair, 2, true)
+    { orth::product<PLANES, SIDE>(a_hi, a_lo, b_hi, b_lo, o_hi, o_lo, p); }
+ORTH_PRODUCT(orth_product_1_64, 1, 64)
+ORTH_PRODUCT(orth_product_2_64, 2, 64)
+ORTH_PRODUCT(orth_product_1_128, 1, 128)
+ORTH_PRODUCT(orth_product_2_128, 2, 128)
+ORTH_PRODUCT(orth_product_1_256, 1, 256)
+ORTH_PRODUCT(orth_product_2_256, 2, 256)

@@ -83,9 +83,9 @@ enum {
     /* layer normalisation: five pairs of types, six forms each; per element type (f32, bf16, f16) the column sums */
     SM100_K_LN_FWD, SM100_K_LN_BWD = SM100_K_LN_FWD + 5 * SM100_LN_FORMS,
     SM100_K_LN_COLUMNS = SM100_K_LN_BWD + 5 * SM100_LN_FORMS, SM100_K_LN_PARAM_GRAD = SM100_K_LN_COLUMNS + 3,
-    /* orthogonalisation: the products by form (single, pair) and planes (1, 2) */
+    /* orthogonalisation: the products by tile side (64, 128, 256) and planes (1, 2) */
     SM100_K_ORTH_NORM = SM100_K_LN_PARAM_GRAD + 3, SM100_K_ORTH_SPLIT, SM100_K_ORTH_PRODUCT,
-    SM100_K_COUNT = SM100_K_ORTH_PRODUCT + 4
+    SM100_K_COUNT = SM100_K_ORTH_PRODUCT + 6
 };
 
 struct sm100_dev {
@@ -119,7 +119,7 @@ struct sm100_dev {
     unsigned    gemm_wait_ms;          /* limit of the GEMM kernel's barrier waits */
     int         orth_pending;          /* an orthogonalisation was enqueued since the last status check */
     int         orth_captured;         /* one was captured into a graph: its replays are not seen here */
-    int         orth_clusters[5];      /* clusters of 2 x split CTAs the GPU holds at once, by split (0 = not asked yet) */
+    int         orth_clusters[9];      /* clusters of so many product CTAs the GPU holds at once (0 = not asked yet) */
     int         orth_smem_set;         /* dynamic shared memory limit raised on the product kernels */
     unsigned    gemm_epoch;            /* tag of the latest persistent GEMM call (never zero once used) */
     int         gemm_clusters;         /* CTA pairs of the persistent GEMM kernel this GPU holds at once (0 = not asked yet) */

@@ -157,7 +157,7 @@ static const char *const k_names[SM100_K_COUNT] = {
     LN_FORM_NAMES("layernorm_bwd_f16"), LN_FORM_NAMES("layernorm_bwd_f16_f32"),
     "layernorm_bwd_columns_f32", "layernorm_bwd_columns_bf16", "layernorm_bwd_columns_f16",
     "layernorm_param_grad_f32", "layernorm_param_grad_bf16", "layernorm_param_grad_f16",
-    "orth_norm", "orth_split", "orth_product_1_single", "orth_product_2_single", "orth_product_1_pair", "orth_product_2_pair",
+    "orth_norm", "orth_split", "orth_product_1_64", "orth_product_2_64", "orth_product_1_128", "orth_product_2_128", "orth_product_1_256", "orth_product_2_256",
 };
 
 int sm100_rt_device_count(void)

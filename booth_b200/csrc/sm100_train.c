@@ -196,12 +196,17 @@ static int orth_layout(const sm100_dev_t *dev, orth_layout_t *o, int batch, int 
     o->s_lo = at; if (two_planes) at += a;
     o->q_hi = at; at += a;
     o->q_lo = at; if (two_planes) at += a;
-    /* K is shared only while all parts of all tiles run at once, so no more CTAs than SMs meet */
-    const long long pairs = batch * ((o->l + 255) / 256) * ((o->s + 255) / 256), ctas = 2 * 4 * pairs < dev->sm_count ? 2 * 4 * pairs : dev->sm_count;
-    o->sums = at; at += (size_t)ctas * 131072;
+    /* sums of shared tiles: 32, 64 or 128 KB a CTA by tile side, eight parts a tile at most (four pairs), all at once on the GPU */
+    size_t sums = 0;
+    for (int side = 64; side <= 256; side *= 2) {
+        const long long ctas = 8ll * batch * ((o->l + side - 1) / side) * ((o->s + side - 1) / side);
+        const size_t need = (size_t)(ctas < dev->sm_count ? ctas : dev->sm_count) * (side == 64 ? 32768u : side == 128 ? 65536u : 131072u);
+        if (need > sums) sums = need;
+    }
+    o->sums = at; at += sums;
     o->bytes = at;
-    const long long t = (o->l + 127) / 128;
-    return t * ((o->s + 127) / 128) <= INT_MAX / batch;
+    const long long t = (o->l + 63) / 64;
+    return t * ((o->s + 63) / 64) <= INT_MAX / batch;
 }
 
 size_t booth_sm100_orthogonalise_workspace(sm100_dev_t *dev, int batch, int rows, int cols, int dtype)
@@ -230,76 +235,79 @@ static int plane_map(sm100_dev_t *dev, CUtensorMap *map, CUdeviceptr p, long lon
 /* cuTensorMapEncodeTiled wants its maps on 64-byte boundaries. */
 typedef struct { CUtensorMap hi __attribute__((aligned(64))), lo __attribute__((aligned(64))); } plane_maps_t;
 
-/* How many clusters of 2 x split CTAs of the product kernels the GPU holds at once
- * (asked of the driver once; else SM pairs, less one in seven for clusters that have
+/* How many clusters of `ctas` CTAs of the product kernels the GPU holds at once (asked of
+ * the driver once; else what the SMs hold, less one in seven for clusters that have
  * to fit inside a group of SMs). Only a measure for the choice below: no cluster waits for another. */
-static int orth_clusters(sm100_dev_t *dev, int split)
+static int orth_clusters(sm100_dev_t *dev, int ctas)
 {
-    if (dev->orth_clusters[split]) return dev->orth_clusters[split];
-    int n = dev->sm_count / (2 * split);
-    if (split > 1) n = n * 6 / 7;
+    if (dev->orth_clusters[ctas]) return dev->orth_clusters[ctas];
+    int n = dev->sm_count / ctas;
+    if (ctas > 2) n = n * 6 / 7;
     if (dev->api->OccupancyMaxActiveClusters) {
         CUlaunchAttribute attr;
         memset(&attr, 0, sizeof attr);
         attr.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
-        attr.value.clusterDim.x = 2u * (unsigned)split; attr.value.clusterDim.y = 1; attr.value.clusterDim.z = 1;
+        attr.value.clusterDim.x = (unsigned)ctas; attr.value.clusterDim.y = 1; attr.value.clusterDim.z = 1;
         CUlaunchConfig cfg;
         memset(&cfg, 0, sizeof cfg);
-        cfg.gridDimX = 2u * (unsigned)split * 64u; cfg.gridDimY = 1; cfg.gridDimZ = 1;
+        cfg.gridDimX = (unsigned)ctas * 64u; cfg.gridDimY = 1; cfg.gridDimZ = 1;
         cfg.blockDimX = 384; cfg.blockDimY = 1; cfg.blockDimZ = 1;
         cfg.sharedMemBytes = ORTH_SMEM;
         cfg.hStream = dev->stream;
         cfg.attrs = &attr; cfg.numAttrs = 1;
         int got = 0;
-        if (dev->api->OccupancyMaxActiveClusters(&got, dev->k[SM100_K_ORTH_PRODUCT + 2], &cfg) == CUDA_SUCCESS && got > 0) n = got;
+        if (dev->api->OccupancyMaxActiveClusters(&got, dev->k[SM100_K_ORTH_PRODUCT + 4], &cfg) == CUDA_SUCCESS && got > 0) n = got;
     }
-    dev->orth_clusters[split] = n > 0 ? n : 1;
-    return dev->orth_clusters[split];
+    dev->orth_clusters[ctas] = n > 0 ? n : 1;
+    return dev->orth_clusters[ctas];
 }
 
-/* Form of a product: pairs of CTAs on 256 x 256 tiles, the K of a tile shared by up to
- * four pairs, or single CTAs on 128 x 128 tiles; the one with the shortest estimate in
- * tensor clocks. A K block of 64 takes a pair 512 clocks a plane product (one or three). A
- * single CTA needs 256 of them, but its narrow tile reads shared memory faster than it
- * delivers: 512 and 1250 measured. Beside that a wave costs its epilogue, some 3000
- * clocks (2000 for the smaller tile), and meeting in the workspace some 3000. */
-static void orth_plan(sm100_dev_t *dev, const orth_product_t *p, int two_planes, int *pairs, int *split)
+typedef struct { int side, split; long long tiles; } orth_plan_t;
+
+/* Tile side of a product and the parts its K is cut into: the shortest estimate in clocks.
+ * A K block of 64 takes a pair 512 clocks of the tensor pipe a plane product (one, or
+ * three); the smaller tiles read shared memory faster than it delivers, measured 512
+ * and 1250 for 128, 250 and 500 for 64. A wave's epilogue costs some 3000, 2000 and 1000, and
+ * parts that meet 3000. K is shared only while everything runs at once. Rows
+ * may span two tiles of the stored triangle, not more (see the kernel). */
+static orth_plan_t orth_plan(sm100_dev_t *dev, const orth_product_t *p, int two_planes)
 {
+    static const double block[3][2] = { { 250, 500 }, { 512, 1250 }, { 512, 1536 } }, wave[3] = { 1000, 2000, 3000 };
     const int sym = p->mode <= ORTH_POLY;
-    const long long pm = (p->rows + 255) / 256, pn = (p->cols + 255) / 256, sm = (p->rows + 127) / 128, sn = (p->cols + 127) / 128;
-    const long long pt = p->batch * (sym ? pm * (pm + 1) / 2 : pm * pn), st = p->batch * (sym ? sm * (sm + 1) / 2 : sm * sn);
     const long long kb = (p->K + 63) / 64, chunks = (kb + 1) / 2;
-    double best = (double)((st + dev->sm_count - 1) / dev->sm_count) * (2000.0 + kb * (two_planes ? 1250.0 : 512.0));
-    *pairs = 0; *split = 1;
-    for (int s = 1; s <= 4 && s <= chunks; s++) {
-        const long long slots = orth_clusters(dev, s), waves = (pt + slots - 1) / slots;
-        if (s > 1 && (waves > 1 || 2 * s * pt > dev->sm_count)) break;
-        const double cost = (double)waves * (3000.0 / s + (s > 1 ? 3000.0 : 0.0) + 2.0 * ((chunks + s - 1) / s) * (two_planes ? 1536.0 : 512.0));
-        if (cost < best) { best = cost; *pairs = 1; *split = s; }
+    orth_plan_t best = { 0, 1, 0 };
+    double least = 0.0;
+    for (int f = 0; f < 3; f++) {
+        const int side = 64 << f, ctas = side == 256 ? 2 : 1;
+        if (p->mode != ORTH_GRAM && side > 2 * p->tri) break;
+        const long long m = (p->rows + side - 1) / side, n = (p->cols + side - 1) / side, tiles = p->batch * (sym ? m * (m + 1) / 2 : m * n);
+        for (int s = 1; s * ctas <= 8 && s <= chunks; s++) {
+            const long long slots = orth_clusters(dev, s * ctas), waves = (tiles + slots - 1) / slots;
+            if (s > 1 && (waves > 1 || s * ctas * tiles > dev->sm_count)) break;
+            const double cost = (double)waves * (wave[f] + (s > 1 ? 3000.0 : 0.0) + 2.0 * ((chunks + s - 1) / s) * block[f][two_planes]);
+            if (!best.side || cost < least) { least = cost; best.side = side; best.split = s; best.tiles = tiles; }
+        }
     }
+    return best;
 }
 
 static int orth_launch(sm100_dev_t *dev, const plane_maps_t *a, const plane_maps_t *b, const plane_maps_t *out, orth_product_t *p, int two_planes)
 {
-    int pairs, split;
-    orth_plan(dev, p, two_planes, &pairs, &split);
-    const int sym = p->mode <= ORTH_POLY;
-    const long long side = pairs ? 256 : 128, tm = (p->rows + side - 1) / side, tn = (p->cols + side - 1) / side;
-    const long long tiles = p->batch * (sym ? tm * (tm + 1) / 2 : tm * tn), slots = pairs ? orth_clusters(dev, 1) : dev->sm_count;
-    /* a split tile's cluster takes that one tile: the parts meet a fixed number of times */
-    const long long groups = split > 1 || tiles < slots ? tiles : slots;
-    p->split = split;
+    const orth_plan_t plan = orth_plan(dev, p, two_planes);
+    const int ctas = (plan.side == 256 ? 2 : 1) * plan.split, form = plan.side == 64 ? 0 : plan.side == 128 ? 2 : 4;
+    /* a shared tile's cluster takes that one tile: the parts meet a fixed number of times */
+    const long long slots = orth_clusters(dev, ctas), groups = plan.split > 1 || plan.tiles < slots ? plan.tiles : slots;
+    p->split = plan.split;
     void *args[] = { (void *)&a->hi, (void *)&a->lo, (void *)&b->hi, (void *)&b->lo, (void *)&out->hi, (void *)&out->lo, p };
-    const int rc = sm100_launch_k_cluster(dev, SM100_K_ORTH_PRODUCT + (pairs ? 2 : 0) + (two_planes ? 1 : 0), (unsigned)(groups * (pairs ? 2 * split : 1)),
-                                          pairs ? 2u * (unsigned)split : 1u, 384, ORTH_SMEM, args);
-    if (sym) p->tri = (int)side;        /* how the product that reads this one finds its triangle */
+    const int rc = sm100_launch_k_cluster(dev, SM100_K_ORTH_PRODUCT + form + (two_planes ? 1 : 0), (unsigned)(groups * ctas), (unsigned)ctas, 384, ORTH_SMEM, args);
+    if (p->mode <= ORTH_POLY) p->tri = plan.side;       /* how the product that reads this one finds its triangle */
     return rc;
 }
 
 static int orth_status_ready(sm100_dev_t *dev)
 {
     if (!dev->orth_smem_set) {
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < 6; i++) {
             CUresult cr = dev->api->FuncSetAttribute(dev->k[SM100_K_ORTH_PRODUCT + i], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)ORTH_SMEM);
             if (cr != CUDA_SUCCESS) return sm100_fail(dev, "raising the product kernels' shared memory limit", cr);
         }
