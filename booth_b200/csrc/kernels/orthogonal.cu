@@ -271,12 +271,12 @@ template <bool PAIR>
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
     if constexpr (PAIR)
-        asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-                     "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                      ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-                     "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                      ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *v)
@@ -295,12 +295,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *v)
 template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar, uint32_t first)
 {
     if constexpr (PAIR)
-        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                     "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                      ::"r"(bar), "h"((uint16_t)(3u << first)) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                     "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
+    else gemm::umma_commit(bar);
+}
+__device__ __forceinline__ bool elected()
+{
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
 }
 __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes)
 {
@@ -609,26 +612,25 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     const uint32_t ak = a_t ? 2048 >> 4 : 32 >> 4, bk = b_t ? 2048 >> 4 : 32 >> 4;
                     // two planes: the small products first. The tensor core truncates what it adds to a sum
                     // to the sum's last bit, so adds to a sum that is still small cost less.
-                    if constexpr (PLANES == 2) {
-                        const uint32_t al = ah + (TILE >> 4), bl = bh + (TILE >> 4);
-#pragma unroll
-                        for (int kk = 0; kk < BK / 16; kk++) {
-                            umma<PAIR>(tacc, desc(al + kk * ak), desc(bh + kk * bk), idesc, acc);
-                            umma<PAIR>(tacc, desc(ah + kk * ak), desc(bl + kk * bk), idesc, 1u);
-                            acc = 1;
-                        }
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < BK / 16; kk++) {
-                        umma<PAIR>(tacc, desc(ah + kk * ak), desc(bh + kk * bk), idesc, acc);
-                        acc = 1;
-                    }
-                    commit<PAIR>(empty, first);
+                    const uint32_t al = ah + (TILE >> 4), bl = bh + (TILE >> 4);
                     const int next = lo && --lo == 0 ? kb0 : kb + 1;
-                    if (next == kb1 || (PLANES == 2 && chunk_ends(kb, i * DIAG, DIAG, a_sym))) {
-                        commit<PAIR>(acc_full0 + 8 * buf, first);
-                        acc = 0;
+                    const bool ends = next == kb1 || (PLANES == 2 && chunk_ends(kb, i * DIAG, DIAG, a_sym));
+                    if (elected()) {
+                        if constexpr (PLANES == 2) {
+#pragma unroll
+                            for (int kk = 0; kk < BK / 16; kk++) {
+                                umma<PAIR>(tacc, desc(al + kk * ak), desc(bh + kk * bk), idesc, kk ? 1u : acc);
+                                umma<PAIR>(tacc, desc(ah + kk * ak), desc(bl + kk * bk), idesc, 1u);
+                            }
+                        }
+#pragma unroll
+                        for (int kk = 0; kk < BK / 16; kk++)
+                            umma<PAIR>(tacc, desc(ah + kk * ak), desc(bh + kk * bk), idesc, PLANES == 2 || kk ? 1u : acc);
+                        commit<PAIR>(empty, first);
+                        if (ends) commit<PAIR>(acc_full0 + 8 * buf, first);
                     }
+                    __syncwarp();
+                    acc = ends ? 0u : 1u;
                     kb = next;
                     s_lo += STAGE >> 4; full += 8; empty += 8;
                     if (full == full0 + 8 * STAGES) { s_lo = desc_lo(smem0, false); full = full0; empty = empty0; ph ^= 1u; }
