@@ -394,9 +394,9 @@ __device__ __forceinline__ void prefetch_result(const Product &p, int lane, int 
     }
 }
 
-// One warp's 32 columns of rows row0 .. rows_end (32 at most), a row a lane, into the caller's matrix. Through 4 KB of the
+// One warp's 32 rows x 32 columns of the result, a row a lane, into the caller's matrix. Through 4 KB of the
 // warp's own shared memory, so that accesses run along the rows; loads ahead of stores.
-__device__ __forceinline__ void store_result(const Product &p, const float (&v)[32], uint32_t buf, int lane, int k, int row0, int rows_end, int col0)
+__device__ __forceinline__ void store_result(const Product &p, const float (&v)[32], uint32_t buf, int lane, int k, int row0, int col0)
 {
     const int row = row0 + lane;
     if (p.tall) {
@@ -406,10 +406,10 @@ __device__ __forceinline__ void store_result(const Product &p, const float (&v)[
             const long long o = k * p.stride_w + (long long)(col0 + j0) * p.ld_w + row;
             float w[16];
 #pragma unroll
-            for (int j = 0; j < 16; j++) w[j] = p.keep != 0.f && row < rows_end && col0 + j0 + j < p.cols ? load1(p.w, p.type_w, o + j * p.ld_w) : 0.f;
+            for (int j = 0; j < 16; j++) w[j] = p.keep != 0.f && row < p.rows && col0 + j0 + j < p.cols ? load1(p.w, p.type_w, o + j * p.ld_w) : 0.f;
 #pragma unroll
             for (int j = 0; j < 16; j++)
-                if (row < rows_end && col0 + j0 + j < p.cols) store1(p.w, p.type_w, o + j * p.ld_w, fmaf(p.keep, w[j], v[j0 + j]));
+                if (row < p.rows && col0 + j0 + j < p.cols) store1(p.w, p.type_w, o + j * p.ld_w, fmaf(p.keep, w[j], v[j0 + j]));
         }
         return;
     }
@@ -425,11 +425,11 @@ __device__ __forceinline__ void store_result(const Product &p, const float (&v)[
 #pragma unroll
         for (int q = 0; q < 8; q++) {
             w[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (p.keep != 0.f && row0 + r0 + 4 * q < rows_end && c < p.cols) w[q] = load4(p.w, p.type_w, o + 4 * q * p.ld_w);
+            if (p.keep != 0.f && row0 + r0 + 4 * q < p.rows && c < p.cols) w[q] = load4(p.w, p.type_w, o + 4 * q * p.ld_w);
         }
 #pragma unroll
         for (int q = 0; q < 8; q++)
-            if (row0 + r0 + 4 * q < rows_end && c < p.cols) {
+            if (row0 + r0 + 4 * q < p.rows && c < p.cols) {
                 const int r = r0 + 4 * q;
                 const uint4 x = lds(buf + (uint32_t)(r * 128 + ((u ^ r) & 7) * 16));
                 store4(p.w, p.type_w, o + 4 * q * p.ld_w, make_float4(fmaf(p.keep, w[q].x, __uint_as_float(x.x)), fmaf(p.keep, w[q].y, __uint_as_float(x.y)),
@@ -443,25 +443,79 @@ __device__ __forceinline__ void store_result(const Product &p, const float (&v)[
             const long long o = k * p.stride_w + (row0 + q0) * p.ld_w + c;
             float w[16];
 #pragma unroll
-            for (int q = 0; q < 16; q++) w[q] = p.keep != 0.f && row0 + q0 + q < rows_end && c < p.cols ? load1(p.w, p.type_w, o + q * p.ld_w) : 0.f;
+            for (int q = 0; q < 16; q++) w[q] = p.keep != 0.f && row0 + q0 + q < p.rows && c < p.cols ? load1(p.w, p.type_w, o + q * p.ld_w) : 0.f;
 #pragma unroll
             for (int q = 0; q < 16; q++) {
                 const int r = q0 + q;
                 float x;
                 asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buf + (uint32_t)(r * 128 + (((lane >> 2) ^ r) & 7) * 16 + (lane & 3) * 4)) : "memory");
-                if (row0 + r < rows_end && c < p.cols) store1(p.w, p.type_w, o + q * p.ld_w, fmaf(p.keep, w[q], x));
+                if (row0 + r < p.rows && c < p.cols) store1(p.w, p.type_w, o + q * p.ld_w, fmaf(p.keep, w[q], x));
             }
         }
     }
     __syncwarp();
 }
 
-constexpr uint32_t OPERAND_BYTES = 196608;          // operand stages; behind them 32 KB in which results are staged
-
-// Two planes: where the accumulator is drained, every other K block and every one on the tile's diagonal.
-__device__ __forceinline__ bool chunk_ends(int kb, int diag0, int diag, bool sym)
+// A lane's part of row r of a 64 x 64 quarter in fp32, from 16-byte unit u0 on.
+template <int N> __device__ __forceinline__ void put_quarter(uint32_t quarter, const uint32_t (&x)[N], int r, int u0)
 {
-    return (kb & 1) || (sym && kb >= diag0 && kb < diag0 + diag);
+#pragma unroll
+    for (int u = 0; u < N / 4; u++)
+        sts(quarter + (uint32_t)(r * 256 + ((u0 + u) ^ (r & 7)) * 16), make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]));
+}
+
+// A 64 x 64 tile of the result, rows of 65 floats in shared memory, into the caller's matrix by 256 threads, along its
+// rows; loads ahead of stores.
+__device__ __forceinline__ void store_result_64(const Product &p, uint32_t tile, int tid, int k, int row0, int col0)
+{
+    const auto at = [&](int r, int c) {
+        float x;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(tile + (uint32_t)(r * 65 + c) * 4) : "memory");
+        return x;
+    };
+    if (p.vec_w && !p.tall) {
+        const int c = 4 * (tid & 15);
+        float4 w[4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const int r = (tid >> 4) + 16 * n;
+            w[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p.keep != 0.f && row0 + r < p.rows && col0 + c < p.cols) w[n] = load4(p.w, p.type_w, k * p.stride_w + (row0 + r) * p.ld_w + col0 + c);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const int r = (tid >> 4) + 16 * n;
+            if (row0 + r < p.rows && col0 + c < p.cols)
+                store4(p.w, p.type_w, k * p.stride_w + (row0 + r) * p.ld_w + col0 + c,
+                       make_float4(fmaf(p.keep, w[n].x, at(r, c)), fmaf(p.keep, w[n].y, at(r, c + 1)), fmaf(p.keep, w[n].z, at(r, c + 2)), fmaf(p.keep, w[n].w, at(r, c + 3))));
+        }
+        return;
+    }
+    // an element a thread, neighbouring threads along the caller's row
+    float w[16];
+#pragma unroll
+    for (int n = 0; n < 16; n++) {
+        const int x = tid & 63, y = (tid >> 6) + 4 * n, r = p.tall ? x : y, c = p.tall ? y : x;
+        const long long o = k * p.stride_w + (p.tall ? (col0 + c) * p.ld_w + row0 + r : (row0 + r) * p.ld_w + col0 + c);
+        w[n] = p.keep != 0.f && row0 + r < p.rows && col0 + c < p.cols ? load1(p.w, p.type_w, o) : 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < 16; n++) {
+        const int x = tid & 63, y = (tid >> 6) + 4 * n, r = p.tall ? x : y, c = p.tall ? y : x;
+        const long long o = k * p.stride_w + (p.tall ? (col0 + c) * p.ld_w + row0 + r : (row0 + r) * p.ld_w + col0 + c);
+        if (row0 + r < p.rows && col0 + c < p.cols) store1(p.w, p.type_w, o, fmaf(p.keep, w[n], at(r, c)));
+    }
+}
+
+// Shared memory: operand stages; behind them 32 KB in which results are staged. 64-tiles: 48 KB in which the quarters of
+// the product meet, and a box each for hi and lo.
+constexpr uint32_t OPERAND_BYTES = 196608, OPERAND_BYTES_64 = 163840, QUARTERS_64 = 49152;
+
+// Two planes: where the accumulator is drained, after every `run` K blocks (64-tiles, whose small products have sums of their
+// own: 4; else 2) and after every one on the tile's diagonal.
+__device__ __forceinline__ bool chunk_ends(int kb, int run, int diag0, int diag, bool sym)
+{
+    return (kb & (run - 1)) == run - 1 || (sym && kb >= diag0 && kb < diag0 + diag);
 }
 
 // 384 threads; grid: any number of CTAs (pairs), each takes every grid-th tile. p.split > 1: a
@@ -478,9 +532,13 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     constexpr int BK = 64, ROWS = SIDE == 64 ? 64 : 128;            // K block; rows of an operand that one CTA holds
     constexpr uint32_t TILE = ROWS * BK * 2;                        // one operand plane of one CTA
     constexpr uint32_t STAGE = 2 * PLANES * TILE;
-    constexpr int STAGES = OPERAND_BYTES / STAGE;
+    constexpr int STAGES = (SIDE == 64 ? OPERAND_BYTES_64 : OPERAND_BYTES) / STAGE;
     constexpr int HALF = SIDE / 2;                                  // columns per epilogue warp
-    constexpr uint32_t TMEM_COLS = 2 * SIDE;                        // two accumulators
+    // Rows and columns of one tensor instruction. 64-tiles in two planes take hi and lo, which lie one below the
+    // other, as one operand of 128: the four quarters of a 128 x 128 product are hi.hi, hi.lo, lo.hi and lo.lo, four
+    // instructions a K block instead of twelve (an instruction takes some 90 clocks however small it is).
+    constexpr int MMA = SIDE == 64 ? 64 * PLANES : SIDE;
+    constexpr uint32_t TMEM_COLS = 2 * MMA;                         // two accumulators
     const WaitCtl status = { p.status, p.wait_ns };
 
     extern __shared__ uint8_t smem_orth[];
@@ -510,7 +568,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     // first K block that comes transposed, of rows that begin at tile index x of SIDE
     const auto turn = [&](int x, bool sym) { return sym ? (x * (SIDE / BK) / tri_kb + 1) * tri_kb : 0x7fffffff; };
     // One plane, Q X: ahead of the K blocks, those on the tile's diagonal with the lo plane of X.
-    constexpr int DIAG = SIDE / BK;
+    constexpr int DIAG = SIDE / BK, RUN = SIDE == 64 ? 4 : 2;
     const auto lo_from = [&](int x) { return max(x * DIAG, kb0); };
     const auto lo_count = [&](int x) { return PLANES == 1 && b_cols ? max(0, min(x * DIAG + DIAG, kb1) - lo_from(x)) : 0; };
 
@@ -600,12 +658,12 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         if (!ok) break;
                         g++;
                     }
-                    const uint32_t tacc = tmem + buf * (uint32_t)SIDE;
+                    const uint32_t tacc = tmem + buf * (uint32_t)MMA;
                     ok = warp_wait(full, ph, status, 2);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const bool a_t = kb >= a_turn, b_t = kb >= b_turn;
-                    const uint32_t idesc = instr_desc(SIDE, SIDE, a_t, b_t);
+                    const uint32_t idesc = instr_desc(MMA, MMA, a_t, b_t);
                     const uint32_t at = a_t ? (8192u >> 4) << 16 : 0u, bt = b_t ? (8192u >> 4) << 16 : 0u;
                     const uint32_t ah = s_lo | at, bh = (s_lo + (PLANES * TILE >> 4)) | bt;
                     // sixteen of K further: 32 bytes along a row, or sixteen rows
@@ -614,9 +672,9 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     // to the sum's last bit, so adds to a sum that is still small cost less.
                     const uint32_t al = ah + (TILE >> 4), bl = bh + (TILE >> 4);
                     const int next = lo && --lo == 0 ? kb0 : kb + 1;
-                    const bool ends = next == kb1 || (PLANES == 2 && chunk_ends(kb, i * DIAG, DIAG, a_sym));
+                    const bool ends = next == kb1 || (PLANES == 2 && chunk_ends(kb, RUN, i * DIAG, DIAG, a_sym));
                     if (elected()) {
-                        if constexpr (PLANES == 2) {
+                        if constexpr (PLANES == 2 && SIDE != 64) {
 #pragma unroll
                             for (int kk = 0; kk < BK / 16; kk++) {
                                 umma<PAIR>(tacc, desc(al + kk * ak), desc(bh + kk * bk), idesc, kk ? 1u : acc);
@@ -625,7 +683,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         }
 #pragma unroll
                         for (int kk = 0; kk < BK / 16; kk++)
-                            umma<PAIR>(tacc, desc(ah + kk * ak), desc(bh + kk * bk), idesc, PLANES == 2 || kk ? 1u : acc);
+                            umma<PAIR>(tacc, desc(ah + kk * ak), desc(bh + kk * bk), idesc, (PLANES == 2 && SIDE != 64) || kk ? 1u : acc);
                         commit<PAIR>(empty, first);
                         if (ends) commit<PAIR>(acc_full0 + 8 * buf, first);
                     }
@@ -645,17 +703,138 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
         const int e = warp - 4, q = warp & 3, h = e >> 2;
         const uint32_t acc_empty = PAIR ? map_to_cta(acc_empty0, first) : acc_empty0;
         const uint32_t staging = smem0 + OPERAND_BYTES;
-        // the warps that store a box of 64 x 64 together: two (q even and odd), each with 32 rows and all columns; with
-        // 64-tiles all eight, each with 16 rows (the lower half of its lanes) and half the columns
-        constexpr int TEAM = SIDE == 64 ? 256 : 64;
-        const int team = SIDE == 64 ? 0 : h * 2 + (q >> 1), team_row = SIDE == 64 ? q * 16 + lane : (q & 1) * 32 + lane;
-        const bool issuer = SIDE == 64 ? e == 0 && lane == 0 : team_row == 0;
+        const bool issuer = SIDE == 64 ? e == 0 && lane == 0 : (q & 1) == 0 && lane == 0;
         uint32_t g = 0;
         bool ok = true;
+        if constexpr (SIDE == 64) {
+            // The quarters of the product meet in shared memory; then each warp has 32 rows x 16 columns of the tile.
+            const uint32_t quarters = smem0 + OPERAND_BYTES_64, box = quarters + QUARTERS_64;
+            const int r = (e & 1) * 32 + lane, c16 = e >> 1;
+            for (int item = cl; ok && item < items; item += C) {
+                int k, i, j;
+                tiles.at(item, k, i, j);
+                if (p.mode == ORTH_RESULT && p.keep != 0.f && part == 0) prefetch_result(p, lane, k, i * 64 + (e & 1) * 32, j * 64 + c16 * 16, 16);
+                if constexpr (PLANES == 1) {
+                    // 64 rows: 16 lanes of each quarter of tensor memory; this warp's half of the columns
+                    const uint32_t buf = g & 1u;
+                    ok = warp_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3);
+                    g++;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    uint32_t x[32];
+                    tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * (uint32_t)MMA + (uint32_t)(h * 32), x);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
+                    if (lane < 16) put_quarter(quarters, x, q * 16 + lane, h * 8);
+                } else {
+                    // rows of hi (q 0, 1) or lo, columns of hi (h 0) or lo; the quarter lo.lo is left out
+                    const bool used = q < 2 || h == 0;
+                    float acc[64];
+#pragma unroll
+                    for (int c = 0; c < 64; c++) acc[c] = 0.f;
+                    for (int kb = kb0; kb < kb1; kb++) {
+                        if (kb + 1 < kb1 && !chunk_ends(kb, RUN, i * DIAG, DIAG, a_sym)) continue;
+                        const uint32_t buf = g & 1u;
+                        ok = ok && warp_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3);
+                        if (!ok) break;
+                        g++;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (used) {
+#pragma unroll
+                            for (int cc = 0; cc < 2; cc++) {
+                                uint32_t x[32];
+                                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * (uint32_t)MMA + (uint32_t)(h * 64 + cc * 32), x);
+                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                                for (int c = 0; c < 32; c++) acc[cc * 32 + c] = __fadd_rn(acc[cc * 32 + c], __uint_as_float(x[c]));
+                            }
+                        }
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
+                    }
+                    if (used) {
+                        uint32_t x[64];
+#pragma unroll
+                        for (int c = 0; c < 64; c++) x[c] = __float_as_uint(acc[c]);
+                        put_quarter(quarters + (q < 2 ? h : 2) * 16384u, x, (q & 1) * 32 + lane, 0);
+                    }
+                }
+                ok = all_ok<256>(1, ok);
+                float v[16];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t at = quarters + (uint32_t)(r * 256 + ((c16 * 4 + u) ^ (r & 7)) * 16);
+                    uint4 x = lds(at);
+                    v[4 * u] = __uint_as_float(x.x); v[4 * u + 1] = __uint_as_float(x.y); v[4 * u + 2] = __uint_as_float(x.z); v[4 * u + 3] = __uint_as_float(x.w);
+                    if constexpr (PLANES == 2) {
+                        const uint4 y = lds(at + 16384u), z = lds(at + 32768u);
+                        v[4 * u] += __uint_as_float(y.x) + __uint_as_float(z.x); v[4 * u + 1] += __uint_as_float(y.y) + __uint_as_float(z.y);
+                        v[4 * u + 2] += __uint_as_float(y.z) + __uint_as_float(z.z); v[4 * u + 3] += __uint_as_float(y.w) + __uint_as_float(z.w);
+                    }
+                }
+                if (split > 1) {        // part 0 has the tile; the others' sums: [part][warp][4 columns][lane][4]
+                    float *const to = p.sums + ((size_t)(cl * split + part) * 8 + e) * 512 + lane * 4;
+                    if (part != 0) {
+#pragma unroll
+                        for (int u = 0; u < 4; u++) __stcg(reinterpret_cast<float4 *>(to + u * 128), make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]));
+                    }
+                    cluster_sync_all();
+                    if (part != 0) continue;
+                    for (int from = 1; from < split; from++) {
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(to + (size_t)from * 4096 + u * 128));
+                            v[4 * u] += x.x; v[4 * u + 1] += x.y; v[4 * u + 2] += x.z; v[4 * u + 3] += x.w;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 16; c++) v[c] *= p.alpha;
+                if (!ok) break;
+                if (p.mode == ORTH_RESULT) {
+                    team_sync<256>(1);          // every warp has read the quarters
+#pragma unroll
+                    for (int c = 0; c < 16; c++)
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(quarters + (uint32_t)(r * 65 + c16 * 16 + c) * 4), "f"(v[c]) : "memory");
+                    team_sync<256>(1);
+                    store_result_64(p, quarters, (int)threadIdx.x - 128, k, i * 64, j * 64);
+                    team_sync<256>(1);
+                    continue;
+                }
+                if (tiles.sym && i == j) {
+#pragma unroll
+                    for (int c = 0; c < 16; c++) v[c] += r == c16 * 16 + c ? p.diag : 0.f;
+                }
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    const __half2 x = __floats2half2_rn(v[2 * c], v[2 * c + 1]);
+                    const float2 f = __half22float2(x);
+                    const __half2 y = __floats2half2_rn(v[2 * c] - f.x, v[2 * c + 1] - f.y);
+                    hi[c] = *reinterpret_cast<const uint32_t *>(&x);
+                    lo[c] = *reinterpret_cast<const uint32_t *>(&y);
+                }
+                if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the boxes' last content has left
+                team_sync<256>(1);
+                put_box(box, hi, r, c16 * 2);
+                if (p.lo) put_box(box + 8192u, lo, r, c16 * 2);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                team_sync<256>(1);
+                if (issuer) {
+                    tma_store(&o_hi, box, j * 64, i * 64, k);
+                    if (p.lo) tma_store(&o_lo, box + 8192u, j * 64, i * 64, k);
+                }
+            }
+        } else {
+        // two warps (q even and odd) store a box of 64 x 64 together
+        constexpr int TEAM = 64;
+        const int team = h * 2 + (q >> 1), team_row = (q & 1) * 32 + lane;
         for (int item = cl; ok && item < items; item += C) {
             int k, i, j;
             tiles.at(item, k, i, j);
-            const int row0 = i * SIDE + (int)rank * 128 + q * (SIDE == 64 ? 16 : 32), col0 = j * SIDE + h * HALF;
+            const int row0 = i * SIDE + (int)rank * 128 + q * 32, col0 = j * SIDE + h * HALF;
             if (p.mode == ORTH_RESULT && p.keep != 0.f) prefetch_result(p, lane, k, row0, col0, HALF);
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * HALF);
             uint32_t buf = g & 1u;
@@ -671,7 +850,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
 #pragma unroll
                 for (int c = 0; c < HALF; c++) acc[c] = 0.f;
                 for (int kb = kb0; kb < kb1; kb++) {
-                    if (kb + 1 < kb1 && !chunk_ends(kb, i * DIAG, DIAG, a_sym)) continue;
+                    if (kb + 1 < kb1 && !chunk_ends(kb, RUN, i * DIAG, DIAG, a_sym)) continue;
                     buf = g & 1u;
                     ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
                     if (!ok) break;
@@ -699,8 +878,8 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
             // where this warp's sums lie when parts meet: [part][CTA][warp][4 columns][lane][4]
             constexpr size_t WARP_SUMS = 32 * HALF, part_step = (size_t)CTAS * 8 * WARP_SUMS;
             const size_t sums_at = (((size_t)cl * split * CTAS + rank) * 8 + e) * WARP_SUMS + lane * 4;
-            constexpr int PIECE = SIDE == 64 ? 32 : 64, PIECES = HALF / PIECE;         // columns that have one owner
-            const int piece0 = SIDE == 64 ? 0 : h * PIECES;
+            constexpr int PIECE = 64, PIECES = HALF / PIECE;                // columns that have one owner
+            const int piece0 = h * PIECES;
             if (split > 1) {
 #pragma unroll 1
                 for (int cc = 0; ok && cc < HALF / 32; cc++) {
@@ -724,8 +903,8 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
             for (int cc = 0; ok && cc < PIECES; cc++) {
                 if (split > 1 && (piece0 + cc) % split != part) continue;
                 const int col = col0 + cc * PIECE;
-                // all warps of a store agree: its first row and column decide
-                if (row0 - (SIDE == 64 ? q * 16 : (q & 1) * 32) >= p.rows || (SIDE == 64 ? j * SIDE : col) >= p.cols) break;
+                // both warps of a store agree: its first row and column decide
+                if (row0 - (q & 1) * 32 >= p.rows || col >= p.cols) break;
                 uint32_t hi[PIECE / 2], lo[PIECE / 2];
 #pragma unroll
                 for (int half = 0; half < PIECE / 32; half++) {
@@ -747,7 +926,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
 #pragma unroll
                     for (int c = 0; c < 32; c++) v[c] *= p.alpha;
                     if (p.mode == ORTH_RESULT) {
-                        store_result(p, v, staging + (uint32_t)e * 4096u, lane, k, row0, SIDE == 64 ? min(p.rows, row0 + 16) : p.rows, col + half * 32);
+                        store_result(p, v, staging + (uint32_t)e * 4096u, lane, k, row0, col + half * 32);
                         continue;
                     }
                     if (tiles.sym && i == j) {
@@ -769,33 +948,33 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     }
                 }
                 if (p.mode != ORTH_RESULT) {
-                    const uint32_t box = roomy ? smem0 + (uint32_t)(team * PIECES + cc) * 16384u : staging + (uint32_t)team * (SIDE == 64 ? 16384u : 8192u);
-                    const bool apart = roomy || SIDE == 64;         // hi and lo have a place each
-                    const int u0 = SIDE == 64 ? h * 4 : 0;
-                    if (issuer && !roomy) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the last content has left
-                    if (!roomy) team_sync<TEAM>(1 + team);
-                    if (SIDE != 64 || lane < 16) put_box(box, hi, team_row, u0);
-                    if (apart && p.lo && (SIDE != 64 || lane < 16)) put_box(box + 8192u, lo, team_row, u0);
+                    const uint32_t box = roomy ? smem0 + (uint32_t)(team * PIECES + cc) * 16384u : staging + (uint32_t)team * 8192u;
+                    if (!roomy) {
+                        if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the last content has left
+                        team_sync<TEAM>(1 + team);
+                    }
+                    put_box(box, hi, team_row, 0);
+                    if (roomy && p.lo) put_box(box + 8192u, lo, team_row, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     team_sync<TEAM>(1 + team);
-                    const int x = SIDE == 64 ? j * SIDE : col;
                     if (issuer) {
-                        tma_store(&o_hi, box, x, row0, k);
-                        if (apart && p.lo) tma_store(&o_lo, box + 8192u, x, row0, k);
+                        tma_store(&o_hi, box, col, row0, k);
+                        if (roomy && p.lo) tma_store(&o_lo, box + 8192u, col, row0, k);
                     }
-                    if (!apart && p.lo) {
+                    if (!roomy && p.lo) {
                         if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         team_sync<TEAM>(1 + team);
-                        put_box(box, lo, team_row, u0);
+                        put_box(box, lo, team_row, 0);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         team_sync<TEAM>(1 + team);
-                        if (issuer) tma_store(&o_lo, box, x, row0, k);
+                        if (issuer) tma_store(&o_lo, box, col, row0, k);
                     }
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
+        }
         }
         if (issuer) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if (!ok) {      // a wait ran out: copies that may still be in flight land before the shared memory is released

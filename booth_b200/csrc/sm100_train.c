@@ -196,11 +196,11 @@ static int orth_layout(const sm100_dev_t *dev, orth_layout_t *o, int batch, int 
     o->s_lo = at; if (two_planes) at += a;
     o->q_hi = at; at += a;
     o->q_lo = at; if (two_planes) at += a;
-    /* sums of shared tiles: 32, 64 or 128 KB a CTA by tile side, eight parts a tile at most (four pairs), all at once on the GPU */
+    /* sums of shared tiles: 16, 64 or 128 KB a CTA by tile side, eight parts a tile at most (four pairs), all at once on the GPU */
     size_t sums = 0;
     for (int side = 64; side <= 256; side *= 2) {
         const long long ctas = 8ll * batch * ((o->l + side - 1) / side) * ((o->s + side - 1) / side);
-        const size_t need = (size_t)(ctas < dev->sm_count ? ctas : dev->sm_count) * (side == 64 ? 32768u : side == 128 ? 65536u : 131072u);
+        const size_t need = (size_t)(ctas < dev->sm_count ? ctas : dev->sm_count) * (side == 64 ? 16384u : side == 128 ? 65536u : 131072u);
         if (need > sums) sums = need;
     }
     o->sums = at; at += sums;
