@@ -54,11 +54,15 @@ using gemm::smem_u32;
 
 constexpr float X_SCALE = 16384.f;       // 2^14
 
-__device__ __forceinline__ float load1(const void *p, int type, long long i)
+// Elements of a type known at run time: first the bits, then the values. (Load and conversion under one branch on the
+// type would wait for each load before the next is issued.)
+__device__ __forceinline__ uint32_t bits1(const void *p, int type, long long i)
 {
-    if (type == ORTH_F32) return static_cast<const float *>(p)[i];
-    if (type == ORTH_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-    return __half2float(static_cast<const __half *>(p)[i]);
+    return type == ORTH_F32 ? static_cast<const uint32_t *>(p)[i] : static_cast<const uint16_t *>(p)[i];
+}
+__device__ __forceinline__ float value1(uint32_t x, int type)
+{
+    return type == ORTH_F32 ? __uint_as_float(x) : type == ORTH_BF16 ? __uint_as_float(x << 16) : __half2float(__ushort_as_half((unsigned short)x));
 }
 __device__ __forceinline__ void store1(void *p, int type, long long i, float v)
 {
@@ -73,10 +77,15 @@ __device__ __forceinline__ float rounded(float v, int type)
 }
 __device__ __forceinline__ float4 rounded4(float4 v, int type) { return make_float4(rounded(v.x, type), rounded(v.y, type), rounded(v.z, type), rounded(v.w, type)); }
 // Four neighbouring elements; p + i is aligned to four elements.
-__device__ __forceinline__ float4 load4(const void *p, int type, long long i)
+__device__ __forceinline__ uint4 bits4(const void *p, int type, long long i)
 {
-    if (type == ORTH_F32) return *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+    if (type == ORTH_F32) return *reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + i);
     const uint2 r = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
+    return make_uint4(r.x, r.y, 0, 0);
+}
+__device__ __forceinline__ float4 values4(uint4 r, int type)
+{
+    if (type == ORTH_F32) return make_float4(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), __uint_as_float(r.w));
     if (type == ORTH_BF16)
         return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u));
     const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&r.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&r.y));
@@ -103,17 +112,9 @@ __device__ __forceinline__ float lerp(float m, float g, float mu) { return fmaf(
 // What is orthogonalised, from the gradient and the stored momentum.
 __device__ __forceinline__ float update_of(float m, float g, const Source &s) { return s.nesterov ? lerp(m, g, s.mu) : m; }
 
-__device__ __forceinline__ float4 source4(const Source &s, int k, int r, int c)
+__device__ __forceinline__ float4 update4(float4 m, float4 g, const Source &s)
 {
-    const float4 g = load4(s.g, s.type_g, k * s.stride_g + r * s.ld_g + c);
-    if (!s.m) return g;
-    const float4 m = load4(s.m, s.type_m, k * s.stride_m + r * s.ld_m + c);
     return make_float4(update_of(m.x, g.x, s), update_of(m.y, g.y, s), update_of(m.z, g.z, s), update_of(m.w, g.w, s));
-}
-__device__ __forceinline__ float source1(const Source &s, int k, int r, int c)
-{
-    const float g = load1(s.g, s.type_g, k * s.stride_g + r * s.ld_g + c);
-    return s.m ? update_of(load1(s.m, s.type_m, k * s.stride_m + r * s.ld_m + c), g, s) : g;
 }
 
 }  // namespace orth
@@ -136,29 +137,50 @@ orth_norm(const __grid_constant__ orth::Source s, double *__restrict__ partial)
     double sum = 0.0;
     for (long long r = r0; r < rows; r += r_step) {
         const long long at_g = k * s.stride_g + r * s.ld_g, at_m = k * s.stride_m + r * s.ld_m;
-        if (s.vec) {
-#pragma unroll 4
-            for (long long c = c0; c < cols; c += c_step) {
-                float4 u = load4(s.g, s.type_g, at_g + c);
-                if (s.m) {
-                    float4 m = load4(s.m, s.type_m, at_m + c);
-                    m = make_float4(lerp(m.x, u.x, s.mu), lerp(m.y, u.y, s.mu), lerp(m.z, u.z, s.mu), lerp(m.w, u.w, s.mu));
-                    m = rounded4(m, s.type_m);
-                    store4(s.m, s.type_m, at_m + c, m);
-                    u = make_float4(update_of(m.x, u.x, s), update_of(m.y, u.y, s), update_of(m.z, u.z, s), update_of(m.w, u.w, s));
+        // several loads ahead of the stores to m, which the compiler has to keep in order
+        constexpr int N = 4;
+        for (long long c = c0; c < cols; c += N * c_step) {
+            if (s.vec) {
+                uint4 g[N], m[N];
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    g[n] = m[n] = make_uint4(0, 0, 0, 0);
+                    if (c + n * c_step < cols) {
+                        g[n] = bits4(s.g, s.type_g, at_g + c + n * c_step);
+                        if (s.m) m[n] = bits4(s.m, s.type_m, at_m + c + n * c_step);
+                    }
                 }
-                sum += ((double)u.x * u.x + (double)u.y * u.y) + ((double)u.z * u.z + (double)u.w * u.w);
-            }
-        } else {
-#pragma unroll 4
-            for (long long c = c0; c < cols; c += c_step) {
-                float u = load1(s.g, s.type_g, at_g + c);
-                if (s.m) {
-                    const float m = rounded(lerp(load1(s.m, s.type_m, at_m + c), u, s.mu), s.type_m);
-                    store1(s.m, s.type_m, at_m + c, m);
-                    u = update_of(m, u, s);
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    float4 u = values4(g[n], s.type_g);
+                    if (s.m && c + n * c_step < cols) {
+                        float4 x = values4(m[n], s.type_m);
+                        x = rounded4(make_float4(lerp(x.x, u.x, s.mu), lerp(x.y, u.y, s.mu), lerp(x.z, u.z, s.mu), lerp(x.w, u.w, s.mu)), s.type_m);
+                        store4(s.m, s.type_m, at_m + c + n * c_step, x);
+                        u = update4(x, u, s);
+                    }
+                    sum += ((double)u.x * u.x + (double)u.y * u.y) + ((double)u.z * u.z + (double)u.w * u.w);
                 }
-                sum += (double)u * u;
+            } else {
+                uint32_t g[N], m[N];
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    g[n] = m[n] = 0;
+                    if (c + n * c_step < cols) {
+                        g[n] = bits1(s.g, s.type_g, at_g + c + n * c_step);
+                        if (s.m) m[n] = bits1(s.m, s.type_m, at_m + c + n * c_step);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    float u = value1(g[n], s.type_g);
+                    if (s.m && c + n * c_step < cols) {
+                        const float x = rounded(lerp(value1(m[n], s.type_m), u, s.mu), s.type_m);
+                        store1(s.m, s.type_m, at_m + c + n * c_step, x);
+                        u = update_of(x, u, s);
+                    }
+                    sum += (double)u * u;
+                }
             }
         }
     }
@@ -173,8 +195,8 @@ orth_norm(const __grid_constant__ orth::Source s, double *__restrict__ partial)
 }
 
 // hi and lo planes of 2^14 u / (|u| + eps), s x l with rows `pitch` apart, transposed
-// when the matrix is tall. One 64 x 64 tile of u a block through shared memory; grid
-// (column tiles, row tiles, matrices).
+// when the matrix is tall. A 64 x 64 tile of u a block; grid (column tiles, row tiles,
+// matrices). A tall tile goes through shared memory, any other straight to its place.
 extern "C" __global__ void __launch_bounds__(256)
 orth_split(const __grid_constant__ orth::Source s, const double *__restrict__ partial, int parts, float eps, __half *__restrict__ hi,
            __half *__restrict__ lo, long long pitch, long long plane, int tall)
@@ -185,6 +207,30 @@ orth_split(const __grid_constant__ orth::Source s, const double *__restrict__ pa
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const int k = (int)blockIdx.z, r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;
+    const int tx = (int)threadIdx.x & 15, ty = (int)threadIdx.x >> 4;
+    uint4 g[4], m[4];
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+        const int r = r0 + ty + 16 * p, c = c0 + 4 * tx;
+        const long long at_g = k * s.stride_g + r * s.ld_g + c, at_m = k * s.stride_m + r * s.ld_m + c;
+        g[p] = m[p] = make_uint4(0, 0, 0, 0);
+        if (r >= s.rows) continue;
+        if (s.vec) {
+            if (c < s.cols) {
+                g[p] = bits4(s.g, s.type_g, at_g);
+                if (s.m) m[p] = bits4(s.m, s.type_m, at_m);
+            }
+        } else {
+            uint32_t x[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[e] = c + e < s.cols ? bits1(s.g, s.type_g, at_g + e) : 0;
+                y[e] = s.m && c + e < s.cols ? bits1(s.m, s.type_m, at_m + e) : 0;
+            }
+            g[p] = s.type_g == ORTH_F32 ? make_uint4(x[0], x[1], x[2], x[3]) : make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, 0, 0);
+            m[p] = s.type_m == ORTH_F32 ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[0] | y[1] << 16, y[2] | y[3] << 16, 0, 0);
+        }
+    }
     if (threadIdx.x < 32) {
         double sum = 0.0;
         for (int i = (int)threadIdx.x; i < parts; i += 32) sum += partial[(size_t)k * parts + i];
@@ -192,22 +238,18 @@ orth_split(const __grid_constant__ orth::Source s, const double *__restrict__ pa
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (threadIdx.x == 0) s_scale = (float)fmin((double)X_SCALE / (sqrt(sum) + (double)eps), 3.4e38);
     }
-    const int tx = (int)threadIdx.x & 15, ty = (int)threadIdx.x >> 4;
+    float4 v[4];
 #pragma unroll
     for (int p = 0; p < 4; p++) {
-        const int r = r0 + ty + 16 * p, c = c0 + 4 * tx;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < s.rows) {
-            if (s.vec && c < s.cols) v = source4(s, k, r, c);
-            else {
-                if (c + 0 < s.cols) v.x = source1(s, k, r, c);
-                if (c + 1 < s.cols) v.y = source1(s, k, r, c + 1);
-                if (c + 2 < s.cols) v.z = source1(s, k, r, c + 2);
-                if (c + 3 < s.cols) v.w = source1(s, k, r, c + 3);
-            }
+        v[p] = values4(g[p], s.type_g);
+        if (s.m) v[p] = update4(values4(m[p], s.type_m), v[p], s);
+    }
+    if (tall) {
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            float *t = &tile[ty + 16 * p][4 * tx];
+            t[0] = v[p].x; t[1] = v[p].y; t[2] = v[p].z; t[3] = v[p].w;
         }
-        float *t = &tile[ty + 16 * p][4 * tx];
-        t[0] = v.x; t[1] = v.y; t[2] = v.z; t[3] = v.w;
     }
     __syncthreads();
     const float f = s_scale;
@@ -217,13 +259,14 @@ orth_split(const __grid_constant__ orth::Source s, const double *__restrict__ pa
         // row (of the plane) a, four columns from b; the pitch is a multiple of 64, so a whole group is in the plane
         const int a = ty + 16 * p, b = 4 * tx;
         const int row = (tall ? c0 : r0) + a, col = (tall ? r0 : c0) + b;
+        if (tall) v[p] = make_float4(tile[b][a], tile[b + 1][a], tile[b + 2][a], tile[b + 3][a]);
         if (row < (tall ? s.cols : s.rows) && col < (tall ? s.rows : s.cols)) {
+            const float x[4] = { f * v[p].x, f * v[p].y, f * v[p].z, f * v[p].w };
             __half h[4], l[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float v = f * (tall ? tile[b + e][a] : tile[a][b + e]);
-                h[e] = __float2half_rn(v);
-                l[e] = __float2half_rn(v - __half2float(h[e]));
+                h[e] = __float2half_rn(x[e]);
+                l[e] = __float2half_rn(x[e] - __half2float(h[e]));
             }
             *reinterpret_cast<uint2 *>(ph + row * pitch + col) = *reinterpret_cast<const uint2 *>(h);
             *reinterpret_cast<uint2 *>(pl + row * pitch + col) = *reinterpret_cast<const uint2 *>(l);
@@ -394,66 +437,92 @@ __device__ __forceinline__ void prefetch_result(const Product &p, int lane, int 
     }
 }
 
-// One warp's 32 rows x 32 columns of the result, a row a lane, into the caller's matrix. Through 4 KB of the
-// warp's own shared memory, so that accesses run along the rows; loads ahead of stores.
-__device__ __forceinline__ void store_result(const Product &p, const float (&v)[32], uint32_t buf, int lane, int k, int row0, int col0)
+// One warp's 32 rows x 32 columns of the caller's matrix: N / 32 of its weights from part `n0` on, as bits, and the result, a
+// row a lane in v. A tall matrix has a column of the piece as a contiguous run of its row: neighbouring lanes hold
+// neighbouring rows. Else the piece goes through 4 KB of the warp's own shared memory, so that accesses run
+// along the rows: eight rows of eight lanes' groups of four elements, or a column a lane.
+template <int N, bool WIDE>
+__device__ __forceinline__ void fetch_weights_of(const Product &p, uint32_t (&w)[N], int n0, int lane, int k, int row0, int col0)
 {
-    const int row = row0 + lane;
+    constexpr int type = WIDE ? ORTH_F32 : ORTH_BF16;       // as bits, 16-bit types are alike
     if (p.tall) {
-        // neighbouring lanes hold neighbouring rows: a column is a contiguous run of the caller's row
+        const long long o = k * p.stride_w + col0 * p.ld_w + row0 + lane;
 #pragma unroll
-        for (int j0 = 0; j0 < 32; j0 += 16) {
-            const long long o = k * p.stride_w + (long long)(col0 + j0) * p.ld_w + row;
-            float w[16];
+        for (int j = 0; j < N; j++)
+            if (row0 + lane < p.rows && col0 + n0 + j < p.cols) w[j] = bits1(p.w, type, o + (n0 + j) * p.ld_w);
+    } else if (p.vec_w) {
+        const int r0 = n0 + (lane >> 3), c = col0 + 4 * (lane & 7);
+        const long long o = k * p.stride_w + (row0 + r0) * p.ld_w + c;
 #pragma unroll
-            for (int j = 0; j < 16; j++) w[j] = p.keep != 0.f && row < p.rows && col0 + j0 + j < p.cols ? load1(p.w, p.type_w, o + j * p.ld_w) : 0.f;
+        for (int q = 0; q < N / 4; q++)
+            if (row0 + r0 + 4 * q < p.rows && c < p.cols) {
+                const uint4 x = bits4(p.w, type, o + 4 * q * p.ld_w);
+                w[4 * q] = x.x; w[4 * q + 1] = x.y; w[4 * q + 2] = x.z; w[4 * q + 3] = x.w;
+            }
+    } else {
+        const long long o = k * p.stride_w + row0 * p.ld_w + col0 + lane;
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (row < p.rows && col0 + j0 + j < p.cols) store1(p.w, p.type_w, o + j * p.ld_w, fmaf(p.keep, w[j], v[j0 + j]));
-        }
-        return;
+        for (int q = 0; q < N; q++)
+            if (row0 + n0 + q < p.rows && col0 + lane < p.cols) w[q] = bits1(p.w, type, o + (n0 + q) * p.ld_w);
     }
+}
+template <int N>
+__device__ __forceinline__ void fetch_weights(const Product &p, uint32_t (&w)[N], int n0, int lane, int k, int row0, int col0)
+{
+#pragma unroll
+    for (int j = 0; j < N; j++) w[j] = 0;
+    if (p.keep == 0.f) return;
+    if (p.type_w == ORTH_F32) fetch_weights_of<N, true>(p, w, n0, lane, k, row0, col0);
+    else fetch_weights_of<N, false>(p, w, n0, lane, k, row0, col0);
+}
+// The result's part `n0`.. with those weights. put_result comes first where the matrix is not tall.
+__device__ __forceinline__ void put_result(const float (&v)[32], uint32_t buf, int lane)
+{
+    __syncwarp();
 #pragma unroll
     for (int u = 0; u < 8; u++)
         sts(buf + (uint32_t)(lane * 128 + ((u ^ lane) & 7) * 16),
             make_uint4(__float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3])));
     __syncwarp();
-    if (p.vec_w) {
-        const int u = lane & 7, r0 = lane >> 3, c = col0 + 4 * u;
+}
+template <int N, int N0, int TYPE>
+__device__ __forceinline__ void store_result_as(const Product &p, const float (&v)[32], const uint32_t (&w)[N], uint32_t buf, int lane, int k, int row0, int col0)
+{
+    if (p.tall) {
+        const long long o = k * p.stride_w + col0 * p.ld_w + row0 + lane;
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (row0 + lane < p.rows && col0 + N0 + j < p.cols) store1(p.w, TYPE, o + (N0 + j) * p.ld_w, fmaf(p.keep, value1(w[j], TYPE), v[N0 + j]));
+    } else if (p.vec_w) {
+        const int u = lane & 7, r0 = N0 + (lane >> 3), c = col0 + 4 * u;
         const long long o = k * p.stride_w + (row0 + r0) * p.ld_w + c;
-        float4 w[8];
 #pragma unroll
-        for (int q = 0; q < 8; q++) {
-            w[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (p.keep != 0.f && row0 + r0 + 4 * q < p.rows && c < p.cols) w[q] = load4(p.w, p.type_w, o + 4 * q * p.ld_w);
-        }
-#pragma unroll
-        for (int q = 0; q < 8; q++)
+        for (int q = 0; q < N / 4; q++)
             if (row0 + r0 + 4 * q < p.rows && c < p.cols) {
                 const int r = r0 + 4 * q;
                 const uint4 x = lds(buf + (uint32_t)(r * 128 + ((u ^ r) & 7) * 16));
-                store4(p.w, p.type_w, o + 4 * q * p.ld_w, make_float4(fmaf(p.keep, w[q].x, __uint_as_float(x.x)), fmaf(p.keep, w[q].y, __uint_as_float(x.y)),
-                                                                     fmaf(p.keep, w[q].z, __uint_as_float(x.z)), fmaf(p.keep, w[q].w, __uint_as_float(x.w))));
+                const float4 y = values4(make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]), TYPE);
+                store4(p.w, TYPE, o + 4 * q * p.ld_w, make_float4(fmaf(p.keep, y.x, __uint_as_float(x.x)), fmaf(p.keep, y.y, __uint_as_float(x.y)),
+                                                                     fmaf(p.keep, y.z, __uint_as_float(x.z)), fmaf(p.keep, y.w, __uint_as_float(x.w))));
             }
     } else {
-        // a column a lane, sixteen rows at a time
-        const int c = col0 + lane;
-#pragma unroll 1
-        for (int q0 = 0; q0 < 32; q0 += 16) {
-            const long long o = k * p.stride_w + (row0 + q0) * p.ld_w + c;
-            float w[16];
+        const long long o = k * p.stride_w + row0 * p.ld_w + col0 + lane;
 #pragma unroll
-            for (int q = 0; q < 16; q++) w[q] = p.keep != 0.f && row0 + q0 + q < p.rows && c < p.cols ? load1(p.w, p.type_w, o + q * p.ld_w) : 0.f;
-#pragma unroll
-            for (int q = 0; q < 16; q++) {
-                const int r = q0 + q;
-                float x;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buf + (uint32_t)(r * 128 + (((lane >> 2) ^ r) & 7) * 16 + (lane & 3) * 4)) : "memory");
-                if (row0 + r < p.rows && c < p.cols) store1(p.w, p.type_w, o + q * p.ld_w, fmaf(p.keep, w[q], x));
-            }
+        for (int q = 0; q < N; q++) {
+            const int r = N0 + q;
+            float x;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buf + (uint32_t)(r * 128 + (((lane >> 2) ^ r) & 7) * 16 + (lane & 3) * 4)) : "memory");
+            if (row0 + r < p.rows && col0 + lane < p.cols) store1(p.w, TYPE, o + r * p.ld_w, fmaf(p.keep, value1(w[q], TYPE), x));
         }
     }
-    __syncwarp();
+}
+
+template <int N, int N0>
+__device__ __forceinline__ void store_result(const Product &p, const float (&v)[32], const uint32_t (&w)[N], uint32_t buf, int lane, int k, int row0, int col0)
+{
+    if (p.type_w == ORTH_F32) store_result_as<N, N0, ORTH_F32>(p, v, w, buf, lane, k, row0, col0);
+    else if (p.type_w == ORTH_BF16) store_result_as<N, N0, ORTH_BF16>(p, v, w, buf, lane, k, row0, col0);
+    else store_result_as<N, N0, ORTH_F16>(p, v, w, buf, lane, k, row0, col0);
 }
 
 // A lane's part of row r of a 64 x 64 quarter in fp32, from 16-byte unit u0 on.
@@ -475,35 +544,36 @@ __device__ __forceinline__ void store_result_64(const Product &p, uint32_t tile,
     };
     if (p.vec_w && !p.tall) {
         const int c = 4 * (tid & 15);
-        float4 w[4];
+        uint4 w[4];
 #pragma unroll
         for (int n = 0; n < 4; n++) {
             const int r = (tid >> 4) + 16 * n;
-            w[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (p.keep != 0.f && row0 + r < p.rows && col0 + c < p.cols) w[n] = load4(p.w, p.type_w, k * p.stride_w + (row0 + r) * p.ld_w + col0 + c);
+            w[n] = make_uint4(0, 0, 0, 0);
+            if (p.keep != 0.f && row0 + r < p.rows && col0 + c < p.cols) w[n] = bits4(p.w, p.type_w, k * p.stride_w + (row0 + r) * p.ld_w + col0 + c);
         }
 #pragma unroll
         for (int n = 0; n < 4; n++) {
             const int r = (tid >> 4) + 16 * n;
+            const float4 y = values4(w[n], p.type_w);
             if (row0 + r < p.rows && col0 + c < p.cols)
                 store4(p.w, p.type_w, k * p.stride_w + (row0 + r) * p.ld_w + col0 + c,
-                       make_float4(fmaf(p.keep, w[n].x, at(r, c)), fmaf(p.keep, w[n].y, at(r, c + 1)), fmaf(p.keep, w[n].z, at(r, c + 2)), fmaf(p.keep, w[n].w, at(r, c + 3))));
+                       make_float4(fmaf(p.keep, y.x, at(r, c)), fmaf(p.keep, y.y, at(r, c + 1)), fmaf(p.keep, y.z, at(r, c + 2)), fmaf(p.keep, y.w, at(r, c + 3))));
         }
         return;
     }
     // an element a thread, neighbouring threads along the caller's row
-    float w[16];
+    uint32_t w[16];
 #pragma unroll
     for (int n = 0; n < 16; n++) {
         const int x = tid & 63, y = (tid >> 6) + 4 * n, r = p.tall ? x : y, c = p.tall ? y : x;
         const long long o = k * p.stride_w + (p.tall ? (col0 + c) * p.ld_w + row0 + r : (row0 + r) * p.ld_w + col0 + c);
-        w[n] = p.keep != 0.f && row0 + r < p.rows && col0 + c < p.cols ? load1(p.w, p.type_w, o) : 0.f;
+        w[n] = p.keep != 0.f && row0 + r < p.rows && col0 + c < p.cols ? bits1(p.w, p.type_w, o) : 0;
     }
 #pragma unroll
     for (int n = 0; n < 16; n++) {
         const int x = tid & 63, y = (tid >> 6) + 4 * n, r = p.tall ? x : y, c = p.tall ? y : x;
         const long long o = k * p.stride_w + (p.tall ? (col0 + c) * p.ld_w + row0 + r : (row0 + r) * p.ld_w + col0 + c);
-        if (row0 + r < p.rows && col0 + c < p.cols) store1(p.w, p.type_w, o, fmaf(p.keep, w[n], at(r, c)));
+        if (row0 + r < p.rows && col0 + c < p.cols) store1(p.w, p.type_w, o, fmaf(p.keep, value1(w[n], p.type_w), at(r, c)));
     }
 }
 
@@ -838,7 +908,17 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
             if (p.mode == ORTH_RESULT && p.keep != 0.f) prefetch_result(p, lane, k, row0, col0, HALF);
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * HALF);
             uint32_t buf = g & 1u;
+            // the first piece of 64 columns this part owns. One plane: its weights a piece ahead; two planes, where the sums
+            // need the registers: half of them at a time, when they are needed.
+            constexpr int PIECE = 64, PIECES = HALF / PIECE;
+            const int piece0 = h * PIECES, own0 = (part + 8 * split - piece0) % split;
+            uint32_t w[2][PLANES == 1 ? 32 : 1];
+            const auto weights = [&](int cc, int half) {
+                if (p.mode == ORTH_RESULT && cc < PIECES) fetch_weights(p, w[half], 0, lane, k, row0, col0 + cc * PIECE + half * 32);
+            };
             if constexpr (PLANES == 1) {
+                weights(own0, 0);
+                weights(own0, 1);
                 ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
                 g++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -878,8 +958,6 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
             // where this warp's sums lie when parts meet: [part][CTA][warp][4 columns][lane][4]
             constexpr size_t WARP_SUMS = 32 * HALF, part_step = (size_t)CTAS * 8 * WARP_SUMS;
             const size_t sums_at = (((size_t)cl * split * CTAS + rank) * 8 + e) * WARP_SUMS + lane * 4;
-            constexpr int PIECE = 64, PIECES = HALF / PIECE;                // columns that have one owner
-            const int piece0 = h * PIECES;
             if (split > 1) {
 #pragma unroll 1
                 for (int cc = 0; ok && cc < HALF / 32; cc++) {
@@ -900,8 +978,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
             // behind the last tile the operand stages are free: every box has its own place there and none waits for another
             const bool roomy = item + C >= items;
 #pragma unroll 1
-            for (int cc = 0; ok && cc < PIECES; cc++) {
-                if (split > 1 && (piece0 + cc) % split != part) continue;
+            for (int cc = own0; ok && cc < PIECES; cc += split) {
                 const int col = col0 + cc * PIECE;
                 // both warps of a store agree: its first row and column decide
                 if (row0 - (q & 1) * 32 >= p.rows || col >= p.cols) break;
@@ -926,7 +1003,19 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
 #pragma unroll
                     for (int c = 0; c < 32; c++) v[c] *= p.alpha;
                     if (p.mode == ORTH_RESULT) {
-                        store_result(p, v, staging + (uint32_t)e * 4096u, lane, k, row0, col + half * 32);
+                        const uint32_t own = staging + (uint32_t)e * 4096u;
+                        const int c0 = col + half * 32;
+                        if (!p.tall) put_result(v, own, lane);
+                        if constexpr (PLANES == 1) {
+                            store_result<32, 0>(p, v, w[half], own, lane, k, row0, c0);
+                            weights(cc + split, half);
+                        } else {
+                            uint32_t x[16];
+                            fetch_weights(p, x, 0, lane, k, row0, c0);
+                            store_result<16, 0>(p, v, x, own, lane, k, row0, c0);
+                            fetch_weights(p, x, 16, lane, k, row0, c0);
+                            store_result<16, 16>(p, v, x, own, lane, k, row0, c0);
+                        }
                         continue;
                     }
                     if (tiles.sym && i == j) {
