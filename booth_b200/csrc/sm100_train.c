@@ -262,45 +262,63 @@ static int orth_clusters(sm100_dev_t *dev, int ctas)
     return dev->orth_clusters[ctas];
 }
 
-typedef struct { int side, split; long long tiles; } orth_plan_t;
+typedef struct { int side, split; long long tiles; double us; } orth_plan_t;
 
-/* Tile side of a product and the parts its K is cut into: the shortest estimate in clocks.
- * A K block of 64 takes a pair 512 clocks of the tensor pipe a plane product (one, or
- * three); the smaller tiles read shared memory faster than it delivers, measured 512
- * and 1250 for 128, 250 and 500 for 64. A wave's epilogue costs some 3000, 2000 and 1000, and
- * parts that meet 3000. K is shared only while everything runs at once. Rows
- * may span two tiles of the stored triangle, not more (see the kernel). */
-static orth_plan_t orth_plan(sm100_dev_t *dev, const orth_product_t *p, int two_planes)
+/* One product with a given tile side: the parts its K is cut into and how long it takes,
+ * in microseconds measured in a chain of products (one plane, two planes). A product costs
+ * `base`, a K block of 64 `block` (64-tiles slow one another down in L2: .001 more for every CTA), a
+ * further wave its K blocks or, if that is longer, its epilogue; parts meet at `meet`. Per
+ * 1000 x 1000 x 1000 product in two planes that makes 10 us with 64-tiles, 13 with 128 and 12 with 256
+ * in three or four parts; at 2048 cubed 59, 36 and 46, and at 2048 x 4096 the largest tile wins.
+ * K is shared only while everything runs at once. */
+static orth_plan_t orth_product_plan(sm100_dev_t *dev, int side, long long rows, long long cols, long long K, int batch, int sym, int two_planes)
 {
-    static const double block[3][2] = { { 250, 500 }, { 512, 1250 }, { 512, 1536 } }, wave[3] = { 1000, 2000, 3000 };
-    const int sym = p->mode <= ORTH_POLY;
-    const long long kb = (p->K + 63) / 64, chunks = (kb + 1) / 2;
-    orth_plan_t best = { 0, 1, 0 };
-    double least = 0.0;
-    for (int f = 0; f < 3; f++) {
-        const int side = 64 << f, ctas = side == 256 ? 2 : 1;
-        if (p->mode != ORTH_GRAM && side > 2 * p->tri) break;
-        const long long m = (p->rows + side - 1) / side, n = (p->cols + side - 1) / side, tiles = p->batch * (sym ? m * (m + 1) / 2 : m * n);
-        for (int s = 1; s * ctas <= 8 && s <= chunks; s++) {
-            const long long slots = orth_clusters(dev, s * ctas), waves = (tiles + slots - 1) / slots;
-            if (s > 1 && (waves > 1 || s * ctas * tiles > dev->sm_count)) break;
-            const double cost = (double)waves * (wave[f] + (s > 1 ? 3000.0 : 0.0) + 2.0 * ((chunks + s - 1) / s) * block[f][two_planes]);
-            if (!best.side || cost < least) { least = cost; best.side = side; best.split = s; best.tiles = tiles; }
-        }
+    static const struct { double base[2], block[2], epilogue, meet; } cost[3] = {
+        { { 3.3, 3.9 }, { 0.22, 0.26 }, 1.5, 1.0 }, { { 4.3, 5.0 }, { 0.33, 0.80 }, 3.0, 2.0 }, { { 6.0, 7.5 }, { 0.32, 0.85 }, 5.0, 3.0 } };
+    const int f = side == 64 ? 0 : side == 128 ? 1 : 2, ctas = side == 256 ? 2 : 1;
+    const long long m = (rows + side - 1) / side, n = (cols + side - 1) / side, chunks = (K + 127) / 128;
+    orth_plan_t best = { side, 1, batch * (sym ? m * (m + 1) / 2 : m * n), 0.0 };
+    for (int s = 1; s * ctas <= 8 && s <= chunks; s++) {
+        const long long slots = orth_clusters(dev, s * ctas), waves = (best.tiles + slots - 1) / slots;
+        if (s > 1 && (waves > 1 || s * ctas * best.tiles > dev->sm_count)) break;
+        const double running = (double)(best.tiles < slots ? best.tiles : slots) * s;
+        const double blocks = 2.0 * ((chunks + s - 1) / s) * (cost[f].block[two_planes] + (f == 0 ? 0.001 * running : 0.0));
+        const double us = cost[f].base[two_planes] + blocks + (waves - 1) * fmax(blocks, cost[f].epilogue) + (s > 1 ? cost[f].meet : 0.0);
+        if (s == 1 || us < best.us) { best.us = us; best.split = s; }
     }
     return best;
 }
 
-static int orth_launch(sm100_dev_t *dev, const plane_maps_t *a, const plane_maps_t *b, const plane_maps_t *out, orth_product_t *p, int two_planes)
+/* Forms of a step's three products, chosen together: rows of a product may span two tiles of the triangle that the
+ * product before it stored, not more (see the kernel), so small tiles for S and Q keep the update from large ones. */
+static void orth_plan(sm100_dev_t *dev, const orth_layout_t *o, int batch, int poly, int two_planes, orth_plan_t plan[3])
 {
-    const orth_plan_t plan = orth_plan(dev, p, two_planes);
-    const int ctas = (plan.side == 256 ? 2 : 1) * plan.split, form = plan.side == 64 ? 0 : plan.side == 128 ? 2 : 4;
+    orth_plan_t g[3], q[3], u[3];
+    double best = 0.0;
+    for (int f = 0; f < 3; f++) {
+        g[f] = orth_product_plan(dev, 64 << f, o->s, o->s, o->l, batch, 1, two_planes);
+        q[f] = orth_product_plan(dev, 64 << f, o->s, o->s, o->s, batch, 1, two_planes);
+        u[f] = orth_product_plan(dev, 64 << f, o->s, o->l, o->s, batch, 0, two_planes);
+    }
+    for (int i = 0; i < 3; i++)
+        for (int j = 0; j < 3; j++)
+            for (int k = 0; k < 3; k++) {
+                if (poly ? j > i + 1 || k > j + 1 : j != i || k > i + 1) continue;
+                const double us = g[i].us + (poly ? q[j].us : 0.0) + u[k].us;
+                if (best == 0.0 || us < best) { best = us; plan[0] = g[i]; plan[1] = q[j]; plan[2] = u[k]; }
+            }
+}
+
+static int orth_launch(sm100_dev_t *dev, const orth_plan_t *plan, const plane_maps_t *a, const plane_maps_t *b, const plane_maps_t *out,
+                       orth_product_t *p, int two_planes)
+{
+    const int ctas = (plan->side == 256 ? 2 : 1) * plan->split, form = plan->side == 64 ? 0 : plan->side == 128 ? 2 : 4;
     /* a shared tile's cluster takes that one tile: the parts meet a fixed number of times */
-    const long long slots = orth_clusters(dev, ctas), groups = plan.split > 1 || plan.tiles < slots ? plan.tiles : slots;
-    p->split = plan.split;
+    const long long slots = orth_clusters(dev, ctas), groups = plan->split > 1 || plan->tiles < slots ? plan->tiles : slots;
+    p->split = plan->split;
     void *args[] = { (void *)&a->hi, (void *)&a->lo, (void *)&b->hi, (void *)&b->lo, (void *)&out->hi, (void *)&out->lo, p };
     const int rc = sm100_launch_k_cluster(dev, SM100_K_ORTH_PRODUCT + form + (two_planes ? 1 : 0), (unsigned)(groups * ctas), (unsigned)ctas, 384, ORTH_SMEM, args);
-    if (p->mode <= ORTH_POLY) p->tri = plan.side;       /* how the product that reads this one finds its triangle */
+    if (p->mode <= ORTH_POLY) p->tri = plan->side;      /* how the product that reads this one finds its triangle */
     return rc;
 }
 
@@ -365,6 +383,8 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
     double qs = 16384.0;
     while (qs * most > 60000.0) qs *= 0.5;
 
+    orth_plan_t plan[3];
+    orth_plan(dev, o, batch, c != 0.0, two_planes, plan);
     orth_product_t q = *last;
     q.batch = batch;
     q.sums = ws + o->sums;
@@ -376,18 +396,18 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
         q.mode = ORTH_GRAM; q.K = (int)o->l; q.lo = two_planes;
         if (c == 0.0) {
             q.alpha = (float)(b * qs / (xs * xs)); q.diag = (float)(a * qs);
-            if ((rc = orth_launch(dev, &x[from], &x[from], &qm, &q, two_planes)) != SM100_OK) return rc;
+            if ((rc = orth_launch(dev, &plan[0], &x[from], &x[from], &qm, &q, two_planes)) != SM100_OK) return rc;
         } else {
             q.alpha = (float)(ss / (xs * xs)); q.diag = (float)(beta * ss);
-            if ((rc = orth_launch(dev, &x[from], &x[from], &sm, &q, two_planes)) != SM100_OK) return rc;
+            if ((rc = orth_launch(dev, &plan[0], &x[from], &x[from], &sm, &q, two_planes)) != SM100_OK) return rc;
             q.mode = ORTH_POLY; q.K = (int)o->s;
             q.alpha = (float)(c * qs / (ss * ss)); q.diag = (float)(gamma * qs);
-            if ((rc = orth_launch(dev, &sm, &sm, &qm, &q, two_planes)) != SM100_OK) return rc;
+            if ((rc = orth_launch(dev, &plan[1], &sm, &sm, &qm, &q, two_planes)) != SM100_OK) return rc;
         }
         q.mode = end ? ORTH_RESULT : ORTH_UPDATE; q.K = (int)o->s; q.lo = 1;
         q.cols = (int)o->l;
         q.alpha = (float)(end ? factor / (qs * xs) : 1.0 / qs); q.diag = 0.0f;
-        if ((rc = orth_launch(dev, &qm, &x[from], &x[to], &q, two_planes)) != SM100_OK) return rc;
+        if ((rc = orth_launch(dev, &plan[2], &qm, &x[from], &x[to], &q, two_planes)) != SM100_OK) return rc;
     }
     return SM100_OK;
 }

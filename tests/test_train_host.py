@@ -104,7 +104,7 @@ go(3, 1000, 500, sm.F32, 1)
 d.sync(); d.close()
 """)
     assert res.returncode == 0, res.stderr
-    assert [l["kernel"] for l in L] == ["orth_norm", "orth_split"] + ["orth_product_1_256"] * 6 + ["orth_norm", "orth_split"] + ["orth_product_2_128"] * 3
+    assert [l["kernel"] for l in L] == ["orth_norm", "orth_split"] + ["orth_product_1_256"] * 6 + ["orth_norm", "orth_split", "orth_product_2_64", "orth_product_2_64", "orth_product_2_128"]
     assert all(l["overlap"] == 1 for l in L)
     assert all(l["shmem"] == 230400 and l["block"] == (384, 1, 1) for l in L if l["kernel"].startswith("orth_product"))
     P = products(lines)
@@ -118,7 +118,7 @@ d.sync(); d.close()
     for p, k in zip(P, (0, 1, 2, 0, 1, 3, 0, 1, 3)):
         assert (p["alpha"], p["diag"]) == pytest.approx(want[k], rel=1e-6)
     maps = [ln for ln in lines if ln.startswith("tensormap3")]
-    # one plane: hi and lo of both copies of X, A and P; rows a multiple of 64 apart
+    # one plane: hi and lo of both copies of X, S and Q; rows a multiple of 64 apart
     assert maps[:6] == ["tensormap3 dims 4096 4096 1 strides 8192 33554432 box 64 64 1"] * 6
     assert maps[6:] == ["tensormap3 dims 1000 500 3 strides 2048 1024000 box 64 64 1"] * 4 + ["tensormap3 dims 500 500 3 strides 1024 512000 box 64 64 1"] * 4
 
@@ -133,7 +133,7 @@ d.sync(); d.close()
     assert res.returncode == 0, res.stderr
     P = products(lines)
     assert [p["mode"] for p in P] == [0, 2, 0, 3]
-    assert [P[0]["alpha"], P[0]["diag"], P[1]["alpha"]] == pytest.approx([-0.5 * 2.0 ** -15, 1.5 * 2 ** 13, 2.0 ** -13])
+    assert [P[0]["alpha"], P[0]["diag"], P[1]["alpha"]] == pytest.approx([-0.5 * 2.0 ** -14, 1.5 * 2 ** 14, 2.0 ** -14])
 
 
 def test_muon_parameters(fake3, tmp_path):
