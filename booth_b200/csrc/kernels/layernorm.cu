@@ -7,12 +7,16 @@
 //     dx = rstd (w dy - p - xhat q);   dw = sum over rows of dy xhat;   db = sum over rows of dy
 //
 // Both read every value once and write every result once, so HBM bounds them. A
-// row belongs to one group of threads that keeps it in registers: 1 to 32 lanes of
-// a warp for narrow rows, a whole block for wider ones, 8, 16 or 32 values a
-// thread. The mean is taken first and the variance from the differences (the
-// row is in registers, a second pass costs no memory), with the differences' own
-// mean as a correction, so a row far from zero loses nothing. Blocks stay and walk
-// over the rows; the next row's loads are issued before the current row is reduced.
+// row belongs to one group of threads: 1 to 32 lanes of a warp for narrow rows, a whole
+// block for wider ones, 8 or 16 values a thread. The mean is taken first and the variance
+// from the differences (the row is on chip, a second pass costs no memory), with the
+// differences' own mean as a correction, so a row far from zero loses nothing.
+//
+// Blocks stay and walk over the rows. Vector forms keep the next few rows on their way
+// with cp.async into a ring in shared memory, in which every thread has places of its
+// own for what it alone reads, so the ring needs no barrier; with the next row held in
+// registers instead, 16 KB an SM were in flight and 16384 x 4096 bf16 took 116 us forward
+// and 128 backward.
 //
 // The backward pass walks the rows once for all three results: each thread adds dy
 // and dy xhat of its own columns into registers over all the rows its block sees,
@@ -22,10 +26,11 @@
 // Sums, statistics and products are fp32 (the last sum over the blocks double);
 // values are rounded to the tensor's type once, when they are stored.
 //
-// Forms: v8, v16, v32 read 16-byte vectors (row starts and parameters 16-byte
-// aligned, cols a multiple of the vector); s8, s16 read single elements, neighbouring
-// threads on neighbouring columns, for any alignment; loop goes through the row
-// several times from cache, for rows no block can hold.
+// Forms: v8, v16, vw read 16-byte vectors (row starts and parameters 16-byte
+// aligned, cols a multiple of the vector), vw up to 1024 threads a row with the parameters
+// from cache; s8, s16 read single elements, neighbouring threads on neighbouring
+// columns, for any alignment; loop goes through the row several times from
+// cache, for rows no block can hold.
 #include "common.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -110,6 +115,45 @@ __device__ __forceinline__ void load_row(Chunk<T, E> (&c)[NCH], const T *row, co
     }
 }
 
+// The ring: `depth` rows ahead of A arrays; chunk j of array a of a stage at ((stage A + a) NCH + j) blockDim 16 bytes,
+// 16 bytes a thread. Every row position commits one group, with or without copies, so that the count of groups
+// tells which row has landed.
+template <int A, int NCH> struct Ring {
+    uint32_t base, row_bytes;
+    int depth, stage;
+    __device__ __forceinline__ Ring(int depth_) : depth(depth_), stage(0)
+    {
+        extern __shared__ uint4 ln_ring[];
+        base = (uint32_t)__cvta_generic_to_shared(ln_ring) + threadIdx.x * 16u;
+        row_bytes = blockDim.x * 16u;
+    }
+    __device__ __forceinline__ uint32_t at(int a, int j) const { return base + (uint32_t)((stage * A + a) * NCH + j) * row_bytes; }
+    template <typename T, int E> __device__ __forceinline__ void fetch(int a, const T *row, const Group &g, int cols, bool live) const
+    {
+#pragma unroll
+        for (int j = 0; j < NCH; j++) {
+            const int col = (j * g.size + g.t) * E;
+            if (live && col < cols) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(a, j)), "l"(row + col) : "memory");
+        }
+    }
+    __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    __device__ __forceinline__ void next() { stage = stage + 1 == depth ? 0 : stage + 1; }
+    // This thread's oldest outstanding row has landed.
+    __device__ __forceinline__ void wait() const
+    {
+        if (depth == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+        else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    template <typename T, int E> __device__ __forceinline__ Chunk<T, E> get(int a, int j, bool live) const
+    {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at(a, j)) : "memory");
+        return *reinterpret_cast<const Chunk<T, E> *>(&v);
+    }
+};
+
 // Mean and 1/deviation of a row held as NCH chunks.
 template <typename T, int E, int NCH>
 __device__ __forceinline__ void row_stats(const Chunk<T, E> (&c)[NCH], Group &g, int cols, float eps, float2 (*sh)[32], float &mean, float &rstd)
@@ -134,40 +178,61 @@ __device__ __forceinline__ void row_stats(const Chunk<T, E> (&c)[NCH], Group &g,
     if (!(t.y == t.y)) rstd = t.y;                               // fmaxf drops a NaN; the row keeps it
 }
 
-template <typename T, typename W, bool VEC, int CPT>
+template <typename T, typename W, bool VEC, int CPT, bool HOLD>
 __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__ x, const W *__restrict__ w, const W *__restrict__ b,
                                         float *__restrict__ mean_out, float *__restrict__ rstd_out, long long rows, int cols,
-                                        long long ldx, long long ldy, float eps, int group)
+                                        long long ldx, long long ldy, float eps, int group, int depth)
 {
     constexpr int E = VEC ? 16 / (int)sizeof(T) : 1, NCH = CPT / E;
-    constexpr bool HOLD = CPT <= 16;            // parameters and the next row in registers too
     __shared__ float2 sh[2][32];
     Group g(group);
-    float pw[HOLD ? NCH : 1][E], pb[HOLD ? NCH : 1][E];
+    float pw[HOLD ? NCH : 1][E], pb[HOLD ? NCH : 1][E];         // the parameters of this thread's columns
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    if constexpr (HOLD) {
-#pragma unroll
-        for (int j = 0; j < NCH; j++) {
-            const int col = (j * g.size + g.t) * E;
-#pragma unroll
-            for (int e = 0; e < E; e++) { pw[j][e] = 1.f; pb[j][e] = 0.f; }
-            if (col < cols) {
-                if (w) load_params<W, E>(w, col, pw[j]);
-                if (b) load_params<W, E>(b, col, pb[j]);
-            }
-        }
-    }
     const long long step = (long long)gridDim.x * g.per_block;
     long long base = (long long)blockIdx.x * g.per_block;
-    Chunk<T, E> cur[NCH];
-    load_row<T, E, NCH>(cur, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
+    Ring<1, VEC ? NCH : 1> ring(depth);
+    Chunk<T, E> cur[NCH], nxt[VEC ? 1 : NCH];
+    if constexpr (VEC) {
+        for (int d = 0; d < depth; d++) {
+            const long long row = base + g.index + d * step;
+            ring.template fetch<T, E>(0, x + row * ldx, g, cols, row < rows);
+            ring.commit();
+            ring.next();
+        }
+    } else {
+        load_row<T, E, NCH>(cur, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
+    }
+    const auto params = [&](int j, float (&qw)[E], float (&qb)[E]) {
+        const int col = (j * g.size + g.t) * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) { qw[e] = 1.f; qb[e] = 0.f; }
+        if (col < cols) {
+            if (w) load_params<W, E>(w, col, qw);
+            if (b) load_params<W, E>(b, col, qb);
+        }
+    };
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int j = 0; j < NCH; j++) params(j, pw[j], pb[j]);
+    }
     for (; base < rows; base += step) {
         const long long row = base + g.index;
-        Chunk<T, E> nxt[HOLD ? NCH : 1];
-        if constexpr (HOLD) load_row<T, E, NCH>(nxt, x + (row + step) * ldx, g, cols, row + step < rows);
+        if constexpr (VEC) {
+            ring.wait();
+#pragma unroll
+            for (int j = 0; j < NCH; j++) cur[j] = ring.template get<T, E>(0, j, row < rows && (j * g.size + g.t) * E < cols);
+        } else {
+            load_row<T, E, NCH>(nxt, x + (row + step) * ldx, g, cols, row + step < rows);
+        }
         float mean, rstd;
         row_stats<T, E, NCH>(cur, g, cols, eps, sh, mean, rstd);
+        if constexpr (VEC) {                    // the row is in registers: its places may fill again
+            const long long ahead = row + depth * step;
+            ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
+            ring.commit();
+            ring.next();
+        }
         if (row < rows) {
             if (g.t == 0) {
                 if (mean_out) mean_out[row] = mean;
@@ -184,10 +249,7 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                         for (int e = 0; e < E; e++) o.v[e] = from_f32<T>(fmaf((to_f32(cur[j].v[e]) - mean) * rstd, pw[j][e], pb[j][e]));
                     } else {
                         float qw[E], qb[E];
-#pragma unroll
-                        for (int e = 0; e < E; e++) { qw[e] = 1.f; qb[e] = 0.f; }
-                        if (w) load_params<W, E>(w, col, qw);
-                        if (b) load_params<W, E>(b, col, qb);
+                        params(j, qw, qb);
 #pragma unroll
                         for (int e = 0; e < E; e++) o.v[e] = from_f32<T>(fmaf((to_f32(cur[j].v[e]) - mean) * rstd, qw[e], qb[e]));
                     }
@@ -195,11 +257,9 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                 }
             }
         }
-        if constexpr (HOLD) {
+        if constexpr (!VEC) {
 #pragma unroll
             for (int j = 0; j < NCH; j++) cur[j] = nxt[j];
-        } else {
-            load_row<T, E, NCH>(cur, x + (row + step) * ldx, g, cols, row + step < rows);
         }
     }
 }
@@ -235,63 +295,73 @@ __device__ __forceinline__ void forward_loop(T *y, const T *x, const W *__restri
 }
 
 // Adds dy and dy xhat of each thread's columns over the rows of its block (partial,
-// when asked for: [block][2][cols]) and writes dx (when asked for).
-template <typename T, typename W, bool VEC, int CPT>
+// when asked for: [block][2][cols]) and writes dx (when asked for). A vector row is read from its ring places twice,
+// for the two sums and for dx, and its places are filled again right behind the second read.
+template <typename T, typename W, bool VEC, int CPT, bool HOLD>
 __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__ partial, const T *__restrict__ dy, const T *__restrict__ x,
                                          const W *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-                                         long long rows, int cols, long long lddx, long long lddy, long long ldx, int group)
+                                         long long rows, int cols, long long lddx, long long lddy, long long ldx, int group, int depth)
 {
     constexpr int E = VEC ? 16 / (int)sizeof(T) : 1, NCH = CPT / E;
-    constexpr bool HOLD = CPT <= 16;            // the weight and the next row in registers too
     __shared__ float2 sh[2][32];
     __shared__ float part[2][256];              // narrow rows: the block's groups add up here
     Group g(group);
     float pw[HOLD ? NCH : 1][E], aw[NCH][E], ab[NCH][E];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-#pragma unroll
-    for (int j = 0; j < NCH; j++) {
-        const int col = (j * g.size + g.t) * E;
-#pragma unroll
-        for (int e = 0; e < E; e++) { aw[j][e] = 0.f; ab[j][e] = 0.f; }
-        if constexpr (HOLD) {
-#pragma unroll
-            for (int e = 0; e < E; e++) pw[j][e] = 1.f;
-            if (w && col < cols) load_params<W, E>(w, col, pw[j]);
-        }
-    }
     const float inv = 1.f / (float)cols;
     const long long step = (long long)gridDim.x * g.per_block;
     long long base = (long long)blockIdx.x * g.per_block;
-    Chunk<T, E> cx[NCH], cd[NCH];
+    Ring<2, VEC ? NCH : 1> ring(depth);
+    Chunk<T, E> sx[VEC ? 1 : NCH], sd[VEC ? 1 : NCH], nx[VEC ? 1 : NCH], nd[VEC ? 1 : NCH];
+    if constexpr (VEC) {
+        for (int d = 0; d < depth; d++) {
+            const long long row = base + g.index + d * step;
+            ring.template fetch<T, E>(0, x + row * ldx, g, cols, row < rows);
+            ring.template fetch<T, E>(1, dy + row * lddy, g, cols, row < rows);
+            ring.commit();
+            ring.next();
+        }
+    } else {
+        load_row<T, E, NCH>(sx, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
+        load_row<T, E, NCH>(sd, dy + (base + g.index) * lddy, g, cols, base + g.index < rows);
+    }
+    const auto weight = [&](int j, float (&q)[E]) {
+        const int col = (j * g.size + g.t) * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) q[e] = 1.f;
+        if (w && col < cols) load_params<W, E>(w, col, q);
+    };
+#pragma unroll
+    for (int j = 0; j < NCH; j++) {
+#pragma unroll
+        for (int e = 0; e < E; e++) { aw[j][e] = 0.f; ab[j][e] = 0.f; }
+        if constexpr (HOLD) weight(j, pw[j]);
+    }
     float cm = 0.f, cr = 0.f;
     if (base + g.index < rows) { cm = mean_in[base + g.index]; cr = rstd_in[base + g.index]; }
-    load_row<T, E, NCH>(cx, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
-    load_row<T, E, NCH>(cd, dy + (base + g.index) * lddy, g, cols, base + g.index < rows);
     for (; base < rows; base += step) {
         const long long row = base + g.index, next = row + step;
-        Chunk<T, E> nx[HOLD ? NCH : 1], nd[HOLD ? NCH : 1];
         float nm = 0.f, nr = 0.f;
         if (next < rows) { nm = mean_in[next]; nr = rstd_in[next]; }
-        if constexpr (HOLD) {
+        if constexpr (VEC) ring.wait();
+        else {
             load_row<T, E, NCH>(nx, x + next * ldx, g, cols, next < rows);
             load_row<T, E, NCH>(nd, dy + next * lddy, g, cols, next < rows);
         }
         float s1 = 0.f, s2 = 0.f;
-        // columns past the end and rows past the last have dy = 0 (and mean = rstd = 0): they add nothing
+        // rows past the last have dy = 0 (and mean = rstd = 0): they add nothing
 #pragma unroll
         for (int j = 0; j < NCH; j++) {
-            const int col = (j * g.size + g.t) * E;
-            float qw[E];
-            if constexpr (!HOLD) {
-#pragma unroll
-                for (int e = 0; e < E; e++) qw[e] = 1.f;
-                if (w && col < cols) load_params<W, E>(w, col, qw);
-            }
-            if (col < cols) {
+            if ((j * g.size + g.t) * E < cols) {
+                float qw[E];
+                if constexpr (!HOLD) weight(j, qw);
+                Chunk<T, E> cx, cd;
+                if constexpr (VEC) { cx = ring.template get<T, E>(0, j, row < rows); cd = ring.template get<T, E>(1, j, row < rows); }
+                else { cx = sx[j]; cd = sd[j]; }
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const float d = to_f32(cd[j].v[e]), xh = (to_f32(cx[j].v[e]) - cm) * cr;
+                    const float d = to_f32(cd.v[e]), xh = (to_f32(cx.v[e]) - cm) * cr;
                     const float wd = d * (HOLD ? pw[HOLD ? j : 0][e] : qw[e]);
                     s1 += wd;
                     s2 = fmaf(wd, xh, s2);
@@ -309,16 +379,14 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                 const int col = (j * g.size + g.t) * E;
                 if (col < cols) {
                     float qw[E];
-                    if constexpr (!HOLD) {
-#pragma unroll
-                        for (int e = 0; e < E; e++) qw[e] = 1.f;
-                        if (w) load_params<W, E>(w, col, qw);
-                    }
-                    Chunk<T, E> o;
+                    if constexpr (!HOLD) weight(j, qw);
+                    Chunk<T, E> cx, cd, o;
+                    if constexpr (VEC) { cx = ring.template get<T, E>(0, j, true); cd = ring.template get<T, E>(1, j, true); }
+                    else { cx = sx[j]; cd = sd[j]; }
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        const float xh = (to_f32(cx[j].v[e]) - cm) * cr;
-                        const float wd = to_f32(cd[j].v[e]) * (HOLD ? pw[HOLD ? j : 0][e] : qw[e]);
+                        const float xh = (to_f32(cx.v[e]) - cm) * cr;
+                        const float wd = to_f32(cd.v[e]) * (HOLD ? pw[HOLD ? j : 0][e] : qw[e]);
                         o.v[e] = from_f32<T>(cr * (wd - p - xh * q));
                     }
                     *reinterpret_cast<Chunk<T, E> *>(out + col) = o;
@@ -326,12 +394,15 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
             }
         }
         cm = nm; cr = nr;
-        if constexpr (HOLD) {
-#pragma unroll
-            for (int j = 0; j < NCH; j++) { cx[j] = nx[j]; cd[j] = nd[j]; }
+        if constexpr (VEC) {
+            const long long ahead = row + depth * step;
+            ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
+            ring.template fetch<T, E>(1, dy + ahead * lddy, g, cols, ahead < rows);
+            ring.commit();
+            ring.next();
         } else {
-            load_row<T, E, NCH>(cx, x + next * ldx, g, cols, next < rows);
-            load_row<T, E, NCH>(cd, dy + next * lddy, g, cols, next < rows);
+#pragma unroll
+            for (int j = 0; j < NCH; j++) { sx[j] = nx[j]; sd[j] = nd[j]; }
         }
     }
     if (!partial) return;
@@ -424,12 +495,12 @@ __device__ __forceinline__ void backward_columns(float *__restrict__ partial, co
     out[cols + c] = ab;
 }
 
-// dw and db: column sums of the `parts` partial rows, 32 columns a block, eight
+// dw and db: column sums of the `parts` partial rows, 32 columns a block, 32
 // threads on each column, in double and in a fixed order. blockIdx.y 0: dw, 1: db.
 template <typename W>
 __device__ __forceinline__ void param_grad(W *__restrict__ dw, W *__restrict__ db, const float *__restrict__ partial, int parts, int cols)
 {
-    __shared__ double sh[8][33];
+    __shared__ double sh[32][33];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     W *out = blockIdx.y ? db : dw;
@@ -439,42 +510,44 @@ __device__ __forceinline__ void param_grad(W *__restrict__ dw, W *__restrict__ d
     if (c < cols) {
         const float *p = partial + (size_t)blockIdx.y * cols + c;
 #pragma unroll 8
-        for (int i = ty; i < parts; i += 8) s += (double)__ldcg(p + (size_t)i * 2 * cols);
+        for (int i = ty; i < parts; i += 32) s += (double)__ldcg(p + (size_t)i * 2 * cols);
     }
     sh[ty][lane] = s;
     __syncthreads();
-    if (ty == 0 && c < cols) {
-        for (int k = 1; k < 8; k++) s += sh[k][lane];
-        out[c] = from_f32<W>((float)s);
-    }
+    // warp ty adds column ty of the block
+    s = sh[lane][ty];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int mine = (int)blockIdx.x * 32 + ty;
+    if (lane == 0 && mine < cols) out[mine] = from_f32<W>((float)s);
 }
 
 }  // namespace ln
 
-#define LN_FORM(name, T, W, form, VEC, CPT)                                                                                              \
-    extern "C" __global__ void __launch_bounds__(512)                                                                                    \
+#define LN_FORM(name, T, W, form, VEC, CPT, HOLD, THREADS)                                                                                \
+    extern "C" __global__ void __launch_bounds__(THREADS)                                                                                \
     layernorm_##name##_##form(T *y, const T *x, const W *w, const W *b, float *mean, float *rstd, long long rows, int cols,              \
-                              long long ldx, long long ldy, float eps, int group)                                                        \
-    { ln::forward<T, W, VEC, CPT>(y, x, w, b, mean, rstd, rows, cols, ldx, ldy, eps, group); }                                           \
-    extern "C" __global__ void __launch_bounds__(512)                                                                                    \
+                              long long ldx, long long ldy, float eps, int group, int depth)                                             \
+    { ln::forward<T, W, VEC, CPT, HOLD>(y, x, w, b, mean, rstd, rows, cols, ldx, ldy, eps, group, depth); }                              \
+    extern "C" __global__ void __launch_bounds__(THREADS)                                                                                \
     layernorm_bwd_##name##_##form(T *dx, float *partial, const T *dy, const T *x, const W *w, const float *mean, const float *rstd,      \
-                                  long long rows, int cols, long long lddx, long long lddy, long long ldx, int group)                    \
-    { ln::backward<T, W, VEC, CPT>(dx, partial, dy, x, w, mean, rstd, rows, cols, lddx, lddy, ldx, group); }
+                                  long long rows, int cols, long long lddx, long long lddy, long long ldx, int group, int depth)         \
+    { ln::backward<T, W, VEC, CPT, HOLD>(dx, partial, dy, x, w, mean, rstd, rows, cols, lddx, lddy, ldx, group, depth); }
 
 #define LN_KERNELS(name, T, W)                                                                                                           \
-    LN_FORM(name, T, W, v8, true, 8)                                                                                                     \
-    LN_FORM(name, T, W, v16, true, 16)                                                                                                   \
-    LN_FORM(name, T, W, v32, true, 32)                                                                                                   \
-    LN_FORM(name, T, W, s8, false, 8)                                                                                                    \
-    LN_FORM(name, T, W, s16, false, 16)                                                                                                  \
+    LN_FORM(name, T, W, v8, true, 8, true, 512)                                                                                          \
+    LN_FORM(name, T, W, v16, true, 16, true, 512)                                                                                        \
+    LN_FORM(name, T, W, vw, true, 16, false, 1024)                                                                                       \
+    LN_FORM(name, T, W, s8, false, 8, true, 512)                                                                                         \
+    LN_FORM(name, T, W, s16, false, 16, true, 512)                                                                                       \
     extern "C" __global__ void __launch_bounds__(512)                                                                                    \
     layernorm_##name##_loop(T *y, const T *x, const W *w, const W *b, float *mean, float *rstd, long long rows, int cols,                \
-                            long long ldx, long long ldy, float eps, int group)                                                          \
-    { (void)group; ln::forward_loop<T, W>(y, x, w, b, mean, rstd, rows, cols, ldx, ldy, eps); }                                          \
+                            long long ldx, long long ldy, float eps, int group, int depth)                                               \
+    { (void)group; (void)depth; ln::forward_loop<T, W>(y, x, w, b, mean, rstd, rows, cols, ldx, ldy, eps); }                             \
     extern "C" __global__ void __launch_bounds__(512)                                                                                    \
     layernorm_bwd_##name##_loop(T *dx, float *partial, const T *dy, const T *x, const W *w, const float *mean, const float *rstd,        \
-                                long long rows, int cols, long long lddx, long long lddy, long long ldx, int group)                      \
-    { (void)group; (void)partial; ln::backward_loop<T, W>(dx, dy, x, w, mean, rstd, rows, cols, lddx, lddy, ldx); }
+                                long long rows, int cols, long long lddx, long long lddy, long long ldx, int group, int depth)           \
+    { (void)group; (void)partial; (void)depth; ln::backward_loop<T, W>(dx, dy, x, w, mean, rstd, rows, cols, lddx, lddy, ldx); }
 
 LN_KERNELS(f32, float, float)
 LN_KERNELS(bf16, __nv_bfloat16, __nv_bfloat16)
@@ -487,7 +560,7 @@ LN_KERNELS(f16_f32, __half, float)
     layernorm_bwd_columns_##name(float *partial, const T *dy, const T *x, const float *mean, const float *rstd, long long rows,          \
                                  int cols, long long lddy, long long ldx)                                                                \
     { ln::backward_columns<T>(partial, dy, x, mean, rstd, rows, cols, lddy, ldx); }                                                      \
-    extern "C" __global__ void __launch_bounds__(256)                                                                                    \
+    extern "C" __global__ void __launch_bounds__(1024)                                                                                    \
     layernorm_param_grad_##name(T *dw, T *db, const float *partial, int parts, int cols)                                                 \
     { ln::param_grad<T>(dw, db, partial, parts, cols); }
 LN_COLUMNS(f32, float)

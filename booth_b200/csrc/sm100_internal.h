@@ -117,6 +117,7 @@ struct sm100_dev {
     int         gemm_pending;          /* a GEMM was enqueued since the last status check */
     int         gemm_smem_set;         /* dynamic shared memory limit raised on the GEMM kernels */
     unsigned    gemm_wait_ms;          /* limit of the GEMM kernel's barrier waits */
+    int         ln_smem_set;           /* dynamic shared memory limit raised on the layer normalisation kernels */
     int         orth_pending;          /* an orthogonalisation was enqueued since the last status check */
     int         orth_captured;         /* one was captured into a graph: its replays are not seen here */
     int         orth_clusters[9];      /* clusters of so many product CTAs the GPU holds at once (0 = not asked yet) */

@@ -144,7 +144,7 @@ int sm100_enter(sm100_dev_t *dev)
 
 /* ---- init / shut ---- */
 
-#define LN_FORM_NAMES(k) k "_v8", k "_v16", k "_v32", k "_s8", k "_s16", k "_loop"
+#define LN_FORM_NAMES(k) k "_v8", k "_v16", k "_vw", k "_s8", k "_s16", k "_loop"
 static const char *const k_names[SM100_K_COUNT] = {
     "vadd_stream", "saxpy_stream", "fill_philox",
     "reduce_sum_i32", "reduce_sum_f32",

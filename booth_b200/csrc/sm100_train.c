@@ -45,21 +45,27 @@ static int ln_pair(int dtype, int wdtype)
     return -1;
 }
 
-enum { LN_V8, LN_V16, LN_V32, LN_S8, LN_S16, LN_LOOP };
+enum { LN_V8, LN_V16, LN_VW, LN_S8, LN_S16, LN_LOOP };
 
-typedef struct { int form, group; unsigned block, grid; } ln_shape_t;
+/* Shared memory for rings: what an SM has less the blocks' own few KB. */
+#define LN_RING_SM (208u << 10)
+
+typedef struct { int form, group, depth; unsigned block, grid, ring; } ln_shape_t;
 
 /* How rows are dealt to threads. Eight values a thread for narrow rows, and for
  * rows so few that each has an SM to itself (more threads shorten the one row);
  * sixteen otherwise, which halves what the reductions and the barriers cost per
- * value; thirty-two for vector rows too wide for 512 threads at sixteen; else the
- * form that walks the row. Blocks stay: as many as an SM holds (`threads`), each
- * taking every grid-th row. */
-static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, int vec, int threads)
+ * value; vector rows too wide for 512 threads get up to 1024; else the form that walks
+ * the row. Blocks stay, each taking every grid-th row: as many as an SM holds by
+ * registers (64 a thread for eight values, 80 to 128 else), and of the vector
+ * forms' rings up to four rows each, as many as fit beside one another. */
+static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, unsigned esz, int vec, int backward)
 {
     ln_shape_t s;
-    int cpt = cols <= 1024 || (cols <= 4096 && rows < 2ll * dev->sm_count) ? 8 : cols <= 8192 ? 16 : cols <= 16384 && vec ? 32 : 0;
-    s.form = cpt == 8 ? (vec ? LN_V8 : LN_S8) : cpt == 16 ? (vec ? LN_V16 : LN_S16) : cpt == 32 ? LN_V32 : LN_LOOP;
+    const int cpt = cols <= 1024 || (cols <= 4096 && rows < 2ll * dev->sm_count) ? 8 : cols <= 8192 || (cols <= 16384 && vec) ? 16 : 0;
+    s.form = cpt == 8 ? (vec ? LN_V8 : LN_S8) : cpt == 16 ? (!vec ? LN_S16 : cols <= 8192 ? LN_V16 : LN_VW) : LN_LOOP;
+    s.depth = 1;
+    s.ring = 0;
     if (!cpt) {
         s.group = 512;
         s.block = 512;
@@ -71,11 +77,32 @@ static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, int
         s.block = g <= 32 ? 128u : (unsigned)g;
     }
     const long long per_block = s.group <= 32 ? (long long)s.block / s.group : 1;
-    long long want = (rows + per_block - 1) / per_block, per_sm = threads / (int)s.block;
-    if (per_sm < 1) per_sm = 1;
-    if (want > dev->sm_count * per_sm) want = dev->sm_count * per_sm;
+    const unsigned threads = cpt == 8 ? (backward && !vec ? 640u : 1024u) : backward ? 512u : 768u;
+    unsigned per_sm = threads / s.block < 1 ? 1 : threads / s.block;
+    if (s.form <= LN_VW) {
+        const unsigned row = s.block * (unsigned)cpt * esz * (backward ? 2u : 1u);
+        s.depth = 4;
+        while (s.depth > 2 && per_sm * (unsigned)s.depth * row > LN_RING_SM) s.depth--;
+        while (per_sm > 1 && per_sm * (unsigned)s.depth * row > LN_RING_SM) per_sm--;
+        if ((unsigned)s.depth * row > LN_RING_SM) s.depth = 1;
+        s.ring = (unsigned)s.depth * row;
+    }
+    long long want = (rows + per_block - 1) / per_block;
+    if (want > (long long)dev->sm_count * per_sm) want = (long long)dev->sm_count * per_sm;
     s.grid = (unsigned)(want < 1 ? 1 : want);
     return s;
+}
+
+static int ln_ready(sm100_dev_t *dev)
+{
+    if (dev->ln_smem_set) return SM100_OK;
+    for (int k = 0; k < 2 * 5 * SM100_LN_FORMS; k++) {
+        if (k % SM100_LN_FORMS > LN_VW) continue;
+        CUresult cr = dev->api->FuncSetAttribute(dev->k[SM100_K_LN_FWD + k], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)LN_RING_SM);
+        if (cr != CUDA_SUCCESS) return sm100_fail(dev, "raising the layer normalisation kernels' shared memory limit", cr);
+    }
+    dev->ln_smem_set = 1;
+    return SM100_OK;
 }
 
 int booth_sm100_layernorm(sm100_dev_t *dev, sm100_ptr_t y, sm100_ptr_t x, sm100_ptr_t w, sm100_ptr_t b,
@@ -93,15 +120,15 @@ int booth_sm100_layernorm(sm100_dev_t *dev, sm100_ptr_t y, sm100_ptr_t x, sm100_
         (x == y && ldx != ldy))
         return bad_arg(dev, "booth_sm100_layernorm: x and y non-NULL, every operand aligned to its element, pitches >= cols (equal ones when y is x)");
     const int vec = !(((x | y | w | b) & 15) || cols % (int)(16 / e) || ldx % (16 / e) || ldy % (16 / e));
-    const ln_shape_t s = ln_shape(dev, rows, cols, vec, 1024);
-    int group = s.group;
-    void *args[] = { &y, &x, &w, &b, &mean, &rstd, &rows, &cols, &ldx, &ldy, &eps, &group };
-    return sm100_launch_k_overlapped(dev, SM100_K_LN_FWD + pair * SM100_LN_FORMS + s.form, s.grid, s.block, 0, args);
+    if ((rc = ln_ready(dev)) != SM100_OK) return rc;
+    const ln_shape_t s = ln_shape(dev, rows, cols, e, vec, 0);
+    int group = s.group, depth = s.depth;
+    void *args[] = { &y, &x, &w, &b, &mean, &rstd, &rows, &cols, &ldx, &ldy, &eps, &group, &depth };
+    return sm100_launch_k_overlapped(dev, SM100_K_LN_FWD + pair * SM100_LN_FORMS + s.form, s.grid, s.block, s.ring, args);
 }
 
 /* Partial rows of the parameters' gradients: one a block, or one a row range in the walking form. */
 #define LN_LOOP_PARTS 64
-#define LN_BWD_THREADS 512
 
 size_t booth_sm100_layernorm_backward_workspace(sm100_dev_t *dev, long long rows, int cols, int dtype, int wdtype)
 {
@@ -111,7 +138,7 @@ size_t booth_sm100_layernorm_backward_workspace(sm100_dev_t *dev, long long rows
     }
     size_t parts = LN_LOOP_PARTS;
     for (int vec = 0; vec < 2; vec++) {
-        const ln_shape_t s = ln_shape(dev, rows, cols, vec, LN_BWD_THREADS);
+        const ln_shape_t s = ln_shape(dev, rows, cols, type_bytes(dtype), vec, 1);
         if (s.form != LN_LOOP && s.grid > parts) parts = s.grid;
     }
     return parts * 2 * (size_t)cols * sizeof(float);
@@ -139,13 +166,14 @@ int booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t
     int parts = 0;
     if (rows > 0 && (dx || params)) {
         const int vec = !(((x | dy | dx | w) & 15) || cols % (int)(16 / e) || ldx % (16 / e) || lddy % (16 / e) || (dx && lddx % (16 / e)));
-        const ln_shape_t s = ln_shape(dev, rows, cols, vec, LN_BWD_THREADS);
-        int group = s.group;
+        if ((rc = ln_ready(dev)) != SM100_OK) return rc;
+        const ln_shape_t s = ln_shape(dev, rows, cols, e, vec, 1);
+        int group = s.group, depth = s.depth;
         sm100_ptr_t partial = params ? ws : 0;
-        void *args[] = { &dx, &partial, &dy, &x, &w, &mean, &rstd, &rows, &cols, &lddx, &lddy, &ldx, &group };
+        void *args[] = { &dx, &partial, &dy, &x, &w, &mean, &rstd, &rows, &cols, &lddx, &lddy, &ldx, &group, &depth };
         parts = (int)s.grid;
         if (s.form != LN_LOOP || dx) {
-            rc = sm100_launch_k_overlapped(dev, SM100_K_LN_BWD + pair * SM100_LN_FORMS + s.form, s.grid, s.block, 0, args);
+            rc = sm100_launch_k_overlapped(dev, SM100_K_LN_BWD + pair * SM100_LN_FORMS + s.form, s.grid, s.block, s.ring, args);
             if (rc != SM100_OK) return rc;
         }
         if (s.form == LN_LOOP && params) {
@@ -157,7 +185,7 @@ int booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t
     }
     if (params) {
         void *pa[] = { &dw, &db, &ws, &parts, &cols };
-        rc = sm100_launch_k3_overlapped(dev, SM100_K_LN_PARAM_GRAD + type_index(wdtype), (unsigned)(((long long)cols + 31) / 32), 2, 1, 256, 1, 1, 0, pa);
+        rc = sm100_launch_k3_overlapped(dev, SM100_K_LN_PARAM_GRAD + type_index(wdtype), (unsigned)(((long long)cols + 31) / 32), 2, 1, 1024, 1, 1, 0, pa);
     }
     return rc;
 }
