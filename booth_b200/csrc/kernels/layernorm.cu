@@ -45,6 +45,39 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// Two fp32 values in a register pair: the packed forms do two operations an instruction, each rounded as by itself.
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair(float a, float b)
+{
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float2 split(Pair p)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ Pair add(Pair a, Pair b) { Pair r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ Pair mul(Pair a, Pair b) { Pair r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) { Pair r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+// Two neighbouring values of a chunk, to and from their type.
+__device__ __forceinline__ Pair widen(const float *v) { return pair(v[0], v[1]); }
+__device__ __forceinline__ Pair widen(const __nv_bfloat16 *v)
+{
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(v);
+    return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ Pair widen(const __half *v)
+{
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(v));
+    return pair(f.x, f.y);
+}
+__device__ __forceinline__ void narrow(float *v, Pair p) { const float2 f = split(p); v[0] = f.x; v[1] = f.y; }
+__device__ __forceinline__ void narrow(__nv_bfloat16 *v, Pair p) { const float2 f = split(p); *reinterpret_cast<__nv_bfloat162 *>(v) = __floats2bfloat162_rn(f.x, f.y); }
+__device__ __forceinline__ void narrow(__half *v, Pair p) { const float2 f = split(p); *reinterpret_cast<__half2 *>(v) = __floats2half2_rn(f.x, f.y); }
+
 // E values read or written by one access: 16 bytes, or one element (E = 1).
 template <typename T, int E> struct __align__(E * sizeof(T)) Chunk { T v[E]; };
 
@@ -74,32 +107,87 @@ struct Group {
         if (size > 32) { t = tid; index = 0; per_block = 1; }
         else { t = tid & (size - 1); index = tid / size; per_block = (int)blockDim.x / size; }
     }
-    // Sums of a and b over the group, the same bits in every thread. Called by all threads of
-    // the block in step. `sh` holds 2 x 32 values; the halves alternate, so one barrier a call is enough.
+    // Sums over the group, the same bits in every thread. Called by all threads of the block in step. `sh` holds
+    // 2 x 32 values; the halves alternate, so one barrier a call is enough.
     __device__ __forceinline__ float2 sum2(float a, float b, float2 (*sh)[32])
     {
-        const int top = size < 32 ? size : 32;
-        for (int o = top >> 1; o > 0; o >>= 1) {
+        if (size < 32) {
+            for (int o = size >> 1; o > 0; o >>= 1) {
+                a += __shfl_xor_sync(0xffffffffu, a, o);
+                b += __shfl_xor_sync(0xffffffffu, b, o);
+            }
+            return make_float2(a, b);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
             a += __shfl_xor_sync(0xffffffffu, a, o);
             b += __shfl_xor_sync(0xffffffffu, b, o);
         }
         if (size > 32) {
-            const int warps = size >> 5, lane = t & 31;
             float2 *s = sh[turn & 1];
             turn++;
-            if (lane == 0) s[t >> 5] = make_float2(a, b);
+            if ((t & 31) == 0) s[t >> 5] = make_float2(a, b);
             __syncthreads();
-            const float2 v = lane < warps ? s[lane] : make_float2(0.f, 0.f);
-            a = v.x; b = v.y;
+            const int warps = size >> 5;
+            if (warps <= 8) {           // a few broadcast reads are shorter than a second tree
+                a = b = 0.f;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                a += __shfl_xor_sync(0xffffffffu, a, o);
-                b += __shfl_xor_sync(0xffffffffu, b, o);
+                for (int i = 0; i < 8; i++)
+                    if (i < warps) { const float2 v = s[i]; a += v.x; b += v.y; }
+            } else {
+                const float2 v = (t & 31) < warps ? s[t & 31] : make_float2(0.f, 0.f);
+                a = v.x; b = v.y;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    a += __shfl_xor_sync(0xffffffffu, a, o);
+                    b += __shfl_xor_sync(0xffffffffu, b, o);
+                }
             }
         }
         return make_float2(a, b);
     }
+    __device__ __forceinline__ float sum(float a, float2 (*sh)[32])
+    {
+        if (size < 32) {
+            for (int o = size >> 1; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+            return a;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (size > 32) {
+            float *s = reinterpret_cast<float *>(sh[turn & 1]);
+            turn++;
+            if ((t & 31) == 0) s[t >> 5] = a;
+            __syncthreads();
+            const int warps = size >> 5;
+            if (warps <= 8) {
+                a = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (i < warps) a += s[i];
+            } else {
+                a = (t & 31) < warps ? s[t & 31] : 0.f;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+            }
+        }
+        return a;
+    }
 };
+
+// The values of NCH chunks of E as pairs; a lone value a chunk (E = 1) pairs with the next chunk's.
+template <typename T, int E, int NCH> __device__ __forceinline__ void widen_all(const Chunk<T, E> (&c)[NCH], Pair (&v)[NCH * E / 2])
+{
+    if constexpr (E == 1) {
+#pragma unroll
+        for (int i = 0; i < NCH / 2; i++) v[i] = pair(to_f32(c[2 * i].v[0]), to_f32(c[2 * i + 1].v[0]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < NCH; j++)
+#pragma unroll
+            for (int i = 0; i < E / 2; i++) v[j * E / 2 + i] = widen(&c[j].v[2 * i]);
+    }
+}
 
 template <typename T, int E, int NCH>
 __device__ __forceinline__ void load_row(Chunk<T, E> (&c)[NCH], const T *row, const Group &g, int cols, bool live)
@@ -154,28 +242,40 @@ template <int A, int NCH> struct Ring {
     }
 };
 
-// Mean and 1/deviation of a row held as NCH chunks.
-template <typename T, int E, int NCH>
-__device__ __forceinline__ void row_stats(const Chunk<T, E> (&c)[NCH], Group &g, int cols, float eps, float2 (*sh)[32], float &mean, float &rstd)
+// Whether pair i of this thread lies in the row: all of it (vectors; cols is a multiple), or its first or second value.
+template <int E> __device__ __forceinline__ bool inside(const Group &g, int i, int half, int cols)
 {
-    float s = 0.f;
+    return E == 1 ? (2 * i + half) * g.size + g.t < cols : ((2 * i / (E < 2 ? 2 : E)) * g.size + g.t) * E < cols;
+}
+
+// v: a row's values in, their differences from `m` out (zero outside the row). mean = m + dm.
+template <int E, int N>
+__device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int cols, float inv, float eps, float2 (*sh)[32], float &m, float &dm, float &rstd)
+{
+    Pair s = pair(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < NCH; j++)
+    for (int i = 0; i < N; i++) s = add(s, v[i]);                // columns past the end hold zero
+    float2 f = split(s);
+    m = g.sum(f.x + f.y, sh) * inv;
+    const Pair nm = pair(-m, -m);
+    Pair d1 = pair(0.f, 0.f), d2 = pair(0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < E; e++) s += to_f32(c[j].v[e]);      // columns past the end hold zero
-    const float m = g.sum2(s, 0.f, sh).x / (float)cols;
-    float d1 = 0.f, d2 = 0.f;
-#pragma unroll
-    for (int j = 0; j < NCH; j++)
-        if ((j * g.size + g.t) * E < cols) {
-#pragma unroll
-            for (int e = 0; e < E; e++) { const float d = to_f32(c[j].v[e]) - m; d1 += d; d2 = fmaf(d, d, d2); }
+    for (int i = 0; i < N; i++) {
+        v[i] = add(v[i], nm);
+        if constexpr (E == 1) {
+            const float2 x = split(v[i]);
+            v[i] = pair(inside<E>(g, i, 0, cols) ? x.x : 0.f, inside<E>(g, i, 1, cols) ? x.y : 0.f);
+        } else {
+            if (!inside<E>(g, i, 0, cols)) v[i] = pair(0.f, 0.f);
         }
-    const float2 t = g.sum2(d1, d2, sh);
-    const float dm = t.x / (float)cols;                          // what rounding left in m
-    mean = m + dm;
-    rstd = __frsqrt_rn(fmaxf(t.y / (float)cols - dm * dm, 0.f) + eps);
-    if (!(t.y == t.y)) rstd = t.y;                               // fmaxf drops a NaN; the row keeps it
+        d1 = add(d1, v[i]);
+        d2 = fma(v[i], v[i], d2);
+    }
+    const float2 a = split(d1), b = split(d2);
+    const float2 t = g.sum2(a.x + a.y, b.x + b.y, sh);
+    dm = t.x * inv;                                              // what rounding left in m
+    const float var = t.y * inv - dm * dm;
+    rstd = __frsqrt_rn((var > 0.f ? var : var == var ? 0.f : var) + eps);      // a NaN stays one
 }
 
 template <typename T, typename W, bool VEC, int CPT, bool HOLD>
@@ -186,7 +286,8 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
     constexpr int E = VEC ? 16 / (int)sizeof(T) : 1, NCH = CPT / E;
     __shared__ float2 sh[2][32];
     Group g(group);
-    float pw[HOLD ? NCH : 1][E], pb[HOLD ? NCH : 1][E];         // the parameters of this thread's columns
+    Pair pw[HOLD ? CPT / 2 : 1], pb[HOLD ? CPT / 2 : 1];           // the parameters of this thread's columns
+    const float inv = 1.f / (float)cols;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const long long step = (long long)gridDim.x * g.per_block;
@@ -203,6 +304,7 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
     } else {
         load_row<T, E, NCH>(cur, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
     }
+    // parameters of chunk j's columns
     const auto params = [&](int j, float (&qw)[E], float (&qb)[E]) {
         const int col = (j * g.size + g.t) * E;
 #pragma unroll
@@ -213,8 +315,14 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
         }
     };
     if constexpr (HOLD) {
+        float qw[NCH][E], qb[NCH][E];
 #pragma unroll
-        for (int j = 0; j < NCH; j++) params(j, pw[j], pb[j]);
+        for (int j = 0; j < NCH; j++) params(j, qw[j], qb[j]);
+#pragma unroll
+        for (int i = 0; i < CPT / 2; i++) {
+            pw[i] = pair(qw[2 * i / E][2 * i % E], qw[(2 * i + 1) / E][(2 * i + 1) % E]);
+            pb[i] = pair(qb[2 * i / E][2 * i % E], qb[(2 * i + 1) / E][(2 * i + 1) % E]);
+        }
     }
     for (; base < rows; base += step) {
         const long long row = base + g.index;
@@ -225,8 +333,10 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
         } else {
             load_row<T, E, NCH>(nxt, x + (row + step) * ldx, g, cols, row + step < rows);
         }
-        float mean, rstd;
-        row_stats<T, E, NCH>(cur, g, cols, eps, sh, mean, rstd);
+        Pair v[CPT / 2];
+        widen_all<T, E, NCH>(cur, v);
+        float m, dm, rstd;
+        row_stats<E, CPT / 2>(v, g, cols, inv, eps, sh, m, dm, rstd);
         if constexpr (VEC) {                    // the row is in registers: its places may fill again
             const long long ahead = row + depth * step;
             ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
@@ -235,25 +345,36 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
         }
         if (row < rows) {
             if (g.t == 0) {
-                if (mean_out) mean_out[row] = mean;
+                if (mean_out) mean_out[row] = m + dm;
                 if (rstd_out) rstd_out[row] = rstd;
             }
             T *out = y + row * ldy;
+            const Pair r2 = pair(rstd, rstd), shift = pair(-dm * rstd, -dm * rstd);
 #pragma unroll
-            for (int j = 0; j < NCH; j++) {
-                const int col = (j * g.size + g.t) * E;
-                if (col < cols) {
-                    Chunk<T, E> o;
-                    if constexpr (HOLD) {
+            for (int i = 0; i < CPT / 2; i++) v[i] = fma(v[i], r2, shift);
+            if constexpr (E == 1) {
 #pragma unroll
-                        for (int e = 0; e < E; e++) o.v[e] = from_f32<T>(fmaf((to_f32(cur[j].v[e]) - mean) * rstd, pw[j][e], pb[j][e]));
-                    } else {
+                for (int i = 0; i < CPT / 2; i++) {
+                    const float2 f = split(fma(v[i], pw[i], pb[i]));
+                    if (inside<E>(g, i, 0, cols)) out[2 * i * g.size + g.t] = from_f32<T>(f.x);
+                    if (inside<E>(g, i, 1, cols)) out[(2 * i + 1) * g.size + g.t] = from_f32<T>(f.y);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NCH; j++) {
+                    const int col = (j * g.size + g.t) * E;
+                    if (col < cols) {
+                        Chunk<T, E> o;
                         float qw[E], qb[E];
-                        params(j, qw, qb);
+                        if constexpr (!HOLD) params(j, qw, qb);
 #pragma unroll
-                        for (int e = 0; e < E; e++) o.v[e] = from_f32<T>(fmaf((to_f32(cur[j].v[e]) - mean) * rstd, qw[e], qb[e]));
+                        for (int i = 0; i < E / 2; i++) {
+                            const int n = j * E / 2 + i;
+                            if constexpr (HOLD) narrow(&o.v[2 * i], fma(v[n], pw[n], pb[n]));
+                            else narrow(&o.v[2 * i], fma(v[n], pair(qw[2 * i], qw[2 * i + 1]), pair(qb[2 * i], qb[2 * i + 1])));
+                        }
+                        *reinterpret_cast<Chunk<T, E> *>(out + col) = o;
                     }
-                    *reinterpret_cast<Chunk<T, E> *>(out + col) = o;
                 }
             }
         }
@@ -278,7 +399,7 @@ __device__ __forceinline__ void forward_loop(T *y, const T *x, const W *__restri
         T *out = y + row * ldy;
         float s = 0.f;
         for (int c = g.t; c < cols; c += g.size) s += to_f32(src[c]);
-        const float m = g.sum2(s, 0.f, sh).x / (float)cols;
+        const float m = g.sum(s, sh) / (float)cols;
         float d1 = 0.f, d2 = 0.f;
         for (int c = g.t; c < cols; c += g.size) { const float d = to_f32(src[c]) - m; d1 += d; d2 = fmaf(d, d, d2); }
         const float2 t = g.sum2(d1, d2, sh);
@@ -295,25 +416,24 @@ __device__ __forceinline__ void forward_loop(T *y, const T *x, const W *__restri
 }
 
 // Adds dy and dy xhat of each thread's columns over the rows of its block (partial,
-// when asked for: [block][2][cols]) and writes dx (when asked for). A vector row is read from its ring places twice,
-// for the two sums and for dx, and its places are filled again right behind the second read.
+// when asked for: [block][2][cols]) and writes dx (when asked for).
 template <typename T, typename W, bool VEC, int CPT, bool HOLD>
 __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__ partial, const T *__restrict__ dy, const T *__restrict__ x,
                                          const W *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
                                          long long rows, int cols, long long lddx, long long lddy, long long ldx, int group, int depth)
 {
-    constexpr int E = VEC ? 16 / (int)sizeof(T) : 1, NCH = CPT / E;
+    constexpr int E = VEC ? 16 / (int)sizeof(T) : 1, NCH = CPT / E, N = CPT / 2;
     __shared__ float2 sh[2][32];
     __shared__ float part[2][256];              // narrow rows: the block's groups add up here
     Group g(group);
-    float pw[HOLD ? NCH : 1][E], aw[NCH][E], ab[NCH][E];
+    Pair pw[HOLD ? N : 1], aw[N], ab[N];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const float inv = 1.f / (float)cols;
     const long long step = (long long)gridDim.x * g.per_block;
     long long base = (long long)blockIdx.x * g.per_block;
     Ring<2, VEC ? NCH : 1> ring(depth);
-    Chunk<T, E> sx[VEC ? 1 : NCH], sd[VEC ? 1 : NCH], nx[VEC ? 1 : NCH], nd[VEC ? 1 : NCH];
+    Chunk<T, E> cx[VEC ? 1 : NCH], cd[VEC ? 1 : NCH], nx[VEC ? 1 : NCH], nd[VEC ? 1 : NCH];
     if constexpr (VEC) {
         for (int d = 0; d < depth; d++) {
             const long long row = base + g.index + d * step;
@@ -323,8 +443,8 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
             ring.next();
         }
     } else {
-        load_row<T, E, NCH>(sx, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
-        load_row<T, E, NCH>(sd, dy + (base + g.index) * lddy, g, cols, base + g.index < rows);
+        load_row<T, E, NCH>(cx, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
+        load_row<T, E, NCH>(cd, dy + (base + g.index) * lddy, g, cols, base + g.index < rows);
     }
     const auto weight = [&](int j, float (&q)[E]) {
         const int col = (j * g.size + g.t) * E;
@@ -332,12 +452,15 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         for (int e = 0; e < E; e++) q[e] = 1.f;
         if (w && col < cols) load_params<W, E>(w, col, q);
     };
+    if constexpr (HOLD) {
+        float q[NCH][E];
 #pragma unroll
-    for (int j = 0; j < NCH; j++) {
+        for (int j = 0; j < NCH; j++) weight(j, q[j]);
 #pragma unroll
-        for (int e = 0; e < E; e++) { aw[j][e] = 0.f; ab[j][e] = 0.f; }
-        if constexpr (HOLD) weight(j, pw[j]);
+        for (int i = 0; i < N; i++) pw[i] = pair(q[2 * i / E][2 * i % E], q[(2 * i + 1) / E][(2 * i + 1) % E]);
     }
+#pragma unroll
+    for (int i = 0; i < N; i++) aw[i] = ab[i] = pair(0.f, 0.f);
     float cm = 0.f, cr = 0.f;
     if (base + g.index < rows) { cm = mean_in[base + g.index]; cr = rstd_in[base + g.index]; }
     for (; base < rows; base += step) {
@@ -349,96 +472,134 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
             load_row<T, E, NCH>(nx, x + next * ldx, g, cols, next < rows);
             load_row<T, E, NCH>(nd, dy + next * lddy, g, cols, next < rows);
         }
-        float s1 = 0.f, s2 = 0.f;
-        // rows past the last have dy = 0 (and mean = rstd = 0): they add nothing
-#pragma unroll
-        for (int j = 0; j < NCH; j++) {
-            if ((j * g.size + g.t) * E < cols) {
-                float qw[E];
-                if constexpr (!HOLD) weight(j, qw);
-                Chunk<T, E> cx, cd;
-                if constexpr (VEC) { cx = ring.template get<T, E>(0, j, row < rows); cd = ring.template get<T, E>(1, j, row < rows); }
-                else { cx = sx[j]; cd = sd[j]; }
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const float d = to_f32(cd.v[e]), xh = (to_f32(cx.v[e]) - cm) * cr;
-                    const float wd = d * (HOLD ? pw[HOLD ? j : 0][e] : qw[e]);
-                    s1 += wd;
-                    s2 = fmaf(wd, xh, s2);
-                    ab[j][e] += d;
-                    aw[j][e] = fmaf(d, xh, aw[j][e]);
-                }
-            }
-        }
-        const float2 t = g.sum2(s1, s2, sh);
-        if (dx && row < rows) {
-            const float p = t.x * inv, q = t.y * inv;
-            T *out = dx + row * lddx;
+        // xhat and w dy of this thread's columns, kept for dx (HOLD) or formed again from the ring. Outside the row and
+        // past the last row dy is zero: such places add nothing (and past the last row mean = rstd = 0).
+        constexpr int KEEP = HOLD ? N : E / 2;
+        Pair xh[KEEP], wd[KEEP];
+        const Pair nmean = pair(-cm, -cm), r2 = pair(cr, cr);
+        Pair s1 = pair(0.f, 0.f), s2 = pair(0.f, 0.f);
+        if constexpr (VEC) {
 #pragma unroll
             for (int j = 0; j < NCH; j++) {
-                const int col = (j * g.size + g.t) * E;
-                if (col < cols) {
-                    float qw[E];
-                    if constexpr (!HOLD) weight(j, qw);
-                    Chunk<T, E> cx, cd, o;
-                    if constexpr (VEC) { cx = ring.template get<T, E>(0, j, true); cd = ring.template get<T, E>(1, j, true); }
-                    else { cx = sx[j]; cd = sd[j]; }
+                const bool live = row < rows && (j * g.size + g.t) * E < cols;
+                const Chunk<T, E> xc = ring.template get<T, E>(0, j, live), dc = ring.template get<T, E>(1, j, live);
+                float q[E];
+                if constexpr (!HOLD) weight(j, q);
 #pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const float xh = (to_f32(cx.v[e]) - cm) * cr;
-                        const float wd = to_f32(cd.v[e]) * (HOLD ? pw[HOLD ? j : 0][e] : qw[e]);
-                        o.v[e] = from_f32<T>(cr * (wd - p - xh * q));
-                    }
-                    *reinterpret_cast<Chunk<T, E> *>(out + col) = o;
+                for (int i = 0; i < E / 2; i++) {
+                    const int n = j * E / 2 + i, k = HOLD ? n : i;
+                    const Pair d = widen(&dc.v[2 * i]);
+                    xh[k] = mul(add(widen(&xc.v[2 * i]), nmean), r2);
+                    ab[n] = add(ab[n], d);
+                    aw[n] = fma(d, xh[k], aw[n]);
+                    if constexpr (HOLD) wd[k] = mul(d, pw[n]);
+                    else wd[k] = mul(d, pair(q[2 * i], q[2 * i + 1]));
+                    s1 = add(s1, wd[k]);
+                    s2 = fma(wd[k], xh[k], s2);
                 }
             }
+        } else {
+            widen_all<T, E, NCH>(cx, xh);
+            widen_all<T, E, NCH>(cd, wd);
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const Pair d = wd[n];
+                xh[n] = mul(add(xh[n], nmean), r2);
+                ab[n] = add(ab[n], d);
+                aw[n] = fma(d, xh[n], aw[n]);
+                wd[n] = mul(d, pw[n]);
+                s1 = add(s1, wd[n]);
+                s2 = fma(wd[n], xh[n], s2);
+            }
         }
-        cm = nm; cr = nr;
-        if constexpr (VEC) {
+        const float2 f1 = split(s1), f2 = split(s2);
+        const float2 t = g.sum2(f1.x + f1.y, f2.x + f2.y, sh);
+        const auto refill = [&]() {             // the row has been read: its places may fill again
             const long long ahead = row + depth * step;
             ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
             ring.template fetch<T, E>(1, dy + ahead * lddy, g, cols, ahead < rows);
             ring.commit();
             ring.next();
-        } else {
+        };
+        if constexpr (VEC && HOLD) refill();
+        if (dx && row < rows) {
+            const float p = t.x * inv, q = t.y * inv;
+            const Pair np = pair(-p, -p), nq = pair(-q, -q);
+            T *out = dx + row * lddx;
+            if constexpr (E == 1) {
 #pragma unroll
-            for (int j = 0; j < NCH; j++) { sx[j] = nx[j]; sd[j] = nd[j]; }
+                for (int i = 0; i < N; i++) {
+                    const float2 f = split(mul(r2, fma(xh[i], nq, add(wd[i], np))));
+                    if (inside<E>(g, i, 0, cols)) out[2 * i * g.size + g.t] = from_f32<T>(f.x);
+                    if (inside<E>(g, i, 1, cols)) out[(2 * i + 1) * g.size + g.t] = from_f32<T>(f.y);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NCH; j++) {
+                    const int col = (j * g.size + g.t) * E;
+                    if (col < cols) {
+                        Chunk<T, E> o;
+                        if constexpr (!HOLD) {
+                            const Chunk<T, E> xc = ring.template get<T, E>(0, j, true), dc = ring.template get<T, E>(1, j, true);
+                            float u[E];
+                            weight(j, u);
+#pragma unroll
+                            for (int i = 0; i < E / 2; i++) {
+                                xh[i] = mul(add(widen(&xc.v[2 * i]), nmean), r2);
+                                wd[i] = mul(widen(&dc.v[2 * i]), pair(u[2 * i], u[2 * i + 1]));
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < E / 2; i++) {
+                            const int k = HOLD ? j * E / 2 + i : i;
+                            narrow(&o.v[2 * i], mul(r2, fma(xh[k], nq, add(wd[k], np))));
+                        }
+                        *reinterpret_cast<Chunk<T, E> *>(out + col) = o;
+                    }
+                }
+            }
+        }
+        if constexpr (VEC && !HOLD) refill();
+        cm = nm; cr = nr;
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int j = 0; j < NCH; j++) { cx[j] = nx[j]; cd[j] = nd[j]; }
         }
     }
     if (!partial) return;
     float *pw_out = partial + (size_t)blockIdx.x * 2 * cols, *pb_out = pw_out + cols;
+    float sw[CPT], sb[CPT];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float2 a = split(aw[i]), b = split(ab[i]);
+        sw[2 * i] = a.x; sw[2 * i + 1] = a.y; sb[2 * i] = b.x; sb[2 * i + 1] = b.y;
+    }
     if (g.size > 32) {
 #pragma unroll
-        for (int j = 0; j < NCH; j++)
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int col = (j * g.size + g.t) * E + e;
-                if (col < cols) { pw_out[col] = aw[j][e]; pb_out[col] = ab[j][e]; }
-            }
+        for (int n = 0; n < CPT; n++) {
+            const int col = (n / E * g.size + g.t) * E + n % E;
+            if (col < cols) { pw_out[col] = sw[n]; pb_out[col] = sb[n]; }
+        }
         return;
     }
     // narrow rows (cols <= 256): first over the groups of a warp, then over the warps in turn
     for (int o = 16; o >= g.size; o >>= 1)
 #pragma unroll
-        for (int j = 0; j < NCH; j++)
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                aw[j][e] += __shfl_xor_sync(0xffffffffu, aw[j][e], o);
-                ab[j][e] += __shfl_xor_sync(0xffffffffu, ab[j][e], o);
-            }
+        for (int n = 0; n < CPT; n++) {
+            sw[n] += __shfl_xor_sync(0xffffffffu, sw[n], o);
+            sb[n] += __shfl_xor_sync(0xffffffffu, sb[n], o);
+        }
     const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
     for (int k = 0; k < ((int)blockDim.x >> 5); k++) {
         if (warp == k && lane < g.size) {
 #pragma unroll
-            for (int j = 0; j < NCH; j++)
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const int col = (j * g.size + g.t) * E + e;
-                    if (col < cols && col < 256) {
-                        part[0][col] = k ? part[0][col] + aw[j][e] : aw[j][e];
-                        part[1][col] = k ? part[1][col] + ab[j][e] : ab[j][e];
-                    }
+            for (int n = 0; n < CPT; n++) {
+                const int col = (n / E * g.size + g.t) * E + n % E;
+                if (col < cols && col < 256) {
+                    part[0][col] = k ? part[0][col] + sw[n] : sw[n];
+                    part[1][col] = k ? part[1][col] + sb[n] : sb[n];
                 }
+            }
         }
         __syncthreads();
     }
@@ -524,8 +685,8 @@ __device__ __forceinline__ void param_grad(W *__restrict__ dw, W *__restrict__ d
 
 }  // namespace ln
 
-#define LN_FORM(name, T, W, form, VEC, CPT, HOLD, THREADS)                                                                                \
-    extern "C" __global__ void __launch_bounds__(THREADS)                                                                                \
+#define LN_FORM(name, T, W, form, VEC, CPT, HOLD, THREADS, BLOCKS)                                                                           \
+    extern "C" __global__ void __launch_bounds__(THREADS, BLOCKS)                                                                        \
     layernorm_##name##_##form(T *y, const T *x, const W *w, const W *b, float *mean, float *rstd, long long rows, int cols,              \
                               long long ldx, long long ldy, float eps, int group, int depth)                                             \
     { ln::forward<T, W, VEC, CPT, HOLD>(y, x, w, b, mean, rstd, rows, cols, ldx, ldy, eps, group, depth); }                              \
@@ -535,11 +696,11 @@ __device__ __forceinline__ void param_grad(W *__restrict__ dw, W *__restrict__ d
     { ln::backward<T, W, VEC, CPT, HOLD>(dx, partial, dy, x, w, mean, rstd, rows, cols, lddx, lddy, ldx, group, depth); }
 
 #define LN_KERNELS(name, T, W)                                                                                                           \
-    LN_FORM(name, T, W, v8, true, 8, true, 512)                                                                                          \
-    LN_FORM(name, T, W, v16, true, 16, true, 512)                                                                                        \
-    LN_FORM(name, T, W, vw, true, 16, false, 1024)                                                                                       \
-    LN_FORM(name, T, W, s8, false, 8, true, 512)                                                                                         \
-    LN_FORM(name, T, W, s16, false, 16, true, 512)                                                                                       \
+    LN_FORM(name, T, W, v8, true, 8, true, 512, 2)                                                                                         \
+    LN_FORM(name, T, W, v16, true, 16, true, 256, 3)                                                                                       \
+    LN_FORM(name, T, W, vw, true, 16, false, 1024, 1)                                                                                      \
+    LN_FORM(name, T, W, s8, false, 8, true, 512, 1)                                                                                        \
+    LN_FORM(name, T, W, s16, false, 16, true, 512, 1)                                                                                      \
     extern "C" __global__ void __launch_bounds__(512)                                                                                    \
     layernorm_##name##_loop(T *y, const T *x, const W *w, const W *b, float *mean, float *rstd, long long rows, int cols,                \
                             long long ldx, long long ldy, float eps, int group, int depth)                                               \

@@ -55,15 +55,15 @@ typedef struct { int form, group, depth; unsigned block, grid, ring; } ln_shape_
 /* How rows are dealt to threads. Eight values a thread for narrow rows, and for
  * rows so few that each has an SM to itself (more threads shorten the one row);
  * sixteen otherwise, which halves what the reductions and the barriers cost per
- * value; vector rows too wide for 512 threads get up to 1024; else the form that walks
+ * value; vector rows too wide for 256 threads get up to 1024, without the parameters in registers; else the form that walks
  * the row. Blocks stay, each taking every grid-th row: as many as an SM holds by
- * registers (64 a thread for eight values, 80 to 128 else), and of the vector
+ * registers (64 to 80 a thread for eight values, 80 to 128 else), and of the vector
  * forms' rings up to four rows each, as many as fit beside one another. */
 static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, unsigned esz, int vec, int backward)
 {
     ln_shape_t s;
     const int cpt = cols <= 1024 || (cols <= 4096 && rows < 2ll * dev->sm_count) ? 8 : cols <= 8192 || (cols <= 16384 && vec) ? 16 : 0;
-    s.form = cpt == 8 ? (vec ? LN_V8 : LN_S8) : cpt == 16 ? (!vec ? LN_S16 : cols <= 8192 ? LN_V16 : LN_VW) : LN_LOOP;
+    s.form = cpt == 8 ? (vec ? LN_V8 : LN_S8) : cpt == 16 ? (!vec ? LN_S16 : cols <= 4096 ? LN_V16 : LN_VW) : LN_LOOP;
     s.depth = 1;
     s.ring = 0;
     if (!cpt) {
@@ -77,7 +77,7 @@ static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, uns
         s.block = g <= 32 ? 128u : (unsigned)g;
     }
     const long long per_block = s.group <= 32 ? (long long)s.block / s.group : 1;
-    const unsigned threads = cpt == 8 ? (backward && !vec ? 640u : 1024u) : backward ? 512u : 768u;
+    const unsigned threads = cpt == 8 ? (!backward ? 1024u : vec ? 768u : 512u) : s.form == LN_VW ? 1024u : backward ? 512u : 768u;
     unsigned per_sm = threads / s.block < 1 ? 1 : threads / s.block;
     if (s.form <= LN_VW) {
         const unsigned row = s.block * (unsigned)cpt * esz * (backward ? 2u : 1u);
