@@ -8,15 +8,17 @@
 //
 // Both read every value once and write every result once, so HBM bounds them. A
 // row belongs to one group of threads: 1 to 32 lanes of a warp for narrow rows, a whole
-// block for wider ones, 8 or 16 values a thread. The mean is taken first and the variance
+// block for wider ones, 8 to 32 values a thread (a row costs a thread some 150 instructions
+// beside its values, 240 before the sums were shortened: with 8 or 16 values that was most of them). The mean is taken first and the variance
 // from the differences (the row is on chip, a second pass costs no memory), with the
 // differences' own mean as a correction, so a row far from zero loses nothing.
 //
-// Blocks stay and walk over the rows. Vector forms keep the next few rows on their way
-// with cp.async into a ring in shared memory, in which every thread has places of its
-// own for what it alone reads, so the ring needs no barrier; with the next row held in
+// Blocks stay and walk over the rows. The next few rows are on their way with cp.async
+// into a ring in shared memory. In vector forms every thread has places of its
+// own for what it alone reads, so the ring needs no barrier. (With the next row held in
 // registers instead, 16 KB an SM were in flight and 16384 x 4096 bf16 took 116 us forward
-// and 128 backward.
+// and 128 backward.) Rows of any other alignment come in 16-byte units all the same and are read
+// value by value.
 //
 // The backward pass walks the rows once for all three results: each thread adds dy
 // and dy xhat of its own columns into registers over all the rows its block sees,
@@ -26,9 +28,9 @@
 // Sums, statistics and products are fp32 (the last sum over the blocks double);
 // values are rounded to the tensor's type once, when they are stored.
 //
-// Forms: v8, v16, vw read 16-byte vectors (row starts and parameters 16-byte
-// aligned, cols a multiple of the vector), vw up to 1024 threads a row with the parameters
-// from cache; s8, s16 read single elements, neighbouring threads on neighbouring
+// Forms: v8, v16, v32, vw, vx read 16-byte vectors (row starts and parameters 16-byte
+// aligned, cols a multiple of the vector); vw is v16 with up to 640 threads, vx v32 with up
+// to 512 and the parameters from cache; s8, s16 read single elements, neighbouring threads on neighbouring
 // columns, for any alignment; loop goes through the row several times from
 // cache, for rows no block can hold.
 #include "common.cuh"
@@ -189,20 +191,6 @@ template <typename T, int E, int NCH> __device__ __forceinline__ void widen_all(
     }
 }
 
-template <typename T, int E, int NCH>
-__device__ __forceinline__ void load_row(Chunk<T, E> (&c)[NCH], const T *row, const Group &g, int cols, bool live)
-{
-#pragma unroll
-    for (int j = 0; j < NCH; j++) {
-        const int col = (j * g.size + g.t) * E;
-        if (live && col < cols) c[j] = *reinterpret_cast<const Chunk<T, E> *>(row + col);
-        else {
-#pragma unroll
-            for (int e = 0; e < E; e++) c[j].v[e] = from_f32<T>(0.f);
-        }
-    }
-}
-
 // The ring: `depth` rows ahead of A arrays; chunk j of array a of a stage at ((stage A + a) NCH + j) blockDim 16 bytes,
 // 16 bytes a thread. Every row position commits one group, with or without copies, so that the count of groups
 // tells which row has landed.
@@ -239,6 +227,94 @@ template <int A, int NCH> struct Ring {
         uint4 v = make_uint4(0, 0, 0, 0);
         if (live) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at(a, j)) : "memory");
         return *reinterpret_cast<const Chunk<T, E> *>(&v);
+    }
+};
+
+// The ring for rows of any alignment: a row has a slot in which its bytes lie as they do in memory modulo 16. Whole
+// 16-byte units come with cp.async, the units at its two ends word by word, and a 16-bit value that shares its word
+// with a neighbour's row through a register, written to the slot at the next step. What one thread brings others read,
+// so a row is ready behind a barrier of its group, and its slot is free behind the next one.
+template <typename T, int A> struct Slots {
+    uint32_t base, pitch, groups, held[A][2];
+    uint16_t edge[A][2];
+    int depth, stage;
+    __device__ __forceinline__ Slots(int depth_, int cols, const Group &g) : depth(depth_), stage(0)
+    {
+        extern __shared__ uint4 ln_ring[];
+        pitch = ((uint32_t)cols * (uint32_t)sizeof(T) + 15u) / 16u * 16u + 16u;
+        groups = (uint32_t)g.per_block;
+        base = (uint32_t)__cvta_generic_to_shared(ln_ring) + (uint32_t)g.index * pitch;
+#pragma unroll
+        for (int a = 0; a < A; a++) { held[a][0] = held[a][1] = 0; edge[a][0] = edge[a][1] = 0; }
+    }
+    __device__ __forceinline__ uint32_t slot(int a) const { return base + (uint32_t)(stage * A + a) * groups * pitch; }
+    __device__ __forceinline__ void fetch(int a, const T *row, const Group &g, int cols, bool live)
+    {
+        if (!live) return;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row);
+        const uint32_t head = (uint32_t)(at & 15), end = head + (uint32_t)cols * (uint32_t)sizeof(T), to = slot(a);
+        const char *const from = reinterpret_cast<const char *>(at - head);
+        for (uint32_t u = (uint32_t)g.t * 16u; u < end; u += (uint32_t)g.size * 16u) {
+            if (u >= head && u + 16u <= end) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u), "l"(from + u) : "memory");
+                continue;
+            }
+#pragma unroll
+            for (uint32_t w = u; w < u + 16u; w += 4u) {
+                if (w >= head && w + 4u <= end) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + w), "l"(from + w) : "memory");
+                else if (sizeof(T) == 2 && w + 4u > head && w < end) {
+                    // one half of the word: the row's first value in its upper half, or its last in the lower
+                    const int tail = w >= head ? 1 : 0;
+                    const uint32_t h = tail ? w : w + 2u;
+                    held[a][tail] = to + h;
+                    edge[a][tail] = *reinterpret_cast<const uint16_t *>(from + h);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    __device__ __forceinline__ void next() { stage = stage + 1 == depth ? 0 : stage + 1; }
+    __device__ __forceinline__ void settle()
+    {
+#pragma unroll
+        for (int a = 0; a < A; a++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                if (held[a][e]) {
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(held[a][e]), "h"(edge[a][e]) : "memory");
+                    held[a][e] = 0;
+                }
+    }
+    static __device__ __forceinline__ void meet(const Group &g) { if (g.size > 32) __syncthreads(); else __syncwarp(); }
+    // The oldest outstanding row is there for the whole group.
+    __device__ __forceinline__ void wait(const Group &g)
+    {
+        settle();
+        if (depth == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+        else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+        meet(g);
+    }
+    // Column c of the row at `row`; zero outside.
+    __device__ __forceinline__ float get(int a, const T *row, int c, int cols, bool live) const
+    {
+        if (!live || c >= cols) return 0.f;
+        const uint32_t at = slot(a) + (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + (uint32_t)c * (uint32_t)sizeof(T);
+        if constexpr (sizeof(T) == 4) {
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+            return v;
+        } else {
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+            return to_f32(*reinterpret_cast<const T *>(&v));
+        }
+    }
+    template <int N> __device__ __forceinline__ void get_all(int a, const T *row, const Group &g, int cols, bool live, Pair (&v)[N]) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = pair(get(a, row, 2 * i * g.size + g.t, cols, live), get(a, row, (2 * i + 1) * g.size + g.t, cols, live));
     }
 };
 
@@ -293,16 +369,19 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
     const long long step = (long long)gridDim.x * g.per_block;
     long long base = (long long)blockIdx.x * g.per_block;
     Ring<1, VEC ? NCH : 1> ring(depth);
-    Chunk<T, E> cur[NCH], nxt[VEC ? 1 : NCH];
-    if constexpr (VEC) {
-        for (int d = 0; d < depth; d++) {
-            const long long row = base + g.index + d * step;
+    Slots<T, 1> slots(depth, cols, g);
+    for (int d = 0; d < depth; d++) {
+        const long long row = base + g.index + d * step;
+        if constexpr (VEC) {
             ring.template fetch<T, E>(0, x + row * ldx, g, cols, row < rows);
             ring.commit();
             ring.next();
+        } else {
+            slots.settle();
+            slots.fetch(0, x + row * ldx, g, cols, row < rows);
+            slots.commit();
+            slots.next();
         }
-    } else {
-        load_row<T, E, NCH>(cur, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
     }
     // parameters of chunk j's columns
     const auto params = [&](int j, float (&qw)[E], float (&qb)[E]) {
@@ -326,22 +405,29 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
     }
     for (; base < rows; base += step) {
         const long long row = base + g.index;
+        Pair v[CPT / 2];
         if constexpr (VEC) {
             ring.wait();
+            Chunk<T, E> cur[NCH];
 #pragma unroll
             for (int j = 0; j < NCH; j++) cur[j] = ring.template get<T, E>(0, j, row < rows && (j * g.size + g.t) * E < cols);
+            widen_all<T, E, NCH>(cur, v);
         } else {
-            load_row<T, E, NCH>(nxt, x + (row + step) * ldx, g, cols, row + step < rows);
+            slots.wait(g);
+            slots.get_all(0, x + row * ldx, g, cols, row < rows, v);
         }
-        Pair v[CPT / 2];
-        widen_all<T, E, NCH>(cur, v);
         float m, dm, rstd;
         row_stats<E, CPT / 2>(v, g, cols, inv, eps, sh, m, dm, rstd);
-        if constexpr (VEC) {                    // the row is in registers: its places may fill again
-            const long long ahead = row + depth * step;
+        const long long ahead = row + depth * step;          // the row is in registers: its places may fill again
+        if constexpr (VEC) {
             ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
             ring.commit();
             ring.next();
+        } else {
+            if (g.size <= 32) __syncwarp();
+            slots.fetch(0, x + ahead * ldx, g, cols, ahead < rows);
+            slots.commit();
+            slots.next();
         }
         if (row < rows) {
             if (g.t == 0) {
@@ -355,7 +441,15 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
             if constexpr (E == 1) {
 #pragma unroll
                 for (int i = 0; i < CPT / 2; i++) {
-                    const float2 f = split(fma(v[i], pw[i], pb[i]));
+                    if constexpr (!HOLD) {
+                        float qw[2][E], qb[2][E];
+                        params(2 * i, qw[0], qb[0]);
+                        params(2 * i + 1, qw[1], qb[1]);
+                        v[i] = fma(v[i], pair(qw[0][0], qw[1][0]), pair(qb[0][0], qb[1][0]));
+                    } else {
+                        v[i] = fma(v[i], pw[i], pb[i]);
+                    }
+                    const float2 f = split(v[i]);
                     if (inside<E>(g, i, 0, cols)) out[2 * i * g.size + g.t] = from_f32<T>(f.x);
                     if (inside<E>(g, i, 1, cols)) out[(2 * i + 1) * g.size + g.t] = from_f32<T>(f.y);
                 }
@@ -377,10 +471,6 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                     }
                 }
             }
-        }
-        if constexpr (!VEC) {
-#pragma unroll
-            for (int j = 0; j < NCH; j++) cur[j] = nxt[j];
         }
     }
 }
@@ -417,14 +507,14 @@ __device__ __forceinline__ void forward_loop(T *y, const T *x, const W *__restri
 
 // Adds dy and dy xhat of each thread's columns over the rows of its block (partial,
 // when asked for: [block][2][cols]) and writes dx (when asked for).
-template <typename T, typename W, bool VEC, int CPT, bool HOLD>
+template <typename T, typename W, bool VEC, int CPT, bool HOLD, bool KEEP_ROW>
 __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__ partial, const T *__restrict__ dy, const T *__restrict__ x,
                                          const W *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
                                          long long rows, int cols, long long lddx, long long lddy, long long ldx, int group, int depth)
 {
     constexpr int E = VEC ? 16 / (int)sizeof(T) : 1, NCH = CPT / E, N = CPT / 2;
     __shared__ float2 sh[2][32];
-    __shared__ float part[2][256];              // narrow rows: the block's groups add up here
+    __shared__ float part[2][512];              // narrow rows: the block's groups add up here
     Group g(group);
     Pair pw[HOLD ? N : 1], aw[N], ab[N];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -433,18 +523,21 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
     const long long step = (long long)gridDim.x * g.per_block;
     long long base = (long long)blockIdx.x * g.per_block;
     Ring<2, VEC ? NCH : 1> ring(depth);
-    Chunk<T, E> cx[VEC ? 1 : NCH], cd[VEC ? 1 : NCH], nx[VEC ? 1 : NCH], nd[VEC ? 1 : NCH];
-    if constexpr (VEC) {
-        for (int d = 0; d < depth; d++) {
-            const long long row = base + g.index + d * step;
+    Slots<T, 2> slots(depth, cols, g);
+    for (int d = 0; d < depth; d++) {
+        const long long row = base + g.index + d * step;
+        if constexpr (VEC) {
             ring.template fetch<T, E>(0, x + row * ldx, g, cols, row < rows);
             ring.template fetch<T, E>(1, dy + row * lddy, g, cols, row < rows);
             ring.commit();
             ring.next();
+        } else {
+            slots.settle();
+            slots.fetch(0, x + row * ldx, g, cols, row < rows);
+            slots.fetch(1, dy + row * lddy, g, cols, row < rows);
+            slots.commit();
+            slots.next();
         }
-    } else {
-        load_row<T, E, NCH>(cx, x + (base + g.index) * ldx, g, cols, base + g.index < rows);
-        load_row<T, E, NCH>(cd, dy + (base + g.index) * lddy, g, cols, base + g.index < rows);
     }
     const auto weight = [&](int j, float (&q)[E]) {
         const int col = (j * g.size + g.t) * E;
@@ -468,13 +561,10 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         float nm = 0.f, nr = 0.f;
         if (next < rows) { nm = mean_in[next]; nr = rstd_in[next]; }
         if constexpr (VEC) ring.wait();
-        else {
-            load_row<T, E, NCH>(nx, x + next * ldx, g, cols, next < rows);
-            load_row<T, E, NCH>(nd, dy + next * lddy, g, cols, next < rows);
-        }
-        // xhat and w dy of this thread's columns, kept for dx (HOLD) or formed again from the ring. Outside the row and
+        else slots.wait(g);
+        // xhat and w dy of this thread's columns, kept for dx (KEEP_ROW) or formed again from the ring. Outside the row and
         // past the last row dy is zero: such places add nothing (and past the last row mean = rstd = 0).
-        constexpr int KEEP = HOLD ? N : E / 2;
+        constexpr int KEEP = KEEP_ROW ? N : E == 1 ? 1 : E / 2;
         Pair xh[KEEP], wd[KEEP];
         const Pair nmean = pair(-cm, -cm), r2 = pair(cr, cr);
         Pair s1 = pair(0.f, 0.f), s2 = pair(0.f, 0.f);
@@ -487,7 +577,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                 if constexpr (!HOLD) weight(j, q);
 #pragma unroll
                 for (int i = 0; i < E / 2; i++) {
-                    const int n = j * E / 2 + i, k = HOLD ? n : i;
+                    const int n = j * E / 2 + i, k = KEEP_ROW ? n : i;
                     const Pair d = widen(&dc.v[2 * i]);
                     xh[k] = mul(add(widen(&xc.v[2 * i]), nmean), r2);
                     ab[n] = add(ab[n], d);
@@ -499,29 +589,52 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                 }
             }
         } else {
-            widen_all<T, E, NCH>(cx, xh);
-            widen_all<T, E, NCH>(cd, wd);
+            const T *const xr = x + row * ldx, *const dr = dy + row * lddy;
+            if constexpr (KEEP_ROW) {
+                slots.get_all(0, xr, g, cols, row < rows, xh);
+                slots.get_all(1, dr, g, cols, row < rows, wd);
+            }
 #pragma unroll
             for (int n = 0; n < N; n++) {
-                const Pair d = wd[n];
-                xh[n] = mul(add(xh[n], nmean), r2);
+                const int k = KEEP_ROW ? n : 0;
+                if constexpr (!KEEP_ROW) {
+                    xh[0] = pair(slots.get(0, xr, 2 * n * g.size + g.t, cols, row < rows), slots.get(0, xr, (2 * n + 1) * g.size + g.t, cols, row < rows));
+                    wd[0] = pair(slots.get(1, dr, 2 * n * g.size + g.t, cols, row < rows), slots.get(1, dr, (2 * n + 1) * g.size + g.t, cols, row < rows));
+                }
+                const Pair d = wd[k];
+                xh[k] = mul(add(xh[k], nmean), r2);
                 ab[n] = add(ab[n], d);
-                aw[n] = fma(d, xh[n], aw[n]);
-                wd[n] = mul(d, pw[n]);
-                s1 = add(s1, wd[n]);
-                s2 = fma(wd[n], xh[n], s2);
+                aw[n] = fma(d, xh[k], aw[n]);
+                if constexpr (HOLD) wd[k] = mul(d, pw[n]);
+                else {
+                    float q0[E], q1[E];
+                    weight(2 * n, q0);
+                    weight(2 * n + 1, q1);
+                    wd[k] = mul(d, pair(q0[0], q1[0]));
+                }
+                s1 = add(s1, wd[k]);
+                s2 = fma(wd[k], xh[k], s2);
             }
         }
         const float2 f1 = split(s1), f2 = split(s2);
         const float2 t = g.sum2(f1.x + f1.y, f2.x + f2.y, sh);
         const auto refill = [&]() {             // the row has been read: its places may fill again
             const long long ahead = row + depth * step;
-            ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
-            ring.template fetch<T, E>(1, dy + ahead * lddy, g, cols, ahead < rows);
-            ring.commit();
-            ring.next();
+            if constexpr (VEC) {
+                ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
+                ring.template fetch<T, E>(1, dy + ahead * lddy, g, cols, ahead < rows);
+                ring.commit();
+                ring.next();
+            } else {
+                if (!KEEP_ROW) Slots<T, 2>::meet(g);          // the sums' barrier lies behind the first reading only
+                else if (g.size <= 32) __syncwarp();
+                slots.fetch(0, x + ahead * ldx, g, cols, ahead < rows);
+                slots.fetch(1, dy + ahead * lddy, g, cols, ahead < rows);
+                slots.commit();
+                slots.next();
+            }
         };
-        if constexpr (VEC && HOLD) refill();
+        if constexpr (KEEP_ROW) refill();
         if (dx && row < rows) {
             const float p = t.x * inv, q = t.y * inv;
             const Pair np = pair(-p, -p), nq = pair(-q, -q);
@@ -529,7 +642,16 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
             if constexpr (E == 1) {
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    const float2 f = split(mul(r2, fma(xh[i], nq, add(wd[i], np))));
+                    const int k = KEEP_ROW ? i : 0;
+                    if constexpr (!KEEP_ROW) {
+                        const T *const xr = x + row * ldx, *const dr = dy + row * lddy;
+                        float q0[E], q1[E];
+                        weight(2 * i, q0);
+                        weight(2 * i + 1, q1);
+                        xh[0] = mul(add(pair(slots.get(0, xr, 2 * i * g.size + g.t, cols, true), slots.get(0, xr, (2 * i + 1) * g.size + g.t, cols, true)), nmean), r2);
+                        wd[0] = mul(pair(slots.get(1, dr, 2 * i * g.size + g.t, cols, true), slots.get(1, dr, (2 * i + 1) * g.size + g.t, cols, true)), pair(q0[0], q1[0]));
+                    }
+                    const float2 f = split(mul(r2, fma(xh[k], nq, add(wd[k], np))));
                     if (inside<E>(g, i, 0, cols)) out[2 * i * g.size + g.t] = from_f32<T>(f.x);
                     if (inside<E>(g, i, 1, cols)) out[(2 * i + 1) * g.size + g.t] = from_f32<T>(f.y);
                 }
@@ -539,7 +661,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                     const int col = (j * g.size + g.t) * E;
                     if (col < cols) {
                         Chunk<T, E> o;
-                        if constexpr (!HOLD) {
+                        if constexpr (!KEEP_ROW) {
                             const Chunk<T, E> xc = ring.template get<T, E>(0, j, true), dc = ring.template get<T, E>(1, j, true);
                             float u[E];
                             weight(j, u);
@@ -551,7 +673,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                         }
 #pragma unroll
                         for (int i = 0; i < E / 2; i++) {
-                            const int k = HOLD ? j * E / 2 + i : i;
+                            const int k = KEEP_ROW ? j * E / 2 + i : i;
                             narrow(&o.v[2 * i], mul(r2, fma(xh[k], nq, add(wd[k], np))));
                         }
                         *reinterpret_cast<Chunk<T, E> *>(out + col) = o;
@@ -559,12 +681,8 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                 }
             }
         }
-        if constexpr (VEC && !HOLD) refill();
+        if constexpr (!KEEP_ROW) refill();
         cm = nm; cr = nr;
-        if constexpr (!VEC) {
-#pragma unroll
-            for (int j = 0; j < NCH; j++) { cx[j] = nx[j]; cd[j] = nd[j]; }
-        }
     }
     if (!partial) return;
     float *pw_out = partial + (size_t)blockIdx.x * 2 * cols, *pb_out = pw_out + cols;
@@ -582,7 +700,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         }
         return;
     }
-    // narrow rows (cols <= 256): first over the groups of a warp, then over the warps in turn
+    // narrow rows (cols <= 512): first over the groups of a warp, then over the warps in turn
     for (int o = 16; o >= g.size; o >>= 1)
 #pragma unroll
         for (int n = 0; n < CPT; n++) {
@@ -595,7 +713,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
 #pragma unroll
             for (int n = 0; n < CPT; n++) {
                 const int col = (n / E * g.size + g.t) * E + n % E;
-                if (col < cols && col < 256) {
+                if (col < cols && col < 512) {
                     part[0][col] = k ? part[0][col] + sw[n] : sw[n];
                     part[1][col] = k ? part[1][col] + sb[n] : sb[n];
                 }
@@ -603,7 +721,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         }
         __syncthreads();
     }
-    for (int c = (int)threadIdx.x; c < cols && c < 256; c += (int)blockDim.x) { pw_out[c] = part[0][c]; pb_out[c] = part[1][c]; }
+    for (int c = (int)threadIdx.x; c < cols && c < 512; c += (int)blockDim.x) { pw_out[c] = part[0][c]; pb_out[c] = part[1][c]; }
 }
 
 template <typename T, typename W>
@@ -656,51 +774,78 @@ __device__ __forceinline__ void backward_columns(float *__restrict__ partial, co
     out[cols + c] = ab;
 }
 
-// dw and db: column sums of the `parts` partial rows, 32 columns a block, 32
-// threads on each column, in double and in a fixed order. blockIdx.y 0: dw, 1: db.
+// dw and db: column sums of the `parts` partial rows, in double and in a fixed order. A block has 128 columns, four a
+// lane, and 32 threads on each; blockIdx.y 0: dw, 1: db.
 template <typename W>
 __device__ __forceinline__ void param_grad(W *__restrict__ dw, W *__restrict__ db, const float *__restrict__ partial, int parts, int cols)
 {
-    __shared__ double sh[32][33];
+    __shared__ double sh[32][129];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     W *out = blockIdx.y ? db : dw;
     if (!out) return;
-    const int lane = (int)threadIdx.x & 31, ty = (int)threadIdx.x >> 5, c = (int)blockIdx.x * 32 + lane;
-    double s = 0.0;
-    if (c < cols) {
-        const float *p = partial + (size_t)blockIdx.y * cols + c;
-#pragma unroll 8
-        for (int i = ty; i < parts; i += 32) s += (double)__ldcg(p + (size_t)i * 2 * cols);
-    }
-    sh[ty][lane] = s;
-    __syncthreads();
-    // warp ty adds column ty of the block
-    s = sh[lane][ty];
+    const int lane = (int)threadIdx.x & 31, ty = (int)threadIdx.x >> 5, c0 = (int)blockIdx.x * 128;
+    const float *p = partial + (size_t)blockIdx.y * cols;
+    double s[4] = { 0.0, 0.0, 0.0, 0.0 };
+    if (cols % 4 == 0) {                        // the partial rows start on 16 bytes
+        const int c = c0 + 4 * lane;
+        if (c < cols) {
+#pragma unroll 4
+            for (int i = ty; i < parts; i += 32) {
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)i * 2 * cols + c));
+                s[0] += (double)v.x; s[1] += (double)v.y; s[2] += (double)v.z; s[3] += (double)v.w;
+            }
+        }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const int mine = (int)blockIdx.x * 32 + ty;
-    if (lane == 0 && mine < cols) out[mine] = from_f32<W>((float)s);
+        for (int e = 0; e < 4; e++) sh[ty][4 * lane + e] = s[e];
+    } else {
+#pragma unroll 4
+        for (int i = ty; i < parts; i += 32)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (c0 + 32 * e + lane < cols) s[e] += (double)__ldcg(p + (size_t)i * 2 * cols + c0 + 32 * e + lane);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sh[ty][32 * e + lane] = s[e];
+    }
+    __syncthreads();
+    // warp ty adds columns 4 ty .. 4 ty + 3 of the block
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        double v = sh[lane][4 * ty + e];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0 && c0 + 4 * ty + e < cols) out[c0 + 4 * ty + e] = from_f32<W>((float)v);
+    }
 }
 
 }  // namespace ln
 
-#define LN_FORM(name, T, W, form, VEC, CPT, HOLD, THREADS, BLOCKS)                                                                           \
+#define LN_FORWARD(name, T, W, form, VEC, CPT, HOLD, THREADS, BLOCKS)                                                                     \
     extern "C" __global__ void __launch_bounds__(THREADS, BLOCKS)                                                                        \
     layernorm_##name##_##form(T *y, const T *x, const W *w, const W *b, float *mean, float *rstd, long long rows, int cols,              \
                               long long ldx, long long ldy, float eps, int group, int depth)                                             \
-    { ln::forward<T, W, VEC, CPT, HOLD>(y, x, w, b, mean, rstd, rows, cols, ldx, ldy, eps, group, depth); }                              \
+    { ln::forward<T, W, VEC, CPT, HOLD>(y, x, w, b, mean, rstd, rows, cols, ldx, ldy, eps, group, depth); }
+#define LN_BACKWARD(name, T, W, form, VEC, CPT, HOLD, KEEP, THREADS)                                                                     \
     extern "C" __global__ void __launch_bounds__(THREADS)                                                                                \
     layernorm_bwd_##name##_##form(T *dx, float *partial, const T *dy, const T *x, const W *w, const float *mean, const float *rstd,      \
                                   long long rows, int cols, long long lddx, long long lddy, long long ldx, int group, int depth)         \
-    { ln::backward<T, W, VEC, CPT, HOLD>(dx, partial, dy, x, w, mean, rstd, rows, cols, lddx, lddy, ldx, group, depth); }
+    { ln::backward<T, W, VEC, CPT, HOLD, KEEP>(dx, partial, dy, x, w, mean, rstd, rows, cols, lddx, lddy, ldx, group, depth); }
 
 #define LN_KERNELS(name, T, W)                                                                                                           \
-    LN_FORM(name, T, W, v8, true, 8, true, 512, 2)                                                                                         \
-    LN_FORM(name, T, W, v16, true, 16, true, 256, 3)                                                                                       \
-    LN_FORM(name, T, W, vw, true, 16, false, 1024, 1)                                                                                      \
-    LN_FORM(name, T, W, s8, false, 8, true, 512, 1)                                                                                        \
-    LN_FORM(name, T, W, s16, false, 16, true, 512, 1)                                                                                      \
+    LN_FORWARD(name, T, W, v8, true, 8, true, 512, 2)                                                                                    \
+    LN_FORWARD(name, T, W, v32, true, 32, true, 256, 2)                                                                                  \
+    LN_FORWARD(name, T, W, vw, true, 16, false, 640, 1)                                                                                  \
+    LN_FORWARD(name, T, W, vx, true, 32, false, 512, 1)                                                                                  \
+    LN_FORWARD(name, T, W, s8, false, 8, true, 512, 1)                                                                                   \
+    LN_FORWARD(name, T, W, s16, false, 16, true, 512, 1)                                                                                 \
+    LN_FORWARD(name, T, W, sx, false, 32, false, 512, 1)                                                                                 \
+    LN_BACKWARD(name, T, W, v8, true, 8, true, true, 512)                                                                                \
+    LN_BACKWARD(name, T, W, v16, true, 16, true, true, 256)                                                                              \
+    LN_BACKWARD(name, T, W, vw, true, 16, false, true, 640)                                                                              \
+    LN_BACKWARD(name, T, W, vx, true, 32, false, false, 512)                                                                             \
+    LN_BACKWARD(name, T, W, s8, false, 8, true, true, 512)                                                                               \
+    LN_BACKWARD(name, T, W, s16, false, 16, true, true, 512)                                                                             \
+    LN_BACKWARD(name, T, W, sx, false, 32, false, false, 512)                                                                            \
     extern "C" __global__ void __launch_bounds__(512)                                                                                    \
     layernorm_##name##_loop(T *y, const T *x, const W *w, const W *b, float *mean, float *rstd, long long rows, int cols,                \
                             long long ldx, long long ldy, float eps, int group, int depth)                                               \

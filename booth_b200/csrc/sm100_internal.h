@@ -70,8 +70,9 @@ typedef struct sm100_api {
 #define SM100_SCRATCH_ORTH_STATUS  160
 #define SM100_SCRATCH_PARTIALS     256
 
-/* Forms of the layer normalisation kernels, the same for both directions. */
-#define SM100_LN_FORMS 6
+/* Forms of the layer normalisation kernels. */
+#define SM100_LN_FWD_FORMS 8
+#define SM100_LN_BWD_FORMS 8
 
 /* Built-in kernels, resolved once per device from the embedded image. */
 enum {
@@ -80,9 +81,9 @@ enum {
     SM100_K_ASIAN_MC, SM100_K_ASIAN_MC_PRECISE,
     SM100_K_ASIAN_PATHS, SM100_K_ASIAN_PATHS_PRECISE,
     SM100_K_GEMM_PREPASS, SM100_K_GEMM_TF32X3, SM100_K_GEMM_TF32X3_N128, SM100_K_GEMM_TF32X3_2CTA, SM100_K_GEMM_TF32X3_2CTA_N128, SM100_K_GEMM_PERSIST,
-    /* layer normalisation: five pairs of types, six forms each; per element type (f32, bf16, f16) the column sums */
-    SM100_K_LN_FWD, SM100_K_LN_BWD = SM100_K_LN_FWD + 5 * SM100_LN_FORMS,
-    SM100_K_LN_COLUMNS = SM100_K_LN_BWD + 5 * SM100_LN_FORMS, SM100_K_LN_PARAM_GRAD = SM100_K_LN_COLUMNS + 3,
+    /* layer normalisation: five pairs of types; per element type (f32, bf16, f16) the column sums */
+    SM100_K_LN_FWD, SM100_K_LN_BWD = SM100_K_LN_FWD + 5 * SM100_LN_FWD_FORMS,
+    SM100_K_LN_COLUMNS = SM100_K_LN_BWD + 5 * SM100_LN_BWD_FORMS, SM100_K_LN_PARAM_GRAD = SM100_K_LN_COLUMNS + 3,
     /* orthogonalisation: the products by tile side (64, 128, 256) and planes (1, 2) */
     SM100_K_ORTH_NORM = SM100_K_LN_PARAM_GRAD + 3, SM100_K_ORTH_SPLIT, SM100_K_ORTH_PRODUCT,
     SM100_K_COUNT = SM100_K_ORTH_PRODUCT + 6

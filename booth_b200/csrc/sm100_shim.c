@@ -144,17 +144,18 @@ int sm100_enter(sm100_dev_t *dev)
 
 /* ---- init / shut ---- */
 
-#define LN_FORM_NAMES(k) k "_v8", k "_v16", k "_vw", k "_s8", k "_s16", k "_loop"
+#define LN_FWD_NAMES(k) k "_v8", k "_v32", k "_vw", k "_vx", k "_s8", k "_s16", k "_sx", k "_loop"
+#define LN_BWD_NAMES(k) k "_v8", k "_v16", k "_vw", k "_vx", k "_s8", k "_s16", k "_sx", k "_loop"
 static const char *const k_names[SM100_K_COUNT] = {
     "vadd_stream", "saxpy_stream", "fill_philox",
     "reduce_sum_i32", "reduce_sum_f32",
     "asian_mc", "asian_mc_precise",
     "asian_paths", "asian_paths_precise",
     "gemm_prepass", "gemm_tf32x3", "gemm_tf32x3_n128", "gemm_tf32x3_2cta", "gemm_tf32x3_2cta_n128", "gemm_tf32x3_persist",
-    LN_FORM_NAMES("layernorm_f32"), LN_FORM_NAMES("layernorm_bf16"), LN_FORM_NAMES("layernorm_bf16_f32"),
-    LN_FORM_NAMES("layernorm_f16"), LN_FORM_NAMES("layernorm_f16_f32"),
-    LN_FORM_NAMES("layernorm_bwd_f32"), LN_FORM_NAMES("layernorm_bwd_bf16"), LN_FORM_NAMES("layernorm_bwd_bf16_f32"),
-    LN_FORM_NAMES("layernorm_bwd_f16"), LN_FORM_NAMES("layernorm_bwd_f16_f32"),
+    LN_FWD_NAMES("layernorm_f32"), LN_FWD_NAMES("layernorm_bf16"), LN_FWD_NAMES("layernorm_bf16_f32"),
+    LN_FWD_NAMES("layernorm_f16"), LN_FWD_NAMES("layernorm_f16_f32"),
+    LN_BWD_NAMES("layernorm_bwd_f32"), LN_BWD_NAMES("layernorm_bwd_bf16"), LN_BWD_NAMES("layernorm_bwd_bf16_f32"),
+    LN_BWD_NAMES("layernorm_bwd_f16"), LN_BWD_NAMES("layernorm_bwd_f16_f32"),
     "layernorm_bwd_columns_f32", "layernorm_bwd_columns_bf16", "layernorm_bwd_columns_f16",
     "layernorm_param_grad_f32", "layernorm_param_grad_bf16", "layernorm_param_grad_f16",
     "orth_norm", "orth_split", "orth_product_1_64", "orth_product_2_64", "orth_product_1_128", "orth_product_2_128", "orth_product_1_256", "orth_product_2_256",

@@ -45,42 +45,54 @@ static int ln_pair(int dtype, int wdtype)
     return -1;
 }
 
-enum { LN_V8, LN_V16, LN_VW, LN_S8, LN_S16, LN_LOOP };
+/* A form of the kernels: its place among the names, the values a thread has, the most threads a row may have, and what
+ * the SM's registers hold of its threads. */
+typedef struct { int at, vec, cpt, most; unsigned resident; } ln_form_t;
+
+/* Rows so few that each has an SM to itself get eight values a thread: more threads
+ * shorten the one row. Else as many values as the registers bear, thirty-two forward and
+ * sixteen backward, which spreads what a row costs each thread beside its values; rows too wide for
+ * these take the forms without parameters or row in registers. */
+static const ln_form_t ln_forward[] = { { 0, 1, 8, 512, 1024 }, { 1, 1, 32, 256, 512 }, { 2, 1, 16, 640, 640 }, { 3, 1, 32, 512, 512 },
+                                        { 4, 0, 8, 512, 768 }, { 5, 0, 16, 512, 512 }, { 6, 0, 32, 512, 512 } };
+static const ln_form_t ln_backward[] = { { 0, 1, 8, 512, 768 }, { 1, 1, 16, 256, 512 }, { 2, 1, 16, 640, 640 }, { 3, 1, 32, 512, 512 },
+                                         { 4, 0, 8, 512, 768 }, { 5, 0, 16, 512, 512 }, { 6, 0, 32, 512, 512 } };
+#define LN_LOOP 7
 
 /* Shared memory for rings: what an SM has less the blocks' own few KB. */
-#define LN_RING_SM (208u << 10)
+#define LN_RING_SM (204u << 10)
 
-typedef struct { int form, group, depth; unsigned block, grid, ring; } ln_shape_t;
+typedef struct { int form, loop, group, depth; unsigned block, grid, ring; } ln_shape_t;
 
-/* How rows are dealt to threads. Eight values a thread for narrow rows, and for
- * rows so few that each has an SM to itself (more threads shorten the one row);
- * sixteen otherwise, which halves what the reductions and the barriers cost per
- * value; vector rows too wide for 256 threads get up to 1024, without the parameters in registers; else the form that walks
- * the row. Blocks stay, each taking every grid-th row: as many as an SM holds by
- * registers (64 to 80 a thread for eight values, 80 to 128 else), and of the vector
- * forms' rings up to four rows each, as many as fit beside one another. */
+/* How rows are dealt to threads: the form, the group of threads a row has, and blocks
+ * that stay, each taking every grid-th row: as many as an SM holds by registers, and by
+ * rings of up to four rows each. */
 static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, unsigned esz, int vec, int backward)
 {
     ln_shape_t s;
-    const int cpt = cols <= 1024 || (cols <= 4096 && rows < 2ll * dev->sm_count) ? 8 : cols <= 8192 || (cols <= 16384 && vec) ? 16 : 0;
-    s.form = cpt == 8 ? (vec ? LN_V8 : LN_S8) : cpt == 16 ? (!vec ? LN_S16 : cols <= 4096 ? LN_V16 : LN_VW) : LN_LOOP;
+    const ln_form_t *forms = backward ? ln_backward : ln_forward, *f = NULL;
+    const int n = LN_LOOP, few = rows < 2ll * dev->sm_count;
+    for (int i = 0; i < n && !f; i++)
+        if (forms[i].vec == vec && (forms[i].cpt > 8 || few) && cols <= forms[i].cpt * forms[i].most) f = &forms[i];
+    s.loop = !f;
+    s.form = f ? f->at : n;
     s.depth = 1;
     s.ring = 0;
-    if (!cpt) {
-        s.group = 512;
-        s.block = 512;
-    } else {
-        int g = (cols + cpt - 1) / cpt;
+    s.group = 512;
+    s.block = 512;
+    if (f) {
+        int g = (cols + f->cpt - 1) / f->cpt;
         if (g <= 32) { int p = 1; while (p < g) p *= 2; g = p; }
         else g = (g + 31) / 32 * 32;
         s.group = g;
         s.block = g <= 32 ? 128u : (unsigned)g;
     }
     const long long per_block = s.group <= 32 ? (long long)s.block / s.group : 1;
-    const unsigned threads = cpt == 8 ? (!backward ? 1024u : vec ? 768u : 512u) : s.form == LN_VW ? 1024u : backward ? 512u : 768u;
-    unsigned per_sm = threads / s.block < 1 ? 1 : threads / s.block;
-    if (s.form <= LN_VW) {
-        const unsigned row = s.block * (unsigned)cpt * esz * (backward ? 2u : 1u);
+    unsigned per_sm = (f ? f->resident : 1024u) / s.block;
+    if (per_sm < 1) per_sm = 1;
+    if (f) {
+        const unsigned arrays = backward ? 2u : 1u, slot = ((unsigned)cols * esz + 15u) / 16u * 16u + 16u;
+        const unsigned row = vec ? s.block * (unsigned)f->cpt * esz * arrays : (unsigned)per_block * slot * arrays;
         s.depth = 4;
         while (s.depth > 2 && per_sm * (unsigned)s.depth * row > LN_RING_SM) s.depth--;
         while (per_sm > 1 && per_sm * (unsigned)s.depth * row > LN_RING_SM) per_sm--;
@@ -96,11 +108,14 @@ static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, uns
 static int ln_ready(sm100_dev_t *dev)
 {
     if (dev->ln_smem_set) return SM100_OK;
-    for (int k = 0; k < 2 * 5 * SM100_LN_FORMS; k++) {
-        if (k % SM100_LN_FORMS > LN_VW) continue;
-        CUresult cr = dev->api->FuncSetAttribute(dev->k[SM100_K_LN_FWD + k], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)LN_RING_SM);
-        if (cr != CUDA_SUCCESS) return sm100_fail(dev, "raising the layer normalisation kernels' shared memory limit", cr);
-    }
+    for (int pair = 0; pair < 5; pair++)
+        for (int backward = 0; backward < 2; backward++)
+            for (int i = 0; i < LN_LOOP; i++) {
+                const ln_form_t *f = backward ? &ln_backward[i] : &ln_forward[i];
+                const int k = (backward ? SM100_K_LN_BWD + pair * SM100_LN_BWD_FORMS : SM100_K_LN_FWD + pair * SM100_LN_FWD_FORMS) + f->at;
+                CUresult cr = dev->api->FuncSetAttribute(dev->k[k], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)LN_RING_SM);
+                if (cr != CUDA_SUCCESS) return sm100_fail(dev, "raising the layer normalisation kernels' shared memory limit", cr);
+            }
     dev->ln_smem_set = 1;
     return SM100_OK;
 }
@@ -124,7 +139,7 @@ int booth_sm100_layernorm(sm100_dev_t *dev, sm100_ptr_t y, sm100_ptr_t x, sm100_
     const ln_shape_t s = ln_shape(dev, rows, cols, e, vec, 0);
     int group = s.group, depth = s.depth;
     void *args[] = { &y, &x, &w, &b, &mean, &rstd, &rows, &cols, &ldx, &ldy, &eps, &group, &depth };
-    return sm100_launch_k_overlapped(dev, SM100_K_LN_FWD + pair * SM100_LN_FORMS + s.form, s.grid, s.block, s.ring, args);
+    return sm100_launch_k_overlapped(dev, SM100_K_LN_FWD + pair * SM100_LN_FWD_FORMS + s.form, s.grid, s.block, s.ring, args);
 }
 
 /* Partial rows of the parameters' gradients: one a block, or one a row range in the walking form. */
@@ -139,7 +154,7 @@ size_t booth_sm100_layernorm_backward_workspace(sm100_dev_t *dev, long long rows
     size_t parts = LN_LOOP_PARTS;
     for (int vec = 0; vec < 2; vec++) {
         const ln_shape_t s = ln_shape(dev, rows, cols, type_bytes(dtype), vec, 1);
-        if (s.form != LN_LOOP && s.grid > parts) parts = s.grid;
+        if (!s.loop && s.grid > parts) parts = s.grid;
     }
     return parts * 2 * (size_t)cols * sizeof(float);
 }
@@ -172,11 +187,11 @@ int booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t
         sm100_ptr_t partial = params ? ws : 0;
         void *args[] = { &dx, &partial, &dy, &x, &w, &mean, &rstd, &rows, &cols, &lddx, &lddy, &ldx, &group, &depth };
         parts = (int)s.grid;
-        if (s.form != LN_LOOP || dx) {
-            rc = sm100_launch_k_overlapped(dev, SM100_K_LN_BWD + pair * SM100_LN_FORMS + s.form, s.grid, s.block, s.ring, args);
+        if (!s.loop || dx) {
+            rc = sm100_launch_k_overlapped(dev, SM100_K_LN_BWD + pair * SM100_LN_BWD_FORMS + s.form, s.grid, s.block, s.ring, args);
             if (rc != SM100_OK) return rc;
         }
-        if (s.form == LN_LOOP && params) {
+        if (s.loop && params) {
             parts = rows < LN_LOOP_PARTS ? (int)rows : LN_LOOP_PARTS;
             void *ca[] = { &partial, &dy, &x, &mean, &rstd, &rows, &cols, &lddy, &ldx };
             rc = sm100_launch_k3_overlapped(dev, SM100_K_LN_COLUMNS + type_index(dtype), (unsigned)(((long long)cols + 255) / 256), (unsigned)parts, 1, 256, 1, 1, 0, ca);
@@ -185,7 +200,7 @@ int booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t
     }
     if (params) {
         void *pa[] = { &dw, &db, &ws, &parts, &cols };
-        rc = sm100_launch_k3_overlapped(dev, SM100_K_LN_PARAM_GRAD + type_index(wdtype), (unsigned)(((long long)cols + 31) / 32), 2, 1, 1024, 1, 1, 0, pa);
+        rc = sm100_launch_k3_overlapped(dev, SM100_K_LN_PARAM_GRAD + type_index(wdtype), (unsigned)(((long long)cols + 127) / 128), 2, 1, 1024, 1, 1, 0, pa);
     }
     return rc;
 }
