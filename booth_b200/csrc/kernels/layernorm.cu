@@ -318,6 +318,40 @@ template <typename T, int A> struct Slots {
     }
 };
 
+// Parameters of wide rows, in fp32 in shared memory behind the ring: each thread has those of its own columns in places
+// of its own, as with the ring. Array n of a chunk j; 16 bytes a thread (E = 1: 4).
+struct Kept {
+    uint32_t base, step;
+    __device__ __forceinline__ Kept(uint32_t ring_bytes)
+    {
+        extern __shared__ uint4 ln_ring[];
+        base = (uint32_t)__cvta_generic_to_shared(ln_ring) + ring_bytes;
+        step = blockDim.x;
+    }
+    template <int E, int NCH> __device__ __forceinline__ uint32_t at(int n, int j, int k) const
+    {
+        return E == 1 ? base + ((uint32_t)(n * NCH + j) * step + threadIdx.x) * 4u : base + ((uint32_t)((n * NCH + j) * (E / 4 < 1 ? 1 : E / 4) + k) * step + threadIdx.x) * 16u;
+    }
+    template <int E, int NCH> __device__ __forceinline__ void put(int n, int j, const float (&q)[E]) const
+    {
+        if constexpr (E == 1) asm volatile("st.shared.f32 [%0], %1;" ::"r"(at<E, NCH>(n, j, 0)), "f"(q[0]) : "memory");
+        else {
+#pragma unroll
+            for (int k = 0; k < E / 4; k++)
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at<E, NCH>(n, j, k)), "f"(q[4 * k]), "f"(q[4 * k + 1]), "f"(q[4 * k + 2]), "f"(q[4 * k + 3]) : "memory");
+        }
+    }
+    template <int E, int NCH> __device__ __forceinline__ void get(int n, int j, float (&q)[E]) const
+    {
+        if constexpr (E == 1) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(q[0]) : "r"(at<E, NCH>(n, j, 0)) : "memory");
+        else {
+#pragma unroll
+            for (int k = 0; k < E / 4; k++)
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q[4 * k]), "=f"(q[4 * k + 1]), "=f"(q[4 * k + 2]), "=f"(q[4 * k + 3]) : "r"(at<E, NCH>(n, j, k)) : "memory");
+        }
+    }
+};
+
 // Whether pair i of this thread lies in the row: all of it (vectors; cols is a multiple), or its first or second value.
 template <int E> __device__ __forceinline__ bool inside(const Group &g, int i, int half, int cols)
 {
@@ -393,6 +427,16 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
             if (b) load_params<W, E>(b, col, qb);
         }
     };
+    const Kept kept(VEC ? (uint32_t)(depth * NCH) * blockDim.x * 16u : (uint32_t)depth * slots.groups * slots.pitch);
+    if constexpr (!HOLD) {
+#pragma unroll
+        for (int j = 0; j < NCH; j++) {
+            float qw[E], qb[E];
+            params(j, qw, qb);
+            kept.template put<E, NCH>(0, j, qw);
+            kept.template put<E, NCH>(1, j, qb);
+        }
+    }
     if constexpr (HOLD) {
         float qw[NCH][E], qb[NCH][E];
 #pragma unroll
@@ -443,8 +487,11 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                 for (int i = 0; i < CPT / 2; i++) {
                     if constexpr (!HOLD) {
                         float qw[2][E], qb[2][E];
-                        params(2 * i, qw[0], qb[0]);
-                        params(2 * i + 1, qw[1], qb[1]);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            kept.template get<E, NCH>(0, 2 * i + h, qw[h]);
+                            kept.template get<E, NCH>(1, 2 * i + h, qb[h]);
+                        }
                         v[i] = fma(v[i], pair(qw[0][0], qw[1][0]), pair(qb[0][0], qb[1][0]));
                     } else {
                         v[i] = fma(v[i], pw[i], pb[i]);
@@ -460,7 +507,7 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                     if (col < cols) {
                         Chunk<T, E> o;
                         float qw[E], qb[E];
-                        if constexpr (!HOLD) params(j, qw, qb);
+                        if constexpr (!HOLD) { kept.template get<E, NCH>(0, j, qw); kept.template get<E, NCH>(1, j, qb); }
 #pragma unroll
                         for (int i = 0; i < E / 2; i++) {
                             const int n = j * E / 2 + i;
@@ -545,6 +592,15 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         for (int e = 0; e < E; e++) q[e] = 1.f;
         if (w && col < cols) load_params<W, E>(w, col, q);
     };
+    const Kept kept(VEC ? (uint32_t)(depth * 2 * NCH) * blockDim.x * 16u : (uint32_t)(depth * 2) * slots.groups * slots.pitch);
+    if constexpr (!HOLD) {
+#pragma unroll
+        for (int j = 0; j < NCH; j++) {
+            float q[E];
+            weight(j, q);
+            kept.template put<E, NCH>(0, j, q);
+        }
+    }
     if constexpr (HOLD) {
         float q[NCH][E];
 #pragma unroll
@@ -574,7 +630,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                 const bool live = row < rows && (j * g.size + g.t) * E < cols;
                 const Chunk<T, E> xc = ring.template get<T, E>(0, j, live), dc = ring.template get<T, E>(1, j, live);
                 float q[E];
-                if constexpr (!HOLD) weight(j, q);
+                if constexpr (!HOLD) kept.template get<E, NCH>(0, j, q);
 #pragma unroll
                 for (int i = 0; i < E / 2; i++) {
                     const int n = j * E / 2 + i, k = KEEP_ROW ? n : i;
@@ -608,8 +664,8 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                 if constexpr (HOLD) wd[k] = mul(d, pw[n]);
                 else {
                     float q0[E], q1[E];
-                    weight(2 * n, q0);
-                    weight(2 * n + 1, q1);
+                    kept.template get<E, NCH>(0, 2 * n, q0);
+                    kept.template get<E, NCH>(0, 2 * n + 1, q1);
                     wd[k] = mul(d, pair(q0[0], q1[0]));
                 }
                 s1 = add(s1, wd[k]);
@@ -646,8 +702,8 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                     if constexpr (!KEEP_ROW) {
                         const T *const xr = x + row * ldx, *const dr = dy + row * lddy;
                         float q0[E], q1[E];
-                        weight(2 * i, q0);
-                        weight(2 * i + 1, q1);
+                        kept.template get<E, NCH>(0, 2 * i, q0);
+                        kept.template get<E, NCH>(0, 2 * i + 1, q1);
                         xh[0] = mul(add(pair(slots.get(0, xr, 2 * i * g.size + g.t, cols, true), slots.get(0, xr, (2 * i + 1) * g.size + g.t, cols, true)), nmean), r2);
                         wd[0] = mul(pair(slots.get(1, dr, 2 * i * g.size + g.t, cols, true), slots.get(1, dr, (2 * i + 1) * g.size + g.t, cols, true)), pair(q0[0], q1[0]));
                     }
@@ -664,7 +720,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                         if constexpr (!KEEP_ROW) {
                             const Chunk<T, E> xc = ring.template get<T, E>(0, j, true), dc = ring.template get<T, E>(1, j, true);
                             float u[E];
-                            weight(j, u);
+                            kept.template get<E, NCH>(0, j, u);
 #pragma unroll
                             for (int i = 0; i < E / 2; i++) {
                                 xh[i] = mul(add(widen(&xc.v[2 * i]), nmean), r2);

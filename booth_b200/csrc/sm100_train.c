@@ -45,18 +45,18 @@ static int ln_pair(int dtype, int wdtype)
     return -1;
 }
 
-/* A form of the kernels: its place among the names, the values a thread has, the most threads a row may have, and what
- * the SM's registers hold of its threads. */
-typedef struct { int at, vec, cpt, most; unsigned resident; } ln_form_t;
+/* A form of the kernels: its place among the names, the values a thread has, the most threads a row may have, what
+ * the SM's registers hold of its threads, and whether the parameters are kept in shared memory. */
+typedef struct { int at, vec, cpt, most; unsigned resident; int kept; } ln_form_t;
 
 /* Rows so few that each has an SM to itself get eight values a thread: more threads
  * shorten the one row. Else as many values as the registers bear, thirty-two forward and
  * sixteen backward, which spreads what a row costs each thread beside its values; rows too wide for
- * these take the forms without parameters or row in registers. */
-static const ln_form_t ln_forward[] = { { 0, 1, 8, 512, 1024 }, { 1, 1, 32, 256, 512 }, { 2, 1, 16, 640, 640 }, { 3, 1, 32, 512, 512 },
-                                        { 4, 0, 8, 512, 768 }, { 5, 0, 16, 512, 512 }, { 6, 0, 32, 512, 512 } };
-static const ln_form_t ln_backward[] = { { 0, 1, 8, 512, 768 }, { 1, 1, 16, 256, 512 }, { 2, 1, 16, 640, 640 }, { 3, 1, 32, 512, 512 },
-                                         { 4, 0, 8, 512, 768 }, { 5, 0, 16, 512, 512 }, { 6, 0, 32, 512, 512 } };
+ * these take the forms that keep parameters or row in shared memory. */
+static const ln_form_t ln_forward[] = { { 0, 1, 8, 512, 1024, 0 }, { 1, 1, 32, 256, 512, 0 }, { 2, 1, 16, 640, 640, 1 }, { 3, 1, 32, 512, 512, 1 },
+                                        { 4, 0, 8, 512, 768, 0 }, { 5, 0, 16, 512, 512, 0 }, { 6, 0, 32, 512, 512, 1 } };
+static const ln_form_t ln_backward[] = { { 0, 1, 8, 512, 768, 0 }, { 1, 1, 16, 256, 512, 0 }, { 2, 1, 16, 640, 640, 1 }, { 3, 1, 32, 512, 512, 1 },
+                                         { 4, 0, 8, 512, 768, 0 }, { 5, 0, 16, 512, 512, 0 }, { 6, 0, 32, 512, 512, 1 } };
 #define LN_LOOP 7
 
 /* Shared memory for rings: what an SM has less the blocks' own few KB. */
@@ -93,11 +93,12 @@ static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, uns
     if (f) {
         const unsigned arrays = backward ? 2u : 1u, slot = ((unsigned)cols * esz + 15u) / 16u * 16u + 16u;
         const unsigned row = vec ? s.block * (unsigned)f->cpt * esz * arrays : (unsigned)per_block * slot * arrays;
+        const unsigned kept = f->kept ? s.block * (unsigned)f->cpt * (backward ? 4u : 8u) : 0u;
         s.depth = 4;
-        while (s.depth > 2 && per_sm * (unsigned)s.depth * row > LN_RING_SM) s.depth--;
-        while (per_sm > 1 && per_sm * (unsigned)s.depth * row > LN_RING_SM) per_sm--;
-        if ((unsigned)s.depth * row > LN_RING_SM) s.depth = 1;
-        s.ring = (unsigned)s.depth * row;
+        while (s.depth > 2 && per_sm * ((unsigned)s.depth * row + kept) > LN_RING_SM) s.depth--;
+        while (per_sm > 1 && per_sm * ((unsigned)s.depth * row + kept) > LN_RING_SM) per_sm--;
+        if ((unsigned)s.depth * row + kept > LN_RING_SM) s.depth = 1;
+        s.ring = (unsigned)s.depth * row + kept;
     }
     long long want = (rows + per_block - 1) / per_block;
     if (want > (long long)dev->sm_count * per_sm) want = (long long)dev->sm_count * per_sm;
