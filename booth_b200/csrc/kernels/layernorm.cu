@@ -233,17 +233,24 @@ template <int A, int NCH> struct Ring {
 // The ring for rows of any alignment: a row has a slot in which its bytes lie as they do in memory modulo 16. Whole
 // 16-byte units come with cp.async, the units at its two ends word by word, and a 16-bit value that shares its word
 // with a neighbour's row through a register, written to the slot at the next step. What one thread brings others read,
-// so a row is ready behind a barrier of its group, and its slot is free behind the next one.
+// so a row is ready behind a barrier of its group, and its slot is free behind the next one. A slot is as long as
+// all values of a group's threads, zero behind the row, so that reading takes no comparisons.
 template <typename T, int A> struct Slots {
     uint32_t base, pitch, groups, held[A][2];
     uint16_t edge[A][2];
     int depth, stage;
-    __device__ __forceinline__ Slots(int depth_, int cols, const Group &g) : depth(depth_), stage(0)
+    template <bool USED> __device__ __forceinline__ void init(int depth_, int cpt, const Group &g)
     {
         extern __shared__ uint4 ln_ring[];
-        pitch = ((uint32_t)cols * (uint32_t)sizeof(T) + 15u) / 16u * 16u + 16u;
+        depth = depth_;
+        stage = 0;
+        pitch = ((uint32_t)(cpt * g.size) * (uint32_t)sizeof(T) + 15u) / 16u * 16u + 16u;
         groups = (uint32_t)g.per_block;
         base = (uint32_t)__cvta_generic_to_shared(ln_ring) + (uint32_t)g.index * pitch;
+        if constexpr (USED) {
+            for (uint32_t u = threadIdx.x; u < (uint32_t)(depth * A) * groups * pitch / 16u; u += blockDim.x) ln_ring[u] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+        }
 #pragma unroll
         for (int a = 0; a < A; a++) { held[a][0] = held[a][1] = 0; edge[a][0] = edge[a][1] = 0; }
     }
@@ -254,6 +261,9 @@ template <typename T, int A> struct Slots {
         const uintptr_t at = reinterpret_cast<uintptr_t>(row);
         const uint32_t head = (uint32_t)(at & 15), end = head + (uint32_t)cols * (uint32_t)sizeof(T), to = slot(a);
         const char *const from = reinterpret_cast<const char *>(at - head);
+        // an earlier row that lay further on may have ended in the unit behind this row's last
+        const uint32_t behind = (end + 15u) / 16u * 16u;
+        if (behind + 16u <= pitch && g.t == 0) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + behind), "r"(0) : "memory");
         for (uint32_t u = (uint32_t)g.t * 16u; u < end; u += (uint32_t)g.size * 16u) {
             if (u >= head && u + 16u <= end) {
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u), "l"(from + u) : "memory");
@@ -262,12 +272,14 @@ template <typename T, int A> struct Slots {
 #pragma unroll
             for (uint32_t w = u; w < u + 16u; w += 4u) {
                 if (w >= head && w + 4u <= end) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + w), "l"(from + w) : "memory");
-                else if (sizeof(T) == 2 && w + 4u > head && w < end) {
+                else if (w >= end) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + w), "r"(0) : "memory");
+                else if (sizeof(T) == 2 && w + 4u > head) {
                     // one half of the word: the row's first value in its upper half, or its last in the lower
                     const int tail = w >= head ? 1 : 0;
                     const uint32_t h = tail ? w : w + 2u;
                     held[a][tail] = to + h;
                     edge[a][tail] = *reinterpret_cast<const uint16_t *>(from + h);
+                    if (tail) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + w + 2u), "h"((uint16_t)0) : "memory");
                 }
             }
         }
@@ -296,11 +308,14 @@ template <typename T, int A> struct Slots {
         else asm volatile("cp.async.wait_group 0;" ::: "memory");
         meet(g);
     }
-    // Column c of the row at `row`; zero outside.
-    __device__ __forceinline__ float get(int a, const T *row, int c, int cols, bool live) const
+    // Where this thread's first value of the row at `row` lies; its others follow `step()` bytes apart.
+    __device__ __forceinline__ uint32_t first(int a, const T *row, const Group &g) const
     {
-        if (!live || c >= cols) return 0.f;
-        const uint32_t at = slot(a) + (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + (uint32_t)c * (uint32_t)sizeof(T);
+        return slot(a) + (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + (uint32_t)g.t * (uint32_t)sizeof(T);
+    }
+    static __device__ __forceinline__ uint32_t step(const Group &g) { return (uint32_t)g.size * (uint32_t)sizeof(T); }
+    static __device__ __forceinline__ float value(uint32_t at)
+    {
         if constexpr (sizeof(T) == 4) {
             float v;
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
@@ -311,10 +326,18 @@ template <typename T, int A> struct Slots {
             return to_f32(*reinterpret_cast<const T *>(&v));
         }
     }
-    template <int N> __device__ __forceinline__ void get_all(int a, const T *row, const Group &g, int cols, bool live, Pair (&v)[N]) const
+    static __device__ __forceinline__ Pair values(uint32_t &at, uint32_t by)
     {
+        const float a = value(at), b = value(at + by);
+        at += 2u * by;
+        return pair(a, b);
+    }
+    template <int N> __device__ __forceinline__ void get_all(int a, const T *row, const Group &g, Pair (&v)[N]) const
+    {
+        uint32_t at = first(a, row, g);
+        const uint32_t by = step(g);
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = pair(get(a, row, 2 * i * g.size + g.t, cols, live), get(a, row, (2 * i + 1) * g.size + g.t, cols, live));
+        for (int i = 0; i < N; i++) v[i] = values(at, by);
     }
 };
 
@@ -352,15 +375,17 @@ struct Kept {
     }
 };
 
-// Whether pair i of this thread lies in the row: all of it (vectors; cols is a multiple), or its first or second value.
-template <int E> __device__ __forceinline__ bool inside(const Group &g, int i, int half, int cols)
+// Whether chunk j of this thread (E > 1: vectors lie in the row whole or not at all), or its value j (E = 1), lies in
+// the row. `valid`: how many of its values do, when they are single.
+template <int E> __device__ __forceinline__ bool inside(const Group &g, int j, int valid, int cols)
 {
-    return E == 1 ? (2 * i + half) * g.size + g.t < cols : ((2 * i / (E < 2 ? 2 : E)) * g.size + g.t) * E < cols;
+    return E == 1 ? j < valid : (j * g.size + g.t) * E < cols;
 }
+__device__ __forceinline__ int valid_of(const Group &g, int cols) { return g.t < cols ? (cols - g.t + g.size - 1) / g.size : 0; }
 
 // v: a row's values in, their differences from `m` out (zero outside the row). mean = m + dm.
 template <int E, int N>
-__device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int cols, float inv, float eps, float2 (*sh)[32], float &m, float &dm, float &rstd)
+__device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int valid, int cols, float inv, float eps, float2 (*sh)[32], float &m, float &dm, float &rstd)
 {
     Pair s = pair(0.f, 0.f);
 #pragma unroll
@@ -374,9 +399,9 @@ __device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int cols, floa
         v[i] = add(v[i], nm);
         if constexpr (E == 1) {
             const float2 x = split(v[i]);
-            v[i] = pair(inside<E>(g, i, 0, cols) ? x.x : 0.f, inside<E>(g, i, 1, cols) ? x.y : 0.f);
+            v[i] = pair(inside<E>(g, 2 * i, valid, cols) ? x.x : 0.f, inside<E>(g, 2 * i + 1, valid, cols) ? x.y : 0.f);
         } else {
-            if (!inside<E>(g, i, 0, cols)) v[i] = pair(0.f, 0.f);
+            if (!inside<E>(g, 2 * i / (E < 2 ? 2 : E), valid, cols)) v[i] = pair(0.f, 0.f);
         }
         d1 = add(d1, v[i]);
         d2 = fma(v[i], v[i], d2);
@@ -403,7 +428,9 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
     const long long step = (long long)gridDim.x * g.per_block;
     long long base = (long long)blockIdx.x * g.per_block;
     Ring<1, VEC ? NCH : 1> ring(depth);
-    Slots<T, 1> slots(depth, cols, g);
+    Slots<T, 1> slots;
+    slots.template init<!VEC>(depth, CPT, g);
+    const int valid = valid_of(g, cols);
     for (int d = 0; d < depth; d++) {
         const long long row = base + g.index + d * step;
         if constexpr (VEC) {
@@ -458,10 +485,10 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
             widen_all<T, E, NCH>(cur, v);
         } else {
             slots.wait(g);
-            slots.get_all(0, x + row * ldx, g, cols, row < rows, v);
+            slots.get_all(0, x + row * ldx, g, v);
         }
         float m, dm, rstd;
-        row_stats<E, CPT / 2>(v, g, cols, inv, eps, sh, m, dm, rstd);
+        row_stats<E, CPT / 2>(v, g, valid, cols, inv, eps, sh, m, dm, rstd);
         const long long ahead = row + depth * step;          // the row is in registers: its places may fill again
         if constexpr (VEC) {
             ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
@@ -483,6 +510,7 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
 #pragma unroll
             for (int i = 0; i < CPT / 2; i++) v[i] = fma(v[i], r2, shift);
             if constexpr (E == 1) {
+                T *to = out + g.t;
 #pragma unroll
                 for (int i = 0; i < CPT / 2; i++) {
                     if constexpr (!HOLD) {
@@ -497,8 +525,9 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                         v[i] = fma(v[i], pw[i], pb[i]);
                     }
                     const float2 f = split(v[i]);
-                    if (inside<E>(g, i, 0, cols)) out[2 * i * g.size + g.t] = from_f32<T>(f.x);
-                    if (inside<E>(g, i, 1, cols)) out[(2 * i + 1) * g.size + g.t] = from_f32<T>(f.y);
+                    if (inside<E>(g, 2 * i, valid, cols)) to[0] = from_f32<T>(f.x);
+                    if (inside<E>(g, 2 * i + 1, valid, cols)) to[g.size] = from_f32<T>(f.y);
+                    to += 2 * g.size;
                 }
             } else {
 #pragma unroll
@@ -570,7 +599,9 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
     const long long step = (long long)gridDim.x * g.per_block;
     long long base = (long long)blockIdx.x * g.per_block;
     Ring<2, VEC ? NCH : 1> ring(depth);
-    Slots<T, 2> slots(depth, cols, g);
+    Slots<T, 2> slots;
+    slots.template init<!VEC>(depth, CPT, g);
+    const int valid = valid_of(g, cols);
     for (int d = 0; d < depth; d++) {
         const long long row = base + g.index + d * step;
         if constexpr (VEC) {
@@ -646,16 +677,22 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
             }
         } else {
             const T *const xr = x + row * ldx, *const dr = dy + row * lddy;
+            uint32_t xa = slots.first(0, xr, g), da = slots.first(1, dr, g);
+            const uint32_t by = slots.step(g);
             if constexpr (KEEP_ROW) {
-                slots.get_all(0, xr, g, cols, row < rows, xh);
-                slots.get_all(1, dr, g, cols, row < rows, wd);
+                slots.get_all(0, xr, g, xh);
+                slots.get_all(1, dr, g, wd);
+            }
+            if (row >= rows) {                  // a group past the end: its slot holds an earlier row
+#pragma unroll
+                for (int k = 0; k < KEEP; k++) xh[k] = wd[k] = pair(0.f, 0.f);
             }
 #pragma unroll
             for (int n = 0; n < N; n++) {
                 const int k = KEEP_ROW ? n : 0;
                 if constexpr (!KEEP_ROW) {
-                    xh[0] = pair(slots.get(0, xr, 2 * n * g.size + g.t, cols, row < rows), slots.get(0, xr, (2 * n + 1) * g.size + g.t, cols, row < rows));
-                    wd[0] = pair(slots.get(1, dr, 2 * n * g.size + g.t, cols, row < rows), slots.get(1, dr, (2 * n + 1) * g.size + g.t, cols, row < rows));
+                    xh[0] = slots.values(xa, by);
+                    wd[0] = slots.values(da, by);
                 }
                 const Pair d = wd[k];
                 xh[k] = mul(add(xh[k], nmean), r2);
@@ -696,20 +733,23 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
             const Pair np = pair(-p, -p), nq = pair(-q, -q);
             T *out = dx + row * lddx;
             if constexpr (E == 1) {
+                T *to = out + g.t;
+                uint32_t xa = slots.first(0, x + row * ldx, g), da = slots.first(1, dy + row * lddy, g);
+                const uint32_t by = slots.step(g);
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     const int k = KEEP_ROW ? i : 0;
                     if constexpr (!KEEP_ROW) {
-                        const T *const xr = x + row * ldx, *const dr = dy + row * lddy;
                         float q0[E], q1[E];
                         kept.template get<E, NCH>(0, 2 * i, q0);
                         kept.template get<E, NCH>(0, 2 * i + 1, q1);
-                        xh[0] = mul(add(pair(slots.get(0, xr, 2 * i * g.size + g.t, cols, true), slots.get(0, xr, (2 * i + 1) * g.size + g.t, cols, true)), nmean), r2);
-                        wd[0] = mul(pair(slots.get(1, dr, 2 * i * g.size + g.t, cols, true), slots.get(1, dr, (2 * i + 1) * g.size + g.t, cols, true)), pair(q0[0], q1[0]));
+                        xh[0] = mul(add(slots.values(xa, by), nmean), r2);
+                        wd[0] = mul(slots.values(da, by), pair(q0[0], q1[0]));
                     }
                     const float2 f = split(mul(r2, fma(xh[k], nq, add(wd[k], np))));
-                    if (inside<E>(g, i, 0, cols)) out[2 * i * g.size + g.t] = from_f32<T>(f.x);
-                    if (inside<E>(g, i, 1, cols)) out[(2 * i + 1) * g.size + g.t] = from_f32<T>(f.y);
+                    if (inside<E>(g, 2 * i, valid, cols)) to[0] = from_f32<T>(f.x);
+                    if (inside<E>(g, 2 * i + 1, valid, cols)) to[g.size] = from_f32<T>(f.y);
+                    to += 2 * g.size;
                 }
             } else {
 #pragma unroll

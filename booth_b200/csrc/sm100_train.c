@@ -91,7 +91,7 @@ static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, uns
     unsigned per_sm = (f ? f->resident : 1024u) / s.block;
     if (per_sm < 1) per_sm = 1;
     if (f) {
-        const unsigned arrays = backward ? 2u : 1u, slot = ((unsigned)cols * esz + 15u) / 16u * 16u + 16u;
+        const unsigned arrays = backward ? 2u : 1u, slot = ((unsigned)(f->cpt * s.group) * esz + 15u) / 16u * 16u + 16u;
         const unsigned row = vec ? s.block * (unsigned)f->cpt * esz * arrays : (unsigned)per_block * slot * arrays;
         const unsigned kept = f->kept ? s.block * (unsigned)f->cpt * (backward ? 4u : 8u) : 0u;
         s.depth = 4;
