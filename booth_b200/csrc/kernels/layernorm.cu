@@ -313,7 +313,20 @@ template <typename T, int A> struct Slots {
     {
         return slot(a) + (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + (uint32_t)g.t * (uint32_t)sizeof(T);
     }
-    static __device__ __forceinline__ uint32_t step(const Group &g) { return (uint32_t)g.size * (uint32_t)sizeof(T); }
+    // OPAQUE: its multiples are added up where they are used and not held in registers from row to row, which thirty-two
+    // values a thread leave no room for (440 bytes of spills).
+    template <bool OPAQUE> static __device__ __forceinline__ uint32_t step(const Group &g)
+    {
+        uint32_t by = (uint32_t)g.size * (uint32_t)sizeof(T);
+        if constexpr (OPAQUE) asm volatile("mov.u32 %0, %0;" : "+r"(by));
+        return by;
+    }
+    static __device__ __forceinline__ void put(char *&to, uint32_t by, float2 v, int left)
+    {
+        if (left > 0) *reinterpret_cast<T *>(to) = from_f32<T>(v.x);
+        if (left > 1) *reinterpret_cast<T *>(to + by) = from_f32<T>(v.y);
+        to += 2u * by;
+    }
     static __device__ __forceinline__ float value(uint32_t at)
     {
         if constexpr (sizeof(T) == 4) {
@@ -335,7 +348,7 @@ template <typename T, int A> struct Slots {
     template <int N> __device__ __forceinline__ void get_all(int a, const T *row, const Group &g, Pair (&v)[N]) const
     {
         uint32_t at = first(a, row, g);
-        const uint32_t by = step(g);
+        const uint32_t by = step<(N > 8)>(g);
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = values(at, by);
     }
@@ -510,7 +523,8 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
 #pragma unroll
             for (int i = 0; i < CPT / 2; i++) v[i] = fma(v[i], r2, shift);
             if constexpr (E == 1) {
-                T *to = out + g.t;
+                char *to = reinterpret_cast<char *>(out + g.t);
+                const uint32_t by = slots.template step<!HOLD>(g);
 #pragma unroll
                 for (int i = 0; i < CPT / 2; i++) {
                     if constexpr (!HOLD) {
@@ -525,9 +539,7 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                         v[i] = fma(v[i], pw[i], pb[i]);
                     }
                     const float2 f = split(v[i]);
-                    if (inside<E>(g, 2 * i, valid, cols)) to[0] = from_f32<T>(f.x);
-                    if (inside<E>(g, 2 * i + 1, valid, cols)) to[g.size] = from_f32<T>(f.y);
-                    to += 2 * g.size;
+                    slots.put(to, by, f, valid - 2 * i);
                 }
             } else {
 #pragma unroll
@@ -678,7 +690,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         } else {
             const T *const xr = x + row * ldx, *const dr = dy + row * lddy;
             uint32_t xa = slots.first(0, xr, g), da = slots.first(1, dr, g);
-            const uint32_t by = slots.step(g);
+            const uint32_t by = slots.template step<!HOLD>(g);
             if constexpr (KEEP_ROW) {
                 slots.get_all(0, xr, g, xh);
                 slots.get_all(1, dr, g, wd);
@@ -733,9 +745,9 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
             const Pair np = pair(-p, -p), nq = pair(-q, -q);
             T *out = dx + row * lddx;
             if constexpr (E == 1) {
-                T *to = out + g.t;
+                char *to = reinterpret_cast<char *>(out + g.t);
                 uint32_t xa = slots.first(0, x + row * ldx, g), da = slots.first(1, dy + row * lddy, g);
-                const uint32_t by = slots.step(g);
+                const uint32_t by = slots.template step<!HOLD>(g);
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     const int k = KEEP_ROW ? i : 0;
@@ -747,9 +759,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                         wd[0] = mul(slots.values(da, by), pair(q0[0], q1[0]));
                     }
                     const float2 f = split(mul(r2, fma(xh[k], nq, add(wd[k], np))));
-                    if (inside<E>(g, 2 * i, valid, cols)) to[0] = from_f32<T>(f.x);
-                    if (inside<E>(g, 2 * i + 1, valid, cols)) to[g.size] = from_f32<T>(f.y);
-                    to += 2 * g.size;
+                    slots.put(to, by, f, valid - 2 * i);
                 }
             } else {
 #pragma unroll
@@ -789,10 +799,21 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         sw[2 * i] = a.x; sw[2 * i + 1] = a.y; sb[2 * i] = b.x; sb[2 * i + 1] = b.y;
     }
     if (g.size > 32) {
+        if constexpr (VEC) {                    // 16 bytes a store: single values E apart cost a 32-byte sector each
 #pragma unroll
-        for (int n = 0; n < CPT; n++) {
-            const int col = (n / E * g.size + g.t) * E + n % E;
-            if (col < cols) { pw_out[col] = sw[n]; pb_out[col] = sb[n]; }
+            for (int n = 0; n < CPT; n += 4) {
+                const int col = (n / E * g.size + g.t) * E + n % E;
+                if (col < cols) {
+                    *reinterpret_cast<float4 *>(pw_out + col) = make_float4(sw[n], sw[n + 1], sw[n + 2], sw[n + 3]);
+                    *reinterpret_cast<float4 *>(pb_out + col) = make_float4(sb[n], sb[n + 1], sb[n + 2], sb[n + 3]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < CPT; n++) {
+                const int col = n * g.size + g.t;
+                if (col < cols) { pw_out[col] = sw[n]; pb_out[col] = sb[n]; }
+            }
         }
         return;
     }
@@ -870,47 +891,47 @@ __device__ __forceinline__ void backward_columns(float *__restrict__ partial, co
     out[cols + c] = ab;
 }
 
-// dw and db: column sums of the `parts` partial rows, in double and in a fixed order. A block has 128 columns, four a
-// lane, and 32 threads on each; blockIdx.y 0: dw, 1: db.
+// dw and db: column sums of the `parts` partial rows, in double and in a fixed order. A block has 32 columns; a warp
+// reads four partial rows at a time, four columns a lane; blockIdx.y 0: dw, 1: db.
 template <typename W>
 __device__ __forceinline__ void param_grad(W *__restrict__ dw, W *__restrict__ db, const float *__restrict__ partial, int parts, int cols)
 {
-    __shared__ double sh[32][129];
+    __shared__ double sh[32][33];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     W *out = blockIdx.y ? db : dw;
     if (!out) return;
-    const int lane = (int)threadIdx.x & 31, ty = (int)threadIdx.x >> 5, c0 = (int)blockIdx.x * 128;
+    const int lane = (int)threadIdx.x & 31, ty = (int)threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
+    const int c0 = (int)blockIdx.x * 32, c = c0 + 4 * (lane & 7);
     const float *p = partial + (size_t)blockIdx.y * cols;
     double s[4] = { 0.0, 0.0, 0.0, 0.0 };
     if (cols % 4 == 0) {                        // the partial rows start on 16 bytes
-        const int c = c0 + 4 * lane;
         if (c < cols) {
 #pragma unroll 4
-            for (int i = ty; i < parts; i += 32) {
+            for (int i = 4 * ty + (lane >> 3); i < parts; i += 4 * warps) {
                 const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)i * 2 * cols + c));
                 s[0] += (double)v.x; s[1] += (double)v.y; s[2] += (double)v.z; s[3] += (double)v.w;
             }
         }
-#pragma unroll
-        for (int e = 0; e < 4; e++) sh[ty][4 * lane + e] = s[e];
     } else {
 #pragma unroll 4
-        for (int i = ty; i < parts; i += 32)
+        for (int i = 4 * ty + (lane >> 3); i < parts; i += 4 * warps)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (c0 + 32 * e + lane < cols) s[e] += (double)__ldcg(p + (size_t)i * 2 * cols + c0 + 32 * e + lane);
-#pragma unroll
-        for (int e = 0; e < 4; e++) sh[ty][32 * e + lane] = s[e];
+                if (c + e < cols) s[e] += (double)__ldcg(p + (size_t)i * 2 * cols + c + e);
     }
-    __syncthreads();
-    // warp ty adds columns 4 ty .. 4 ty + 3 of the block
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        double v = sh[lane][4 * ty + e];
+        s[e] += __shfl_xor_sync(0xffffffffu, s[e], 8);
+        s[e] += __shfl_xor_sync(0xffffffffu, s[e], 16);
+        if (lane < 8) sh[ty][4 * lane + e] = s[e];
+    }
+    __syncthreads();
+    for (int n = ty; n < 32; n += warps) {
+        double v = lane < warps ? sh[lane][n] : 0.0;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0 && c0 + 4 * ty + e < cols) out[c0 + 4 * ty + e] = from_f32<W>((float)v);
+        if (lane == 0 && c0 + n < cols) out[c0 + n] = from_f32<W>((float)v);
     }
 }
 
@@ -937,7 +958,7 @@ __device__ __forceinline__ void param_grad(W *__restrict__ dw, W *__restrict__ d
     LN_FORWARD(name, T, W, sx, false, 32, false, 512, 1)                                                                                 \
     LN_BACKWARD(name, T, W, v8, true, 8, true, true, 512)                                                                                \
     LN_BACKWARD(name, T, W, v16, true, 16, true, true, 256)                                                                              \
-    LN_BACKWARD(name, T, W, vw, true, 16, false, true, 640)                                                                              \
+    LN_BACKWARD(name, T, W, vw, true, (sizeof(T) == 4 ? 20 : 16), false, true, (sizeof(T) == 4 ? 512 : 640))                                                                              \
     LN_BACKWARD(name, T, W, vx, true, 32, false, false, 512)                                                                             \
     LN_BACKWARD(name, T, W, s8, false, 8, true, true, 512)                                                                               \
     LN_BACKWARD(name, T, W, s16, false, 16, true, true, 512)                                                                             \
@@ -962,7 +983,7 @@ LN_KERNELS(f16_f32, __half, float)
     layernorm_bwd_columns_##name(float *partial, const T *dy, const T *x, const float *mean, const float *rstd, long long rows,          \
                                  int cols, long long lddy, long long ldx)                                                                \
     { ln::backward_columns<T>(partial, dy, x, mean, rstd, rows, cols, lddy, ldx); }                                                      \
-    extern "C" __global__ void __launch_bounds__(1024)                                                                                    \
+    extern "C" __global__ void __launch_bounds__(1024)                                                                                   \
     layernorm_param_grad_##name(T *dw, T *db, const float *partial, int parts, int cols)                                                 \
     { ln::param_grad<T>(dw, db, partial, parts, cols); }
 LN_COLUMNS(f32, float)
