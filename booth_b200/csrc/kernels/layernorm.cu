@@ -231,12 +231,12 @@ template <int A, int NCH> struct Ring {
 };
 
 // The ring for rows of any alignment: a row has a slot in which its bytes lie as they do in memory modulo 16. Whole
-// 16-byte units come with cp.async, the units at its two ends word by word, and a 16-bit value that shares its word
-// with a neighbour's row through a register, written to the slot at the next step. What one thread brings others read,
-// so a row is ready behind a barrier of its group, and its slot is free behind the next one. A slot is as long as
-// all values of a group's threads, zero behind the row, so that reading takes no comparisons.
+// 16-byte units come with cp.async; of the values at its two ends each thread brings at most one of either (a group has
+// eight threads at least), 16-bit ones through a register, written to the slot at the next step. What one thread
+// brings others read, so a row is ready behind a barrier of its group, and its slot is free behind the next one. A slot
+// is as long as all values of a group's threads, zero behind the row, so that reading takes no comparisons.
 template <typename T, int A> struct Slots {
-    uint32_t base, pitch, groups, held[A][2];
+    uint32_t base, pitch, groups, held[A][2], low[A], by_row[A];
     uint16_t edge[A][2];
     int depth, stage;
     template <bool USED> __device__ __forceinline__ void init(int depth_, int cpt, const Group &g)
@@ -254,40 +254,52 @@ template <typename T, int A> struct Slots {
 #pragma unroll
         for (int a = 0; a < A; a++) { held[a][0] = held[a][1] = 0; edge[a][0] = edge[a][1] = 0; }
     }
+    // Array a: its first row and the distance of its rows, modulo 2^32 bytes.
+    __device__ __forceinline__ void source(int a, const T *p, long long ld)
+    {
+        low[a] = (uint32_t)reinterpret_cast<uintptr_t>(p);
+        by_row[a] = (uint32_t)ld * (uint32_t)sizeof(T);
+    }
     __device__ __forceinline__ uint32_t slot(int a) const { return base + (uint32_t)(stage * A + a) * groups * pitch; }
     __device__ __forceinline__ void fetch(int a, const T *row, const Group &g, int cols, bool live)
     {
         if (!live) return;
-        const uintptr_t at = reinterpret_cast<uintptr_t>(row);
-        const uint32_t head = (uint32_t)(at & 15), end = head + (uint32_t)cols * (uint32_t)sizeof(T), to = slot(a);
-        const char *const from = reinterpret_cast<const char *>(at - head);
-        // an earlier row that lay further on may have ended in the unit behind this row's last
-        const uint32_t behind = (end + 15u) / 16u * 16u;
-        if (behind + 16u <= pitch && g.t == 0) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + behind), "r"(0) : "memory");
-        for (uint32_t u = (uint32_t)g.t * 16u; u < end; u += (uint32_t)g.size * 16u) {
-            if (u >= head && u + 16u <= end) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u), "l"(from + u) : "memory");
-                continue;
+        const uint32_t head = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u, bytes = (uint32_t)cols * (uint32_t)sizeof(T), to = slot(a) + head;
+        const uint32_t gap = (16u - head) & 15u, lead = gap < bytes ? gap : bytes, units = (bytes - lead) / 16u, tail = (bytes - lead) & 15u;
+        const uint32_t at = (uint32_t)g.t * (uint32_t)sizeof(T);
+        const char *const from = reinterpret_cast<const char *>(row);
+        if (at < 16u) {
+            // an earlier row may have ended up to 15 bytes further on
+            if (head + bytes + at < pitch) {
+                if constexpr (sizeof(T) == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + bytes + at), "h"((uint16_t)0) : "memory");
+                else asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + bytes + at), "r"(0) : "memory");
             }
 #pragma unroll
-            for (uint32_t w = u; w < u + 16u; w += 4u) {
-                if (w >= head && w + 4u <= end) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + w), "l"(from + w) : "memory");
-                else if (w >= end) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + w), "r"(0) : "memory");
-                else if (sizeof(T) == 2 && w + 4u > head) {
-                    // one half of the word: the row's first value in its upper half, or its last in the lower
-                    const int tail = w >= head ? 1 : 0;
-                    const uint32_t h = tail ? w : w + 2u;
-                    held[a][tail] = to + h;
-                    edge[a][tail] = *reinterpret_cast<const uint16_t *>(from + h);
-                    if (tail) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + w + 2u), "h"((uint16_t)0) : "memory");
+            for (int e = 0; e < 2; e++) {
+                const uint32_t o = e ? bytes - tail + at : at;
+                if (at < (e ? tail : lead)) {
+                    if constexpr (sizeof(T) == 2) {
+                        held[a][e] = to + o;
+                        edge[a][e] = *reinterpret_cast<const uint16_t *>(from + o);
+                    } else {
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + o), "l"(from + o) : "memory");
+                    }
                 }
             }
+        }
+        const char *src = from + lead + (uint32_t)g.t * 16u;
+        uint32_t dst = to + lead + (uint32_t)g.t * 16u;
+        for (uint32_t u = (uint32_t)g.t; u < units; u += (uint32_t)g.size) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+            src += (uint32_t)g.size * 16u;
+            dst += (uint32_t)g.size * 16u;
         }
     }
     __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
     __device__ __forceinline__ void next() { stage = stage + 1 == depth ? 0 : stage + 1; }
     __device__ __forceinline__ void settle()
     {
+        if constexpr (sizeof(T) == 2)
 #pragma unroll
         for (int a = 0; a < A; a++)
 #pragma unroll
@@ -308,10 +320,10 @@ template <typename T, int A> struct Slots {
         else asm volatile("cp.async.wait_group 0;" ::: "memory");
         meet(g);
     }
-    // Where this thread's first value of the row at `row` lies; its others follow `step()` bytes apart.
-    __device__ __forceinline__ uint32_t first(int a, const T *row, const Group &g) const
+    // Where this thread's first value of row `row` lies; its others follow `step()` bytes apart.
+    __device__ __forceinline__ uint32_t first(int a, long long row, const Group &g) const
     {
-        return slot(a) + (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + (uint32_t)g.t * (uint32_t)sizeof(T);
+        return slot(a) + ((low[a] + (uint32_t)row * by_row[a]) & 15u) + (uint32_t)g.t * (uint32_t)sizeof(T);
     }
     // OPAQUE: its multiples are added up where they are used and not held in registers from row to row, which thirty-two
     // values a thread leave no room for (440 bytes of spills).
@@ -345,7 +357,7 @@ template <typename T, int A> struct Slots {
         at += 2u * by;
         return pair(a, b);
     }
-    template <int N> __device__ __forceinline__ void get_all(int a, const T *row, const Group &g, Pair (&v)[N]) const
+    template <int N> __device__ __forceinline__ void get_all(int a, long long row, const Group &g, Pair (&v)[N]) const
     {
         uint32_t at = first(a, row, g);
         const uint32_t by = step<(N > 8)>(g);
@@ -443,6 +455,7 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
     Ring<1, VEC ? NCH : 1> ring(depth);
     Slots<T, 1> slots;
     slots.template init<!VEC>(depth, CPT, g);
+    slots.source(0, x, ldx);
     const int valid = valid_of(g, cols);
     for (int d = 0; d < depth; d++) {
         const long long row = base + g.index + d * step;
@@ -498,7 +511,7 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
             widen_all<T, E, NCH>(cur, v);
         } else {
             slots.wait(g);
-            slots.get_all(0, x + row * ldx, g, v);
+            slots.get_all(0, row, g, v);
         }
         float m, dm, rstd;
         row_stats<E, CPT / 2>(v, g, valid, cols, inv, eps, sh, m, dm, rstd);
@@ -613,6 +626,8 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
     Ring<2, VEC ? NCH : 1> ring(depth);
     Slots<T, 2> slots;
     slots.template init<!VEC>(depth, CPT, g);
+    slots.source(0, x, ldx);
+    slots.source(1, dy, lddy);
     const int valid = valid_of(g, cols);
     for (int d = 0; d < depth; d++) {
         const long long row = base + g.index + d * step;
@@ -688,12 +703,11 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                 }
             }
         } else {
-            const T *const xr = x + row * ldx, *const dr = dy + row * lddy;
-            uint32_t xa = slots.first(0, xr, g), da = slots.first(1, dr, g);
+            uint32_t xa = slots.first(0, row, g), da = slots.first(1, row, g);
             const uint32_t by = slots.template step<!HOLD>(g);
             if constexpr (KEEP_ROW) {
-                slots.get_all(0, xr, g, xh);
-                slots.get_all(1, dr, g, wd);
+                slots.get_all(0, row, g, xh);
+                slots.get_all(1, row, g, wd);
             }
             if (row >= rows) {                  // a group past the end: its slot holds an earlier row
 #pragma unroll
@@ -746,7 +760,7 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
             T *out = dx + row * lddx;
             if constexpr (E == 1) {
                 char *to = reinterpret_cast<char *>(out + g.t);
-                uint32_t xa = slots.first(0, x + row * ldx, g), da = slots.first(1, dy + row * lddy, g);
+                uint32_t xa = slots.first(0, row, g), da = slots.first(1, row, g);
                 const uint32_t by = slots.template step<!HOLD>(g);
 #pragma unroll
                 for (int i = 0; i < N; i++) {

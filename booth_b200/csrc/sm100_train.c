@@ -55,7 +55,7 @@ typedef struct { int at, vec, cpt, most; unsigned resident; int kept, bytes; } l
  * sixteen backward, which spreads what a row costs each thread beside its values; rows too wide for
  * these take the forms that keep parameters or row in shared memory. */
 static const ln_form_t ln_forward[] = { { 0, 1, 8, 512, 1024, 0, 0 }, { 1, 1, 32, 256, 512, 0, 0 }, { 2, 1, 16, 640, 640, 1, 0 }, { 3, 1, 32, 512, 512, 1, 0 },
-                                        { 4, 0, 8, 512, 768, 0, 0 }, { 5, 0, 16, 512, 512, 0, 0 }, { 6, 0, 32, 512, 512, 1, 0 } };
+                                        { 4, 0, 8, 512, 768, 0, 0 }, { 5, 0, 16, 512, 640, 0, 0 }, { 6, 0, 32, 512, 512, 1, 0 } };
 static const ln_form_t ln_backward[] = { { 0, 1, 8, 512, 768, 0, 0 }, { 1, 1, 16, 256, 512, 0, 0 }, { 2, 1, 20, 512, 512, 1, 4 }, { 2, 1, 16, 640, 640, 1, 2 },
                                          { 3, 1, 32, 512, 512, 1, 0 },
                                          { 4, 0, 8, 512, 768, 0, 0 }, { 5, 0, 16, 512, 512, 0, 0 }, { 6, 0, 32, 512, 512, 1, 0 } };
@@ -76,7 +76,7 @@ static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, uns
     const ln_form_t *forms = backward ? ln_backward : ln_forward, *f = NULL;
     const int n = backward ? LN_COUNT(ln_backward) : LN_COUNT(ln_forward), few = rows < 2ll * dev->sm_count;
     for (int i = 0; i < n && !f; i++)
-        if (forms[i].vec == vec && (!forms[i].bytes || forms[i].bytes == (int)esz) && (forms[i].cpt > 8 || few) && cols <= forms[i].cpt * forms[i].most) f = &forms[i];
+        if (forms[i].vec == vec && (!forms[i].bytes || forms[i].bytes == (int)esz) && (forms[i].cpt > 8 || few || (!vec && cols <= 64)) && cols <= forms[i].cpt * forms[i].most) f = &forms[i];
     s.loop = !f;
     s.form = f ? f->at : LN_LOOP;
     s.depth = 1;
@@ -85,7 +85,7 @@ static ln_shape_t ln_shape(const sm100_dev_t *dev, long long rows, int cols, uns
     s.block = 512;
     if (f) {
         int g = (cols + f->cpt - 1) / f->cpt;
-        if (g <= 32) { int p = 1; while (p < g) p *= 2; g = p; }
+        if (g <= 32) { int p = vec ? 1 : 8; while (p < g) p *= 2; g = p; }
         else g = (g + 31) / 32 * 32;
         s.group = g;
         s.block = g <= 32 ? 128u : (unsigned)g;
