@@ -191,6 +191,14 @@ template <typename T, int E, int NCH> __device__ __forceinline__ void widen_all(
     }
 }
 
+// A distance in bytes. OPAQUE: its multiples are added up where they are used and not held in registers from row to
+// row, which many values a thread leave no room for (up to 440 bytes of spills).
+template <bool OPAQUE> __device__ __forceinline__ uint32_t stride(uint32_t by)
+{
+    if constexpr (OPAQUE) asm volatile("mov.u32 %0, %0;" : "+r"(by));
+    return by;
+}
+
 // The ring: `depth` rows ahead of A arrays; chunk j of array a of a stage at ((stage A + a) NCH + j) blockDim 16 bytes,
 // 16 bytes a thread. Every row position commits one group, with or without copies, so that the count of groups
 // tells which row has landed.
@@ -203,13 +211,20 @@ template <int A, int NCH> struct Ring {
         base = (uint32_t)__cvta_generic_to_shared(ln_ring) + threadIdx.x * 16u;
         row_bytes = blockDim.x * 16u;
     }
-    __device__ __forceinline__ uint32_t at(int a, int j) const { return base + (uint32_t)((stage * A + a) * NCH + j) * row_bytes; }
-    template <typename T, int E> __device__ __forceinline__ void fetch(int a, const T *row, const Group &g, int cols, bool live) const
+    // Where this thread's first chunk of array a lies; its others follow `step()` bytes apart.
+    __device__ __forceinline__ uint32_t first(int a) const { return base + (uint32_t)((stage * A + a) * NCH) * row_bytes; }
+    __device__ __forceinline__ uint32_t step() const { return stride<(NCH > 4)>(row_bytes); }
+    // `valid`: this thread's chunks in the row
+    template <typename T, int E> __device__ __forceinline__ void fetch(int a, const T *row, const Group &g, int valid, bool live) const
     {
+        uint32_t to = first(a);
+        const uint32_t by = step(), far = stride<(NCH > 4)>((uint32_t)g.size * 16u);
+        const char *from = reinterpret_cast<const char *>(row + g.t * E);
 #pragma unroll
         for (int j = 0; j < NCH; j++) {
-            const int col = (j * g.size + g.t) * E;
-            if (live && col < cols) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(a, j)), "l"(row + col) : "memory");
+            if (live && j < valid) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+            to += by;
+            from += far;
         }
     }
     __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -222,10 +237,11 @@ template <int A, int NCH> struct Ring {
         else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
         else asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    template <typename T, int E> __device__ __forceinline__ Chunk<T, E> get(int a, int j, bool live) const
+    // The chunk at `at`, zero unless `live`.
+    template <typename T, int E> static __device__ __forceinline__ Chunk<T, E> get(uint32_t at, bool live)
     {
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (live) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at(a, j)) : "memory");
+        if (live) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
         return *reinterpret_cast<const Chunk<T, E> *>(&v);
     }
 };
@@ -325,14 +341,7 @@ template <typename T, int A> struct Slots {
     {
         return slot(a) + ((low[a] + (uint32_t)row * by_row[a]) & 15u) + (uint32_t)g.t * (uint32_t)sizeof(T);
     }
-    // OPAQUE: its multiples are added up where they are used and not held in registers from row to row, which thirty-two
-    // values a thread leave no room for (440 bytes of spills).
-    template <bool OPAQUE> static __device__ __forceinline__ uint32_t step(const Group &g)
-    {
-        uint32_t by = (uint32_t)g.size * (uint32_t)sizeof(T);
-        if constexpr (OPAQUE) asm volatile("mov.u32 %0, %0;" : "+r"(by));
-        return by;
-    }
+    template <bool OPAQUE> static __device__ __forceinline__ uint32_t step(const Group &g) { return stride<OPAQUE>((uint32_t)g.size * (uint32_t)sizeof(T)); }
     static __device__ __forceinline__ void put(char *&to, uint32_t by, float2 v, int left)
     {
         if (left > 0) *reinterpret_cast<T *>(to) = from_f32<T>(v.x);
@@ -400,17 +409,15 @@ struct Kept {
     }
 };
 
-// Whether chunk j of this thread (E > 1: vectors lie in the row whole or not at all), or its value j (E = 1), lies in
-// the row. `valid`: how many of its values do, when they are single.
-template <int E> __device__ __forceinline__ bool inside(const Group &g, int j, int valid, int cols)
+// How many of a thread's chunks of E values lie in the row (whole or not at all: cols is a multiple of E).
+template <int E> __device__ __forceinline__ int valid_of(const Group &g, int cols)
 {
-    return E == 1 ? j < valid : (j * g.size + g.t) * E < cols;
+    return g.t * E < cols ? (cols / E - g.t + g.size - 1) / g.size : 0;
 }
-__device__ __forceinline__ int valid_of(const Group &g, int cols) { return g.t < cols ? (cols - g.t + g.size - 1) / g.size : 0; }
 
 // v: a row's values in, their differences from `m` out (zero outside the row). mean = m + dm.
 template <int E, int N>
-__device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int valid, int cols, float inv, float eps, float2 (*sh)[32], float &m, float &dm, float &rstd)
+__device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int valid, float inv, float eps, float2 (*sh)[32], float &m, float &dm, float &rstd)
 {
     Pair s = pair(0.f, 0.f);
 #pragma unroll
@@ -424,9 +431,9 @@ __device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int valid, int
         v[i] = add(v[i], nm);
         if constexpr (E == 1) {
             const float2 x = split(v[i]);
-            v[i] = pair(inside<E>(g, 2 * i, valid, cols) ? x.x : 0.f, inside<E>(g, 2 * i + 1, valid, cols) ? x.y : 0.f);
+            v[i] = pair(2 * i < valid ? x.x : 0.f, 2 * i + 1 < valid ? x.y : 0.f);
         } else {
-            if (!inside<E>(g, 2 * i / (E < 2 ? 2 : E), valid, cols)) v[i] = pair(0.f, 0.f);
+            if (2 * i / (E < 2 ? 2 : E) >= valid) v[i] = pair(0.f, 0.f);
         }
         d1 = add(d1, v[i]);
         d2 = fma(v[i], v[i], d2);
@@ -456,11 +463,11 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
     Slots<T, 1> slots;
     slots.template init<!VEC>(depth, CPT, g);
     slots.source(0, x, ldx);
-    const int valid = valid_of(g, cols);
+    const int valid = valid_of<E>(g, cols);
     for (int d = 0; d < depth; d++) {
         const long long row = base + g.index + d * step;
         if constexpr (VEC) {
-            ring.template fetch<T, E>(0, x + row * ldx, g, cols, row < rows);
+            ring.template fetch<T, E>(0, x + row * ldx, g, valid, row < rows);
             ring.commit();
             ring.next();
         } else {
@@ -506,18 +513,23 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
         if constexpr (VEC) {
             ring.wait();
             Chunk<T, E> cur[NCH];
+            uint32_t at = ring.first(0);
+            const uint32_t by = ring.step();
 #pragma unroll
-            for (int j = 0; j < NCH; j++) cur[j] = ring.template get<T, E>(0, j, row < rows && (j * g.size + g.t) * E < cols);
+            for (int j = 0; j < NCH; j++) {
+                cur[j] = ring.template get<T, E>(at, row < rows && j < valid);
+                at += by;
+            }
             widen_all<T, E, NCH>(cur, v);
         } else {
             slots.wait(g);
             slots.get_all(0, row, g, v);
         }
         float m, dm, rstd;
-        row_stats<E, CPT / 2>(v, g, valid, cols, inv, eps, sh, m, dm, rstd);
+        row_stats<E, CPT / 2>(v, g, valid, inv, eps, sh, m, dm, rstd);
         const long long ahead = row + depth * step;          // the row is in registers: its places may fill again
         if constexpr (VEC) {
-            ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
+            ring.template fetch<T, E>(0, x + ahead * ldx, g, valid, ahead < rows);
             ring.commit();
             ring.next();
         } else {
@@ -555,10 +567,11 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                     slots.put(to, by, f, valid - 2 * i);
                 }
             } else {
+                char *to = reinterpret_cast<char *>(out + g.t * E);
+                const uint32_t far = stride<(NCH > 4)>((uint32_t)g.size * 16u);
 #pragma unroll
                 for (int j = 0; j < NCH; j++) {
-                    const int col = (j * g.size + g.t) * E;
-                    if (col < cols) {
+                    if (j < valid) {
                         Chunk<T, E> o;
                         float qw[E], qb[E];
                         if constexpr (!HOLD) { kept.template get<E, NCH>(0, j, qw); kept.template get<E, NCH>(1, j, qb); }
@@ -568,8 +581,9 @@ __device__ __forceinline__ void forward(T *__restrict__ y, const T *__restrict__
                             if constexpr (HOLD) narrow(&o.v[2 * i], fma(v[n], pw[n], pb[n]));
                             else narrow(&o.v[2 * i], fma(v[n], pair(qw[2 * i], qw[2 * i + 1]), pair(qb[2 * i], qb[2 * i + 1])));
                         }
-                        *reinterpret_cast<Chunk<T, E> *>(out + col) = o;
+                        *reinterpret_cast<Chunk<T, E> *>(to) = o;
                     }
+                    to += far;
                 }
             }
         }
@@ -628,12 +642,12 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
     slots.template init<!VEC>(depth, CPT, g);
     slots.source(0, x, ldx);
     slots.source(1, dy, lddy);
-    const int valid = valid_of(g, cols);
+    const int valid = valid_of<E>(g, cols);
     for (int d = 0; d < depth; d++) {
         const long long row = base + g.index + d * step;
         if constexpr (VEC) {
-            ring.template fetch<T, E>(0, x + row * ldx, g, cols, row < rows);
-            ring.template fetch<T, E>(1, dy + row * lddy, g, cols, row < rows);
+            ring.template fetch<T, E>(0, x + row * ldx, g, valid, row < rows);
+            ring.template fetch<T, E>(1, dy + row * lddy, g, valid, row < rows);
             ring.commit();
             ring.next();
         } else {
@@ -683,10 +697,14 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         const Pair nmean = pair(-cm, -cm), r2 = pair(cr, cr);
         Pair s1 = pair(0.f, 0.f), s2 = pair(0.f, 0.f);
         if constexpr (VEC) {
+            uint32_t xa = ring.first(0), da = ring.first(1);
+            const uint32_t by = ring.step();
 #pragma unroll
             for (int j = 0; j < NCH; j++) {
-                const bool live = row < rows && (j * g.size + g.t) * E < cols;
-                const Chunk<T, E> xc = ring.template get<T, E>(0, j, live), dc = ring.template get<T, E>(1, j, live);
+                const bool live = row < rows && j < valid;
+                const Chunk<T, E> xc = ring.template get<T, E>(xa, live), dc = ring.template get<T, E>(da, live);
+                xa += by;
+                da += by;
                 float q[E];
                 if constexpr (!HOLD) kept.template get<E, NCH>(0, j, q);
 #pragma unroll
@@ -740,8 +758,8 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
         const auto refill = [&]() {             // the row has been read: its places may fill again
             const long long ahead = row + depth * step;
             if constexpr (VEC) {
-                ring.template fetch<T, E>(0, x + ahead * ldx, g, cols, ahead < rows);
-                ring.template fetch<T, E>(1, dy + ahead * lddy, g, cols, ahead < rows);
+                ring.template fetch<T, E>(0, x + ahead * ldx, g, valid, ahead < rows);
+                ring.template fetch<T, E>(1, dy + ahead * lddy, g, valid, ahead < rows);
                 ring.commit();
                 ring.next();
             } else {
@@ -776,13 +794,15 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                     slots.put(to, by, f, valid - 2 * i);
                 }
             } else {
+                char *to = reinterpret_cast<char *>(out + g.t * E);
+                uint32_t xa = ring.first(0), da = ring.first(1);
+                const uint32_t by = ring.step(), far = stride<(NCH > 4)>((uint32_t)g.size * 16u);
 #pragma unroll
                 for (int j = 0; j < NCH; j++) {
-                    const int col = (j * g.size + g.t) * E;
-                    if (col < cols) {
+                    if (j < valid) {
                         Chunk<T, E> o;
                         if constexpr (!KEEP_ROW) {
-                            const Chunk<T, E> xc = ring.template get<T, E>(0, j, true), dc = ring.template get<T, E>(1, j, true);
+                            const Chunk<T, E> xc = ring.template get<T, E>(xa, true), dc = ring.template get<T, E>(da, true);
                             float u[E];
                             kept.template get<E, NCH>(0, j, u);
 #pragma unroll
@@ -796,8 +816,11 @@ __device__ __forceinline__ void backward(T *__restrict__ dx, float *__restrict__
                             const int k = KEEP_ROW ? j * E / 2 + i : i;
                             narrow(&o.v[2 * i], mul(r2, fma(xh[k], nq, add(wd[k], np))));
                         }
-                        *reinterpret_cast<Chunk<T, E> *>(out + col) = o;
+                        *reinterpret_cast<Chunk<T, E> *>(to) = o;
                     }
+                    to += far;
+                    xa += by;
+                    da += by;
                 }
             }
         }
