@@ -20,8 +20,8 @@ d.sync(); d.close()
 """)
     assert res.returncode == 0, res.stderr
     assert [(l["kernel"], l["grid"][0], l["block"][0]) for l in L] == [
-        ("layernorm_bf16_v8", 1, 128), ("layernorm_bf16_f32_v16", 444, 256), ("layernorm_f32_s16", 1184, 96),
-        ("layernorm_f16_v8", 63, 128), ("layernorm_f16_s8", 63, 128), ("layernorm_f32_vx", 5, 512), ("layernorm_f32_loop", 5, 512),
+        ("layernorm_bf16_v8", 1, 128), ("layernorm_bf16_f32_v32", 592, 128), ("layernorm_f32_s16", 888, 96),
+        ("layernorm_f16_v32", 16, 128), ("layernorm_f16_s8", 63, 128), ("layernorm_f32_vx", 5, 512), ("layernorm_f32_sx", 5, 512),
         ("layernorm_f32_s8", 1, 128)]
     assert all(l["overlap"] == 1 for l in L)
 
