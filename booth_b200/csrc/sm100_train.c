@@ -36,6 +36,9 @@ static int matrix_ok(sm100_ptr_t p, unsigned esz, long long rows, long long cols
 
 /* ---- layer normalisation ---- */
 
+/* Columns are counted in 32 bits, and the last step past them has to fit as well. */
+#define LN_MAX_COLS (1 << 30)
+
 /* Kernel of a (value type, parameter type) pair, in the order of the names in sm100_shim.c; -1: no such pair. */
 static int ln_pair(int dtype, int wdtype)
 {
@@ -131,12 +134,13 @@ int booth_sm100_layernorm(sm100_dev_t *dev, sm100_ptr_t y, sm100_ptr_t x, sm100_
     if (rc != SM100_OK) return rc;
     const int pair = ln_pair(dtype, wdtype);
     if (pair < 0) return bad_arg(dev, "booth_sm100_layernorm: types are f32 with f32 parameters, or bf16 or f16 with parameters of the same type or f32");
-    if (rows < 0 || cols < 1 || !(eps >= 0.0f)) return bad_arg(dev, "booth_sm100_layernorm: need rows >= 0, cols >= 1, eps >= 0");
+    if (rows < 0 || cols < 1 || cols > LN_MAX_COLS || !(eps >= 0.0f)) return bad_arg(dev, "booth_sm100_layernorm: need rows >= 0, 1 to 2^30 columns, eps >= 0");
     if (rows == 0) return SM100_OK;
     const unsigned e = type_bytes(dtype), we = type_bytes(wdtype);
     if (!matrix_ok(x, e, rows, cols, ldx) || !matrix_ok(y, e, rows, cols, ldy) || (w & (we - 1)) || (b & (we - 1)) || ((mean | rstd) & 3) ||
-        (x == y && ldx != ldy))
-        return bad_arg(dev, "booth_sm100_layernorm: x and y non-NULL, every operand aligned to its element, pitches >= cols (equal ones when y is x)");
+        (x == y && ldx != ldy) || (mean && mean == rstd))
+        return bad_arg(dev, "booth_sm100_layernorm: x and y non-NULL, every operand aligned to its element, pitches >= cols (equal ones when y is x), "
+                            "mean apart from rstd");
     const int vec = !(((x | y | w | b) & 15) || cols % (int)(16 / e) || ldx % (16 / e) || ldy % (16 / e));
     if ((rc = ln_ready(dev)) != SM100_OK) return rc;
     const ln_shape_t s = ln_shape(dev, rows, cols, e, vec, 0);
@@ -150,7 +154,7 @@ int booth_sm100_layernorm(sm100_dev_t *dev, sm100_ptr_t y, sm100_ptr_t x, sm100_
 
 size_t booth_sm100_layernorm_backward_workspace(sm100_dev_t *dev, long long rows, int cols, int dtype, int wdtype)
 {
-    if (!dev || rows < 0 || cols < 1 || ln_pair(dtype, wdtype) < 0) {
+    if (!dev || rows < 0 || cols < 1 || cols > LN_MAX_COLS || ln_pair(dtype, wdtype) < 0) {
         bad_arg(dev, "booth_sm100_layernorm_backward_workspace: bad argument");
         return 0;
     }
@@ -171,14 +175,14 @@ int booth_sm100_layernorm_backward(sm100_dev_t *dev, sm100_ptr_t dx, sm100_ptr_t
     if (rc != SM100_OK) return rc;
     const int pair = ln_pair(dtype, wdtype);
     if (pair < 0) return bad_arg(dev, "booth_sm100_layernorm_backward: types are f32 with f32 parameters, or bf16 or f16 with parameters of the same type or f32");
-    if (rows < 0 || cols < 1) return bad_arg(dev, "booth_sm100_layernorm_backward: need rows >= 0, cols >= 1");
+    if (rows < 0 || cols < 1 || cols > LN_MAX_COLS) return bad_arg(dev, "booth_sm100_layernorm_backward: need rows >= 0, 1 to 2^30 columns");
     const unsigned e = type_bytes(dtype), we = type_bytes(wdtype);
     const int params = dw || db;
     if (rows > 0 && (!matrix_ok(dy, e, rows, cols, lddy) || !matrix_ok(x, e, rows, cols, ldx) || (dx && !matrix_ok(dx, e, rows, cols, lddx)) ||
                      !mean || !rstd || ((mean | rstd) & 3) || (w & (we - 1)) || (dx && (dx == dy || dx == x))))
         return bad_arg(dev, "booth_sm100_layernorm_backward: dy, x, mean and rstd non-NULL, every operand aligned to its element, "
                             "pitches >= cols, dx apart from dy and x");
-    if ((dw | db) & (we - 1)) return bad_arg(dev, "booth_sm100_layernorm_backward: dw and db must be aligned to their element");
+    if (((dw | db) & (we - 1)) || (params && dw == db)) return bad_arg(dev, "booth_sm100_layernorm_backward: dw and db must be aligned to their element and apart");
     if (params && (!ws || (ws & 15) || ws_bytes < booth_sm100_layernorm_backward_workspace(dev, rows, cols, dtype, wdtype)))
         return bad_arg(dev, "booth_sm100_layernorm_backward: workspace missing, not 16-byte aligned or too small");
     int parts = 0;
@@ -396,6 +400,19 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
 {
     int rc = orth_status_ready(dev);
     if (rc != SM100_OK) return rc;
+    /* the maps first: whatever can fail fails before the momentum changes */
+    plane_maps_t x[2], sm, qm;
+    for (int i = 0; i < 2; i++) {
+        if ((rc = plane_map(dev, &x[i].hi, ws + o->x_hi[i], o->s, o->l, o->x_pitch, batch)) != SM100_OK) return rc;
+        if ((rc = plane_map(dev, &x[i].lo, ws + o->x_lo[i], o->s, o->l, o->x_pitch, batch)) != SM100_OK) return rc;
+    }
+    if ((rc = plane_map(dev, &sm.hi, ws + o->s_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+    if ((rc = plane_map(dev, &qm.hi, ws + o->q_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+    sm.lo = sm.hi; qm.lo = qm.hi;       /* not read or written by the one-plane kernels */
+    if (two_planes) {
+        if ((rc = plane_map(dev, &sm.lo, ws + o->s_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+        if ((rc = plane_map(dev, &qm.lo, ws + o->q_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
+    }
     const int tall = src->rows > src->cols;
     CUdeviceptr partial = ws;
     int parts = o->parts;
@@ -410,19 +427,6 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
     rc = sm100_launch_k3_overlapped(dev, SM100_K_ORTH_SPLIT, (unsigned)((src->cols + 63) / 64), (unsigned)((src->rows + 63) / 64), (unsigned)batch,
                                     256, 1, 1, 0, sa);
     if (rc != SM100_OK) return rc;
-
-    plane_maps_t x[2], sm, qm;
-    for (int i = 0; i < 2; i++) {
-        if ((rc = plane_map(dev, &x[i].hi, ws + o->x_hi[i], o->s, o->l, o->x_pitch, batch)) != SM100_OK) return rc;
-        if ((rc = plane_map(dev, &x[i].lo, ws + o->x_lo[i], o->s, o->l, o->x_pitch, batch)) != SM100_OK) return rc;
-    }
-    if ((rc = plane_map(dev, &sm.hi, ws + o->s_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
-    if ((rc = plane_map(dev, &qm.hi, ws + o->q_hi, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
-    sm.lo = sm.hi; qm.lo = qm.hi;       /* not read or written by the one-plane kernels */
-    if (two_planes) {
-        if ((rc = plane_map(dev, &sm.lo, ws + o->s_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
-        if ((rc = plane_map(dev, &qm.lo, ws + o->q_lo, o->s, o->s, o->a_pitch, batch)) != SM100_OK) return rc;
-    }
     /* a I + b A + c A A = c (A + beta I)^2 + gamma I; without the square, b A + a I. X is held times 2^14, S times
      * 2^12 (|A| < 4 and |beta| <= 4), Q times what its largest value over singular values below 2 allows. */
     const double a = ns->a, b = ns->b, c = ns->c, xs = 16384.0, ss = 4096.0;

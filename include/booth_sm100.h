@@ -284,7 +284,7 @@ int  booth_sm100_asian_paths(sm100_dev_t *dev, const booth_asian_t *p,
  * fp32, y is rounded once. y may be x (same pitch); otherwise outputs must not
  * overlap inputs. Rows beyond `rows` and columns beyond `cols` are neither read nor
  * written. Any alignment of whole elements; rows that start on 16 bytes and are a
- * multiple of 16 bytes long are read in 16-byte vectors. rows = 0 does nothing. */
+ * multiple of 16 bytes long are read in 16-byte vectors. At most 2^30 columns; rows = 0 does nothing. */
 int  booth_sm100_layernorm(sm100_dev_t *dev, sm100_ptr_t y, sm100_ptr_t x, sm100_ptr_t w, sm100_ptr_t b,
                            sm100_ptr_t mean, sm100_ptr_t rstd, long long rows, int cols,
                            long long ldx, long long ldy, float eps, int dtype, int wdtype);
@@ -292,7 +292,7 @@ int  booth_sm100_layernorm(sm100_dev_t *dev, sm100_ptr_t y, sm100_ptr_t x, sm100
  * p = mean over the row of w dy, q = mean over the row of w dy xhat,
  *   dx = rstd (w dy - p - xhat q),  dw = sum over rows of dy xhat,  db = sum over rows of dy
  * dx (x's type), dw and db (wdtype) are overwritten; any of them may be NULL. w may
- * be NULL (ones). dx must not be dy or x, nor overlap any input. With rows = 0 dw and db
+ * be NULL (ones). dx must not be dy or x, nor overlap any input; dw and db are apart. With rows = 0 dw and db
  * become zero. The sums over rows are taken in a fixed order: the same call gives
  * the same bits. ws: booth_sm100_layernorm_backward_workspace bytes, 16-byte
  * aligned, any contents; NULL when neither dw nor db is asked for. */

@@ -59,6 +59,9 @@ d.sync(); d.close()
     "d.layernorm_backward(p, p, p, 2 * p, 3 * p, p, p, p, 4, 8, p, 16)", "d.layernorm_backward(p, p, p, 2 * p, 3 * p, p, p, p, 4, 8, 0, 0)",
     "d.layernorm_backward(p, p, p, 2 * p, 3 * p, p, p, p, 4, 8, p + 8, 1 << 20)", "d.layernorm_backward(p, p + 1, p, 2 * p, 3 * p, p, p, p, 4, 8, p, 1 << 20)",
     "d.layernorm_backward(p, p, p, 2 * p, 3 * p, p, p, p, 4, 8, p, 1 << 20, lddy=3)", "d.layernorm_backward(p, p, p, 2 * p, 3 * p, p, p, p, 4, 0, p, 1 << 20)",
+    "d.layernorm(p, 2 * p, p, p, 4, (1 << 30) + 1)", "d.layernorm(p, 2 * p, p, p, 4, 8, mean=p, rstd=p)",
+    "d.layernorm_backward(4 * p, p, 5 * p, 2 * p, 3 * p, p, p, p, 1, (1 << 30) + 1, p, 1 << 50)", "d.layernorm_backward_workspace(1, (1 << 30) + 1)",
+    "d.layernorm_backward(4 * p, 5 * p, 5 * p, 2 * p, 3 * p, p, p, p, 4, 8, p, 1 << 20)",
     "d.layernorm_backward_workspace(4, 0)", "d.layernorm_backward_workspace(-1, 8)", "d.layernorm_backward_workspace(1, 8, sm.I32)",
 ])
 def test_layernorm_refusals(fake, tmp_path, call):  # noqa: F811
@@ -201,3 +204,20 @@ d.close()
 """ % call)
     assert res.returncode == 0, res.stderr
     assert not L
+
+
+def test_muon_launches_nothing_when_a_map_fails(fake, tmp_path):  # noqa: F811
+    """The plain stand-in driver refuses maps of three dimensions: the momentum must not have changed by then."""
+    res, L, _ = run(fake, tmp_path, """
+d = sm.Device(0); p = 1 << 20
+n = d.orthogonalise_workspace(1, 64, 64, sm.F32)
+try:
+    d.muon_step(p, 2 * p, 3 * p, 1, 64, 64, 4 * p, n, lr=0.1)
+except sm.Sm100Error as e:
+    assert e.code != sm.ERR_ARG, e
+else:
+    raise SystemExit("not refused")
+d.close()
+""")
+    assert res.returncode == 0, res.stderr
+    assert not [l for l in L if l["kernel"].startswith("orth")]
