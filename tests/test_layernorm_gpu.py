@@ -265,3 +265,53 @@ def test_gradient_agrees_with_differences(dev, sm, cols):
             lo = loss(x, w, b)
             flat[i] = old
             assert abs(((hi - lo) / (2 * step)).item() - grad.view(-1)[i].item()) < 1e-4 * (1 + grad.abs().max().item())
+
+
+# every group of threads takes more rows than its ring holds, rows start at every offset from 16 bytes
+WALKS = [(60000, 7, 2, 1), (60000, 33, 4, 3), (15000, 257, 2, 5), (7000, 1001, 4, 1), (1500, 4099, 2, 7), (800, 9001, 6, 3), (20000, 40, 8, 8), (3000, 5000, 8, 16)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,pad,offset", WALKS)
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_long_walks_take_nothing_from_neighbours(dev, sm, rows, cols, pad, offset, t):
+    """What lies between the rows is NaN, and in the second half so is every seventh row of x: neither may reach another row."""
+    x, w, b, dy = make(rows, cols, TYPES[t], torch.float32, seed=rows)
+
+    def within_nan(v):
+        flat, view = strided(v, pad, offset)
+        hold = v.clone()
+        flat.fill_(float("nan"))
+        view.copy_(hold)
+        return view
+
+    xs, ds = within_nan(x), within_nan(dy)
+    y, mean, rstd = run_forward(dev, sm, xs, w, b)
+    check_forward(x, w, b, 1e-5, y, mean, rstd)
+    check_backward(dy, x, w, mean, rstd, *run_backward(dev, sm, ds, xs, w, mean, rstd))
+    bad = torch.arange(3, rows, 7, device="cuda")
+    keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+    keep[bad] = False
+    xs[bad] = float("nan")
+    y, mean, rstd = run_forward(dev, sm, xs, w, b)
+    check_forward(x[keep], w, b, 1e-5, y[keep], mean[keep], rstd[keep])
+    assert bool(y[bad].isnan().all())
+    dx, _, _ = run_backward(dev, sm, ds, xs, w, mean, rstd)
+    rdx = run_backward(dev, sm, dy[keep].contiguous(), x[keep].contiguous(), w, mean[keep], rstd[keep], want="dx")[0]
+    check_backward(dy[keep], x[keep], w, mean[keep], rstd[keep], dx[keep], None, None)
+    check_backward(dy[keep], x[keep], w, mean[keep], rstd[keep], rdx, None, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [1, 2, 3, 5, 7, 9, 15, 17])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_short_rows_at_every_offset(dev, sm, cols, t):
+    for offset in range(9):
+        x, w, b, dy = make(200, cols, TYPES[t], torch.float32, seed=offset)
+        _, xs = strided(x, 1 + offset % 3, offset)
+        _, ds = strided(dy, 2, 8 - offset)
+        flat, ys = strided(torch.zeros_like(x), 3, 2)
+        y, mean, rstd = run_forward(dev, sm, xs, w, b, y=ys)
+        check_forward(x, w, b, 1e-5, y, mean, rstd)
+        assert bool((flat[2:].view(200, -1)[:, cols:] == 7.25).all())
+        check_backward(dy, x, w, mean, rstd, *run_backward(dev, sm, ds, xs, w, mean, rstd))
