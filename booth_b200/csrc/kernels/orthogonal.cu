@@ -991,13 +991,21 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     float v[32];
 #pragma unroll
                     for (int c = 0; c < 32; c++) v[c] = __uint_as_float(r[c]);
-                    for (int from = 0; from < split; from++) {
-                        if (from == part) continue;
-                        const float *const at = p.sums + sums_at + from * part_step + (cc * PIECE + half * 32) * 32;
+                    // the other parts' sums, two at a time so that their loads wait together, always from the next part on
+                    for (int n = 1; n < split; n += 2) {
+                        const int from[2] = { part + n < split ? part + n : part + n - split, part + n + 1 < split ? part + n + 1 : part + n + 1 - split };
+                        float4 x[2][8];
+#pragma unroll
+                        for (int o = 0; o < 2; o++) {
+                            const float *const at = p.sums + sums_at + from[o] * part_step + (cc * PIECE + half * 32) * 32;
+#pragma unroll
+                            for (int u = 0; u < 8; u++)
+                                x[o][u] = n + o < split ? __ldcg(reinterpret_cast<const float4 *>(at + u * 128)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
 #pragma unroll
                         for (int u = 0; u < 8; u++) {
-                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(at + u * 128));
-                            v[4 * u] += x.x; v[4 * u + 1] += x.y; v[4 * u + 2] += x.z; v[4 * u + 3] += x.w;
+                            v[4 * u] += x[0][u].x + x[1][u].x; v[4 * u + 1] += x[0][u].y + x[1][u].y;
+                            v[4 * u + 2] += x[0][u].z + x[1][u].z; v[4 * u + 3] += x[0][u].w + x[1][u].w;
                         }
                     }
 #pragma unroll
