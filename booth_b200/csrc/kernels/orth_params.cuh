@@ -38,6 +38,9 @@ typedef struct orth_product {
     int tri;                                            /* tile side of the stored triangle of the symmetric operand */
     int split;                                          /* parts of K, one CTA (pair) of a cluster each */
     int lo;                                             /* whether out has a lo plane */
+    ORTH_PTR(void) out_hi;                              /* the planes of out, rows out_pitch and matrices out_plane halves apart */
+    ORTH_PTR(void) out_lo;
+    long long out_pitch, out_plane;
     /* RESULT: element (r, c) of matrix k at k * stride_w + r * ld_w + c; transposed when tall */
     int type_w, tall, vec_w;
     float keep;                                         /* 0: w is not read */

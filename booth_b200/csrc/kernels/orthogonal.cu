@@ -35,7 +35,7 @@
 // the normalised, possibly transposed matrix), then steps x 3 products. A product kernel
 // keeps one CTA or CTA pair per SM (pair) and walks over the tiles of all matrices of
 // the batch; the roles inside are those of the fp32 GEMM: warp 0 TMA, warp 1 MMA, warps 4-11
-// drain tensor memory, apply the epilogue and store, planes by TMA from shared memory.
+// drain tensor memory, apply the epilogue and store.
 //   256: 256 x 256 tile per two CTAs, tcgen05.mma.cta_group::2
 //   128: 128 x 128 tile per CTA
 //   64:  64 x 64 tile per CTA, for products so small that they are all latency
@@ -322,6 +322,14 @@ __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a, uint64_t b, ui
                      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                      ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// 32 halves of a row, whole 32-byte sectors at a time.
+__device__ __forceinline__ void put_row(char *to, const uint32_t (&v)[16])
+{
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + 32 * i), "r"(v[8 * i]), "r"(v[8 * i + 1]), "r"(v[8 * i + 2]), "r"(v[8 * i + 3]),
+                     "r"(v[8 * i + 4]), "r"(v[8 * i + 5]), "r"(v[8 * i + 6]), "r"(v[8 * i + 7]) : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *v)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
@@ -404,7 +412,7 @@ __device__ __forceinline__ void tma_store(const CUtensorMap *map, uint32_t src, 
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-// Results go out by TMA in boxes of 64 x 64 of a plane, which clips them at the matrix's edges: a lane puts its
+// 64-tiles go out by TMA in boxes of 64 x 64 of a plane, which clips them at the matrix's edges: a lane puts its
 // packed halves of row r, from 16-byte unit u0 on, into the box in the map's 128-byte swizzle.
 template <int N>
 __device__ __forceinline__ void put_box(uint32_t box, const uint32_t (&packed)[N], int r, int u0)
@@ -590,7 +598,7 @@ __device__ __forceinline__ bool chunk_ends(int kb, int run, int diag0, int diag,
 
 // 384 threads; grid: any number of CTAs (pairs), each takes every grid-th tile. p.split > 1: a
 // cluster of that many CTAs (pairs) shares one tile, each takes a range of K, and the sums meet in the
-// workspace, 64 columns of the tile with each owner; the grid is then one cluster a tile. Few tiles
+// workspace, every split-th 32 columns of the tile with each owner; the grid is then one cluster a tile. Few tiles
 // leave most of the GPU idle: the 10 tiles of a 1000 x 1000 symmetric product with K = 2049 took 33 us
 // on 36 single CTAs. (Through distributed shared memory instead of L2 the meeting alone took 10 us.)
 template <int PLANES, int SIDE>
@@ -773,7 +781,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
         const int e = warp - 4, q = warp & 3, h = e >> 2;
         const uint32_t acc_empty = PAIR ? map_to_cta(acc_empty0, first) : acc_empty0;
         const uint32_t staging = smem0 + OPERAND_BYTES;
-        const bool issuer = SIDE == 64 ? e == 0 && lane == 0 : (q & 1) == 0 && lane == 0;
+        const bool issuer = e == 0 && lane == 0;      // of the 64-tiles' stores
         uint32_t g = 0;
         bool ok = true;
         if constexpr (SIDE == 64) {
@@ -898,9 +906,6 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                 }
             }
         } else {
-        // two warps (q even and odd) store a box of 64 x 64 together
-        constexpr int TEAM = 64;
-        const int team = h * 2 + (q >> 1), team_row = (q & 1) * 32 + lane;
         for (int item = cl; ok && item < items; item += C) {
             int k, i, j;
             tiles.at(item, k, i, j);
@@ -908,23 +913,22 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
             if (p.mode == ORTH_RESULT && p.keep != 0.f) prefetch_result(p, lane, k, row0, col0, HALF);
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * HALF);
             uint32_t buf = g & 1u;
-            // the first piece of 64 columns this part owns. One plane: its weights a piece ahead; two planes, where the sums
+            // the first piece of 32 columns this part owns. One plane: its weights a piece ahead; two planes, where the sums
             // need the registers: half of them at a time, when they are needed.
-            constexpr int PIECE = 64, PIECES = HALF / PIECE;
+            constexpr int PIECES = HALF / 32;
             const int piece0 = h * PIECES, own0 = (part + 8 * split - piece0) % split;
-            uint32_t w[2][PLANES == 1 ? 32 : 1];
-            const auto weights = [&](int cc, int half) {
-                if (p.mode == ORTH_RESULT && cc < PIECES) fetch_weights(p, w[half], 0, lane, k, row0, col0 + cc * PIECE + half * 32);
+            uint32_t w[PLANES == 1 ? 32 : 1];
+            const auto weights = [&](int cc) {
+                if (p.mode == ORTH_RESULT && cc < PIECES) fetch_weights(p, w, 0, lane, k, row0, col0 + cc * 32);
             };
             if constexpr (PLANES == 1) {
-                weights(own0, 0);
-                weights(own0, 1);
+                weights(own0);
                 ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (g >> 1) & 1u, status, 3));
                 g++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             } else {
                 // the chunks' sums in registers; the total goes back to tensor memory in place of the last chunk, so
-                // that the epilogue below holds 64 columns at a time (with all of them in registers it
+                // that the epilogue below holds 32 columns at a time (with all of them in registers it
                 // spilled, and beside 225 KB of shared memory there is no first-level cache to spill to)
                 float acc[HALF];
 #pragma unroll
@@ -961,7 +965,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
             if (split > 1) {
 #pragma unroll 1
                 for (int cc = 0; ok && cc < HALF / 32; cc++) {
-                    if ((piece0 + cc * 32 / PIECE) % split == part) continue;
+                    if ((piece0 + cc) % split == part) continue;
                     uint32_t r[32];
                     tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 32), r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -973,100 +977,77 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                 }
                 cluster_sync_all();
             }
-            // the warps of a store go on only if all of them may
-            ok = all_ok<TEAM>(1 + team, ok);
-            // behind the last tile the operand stages are free: every box has its own place there and none waits for another
-            const bool roomy = item + C >= items;
+            // Planes are stored from registers: a piece is 64 bytes of a row. (Through 64 x 64 boxes in shared memory and TMA it took
+            // as long, with two barriers a box; and the code, a piece long, is fetched once instead of unrolled: the first
+            // pass over it costs a microsecond of each product.)
 #pragma unroll 1
             for (int cc = own0; ok && cc < PIECES; cc += split) {
-                const int col = col0 + cc * PIECE;
-                // both warps of a store agree: its first row and column decide
-                if (row0 - (q & 1) * 32 >= p.rows || col >= p.cols) break;
-                uint32_t hi[PIECE / 2], lo[PIECE / 2];
+                const int col = col0 + cc * 32;
+                if (row0 >= p.rows || col >= p.cols) break;
+                uint32_t r[32];
+                tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * 32), r);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                float v[32];
 #pragma unroll
-                for (int half = 0; half < PIECE / 32; half++) {
-                    uint32_t r[32];
-                    tmem_ld32(lanes + buf * (uint32_t)SIDE + (uint32_t)(cc * PIECE + half * 32), r);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    float v[32];
+                for (int c = 0; c < 32; c++) v[c] = __uint_as_float(r[c]);
+                // the other parts' sums, two at a time so that their loads wait together, always from the next part on
+                for (int n = 1; n < split; n += 2) {
+                    const int from[2] = { part + n < split ? part + n : part + n - split, part + n + 1 < split ? part + n + 1 : part + n + 1 - split };
+                    float4 x[2][8];
 #pragma unroll
-                    for (int c = 0; c < 32; c++) v[c] = __uint_as_float(r[c]);
-                    // the other parts' sums, two at a time so that their loads wait together, always from the next part on
-                    for (int n = 1; n < split; n += 2) {
-                        const int from[2] = { part + n < split ? part + n : part + n - split, part + n + 1 < split ? part + n + 1 : part + n + 1 - split };
-                        float4 x[2][8];
+                    for (int o = 0; o < 2; o++) {
+                        const float *const at = p.sums + sums_at + from[o] * part_step + cc * 1024;
 #pragma unroll
-                        for (int o = 0; o < 2; o++) {
-                            const float *const at = p.sums + sums_at + from[o] * part_step + (cc * PIECE + half * 32) * 32;
-#pragma unroll
-                            for (int u = 0; u < 8; u++)
-                                x[o][u] = n + o < split ? __ldcg(reinterpret_cast<const float4 *>(at + u * 128)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        }
-#pragma unroll
-                        for (int u = 0; u < 8; u++) {
-                            v[4 * u] += x[0][u].x + x[1][u].x; v[4 * u + 1] += x[0][u].y + x[1][u].y;
-                            v[4 * u + 2] += x[0][u].z + x[1][u].z; v[4 * u + 3] += x[0][u].w + x[1][u].w;
-                        }
+                        for (int u = 0; u < 8; u++)
+                            x[o][u] = n + o < split ? __ldcg(reinterpret_cast<const float4 *>(at + u * 128)) : make_float4(0.f, 0.f, 0.f, 0.f);
                     }
 #pragma unroll
-                    for (int c = 0; c < 32; c++) v[c] *= p.alpha;
-                    if (p.mode == ORTH_RESULT) {
-                        const uint32_t own = staging + (uint32_t)e * 4096u;
-                        const int c0 = col + half * 32;
-                        if (!p.tall) put_result(v, own, lane);
-                        if constexpr (PLANES == 1) {
-                            store_result<32, 0>(p, v, w[half], own, lane, k, row0, c0);
-                            weights(cc + split, half);
-                        } else {
-                            uint32_t x[16];
-                            fetch_weights(p, x, 0, lane, k, row0, c0);
-                            store_result<16, 0>(p, v, x, own, lane, k, row0, c0);
-                            fetch_weights(p, x, 16, lane, k, row0, c0);
-                            store_result<16, 16>(p, v, x, own, lane, k, row0, c0);
-                        }
-                        continue;
+                    for (int u = 0; u < 8; u++) {
+                        v[4 * u] += x[0][u].x + x[1][u].x; v[4 * u + 1] += x[0][u].y + x[1][u].y;
+                        v[4 * u + 2] += x[0][u].z + x[1][u].z; v[4 * u + 3] += x[0][u].w + x[1][u].w;
                     }
-                    if (tiles.sym && i == j) {
+                }
 #pragma unroll
-                        for (int c = 0; c < 32; c++) v[c] += row0 + lane == col + half * 32 + c ? p.diag : 0.f;
+                for (int c = 0; c < 32; c++) v[c] *= p.alpha;
+                if (p.mode == ORTH_RESULT) {
+                    const uint32_t own = staging + (uint32_t)e * 4096u;
+                    if (!p.tall) put_result(v, own, lane);
+                    if constexpr (PLANES == 1) {
+                        store_result<32, 0>(p, v, w, own, lane, k, row0, col);
+                        weights(cc + split);
+                    } else {
+                        uint32_t x[16];
+                        fetch_weights(p, x, 0, lane, k, row0, col);
+                        store_result<16, 0>(p, v, x, own, lane, k, row0, col);
+                        fetch_weights(p, x, 16, lane, k, row0, col);
+                        store_result<16, 16>(p, v, x, own, lane, k, row0, col);
                     }
+                    continue;
+                }
+                if (tiles.sym && i == j) {
+#pragma unroll
+                    for (int c = 0; c < 32; c++) v[c] += row0 + lane == col + c ? p.diag : 0.f;
+                }
+                const bool live = row0 + lane < p.rows;
+                const long long at = (k * p.out_plane + (row0 + lane) * p.out_pitch + col) * 2;
+                uint32_t y[16];
+#pragma unroll
+                for (int c = 0; c < 16; c++) {
+                    const __half2 x = __floats2half2_rn(v[2 * c], v[2 * c + 1]);
+                    const float2 f = __half22float2(x);
+                    y[c] = *reinterpret_cast<const uint32_t *>(&x);
+                    v[2 * c] -= f.x; v[2 * c + 1] -= f.y;
+                }
+                if (live) put_row(static_cast<char *>(p.out_hi) + at, y);
+                if (p.lo) {
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
                         const __half2 x = __floats2half2_rn(v[2 * c], v[2 * c + 1]);
-                        hi[half * 16 + c] = *reinterpret_cast<const uint32_t *>(&x);
+                        y[c] = *reinterpret_cast<const uint32_t *>(&x);
                     }
-                    if (p.lo) {
-#pragma unroll
-                        for (int c = 0; c < 16; c++) {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[half * 16 + c]));
-                            const __half2 y = __floats2half2_rn(v[2 * c] - f.x, v[2 * c + 1] - f.y);
-                            lo[half * 16 + c] = *reinterpret_cast<const uint32_t *>(&y);
-                        }
-                    }
+                    if (live) put_row(static_cast<char *>(p.out_lo) + at, y);
                 }
-                if (p.mode != ORTH_RESULT) {
-                    const uint32_t box = roomy ? smem0 + (uint32_t)(team * PIECES + cc) * 16384u : staging + (uint32_t)team * 8192u;
-                    if (!roomy) {
-                        if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the last content has left
-                        team_sync<TEAM>(1 + team);
-                    }
-                    put_box(box, hi, team_row, 0);
-                    if (roomy && p.lo) put_box(box + 8192u, lo, team_row, 0);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    team_sync<TEAM>(1 + team);
-                    if (issuer) {
-                        tma_store(&o_hi, box, col, row0, k);
-                        if (roomy && p.lo) tma_store(&o_lo, box + 8192u, col, row0, k);
-                    }
-                    if (!roomy && p.lo) {
-                        if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                        team_sync<TEAM>(1 + team);
-                        put_box(box, lo, team_row, 0);
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        team_sync<TEAM>(1 + team);
-                        if (issuer) tma_store(&o_lo, box, col, row0, k);
-                    }
-                }
+                __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();

@@ -447,6 +447,8 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
         const int from = i & 1, to = from ^ 1, end = i == ns->steps - 1;
         q.rows = q.cols = (int)o->s;
         q.mode = ORTH_GRAM; q.K = (int)o->l; q.lo = two_planes;
+        q.out_hi = ws + (c == 0.0 ? o->q_hi : o->s_hi); q.out_lo = ws + (c == 0.0 ? o->q_lo : o->s_lo);
+        q.out_pitch = o->a_pitch; q.out_plane = o->a_pitch * o->s;
         if (c == 0.0) {
             q.alpha = (float)(b * qs / (xs * xs)); q.diag = (float)(a * qs);
             if ((rc = orth_launch(dev, &plan[0], &x[from], &x[from], &qm, &q, two_planes)) != SM100_OK) return rc;
@@ -454,11 +456,14 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
             q.alpha = (float)(ss / (xs * xs)); q.diag = (float)(beta * ss);
             if ((rc = orth_launch(dev, &plan[0], &x[from], &x[from], &sm, &q, two_planes)) != SM100_OK) return rc;
             q.mode = ORTH_POLY; q.K = (int)o->s;
+            q.out_hi = ws + o->q_hi; q.out_lo = ws + o->q_lo;
             q.alpha = (float)(c * qs / (ss * ss)); q.diag = (float)(gamma * qs);
             if ((rc = orth_launch(dev, &plan[1], &sm, &sm, &qm, &q, two_planes)) != SM100_OK) return rc;
         }
         q.mode = end ? ORTH_RESULT : ORTH_UPDATE; q.K = (int)o->s; q.lo = 1;
         q.cols = (int)o->l;
+        q.out_hi = ws + o->x_hi[to]; q.out_lo = ws + o->x_lo[to];
+        q.out_pitch = o->x_pitch; q.out_plane = o->x_pitch * o->s;
         q.alpha = (float)(end ? factor / (qs * xs) : 1.0 / qs); q.diag = 0.0f;
         if ((rc = orth_launch(dev, &plan[2], &qm, &x[from], &x[to], &q, two_planes)) != SM100_OK) return rc;
     }
