@@ -320,14 +320,15 @@ typedef struct { int side, split; long long tiles; double us; } orth_plan_t;
 /* One product with a given tile side: the parts its K is cut into and how long it takes,
  * in microseconds measured in a chain of products (one plane, two planes). A product costs
  * `base`, a K block of 64 `block` (64-tiles slow one another down in L2: .001 more for every CTA), a
- * further wave its K blocks or, if that is longer, its epilogue; parts meet at `meet`. Per
- * 1000 x 1000 x 1000 product in two planes that makes 10 us with 64-tiles, 13 with 128 and 12 with 256
- * in three or four parts; at 2048 cubed 59, 36 and 46, and at 2048 x 4096 the largest tile wins.
+ * further wave its K blocks or, if that is longer, its epilogue; parts meet at `meet`. A
+ * 1000 x 1000 x 1000 product in two planes comes to 17, 12 (two parts) and 15 us by side, 2048 cubed to 95, 53 and 34.
+ * The choice is worth: 1024 x 4096 f32 322 us, 334 with the larger `base` and `meet` of an epilogue through shared
+ * memory; 2048 x 8192 bf16 624 against 648; 768 x 768 bf16 132 against 128 the other way.
  * K is shared only while everything runs at once. */
 static orth_plan_t orth_product_plan(sm100_dev_t *dev, int side, long long rows, long long cols, long long K, int batch, int sym, int two_planes)
 {
     static const struct { double base[2], block[2], epilogue, meet; } cost[3] = {
-        { { 3.3, 3.9 }, { 0.22, 0.26 }, 1.5, 1.0 }, { { 4.3, 5.0 }, { 0.33, 0.80 }, 3.0, 2.0 }, { { 6.0, 7.5 }, { 0.32, 0.85 }, 5.0, 3.0 } };
+        { { 3.3, 3.9 }, { 0.22, 0.26 }, 1.5, 1.0 }, { { 4.0, 4.5 }, { 0.30, 0.75 }, 2.5, 1.5 }, { { 6.0, 7.0 }, { 0.32, 0.85 }, 4.5, 2.5 } };
     const int f = side == 64 ? 0 : side == 128 ? 1 : 2, ctas = side == 256 ? 2 : 1;
     const long long m = (rows + side - 1) / side, n = (cols + side - 1) / side, chunks = (K + 127) / 128;
     orth_plan_t best = { side, 1, batch * (sym ? m * (m + 1) / 2 : m * n), 0.0 };

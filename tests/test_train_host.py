@@ -107,7 +107,7 @@ go(3, 1000, 500, sm.F32, 1)
 d.sync(); d.close()
 """)
     assert res.returncode == 0, res.stderr
-    assert [l["kernel"] for l in L] == ["orth_norm", "orth_split"] + ["orth_product_1_256"] * 6 + ["orth_norm", "orth_split", "orth_product_2_64", "orth_product_2_64", "orth_product_2_128"]
+    assert [l["kernel"] for l in L] == ["orth_norm", "orth_split"] + ["orth_product_1_256"] * 6 + ["orth_norm", "orth_split", "orth_product_2_128", "orth_product_2_64", "orth_product_2_128"]
     assert all(l["overlap"] == 1 for l in L)
     assert all(l["shmem"] == 230400 and l["block"] == (384, 1, 1) for l in L if l["kernel"].startswith("orth_product"))
     P = products(lines)
