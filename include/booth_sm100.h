@@ -281,7 +281,8 @@ int  booth_sm100_asian_paths(sm100_dev_t *dev, const booth_asian_t *p,
  * w and b [cols] may be NULL (ones, zeros); mean and rstd [rows], fp32, may be NULL
  * and are what the backward pass wants. dtype is x's and y's type, wdtype w's and
  * b's (SM100_F32, SM100_BF16 or SM100_F16): the same, or SM100_F32 beside 16-bit values. Statistics and products are
- * fp32, y is rounded once. y may be x (same pitch); otherwise outputs must not
+ * fp32, y is rounded once. A row with infinities of one sign has that infinity as its mean, with both signs or a
+ * NaN no mean; its y and rstd are NaN in either case. y may be x (same pitch); otherwise outputs must not
  * overlap inputs. Rows beyond `rows` and columns beyond `cols` are neither read nor
  * written. Any alignment of whole elements; rows that start on 16 bytes and are a
  * multiple of 16 bytes long are read in 16-byte vectors. At most 2^30 columns; rows = 0 does nothing. */

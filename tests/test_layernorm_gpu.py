@@ -315,3 +315,77 @@ def test_short_rows_at_every_offset(dev, sm, cols, t):
         check_forward(x, w, b, 1e-5, y, mean, rstd)
         assert bool((flat[2:].view(200, -1)[:, cols:] == 7.25).all())
         check_backward(dy, x, w, mean, rstd, *run_backward(dev, sm, ds, xs, w, mean, rstd))
+
+
+def exact_sums(rows, cols, t, seed=0):
+    """Values n / 64 with whole n, |n| <= 200, and row sums of their own choice: any order of adding up to 2^24 / 200
+    of them is exact in fp32. Means between 1e-4 and 1e-2 where the width allows, both signs."""
+    g = torch.Generator().manual_seed(seed)
+    n = (64 * torch.randn(rows, cols, generator=g)).round().clamp(-190, 190).long()
+    want = (64 * cols * 10 ** (-4 + 2 * torch.rand(rows, generator=g))).round().long().clamp_min(1) * (1 - 2 * (torch.arange(rows) % 2))
+    off = want - n.sum(1)
+    n += off.div(cols, rounding_mode="floor")[:, None] + (torch.arange(cols)[None] < (off % cols)[:, None])
+    assert bool((n.sum(1) == want).all()) and int(n.abs().max()) <= 200
+    return (n / 64).to(TYPES[t]).cuda(), want.double().cuda() / 64 / cols
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(1, 1024), (5, 1031), (400, 1024), (400, 600), (300, 1031), (300, 5000), (3, 5001), (2, 10000), (3, 12001), (3, 20000), (2, 40000)])
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_small_means_keep_their_digits(dev, sm, rows, cols, t):
+    """The sum is exact; 1 / cols and the product with it are rounded once each (2 steps of 2^-24, and their product)."""
+    x, want = exact_sums(rows, cols, t, seed=cols)
+    assert torch.equal(x.double().mean(1), want)
+    _, mean, rstd = run_forward(dev, sm, x, None, None)
+    off = (mean.double() - want).abs() / want.abs()
+    assert bool((off <= 2.01 * U).all()), off.max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [64, 1024, 1031, 5000, 10000, 20000])
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_means_of_rows_far_from_zero(dev, sm, cols, t):
+    """m + dm: the correction dm is a mean of differences x - m, each rounded by U of itself and added up with SUMS roundings;
+    1 / cols, the product with it and the last sum are rounded once each."""
+    g = torch.Generator().manual_seed(cols)
+    x = (torch.randn(50, cols, generator=g) + 1000 * (1 - 2 * (torch.arange(50) % 2))[:, None]).to(TYPES[t]).cuda()
+    _, mean, _ = run_forward(dev, sm, x, None, None)
+    want = x.double().mean(1)
+    spread = (x.double() - want[:, None]).abs().mean(1) + 2 * SUMS(cols) * U * want.abs()      # about m, which itself is off by a sum's roundings
+    assert bool(((mean.double() - want).abs() <= U * want.abs() + (SUMS(cols) + 4) * U * spread).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [24, 1000, 1024, 6001, 20000])
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_the_mean_of_a_row_with_infinities(dev, sm, cols, t):
+    """One infinity, or several of one sign, are the row's mean; both signs, or a NaN beside them, leave none."""
+    inf, nan = float("inf"), float("nan")
+    x = make(6, cols, TYPES[t], TYPES[t], seed=cols)[0]
+    x[0, cols // 2] = inf
+    x[1, 0] = -inf
+    x[2, 0] = x[2, cols - 1] = inf
+    x[3, 1], x[3, cols - 2] = inf, -inf
+    x[4, 3], x[4, cols - 4] = inf, nan
+    y, mean, rstd = run_forward(dev, sm, x, None, None)
+    assert mean[:3].tolist() == [inf, -inf, inf] and bool(mean[3:5].isnan().all()) and bool(mean[5].isfinite())
+    assert bool(y[:5].isnan().all()) and bool(rstd[:5].isnan().all()) and bool(y[5].isfinite().all())
+
+
+def residual_rows(rows, cols, seed):
+    """Rows of a residual stream: a few channels larger than the rest, a small mean of its own in every row."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * (1 + 4 * (torch.rand(cols, generator=g) < 0.02))
+    return x - x.mean(1, keepdim=True) + 2e-3 * torch.randn(rows, 1, generator=g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("each", [1, 300])
+def test_means_of_centred_rows_carry_a_sums_rounding_and_no_bias(dev, sm, t, each):
+    """Row by row (the form of few rows) and all at once. The partial sums of such a row reach 2^5 to 2^6 at the last two levels of
+    the tree, where a rounding is 2^-18 / sqrt(12) in the root mean square, and halve with every second level below: some 2.5e-6 in
+    all, 2.4e-9 of the mean. Four times that is allowed; what differences from a mean of their own lose together is 2e-8."""
+    x = residual_rows(300, 1024, 11).to(TYPES[t]).cuda()
+    mean = torch.cat([run_forward(dev, sm, x[i:i + each], None, None)[1] for i in range(0, 300, each)])
+    assert (mean.double() - x.double().mean(1)).square().mean().sqrt().item() <= 1e-8
