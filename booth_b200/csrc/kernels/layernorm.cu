@@ -425,6 +425,9 @@ template <int E> __device__ __forceinline__ int valid_of(const Group &g, int col
 // infinity leaves no dm, and m is the mean. (y takes the same rounded differences and is right with dm either way.)
 __device__ __forceinline__ float mean_of(float m, float dm, float var) { return m * m > var && fabsf(dm) < INFINITY ? m + dm : m; }
 
+// Rounding may leave a variance below zero; a NaN (of a row that holds one, or whose sums overflow) stays one.
+__device__ __forceinline__ float rstd_of(float var, float eps) { return __frsqrt_rn((var > 0.f ? var : var == var ? 0.f : var) + eps); }
+
 // v: a row's values in, their differences from `m` out (zero outside the row). Their mean is `dm`; `mean` as above.
 template <int E, int N>
 __device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int valid, float inv, float eps, float2 (*sh)[32], float &mean, float &dm, float &rstd)
@@ -453,7 +456,7 @@ __device__ __forceinline__ void row_stats(Pair (&v)[N], Group &g, int valid, flo
     dm = t.x * inv;
     const float var = t.y * inv - dm * dm;
     mean = mean_of(m, dm, var);
-    rstd = __frsqrt_rn((var > 0.f ? var : var == var ? 0.f : var) + eps);      // a NaN stays one
+    rstd = rstd_of(var, eps);
 }
 
 template <typename T, typename W, bool VEC, int CPT, bool HOLD>
@@ -619,11 +622,10 @@ __device__ __forceinline__ void forward_loop(T *y, const T *x, const W *__restri
         float d1 = 0.f, d2 = 0.f;
         for (int c = g.t; c < cols; c += g.size) { const float d = to_f32(src[c]) - m; d1 += d; d2 = fmaf(d, d, d2); }
         const float2 t = g.sum2(d1, d2, sh);
-        const float dm = t.x / (float)cols, mean = m + dm;
-        float rstd = __frsqrt_rn(fmaxf(t.y / (float)cols - dm * dm, 0.f) + eps);
-        if (!(t.y == t.y)) rstd = t.y;
+        const float dm = t.x / (float)cols, mean = m + dm, var = t.y / (float)cols - dm * dm;
+        const float rstd = rstd_of(var, eps);
         if (g.t == 0) {
-            if (mean_out) mean_out[row] = mean_of(m, dm, t.y / (float)cols - dm * dm);
+            if (mean_out) mean_out[row] = mean_of(m, dm, var);
             if (rstd_out) rstd_out[row] = rstd;
         }
         for (int c = g.t; c < cols; c += g.size)

@@ -389,3 +389,16 @@ def test_means_of_centred_rows_carry_a_sums_rounding_and_no_bias(dev, sm, t, eac
     x = residual_rows(300, 1024, 11).to(TYPES[t]).cuda()
     mean = torch.cat([run_forward(dev, sm, x[i:i + each], None, None)[1] for i in range(0, 300, each)])
     assert (mean.double() - x.double().mean(1)).square().mean().sqrt().item() <= 1e-8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [1024, 1031, 6001, 20000])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_a_row_whose_sum_overflows_has_no_rstd(dev, sm, cols, t):
+    """1024 values of 3e36 are beyond fp32: no form may make a finite rstd out of that."""
+    x = make(3, cols, TYPES[t], TYPES[t], seed=cols)[0]
+    x[1] = 3e36
+    y, mean, rstd = run_forward(dev, sm, x, None, None)
+    assert not bool(mean[1].isfinite()) and bool(rstd[1].isnan()) and bool(y[1].isnan().all())
+    keep = [0, 2]
+    check_forward(x[keep], None, None, 1e-5, y[keep], mean[keep], rstd[keep])
