@@ -22,6 +22,7 @@ OK, ERR_DL, ERR_SYM, ERR_CUDA, ERR_NO_GPU, ERR_IO, ERR_KERN, ERR_ARG, ERR_NCCL =
 FILL_F32_PM1, FILL_F32_01, FILL_I32_1000, FILL_U32_RAW = 0, 1, 2, 3
 I32, F32, F64, BF16, F16 = 0, 1, 2, 3, 4
 GEMM_B_UNCHANGED, GEMM_TEST_SILENT_PRODUCER = 1, 0x80000000
+NS_TEST_SILENT_PRODUCER = 0x40000000
 COMM_ID_BYTES = 128
 
 _ptr = C.c_ulonglong

@@ -49,5 +49,6 @@ typedef struct orth_product {
     ORTH_PTR(float) sums;                               /* where the parts of a tile meet */
     ORTH_PTR(int) status;
     unsigned long long wait_ns;
+    int silent;                                         /* the tests' way to see a wait run out: nothing is loaded */
 } orth_product_t;
 #endif

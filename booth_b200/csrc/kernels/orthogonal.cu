@@ -431,6 +431,16 @@ template <int THREADS> __device__ __forceinline__ bool all_ok(int bar, bool ok)
     return all != 0;
 }
 
+// Whether a wait has run out in a product of this handle that nobody has asked about yet, this call's earlier ones among
+// them: its planes are incomplete, and the caller's matrix is left as it is. Asked once a tile, behind its sums, where the answer
+// is on its way while they are read back.
+__device__ __forceinline__ int gave_up(const Product &p)
+{
+    int v = 0;
+    if (p.mode == ORTH_RESULT) asm volatile("ld.relaxed.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p.status) : "memory");
+    return v;
+}
+
 // Brings the weights a warp's rows will read into L2 while the products run.
 __device__ __forceinline__ void prefetch_result(const Product &p, int lane, int k, int row0, int col0, int cols)
 {
@@ -687,7 +697,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
         {
             uint32_t st = smem0, full = full0, empty = empty0, ph = 1;      // stage and its barriers
             bool ok = true;
-            for (int item = cl; ok && item < items; item += C) {
+            for (int item = cl; ok && !p.silent && item < items; item += C) {
                 int k, i, j;
                 tiles.at(item, k, i, j);
                 const int m0 = i * SIDE + (int)rank * 128, n0 = j * SIDE + (int)rank * 128;
@@ -839,6 +849,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         put_quarter(quarters + (q < 2 ? h : 2) * 16384u, x, (q & 1) * 32 + lane, 0);
                     }
                 }
+                const int stop = gave_up(p);
                 ok = all_ok<256>(1, ok);
                 float v[16];
 #pragma unroll
@@ -877,7 +888,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     for (int c = 0; c < 16; c++)
                         asm volatile("st.shared.f32 [%0], %1;" ::"r"(quarters + (uint32_t)(r * 65 + c16 * 16 + c) * 4), "f"(v[c]) : "memory");
                     team_sync<256>(1);
-                    store_result_64(p, quarters, (int)threadIdx.x - 128, k, i * 64, j * 64);
+                    if (!__any_sync(0xffffffffu, stop)) store_result_64(p, quarters, (int)threadIdx.x - 128, k, i * 64, j * 64);
                     team_sync<256>(1);
                     continue;
                 }
@@ -959,6 +970,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     }
                 }
             }
+            const int stop = gave_up(p);
             // where this warp's sums lie when parts meet: [part][CTA][warp][4 columns][lane][4]
             constexpr size_t WARP_SUMS = 32 * HALF, part_step = (size_t)CTAS * 8 * WARP_SUMS;
             const size_t sums_at = (((size_t)cl * split * CTAS + rank) * 8 + e) * WARP_SUMS + lane * 4;
@@ -1013,9 +1025,9 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     const uint32_t own = staging + (uint32_t)e * 4096u;
                     if (!p.tall) put_result(v, own, lane);
                     if constexpr (PLANES == 1) {
-                        store_result<32, 0>(p, v, w, own, lane, k, row0, col);
+                        if (!__any_sync(0xffffffffu, stop)) store_result<32, 0>(p, v, w, own, lane, k, row0, col);
                         weights(cc + split);
-                    } else {
+                    } else if (!__any_sync(0xffffffffu, stop)) {
                         uint32_t x[16];
                         fetch_weights(p, x, 0, lane, k, row0, col);
                         store_result<16, 0>(p, v, x, own, lane, k, row0, col);

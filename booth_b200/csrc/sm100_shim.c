@@ -451,7 +451,8 @@ static int orth_outcome(sm100_dev_t *dev)
     CUresult cr = dev->api->MemcpyDtoH(&st, word, sizeof st);
     if (cr != CUDA_SUCCESS) return sm100_fail(dev, "reading the orthogonalisation's status", cr);
     if (st != 0) {
-        (void)dev->api->MemsetD8Async(word, 0, sizeof st, dev->stream);
+        /* cleared before this returns: a graph replayed on another stream must not find it still set and leave its result */
+        if (dev->api->MemsetD8Async(word, 0, sizeof st, dev->stream) == CUDA_SUCCESS) (void)dev->api->StreamSynchronize(dev->stream);
         snprintf(dev->err, sizeof dev->err, "orth_product gave up waiting on a barrier (code %d: "
                  "1 = producer, 2 = MMA issuer on operands, 3 = epilogue, 4 = MMA issuer on a free accumulator)", st);
         fprintf(stderr, "sm100_rt: %s\n", dev->err);

@@ -372,6 +372,7 @@ static int orth_launch(sm100_dev_t *dev, const orth_plan_t *plan, const plane_ma
     p->split = plan->split;
     void *args[] = { (void *)&a->hi, (void *)&a->lo, (void *)&b->hi, (void *)&b->lo, (void *)&out->hi, (void *)&out->lo, p };
     const int rc = sm100_launch_k_cluster(dev, SM100_K_ORTH_PRODUCT + form + (two_planes ? 1 : 0), (unsigned)(groups * ctas), (unsigned)ctas, 384, ORTH_SMEM, args);
+    p->silent = 0;
     if (p->mode <= ORTH_POLY) p->tri = plan->side;      /* how the product that reads this one finds its triangle */
     return rc;
 }
@@ -444,8 +445,10 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
     q.sums = ws + o->sums;
     q.status = dev->scratch + SM100_SCRATCH_ORTH_STATUS;
     q.wait_ns = (unsigned long long)dev->gemm_wait_ms * 1000000ull;
-    for (int i = 0; i < ns->steps; i++) {
-        const int from = i & 1, to = from ^ 1, end = i == ns->steps - 1;
+    const int steps = ns->steps & ~BOOTH_NS_TEST_SILENT_PRODUCER;
+    q.silent = (ns->steps & BOOTH_NS_TEST_SILENT_PRODUCER) != 0;        /* the first product's producers issue nothing */
+    for (int i = 0; i < steps; i++) {
+        const int from = i & 1, to = from ^ 1, end = i == steps - 1;
         q.rows = q.cols = (int)o->s;
         q.mode = ORTH_GRAM; q.K = (int)o->l; q.lo = two_planes;
         q.out_hi = ws + (c == 0.0 ? o->q_hi : o->s_hi); q.out_lo = ws + (c == 0.0 ? o->q_lo : o->s_lo);
@@ -475,7 +478,8 @@ static const booth_newton_schulz_t ns_default = { 5, 3.4445f, -4.7750f, 2.0315f,
 
 static int ns_ok(const booth_newton_schulz_t *ns)
 {
-    return ns->steps >= 1 && ns->steps <= 64 && isfinite(ns->a) && isfinite(ns->b) && isfinite(ns->c) && isfinite(ns->eps) && ns->eps > 0.0f &&
+    const int steps = ns->steps & ~BOOTH_NS_TEST_SILENT_PRODUCER;
+    return steps >= 1 && steps <= 64 && isfinite(ns->a) && isfinite(ns->b) && isfinite(ns->c) && isfinite(ns->eps) && ns->eps > 0.0f &&
            (ns->c == 0.0f || fabsf(ns->b) <= 8.0f * fabsf(ns->c));
 }
 

@@ -309,9 +309,13 @@ size_t booth_sm100_layernorm_backward_workspace(sm100_dev_t *dev, long long rows
  * (for a matrix with more rows than columns X is its transpose, the result is the same
  * polynomial). NULL where one is expected means five steps of the Muon optimiser's
  * quintic, 3.4445, -4.7750, 2.0315, and eps = 1e-7. 1 to 64 steps; eps > 0; c = 0 or
- * |b| <= 8 |c| (the square is completed: b / 2c must be of the size of the rest). The
+ * |b| <= 8 |c| (the square is completed: b / 2c must be of the size of the rest).
+ * Waits inside the products have the limit of booth_sm100_gemm_wait_limit; one that ran out is reported as a GEMM's is,
+ * and from then until it is reported the calls on this handle leave `out` or `w` as it was (a Muon step's momentum
+ * has advanced by then). Only where the last product itself gave up may some of its tiles be written. The
  * coefficients must keep the singular values below 2, as every scheme that converges
  * from [0, 1] does (the operands are fp16, scaled for that range): beyond, results are not finite. */
+#define BOOTH_NS_TEST_SILENT_PRODUCER 0x40000000    /* or'ed into steps, for tests: the first product loads nothing, so its waits run out */
 typedef struct booth_newton_schulz {
     int32_t steps;
     float   a, b, c, eps;

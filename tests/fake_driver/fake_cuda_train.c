@@ -30,10 +30,10 @@ CUresult cuLaunchKernelEx(const CUlaunchConfig *c, CUfunction f, void **params, 
     if (strncmp(((fake_func_t *)f)->name, "orth_product", 12) == 0) {
         const orth_product_t *p = (const orth_product_t *)params[6];
         const char *code = getenv("FAKE_CUDA_ORTH_STATUS");
-        char line[192];
+        char line[224];
         if (code) *(int *)(size_t)p->status = atoi(code);
-        snprintf(line, sizeof line, "product mode %d rows %d cols %d K %d batch %d alpha %.9g diag %.9g keep %.9g tall %d vec %d\n",
-                 p->mode, p->rows, p->cols, p->K, p->batch, p->alpha, p->diag, p->keep, p->tall, p->vec_w);
+        snprintf(line, sizeof line, "product mode %d rows %d cols %d K %d batch %d alpha %.9g diag %.9g keep %.9g tall %d vec %d silent %d\n",
+                 p->mode, p->rows, p->cols, p->K, p->batch, p->alpha, p->diag, p->keep, p->tall, p->vec_w, p->silent);
         logf_line(line);
     }
     return base_cuLaunchKernelEx(c, f, params, extra);

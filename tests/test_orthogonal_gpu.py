@@ -333,3 +333,37 @@ def test_a_training_step_of_a_normalised_linear_layer(dev, sm):
         assert (got.double() - leaf.grad).norm() <= 1e-5 * leaf.grad.norm()
     want, want_m, err = muon64(leaves[3].detach()[None], torch.zeros_like(m)[None], dw[None], 0.02, 1.0, 0.95, 0.0, True, torch.float32)
     assert bool(((w.double() - want[0]).norm() <= err + 4 * 2.0 ** -24 * want.norm()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wt", ["f32", "bf16"])
+@pytest.mark.parametrize("batch,rows,cols", [(1, 64, 64), (3, 130, 61), (1, 700, 500), (1, 600, 1000), (2, 2304, 2200)])
+def test_a_wait_that_runs_out_leaves_the_weights(sm, wt, batch, rows, cols):
+    """Failure detection without a fault: the first product's producers stay silent, so its bounded waits (50 ms here) run out and
+    everything behind it works on planes nobody wrote. The weights, and an orthogonalisation's result, stay as they were;
+    the next call that waits reports it, and the handle works as before."""
+    d = sm.Device(0)
+    try:
+        d.gemm_wait_limit(50)
+        w, m, g = (matrices(batch, rows, cols, TYPES[wt], seed=s) for s in (11, 12, 13))
+        w0, m0, args = w.clone(), m.clone(), dict(lr=0.02, scale=1.0, weight_decay=0.1)
+        with pytest.raises(sm.Sm100Error, match="gave up waiting on a barrier"):
+            run_muon(d, sm, w, m, g, steps=5 | sm.NS_TEST_SILENT_PRODUCER, **args)
+        assert torch.equal(w, w0) and not torch.equal(m, m0)
+        out = torch.full_like(g, 5.0)
+        size = d.orthogonalise_workspace(batch, rows, cols, code(sm, g.dtype))
+        ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for steps in (1 | sm.NS_TEST_SILENT_PRODUCER, 5):       # the call behind it, before anybody has asked, leaves its result too
+            d.orthogonalise(out.data_ptr(), g.data_ptr(), batch, rows, cols, ws.data_ptr(), size, dtype=code(sm, g.dtype), steps=steps)
+        with pytest.raises(sm.Sm100Error, match="gave up waiting on a barrier"):
+            d.sync()
+        assert bool((out == 5).all())
+        d.sync()
+        check(run(d, sm, g), *iterate64(g, g.dtype))
+        m.copy_(m0)
+        run_muon(d, sm, w, m, g, **args)
+        want, _, _ = muon64(w0, m0, g, 0.02, 1.0, 0.95, 0.1, True, w.dtype)
+        assert not torch.equal(w, w0) and bool(((w.double() - want).norm() < 0.1 * (w0.double() - want).norm()))
+    finally:
+        d.close()

@@ -221,3 +221,22 @@ d.close()
 """)
     assert res.returncode == 0, res.stderr
     assert not [l for l in L if l["kernel"].startswith("orth")]
+
+
+def test_the_silent_producer_is_the_first_product_only(fake3, tmp_path):
+    res, _, lines = run(fake3, tmp_path, """
+d = sm.Device(0); p = 1 << 20
+n = d.orthogonalise_workspace(1, 64, 64)
+d.orthogonalise(p, 2 * p, 1, 64, 64, 4 * p, n, steps=2 | sm.NS_TEST_SILENT_PRODUCER)
+d.orthogonalise(p, 2 * p, 1, 64, 64, 4 * p, n, steps=1)
+for steps in (sm.NS_TEST_SILENT_PRODUCER, 65 | sm.NS_TEST_SILENT_PRODUCER):
+    try:
+        d.orthogonalise(p, 2 * p, 1, 64, 64, 4 * p, n, steps=steps)
+    except sm.Sm100Error as e:
+        assert e.code == sm.ERR_ARG, e
+    else:
+        raise SystemExit("not refused")
+d.sync(); d.close()
+""")
+    assert res.returncode == 0, res.stderr
+    assert [p["silent"] for p in products(lines)] == [1, 0, 0, 0, 0, 0, 0, 0, 0]
