@@ -490,6 +490,19 @@ static int matrices_ok(sm100_ptr_t p, int dtype, int batch, int rows, int cols, 
     return batch <= 1 || (stride >= cols && stride <= (1ll << 59) / batch);
 }
 
+/* Whether the rows of all matrices lie apart, as what is written must: one matrix behind the other, side by side, or in any
+ * other way in which no row of the matrix k further on begins inside a row of this one, or the other way round. */
+static int apart(int batch, int rows, int cols, long long ld, long long stride)
+{
+    if (batch <= 1 || stride >= (rows - 1) * ld + cols || ld >= (batch - 1) * stride + cols) return 1;
+    for (long long k = 1; k < batch; k++) {
+        const long long row = k * stride / ld, in = k * stride - row * ld;
+        if (row >= rows) break;
+        if (in < cols || (row + 1 < rows && ld - in < cols)) return 0;
+    }
+    return 1;
+}
+
 /* Whether groups of four elements of every row are aligned to their size. */
 static int four_ok(sm100_ptr_t p, int dtype, int batch, int cols, long long ld, long long stride)
 {
@@ -507,9 +520,10 @@ int booth_sm100_orthogonalise(sm100_dev_t *dev, sm100_ptr_t out, sm100_ptr_t in,
     if (type_index(dtype) < 0) return bad_arg(dev, "booth_sm100_orthogonalise: the type is f32, bf16 or f16");
     if (!ns_ok(ns)) return bad_arg(dev, "booth_sm100_orthogonalise: need 1 to 64 steps, finite coefficients with c = 0 or |b| <= 8 |c|, and eps > 0");
     if (!orth_layout(dev, &o, batch, rows, cols, dtype != SM100_BF16) || !matrices_ok(in, dtype, batch, rows, cols, ld_in, stride_in) ||
-        !matrices_ok(out, dtype, batch, rows, cols, ld_out, stride_out) || (in == out && (ld_in != ld_out || (batch > 1 && stride_in != stride_out))))
+        !matrices_ok(out, dtype, batch, rows, cols, ld_out, stride_out) || !apart(batch, rows, cols, ld_out, stride_out) ||
+        (in == out && (ld_in != ld_out || (batch > 1 && stride_in != stride_out))))
         return bad_arg(dev, "booth_sm100_orthogonalise: need 1 to 65535 matrices of 1 to 2^20 rows and columns, operands non-NULL and aligned to "
-                            "their element, pitches >= cols, strides >= cols (equal ones when out is in)");
+                            "their element, pitches >= cols, strides >= cols (equal ones when out is in), matrices of out apart from one another");
     if (!ws || (ws & 127) || ws_bytes < o.bytes)
         return bad_arg(dev, "booth_sm100_orthogonalise: workspace missing, not 128-byte aligned or too small");
     orth_source_t src;
@@ -540,10 +554,11 @@ int booth_sm100_muon_step(sm100_dev_t *dev, sm100_ptr_t w, sm100_ptr_t m, sm100_
         return bad_arg(dev, "booth_sm100_muon_step: need a finite learning rate, scale and weight decay, and momentum in [0, 1]");
     const int two_planes = p->wdtype != SM100_BF16;
     if (!orth_layout(dev, &o, batch, rows, cols, two_planes) || !matrices_ok(w, p->wdtype, batch, rows, cols, p->ld_w, p->stride_w) ||
-        !matrices_ok(m, p->mdtype, batch, rows, cols, p->ld_m, p->stride_m) || !matrices_ok(g, p->gdtype, batch, rows, cols, p->ld_g, p->stride_g) ||
+        !matrices_ok(m, p->mdtype, batch, rows, cols, p->ld_m, p->stride_m) || !apart(batch, rows, cols, p->ld_w, p->stride_w) ||
+        !apart(batch, rows, cols, p->ld_m, p->stride_m) || !matrices_ok(g, p->gdtype, batch, rows, cols, p->ld_g, p->stride_g) ||
         w == m || w == g || m == g)
         return bad_arg(dev, "booth_sm100_muon_step: need 1 to 65535 matrices of 1 to 2^20 rows and columns; w, m and g non-NULL, apart from one "
-                            "another and aligned to their element; pitches >= cols, strides >= cols");
+                            "another and aligned to their element; pitches >= cols, strides >= cols, matrices of w and of m apart");
     if (!ws || (ws & 127) || ws_bytes < o.bytes)
         return bad_arg(dev, "booth_sm100_muon_step: workspace missing, not 128-byte aligned or too small");
     orth_source_t src;

@@ -328,7 +328,8 @@ typedef struct booth_newton_schulz {
  * of bf16, where the usual bf16 iteration is off by 1 to 50 percent. A matrix of zeros
  * gives zeros; one that holds an infinity or NaN gives no finite result, without
  * touching the others. out may be in (same pitch and stride); otherwise they must not
- * overlap. ws: booth_sm100_orthogonalise_workspace bytes for the same batch, rows,
+ * overlap. No two matrices of out may share an element (they may lie side by side, ld = batch cols and stride = cols);
+ * those of in may. ws: booth_sm100_orthogonalise_workspace bytes for the same batch, rows,
  * cols and dtype, 128-byte aligned, any contents. */
 int  booth_sm100_orthogonalise(sm100_dev_t *dev, sm100_ptr_t out, sm100_ptr_t in, int batch, int rows, int cols,
                                long long ld_in, long long stride_in, long long ld_out, long long stride_out,
@@ -339,7 +340,7 @@ size_t booth_sm100_orthogonalise_workspace(sm100_dev_t *dev, int batch, int rows
 /* One Muon update of `batch` weights w with their momentum m and gradient g:
  *   m = momentum m + (1 - momentum) g,  u = nesterov ? momentum m + (1 - momentum) g : m,
  *   w = (1 - lr weight_decay) w - lr scale NS(u)
- * w and m are updated in place, g is read only; u is formed from m as stored. The three
+ * w and m are updated in place, and no two of their matrices may share an element; g is read only; u is formed from m as stored. The three
  * may have different types; the products' precision goes by w's (see above). `scale`
  * is the caller's choice of update size, for instance 0.2 sqrt(max(rows, cols)). The
  * workspace is booth_sm100_orthogonalise_workspace(batch, rows, cols, wdtype). */

@@ -240,3 +240,41 @@ d.sync(); d.close()
 """)
     assert res.returncode == 0, res.stderr
     assert [p["silent"] for p in products(lines)] == [1, 0, 0, 0, 0, 0, 0, 0, 0]
+
+
+# (batch, rows, cols, ld, stride) of matrices that share elements, and of such that do not
+SHARED = [(2, 8, 8, 8, 8), (2, 8, 8, 16, 16), (3, 4, 8, 8, 24), (2, 8, 8, 20, 14), (4, 5, 6, 18, 10), (65535, 8, 8, 1 << 19, 9), (2, 8, 8, 9, 65)]
+APART = [(2, 8, 8, 8, 64), (2, 8, 8, 16, 8), (3, 8, 8, 24, 8), (4, 2, 4, 12, 8 * 3 + 4), (3, 2, 4, 12, 8), (2, 1, 8, 8, 8), (2, 8, 1, 2, 1), (2, 8, 8, 9, 71), (2, 8, 8, 20, 10)]
+
+
+def elements_apart(batch, rows, cols, ld, stride):
+    starts = sorted(k * stride + r * ld for k in range(batch) for r in range(rows))
+    return all(b - a >= cols for a, b in zip(starts, starts[1:]))
+
+
+def test_layouts_are_what_they_are_listed_as():
+    assert not any(elements_apart(*s) for s in SHARED) and all(elements_apart(*s) for s in APART)
+
+
+@pytest.mark.parametrize("shape", SHARED + APART)
+def test_matrices_that_are_written_lie_apart(fake3, tmp_path, shape):
+    """What two matrices share would be written by two blocks in no order: refused for out, w and m, allowed for what is only read."""
+    res, L, _ = run(fake3, tmp_path, """
+d = sm.Device(0); p = 1 << 20; big = 1 << 34
+n, r, c, ld, stride = %s
+wide = dict(ld_in=c, stride_in=r * c)
+calls = [lambda: d.orthogonalise(p, 2 * p, n, r, c, 4 * p, big, ld_out=ld, stride_out=stride, steps=1, **wide),
+         lambda: d.orthogonalise(p, p, n, r, c, 4 * p, big, ld_out=ld, stride_out=stride, ld_in=ld, stride_in=stride, steps=1),
+         lambda: d.muon_step(p, 2 * p, 3 * p, n, r, c, 4 * p, big, lr=0.1, ld_w=ld, stride_w=stride, steps=1),
+         lambda: d.muon_step(p, 2 * p, 3 * p, n, r, c, 4 * p, big, lr=0.1, ld_m=ld, stride_m=stride, steps=1)]
+for call in calls:
+    try:
+        call()
+        assert %s, "not refused"
+    except sm.Sm100Error as e:
+        assert not %s and e.code == sm.ERR_ARG, e
+d.orthogonalise(p, 2 * p, n, r, c, 4 * p, big, ld_in=ld, stride_in=stride, steps=1)
+d.muon_step(p, 2 * p, 3 * p, n, r, c, 4 * p, big, lr=0.1, ld_g=ld, stride_g=stride, steps=1)
+d.sync(); d.close()
+""" % (shape, shape in APART, shape in APART))
+    assert res.returncode == 0, res.stderr
