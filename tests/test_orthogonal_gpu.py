@@ -373,12 +373,12 @@ def test_a_wait_that_runs_out_leaves_the_weights(sm, wt, batch, rows, cols):
 @pytest.mark.parametrize("rows,cols", [(70, 90), (200, 64)])
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_matrices_side_by_side_and_shared_sources(dev, sm, rows, cols, t):
-    """Three matrices as column ranges of one wide matrix, out of one wide source; and one source matrix read three times."""
+    """Three matrices as column ranges of one wide matrix, out of one wide source; and three windows of one source, a row further on each."""
     g = matrices(1, rows, 3 * cols, TYPES[t], seed=21)[0]
     out = torch.full((rows, 3 * cols + 5), 5.0, dtype=g.dtype, device="cuda")
     side = [x.as_strided((3, rows, cols), (cols, x.stride(0), 1)) for x in (g, out)]
     check(run(dev, sm, side[0], out=side[1]), *iterate64(side[0], g.dtype))
     assert bool((out[:, 3 * cols:] == 5.0).all())
-    overlap = g.as_strided((3, rows, cols), (cols // 2, 3 * cols, 1))
+    overlap = g.as_strided((3, rows, cols), (cols, cols, 1))
     got = run(dev, sm, overlap, out=torch.zeros(3, rows, cols, dtype=g.dtype, device="cuda"))
     check(got, *iterate64(overlap, g.dtype))
