@@ -188,22 +188,41 @@ def _plain(s):
 _program = {}
 
 
-def _device():
-    """This program's device handle. Its torch work runs on the handle's stream from the first call on, so
-    the operators and torch's own kernels are ordered by that one stream."""
-    if not _program:
+def _device(gpu):
+    """This program's handle of a GPU, and its stream with its raw address."""
+    if gpu not in _program:
         import booth_b200
-        dev = booth_b200.Device(torch.cuda.current_device())
-        stream = torch.cuda.ExternalStream(dev.stream)
-        stream.wait_stream(torch.cuda.current_stream())
-        torch.cuda.set_stream(stream)
+        dev = booth_b200.Device(gpu)
         types = {torch.float32: booth_b200.F32, torch.bfloat16: booth_b200.BF16, torch.float16: booth_b200.F16}
-        _program.update(dev=dev, types=types)
-    return _program["dev"], _program["types"]
+        _program[gpu] = dev, types, torch.cuda.ExternalStream(dev.stream, device=gpu), dev.stream
+    return _program[gpu]
 
 
 def _framework(s):
-    dev, types = _device()
+    """The operators run on their handle's stream. The program's torch work joins it from the first call on, so that one stream
+    orders everything; a caller on another stream (inside a `with torch.cuda.stream(...)`, in another thread) is ordered by
+    events on both sides, and the allocator is told of the tensors that both streams use."""
+    gpu = (s["x"] if "x" in s else s["g"]).get_device()
+    first = gpu not in _program
+    dev, types, stream, raw = _device(gpu)
+    if torch._C._cuda_getCurrentRawStream(gpu) == raw:      # 0.1 us; torch.cuda.current_stream makes an object, 1.2 us
+        return _calls(s, dev, types)
+    caller = torch.cuda.current_stream(gpu)
+    stream.wait_stream(caller)
+    with torch.cuda.stream(stream):
+        out = _calls(s, dev, types)
+    caller.wait_stream(stream)
+    for t in s.values():
+        if isinstance(t, torch.Tensor):
+            t.record_stream(stream)
+    for t in out.values():
+        t.record_stream(caller)
+    if first and gpu == torch.cuda.current_device():
+        torch.cuda.set_stream(stream)
+    return out
+
+
+def _calls(s, dev, types):
     case = s["case"]
     op = case["op"]
     if op == "layernorm":
