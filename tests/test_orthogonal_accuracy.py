@@ -1,0 +1,148 @@
+"""How exact the orthogonalisation is, beside the bounds of test_orthogonal_gpu.py: those are worst cases, for bf16 results and
+low ranks larger than the result itself. Here an error is the Frobenius norm of the difference from the iteration in 64 bits
+over the norm of that, and may be
+
+    f32   3 times that of the same iteration in fp32 products, and 2^-20
+    f16   the same, and half a step of f16, 2^-11
+    bf16  5e-3: half a step is at most 2^-8 = 3.9e-3 of a value, 1.7e-3 in the norm of many
+
+emulate() is the kernels' arithmetic in 64 bits: fp16 planes hi and lo, products of sixteen added to a sum of 24 bits with what lies
+below the 26th dropped, sums of 256 added up in fp32. Over the shapes below and 256 x 256, 40 x 3000 and 520 x 700 it gives 0.1 to
+1.7 times the error of fp32 products (2.8e-6 against 1.7e-6 at 256 x 256), and 1.2e-3 to 3.9e-3 for bf16 results. What the
+criterion has to reject lies far off: one plane where there should be two 1e-3 and more, bf16 without the lo plane of X 2e-2 to 4e-2
+for matrices of low rank. The CPU tests say so."""
+import pytest
+import torch
+
+from test_orthogonal_gpu import ABC, SHAPES, TYPES, run, run_muon
+
+EMULATED = [(1, 16, 16), (2, 8, 200), (2, 33, 31), (1, 65, 130)]
+
+
+def coefficients():
+    return [torch.tensor(v, dtype=torch.float32).double().item() for v in ABC]
+
+
+def iterate(g, dtype, steps=5, eps=1e-7):
+    a, b, c = coefficients()
+    x = g.to(dtype)
+    tall = x.shape[1] > x.shape[2]
+    x = x.mT if tall else x
+    x = x / (x.square().sum((1, 2), keepdim=True).sqrt() + eps)
+    for _ in range(steps):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.mT if tall else x
+
+
+def error(got, want):
+    d = got.double() - want
+    return (d.square().sum((1, 2)).sqrt() / want.square().sum((1, 2)).sqrt()).max().item()
+
+
+def allowed(g, want, t):
+    if t == torch.bfloat16:
+        return 5e-3
+    return 3 * error(iterate(g, torch.float32), want) + 2.0 ** -20 + (2.0 ** -11 if t == torch.float16 else 0)
+
+
+def samples(batch, rows, cols, t, kind, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(batch, rows, cols, generator=g)
+    if kind == "rank":          # a few directions far above the rest
+        k = min(4, rows, cols)
+        x = 1e-2 * x + torch.randn(batch, rows, k, generator=g) @ torch.randn(batch, k, cols, generator=g)
+    return (1e-3 * x).to(t)
+
+
+def planes(x, n):
+    hi = x.half().double()
+    return [hi, (x - hi).half().double() if n == 2 else torch.zeros_like(x)]
+
+
+def add_dropping(acc, p):
+    unit = 2.0 ** (torch.maximum(acc.abs(), p.abs()).clamp_min(2.0 ** -100).log2().floor() - 25)
+    s = (acc / unit).trunc() * unit + (p / unit).trunc() * unit
+    unit = 2.0 ** (s.abs().clamp_min(2.0 ** -100).log2().floor() - 23)
+    return (s / unit).trunc() * unit
+
+
+def product(x, y, terms, chunk=256):
+    total = 0
+    for k0 in range(0, x[0].shape[2], chunk):
+        acc = torch.zeros(*x[0].shape[:2], y[0].shape[2], dtype=torch.float64)
+        for i, j in terms:
+            for k in range(k0, min(x[0].shape[2], k0 + chunk), 16):
+                acc = add_dropping(acc, x[i][:, :, k:k + 16] @ y[j][:, k:k + 16])
+        total = (total + acc).float().double()
+    return total
+
+
+def emulate(g, n, terms=None, lo_of_x=True, steps=5, eps=1e-7):
+    """The result for planes n = 2 or 1 before its last rounding; `terms`: the products of planes that are taken."""
+    a, b, c = coefficients()
+    beta, gamma, xs, ss, qs = b / (2 * c), a - b * b / (4 * c), 2.0 ** 14, 2.0 ** 12, 2.0 ** 11
+    terms = terms or ([(1, 0), (0, 1), (0, 0)] if n == 2 else [(0, 0)])
+    x = g.double()
+    tall = x.shape[1] > x.shape[2]
+    x = x.mT if tall else x
+    x = xs * x / (x.square().sum((1, 2), keepdim=True).sqrt() + eps)
+    eye = torch.eye(x.shape[1], dtype=torch.float64)
+    for _ in range(steps):
+        xp = planes(x.float().double(), 2)
+        s = planes((product(xp, [p.mT for p in xp], terms) * (ss / xs ** 2) + beta * ss * eye).float().double(), n)
+        q = planes((product(s, s, terms) * (c * qs / ss ** 2) + gamma * qs * eye).float().double(), n)
+        x = product(q, xp, terms)
+        if n == 1 and lo_of_x:
+            for d in range(0, x.shape[1], 64):
+                x[:, d:d + 64] += q[0][:, d:d + 64, d:d + 64] @ xp[1][:, d:d + 64]
+        x = x / qs
+    x = x.float().double() / xs
+    return x.mT if tall else x
+
+
+@pytest.mark.parametrize("batch,rows,cols", EMULATED)
+@pytest.mark.parametrize("kind", ["noise", "rank"])
+def test_the_criterion_accepts_the_arithmetic_and_rejects_less(batch, rows, cols, kind):
+    for t, n in (("f32", 2), ("f16", 2), ("bf16", 1)):
+        g = samples(batch, rows, cols, TYPES[t], kind, seed=rows + cols)
+        want = iterate(g, torch.float64)
+        most = allowed(g, want, g.dtype)
+        right = emulate(g, n)
+        assert error(right.to(g.dtype), want) <= most < 0.1
+        assert error(torch.zeros_like(right), want) > most and error(-right, want) > most
+        assert error(emulate(g, n, steps=4), want) > most
+        if t == "f32":
+            assert error(emulate(g, 1).float(), want) > most
+            for terms in ([(1, 0), (0, 0)], [(0, 1), (0, 0)]):
+                assert error(emulate(g, 2, terms).float(), want) > 10 * most
+        if t == "bf16" and kind == "rank":
+            assert error(emulate(g, 1, lo_of_x=False).to(g.dtype), want) > 3 * most
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols", SHAPES + [(1, 2304, 2304), (40, 256, 300), (1, 1100, 4200), (9, 700, 513), (1, 1000, 2049), (12, 768, 2048)])
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind", ["noise", "rank"])
+def test_orthogonalise_is_as_exact_as_stated(dev, sm, batch, rows, cols, t, kind):
+    g = samples(batch, rows, cols, TYPES[t], kind, seed=rows + cols).cuda()
+    want = iterate(g, torch.float64)
+    most = allowed(g, want, g.dtype)
+    assert most < 0.1 and error(run(dev, sm, g), want) <= most
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols", [(1, 16, 16), (2, 64, 96), (1, 130, 61), (3, 200, 259), (1, 513, 300), (1, 1024, 2048), (1, 2100, 2300)])
+@pytest.mark.parametrize("wt", ["f32", "bf16", "f16"])
+def test_a_muon_step_is_as_exact_as_stated(dev, sm, batch, rows, cols, wt):
+    """From weights of zero and momentum in fp32 the new weights are the update itself; it is formed in fp32 from two products and
+    a sum twice over, 6 roundings of 2^-24 that the 2^-20 covers."""
+    m, g = (samples(batch, rows, cols, torch.float32, "noise", seed=s).cuda() for s in (1, 2))
+    mu, lr, scale = (torch.tensor(v, dtype=torch.float32).double().item() for v in (0.95, 0.5, 2.0))
+    m64 = (mu * m.double() + (1 - mu) * g.double()).float()
+    u = mu * m64.double() + (1 - mu) * g.double()
+    want = -lr * scale * iterate(u, torch.float64)
+    most = allowed(u, -want, TYPES[wt])           # lr scale = 1
+    w = torch.zeros(batch, rows, cols, dtype=TYPES[wt], device="cuda")
+    run_muon(dev, sm, w, m, g, lr=0.5, scale=2.0)
+    assert most < 0.1 and error(w, want) <= most
