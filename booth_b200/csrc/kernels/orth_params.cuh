@@ -47,7 +47,8 @@ typedef struct orth_product {
     ORTH_PTR(void) w;
     long long ld_w, stride_w;
     ORTH_PTR(float) sums;                               /* where the parts of a tile meet */
-    ORTH_PTR(int) status;
+    ORTH_PTR(int) status;                               /* the code of the first wait that ran out */
+    ORTH_PTR(int) told;                                 /* in the host's memory: set when one has, for calls the host does not see */
     unsigned long long wait_ns;
     int silent;                                         /* the tests' way to see a wait run out: nothing is loaded */
 } orth_product_t;

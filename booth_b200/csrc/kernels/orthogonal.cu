@@ -1067,7 +1067,11 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
         }
         }
         if (issuer) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        if (!ok) {      // a wait ran out: copies that may still be in flight land before the shared memory is released
+        if (!ok) {      // a wait ran out: the host hears of it; copies that may still be in flight land before the shared memory is released
+            if (lane == 0) {
+                __threadfence_system();         // behind the status word
+                asm volatile("st.relaxed.sys.global.b32 [%0], %1;" ::"l"(p.told), "r"(1) : "memory");
+            }
             for (int n = 0; n < 64; n++) __nanosleep(4000);
         }
     }

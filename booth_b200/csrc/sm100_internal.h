@@ -41,7 +41,6 @@ typedef struct sm100_api {
     CUresult (*StreamCreate)(CUstream *, unsigned);
     CUresult (*StreamDestroy)(CUstream);
     CUresult (*StreamSynchronize)(CUstream);
-    CUresult (*StreamIsCapturing)(CUstream, CUstreamCaptureStatus *);       /* optional */
     CUresult (*StreamWaitEvent)(CUstream, CUevent, unsigned);
     CUresult (*EventCreate)(CUevent *, unsigned);
     CUresult (*EventDestroy)(CUevent);
@@ -120,7 +119,7 @@ struct sm100_dev {
     unsigned    gemm_wait_ms;          /* limit of the GEMM kernel's barrier waits */
     int         ln_smem_set;           /* dynamic shared memory limit raised on the layer normalisation kernels */
     int         orth_pending;          /* an orthogonalisation was enqueued since the last status check */
-    int         orth_captured;         /* one was captured into a graph: its replays are not seen here */
+    volatile int *orth_told;           /* page-locked: set by an orthogonalisation whose wait ran out, also by a graph's replay */
     int         orth_clusters[9];      /* clusters of so many product CTAs the GPU holds at once (0 = not asked yet) */
     int         orth_smem_set;         /* dynamic shared memory limit raised on the product kernels */
     unsigned    gemm_epoch;            /* tag of the latest persistent GEMM call (never zero once used) */

@@ -87,7 +87,6 @@ static int api_load(void)
     SYM(EventSynchronize, "cuEventSynchronize");
     SYM(EventElapsedTime, "cuEventElapsedTime");
     SYM(LaunchKernel, "cuLaunchKernel");
-    OPT(StreamIsCapturing, "cuStreamIsCapturing");
     OPT(LaunchKernelEx, "cuLaunchKernelEx");
     OPT(OccupancyMaxActiveClusters, "cuOccupancyMaxActiveClusters");
     SYM(GetErrorString, "cuGetErrorString");
@@ -242,6 +241,12 @@ int sm100_rt_init(sm100_dev_t **out, int ordinal)
         (cr = a->StreamSynchronize(d->stream)) != CUDA_SUCCESS) {
         rc = sm100_fail(NULL, "clearing scratch", cr); a->MemFree(d->scratch); goto drop_image;
     }
+    void *told = NULL;
+    if ((cr = a->MemHostAlloc(&told, sizeof(int), CU_MEMHOSTALLOC_PORTABLE | CU_MEMHOSTALLOC_DEVICEMAP)) != CUDA_SUCCESS) {
+        rc = sm100_fail(NULL, "cuMemHostAlloc(orthogonalisation's word)", cr); a->MemFree(d->scratch); goto drop_image;
+    }
+    d->orth_told = (volatile int *)told;
+    *d->orth_told = 0;
     {   /* limit of the GEMM kernel's barrier waits: BOOTH_SM100_GEMM_WAIT_MS at start-up, else 4 s */
         const char *e = getenv("BOOTH_SM100_GEMM_WAIT_MS");
         int ms = (e && *e) ? atoi(e) : 4000;
@@ -282,6 +287,7 @@ void sm100_rt_shut(sm100_dev_t *dev)
         }
         if (dev->gemm_ws) a->MemFree(dev->gemm_ws);
         if (dev->scratch) a->MemFree(dev->scratch);
+        a->MemFreeHost((void *)(size_t)dev->orth_told);
         a->ModuleUnload(dev->image);
         a->EventDestroy(dev->ev0);
         a->EventDestroy(dev->ev1);
@@ -444,9 +450,11 @@ void sm100_rt_unload(sm100_dev_t *dev, sm100_kern_t *kern)
  * idle when this is called. */
 static int orth_outcome(sm100_dev_t *dev)
 {
-    if (!dev->orth_pending && !dev->orth_captured) return SM100_OK;
+    /* A captured call runs when its graph is replayed, which this library does not see: such a call sets the host's word. */
+    if (!dev->orth_pending && !*dev->orth_told) return SM100_OK;
     int st = 0;
     dev->orth_pending = 0;
+    *dev->orth_told = 0;
     const CUdeviceptr word = dev->scratch + SM100_SCRATCH_ORTH_STATUS;
     CUresult cr = dev->api->MemcpyDtoH(&st, word, sizeof st);
     if (cr != CUDA_SUCCESS) return sm100_fail(dev, "reading the orthogonalisation's status", cr);

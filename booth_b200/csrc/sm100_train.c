@@ -386,12 +386,6 @@ static int orth_status_ready(sm100_dev_t *dev)
         }
         dev->orth_smem_set = 1;
     }
-    /* A captured call runs when its graph is replayed, which this library does not see: from then on the
-     * status word is read at every wait. */
-    CUstreamCaptureStatus capturing = CU_STREAM_CAPTURE_STATUS_NONE;
-    if (dev->api->StreamIsCapturing && dev->api->StreamIsCapturing(dev->stream, &capturing) == CUDA_SUCCESS &&
-        capturing != CU_STREAM_CAPTURE_STATUS_NONE)
-        dev->orth_captured = 1;
     dev->orth_pending = 1;
     return SM100_OK;
 }
@@ -444,6 +438,7 @@ static int newton_schulz(sm100_dev_t *dev, orth_source_t *src, const orth_produc
     q.batch = batch;
     q.sums = ws + o->sums;
     q.status = dev->scratch + SM100_SCRATCH_ORTH_STATUS;
+    q.told = (unsigned long long)(size_t)dev->orth_told;        /* page-locked memory has one address for both sides */
     q.wait_ns = (unsigned long long)dev->gemm_wait_ms * 1000000ull;
     const int steps = ns->steps & ~BOOTH_NS_TEST_SILENT_PRODUCER;
     q.silent = (ns->steps & BOOTH_NS_TEST_SILENT_PRODUCER) != 0;        /* the first product's producers issue nothing */

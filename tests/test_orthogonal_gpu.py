@@ -382,3 +382,37 @@ def test_matrices_side_by_side_and_shared_sources(dev, sm, rows, cols, t):
     overlap = g.as_strided((3, rows, cols), (cols, cols, 1))
     got = run(dev, sm, overlap, out=torch.zeros(3, rows, cols, dtype=g.dtype, device="cuda"))
     check(got, *iterate64(overlap, g.dtype))
+
+
+@pytest.mark.gpu
+def test_a_replayed_wait_that_runs_out_is_reported(sm):
+    """The same out of a graph: the library does not see the replay, and hears of it by the word in the host's memory."""
+    d = sm.Device(0)
+    try:
+        d.gemm_wait_limit(50)
+        g = matrices(1, 200, 300, torch.float32, seed=14)
+        out = torch.full_like(g, 5.0)
+        size = d.orthogonalise_workspace(1, 200, 300)
+        ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+        graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+        torch.cuda.synchronize()
+        for graph, steps in zip(graphs, (5 | sm.NS_TEST_SILENT_PRODUCER, 5)):
+            with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(d.stream)):
+                d.orthogonalise(out.data_ptr(), g.data_ptr(), 1, 200, 300, ws.data_ptr(), size, steps=steps)
+        d.sync()
+        side = torch.cuda.Stream()
+        for _ in range(2):
+            with torch.cuda.stream(side):
+                graphs[0].replay()
+            torch.cuda.synchronize()
+            assert bool((out == 5).all())
+            with pytest.raises(sm.Sm100Error, match="gave up waiting on a barrier"):
+                d.sync()
+            d.sync()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        d.sync()
+        check(out, *iterate64(g, g.dtype))
+    finally:
+        d.close()

@@ -278,3 +278,30 @@ d.muon_step(p, 2 * p, 3 * p, n, r, c, 4 * p, big, lr=0.1, ld_g=ld, stride_g=stri
 d.sync(); d.close()
 """ % (shape, shape in APART, shape in APART))
     assert res.returncode == 0, res.stderr
+
+
+def test_a_replay_whose_wait_ran_out_is_reported_and_others_cost_no_copy(fake3, tmp_path):
+    """A captured call runs behind the library's back. Its word in the host's memory says when the status is worth
+    reading; as long as it does not, waits read nothing from the GPU."""
+    res, _, lines = run(fake3, tmp_path, """
+import ctypes
+libc = ctypes.CDLL(None)
+d = sm.Device(0); p = 1 << 20
+n = d.orthogonalise_workspace(1, 64, 64)
+d.orthogonalise(p, 2 * p, 1, 64, 64, 4 * p, n)
+d.sync()                        # reads the status once: a call was enqueued
+for _ in range(5):
+    d.sync()
+libc.setenv(b"FAKE_CUDA_ORTH_REPLAY", b"3", 1)
+try:
+    d.sync()
+except sm.Sm100Error as e:
+    assert e.code == sm.ERR_CUDA and "code 3" in str(e), e
+else:
+    raise SystemExit("not reported")
+for _ in range(5):
+    d.sync()
+d.close()
+""")
+    assert res.returncode == 0, res.stderr
+    assert lines.count("d2h_now") == 2, lines
