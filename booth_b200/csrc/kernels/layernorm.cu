@@ -6,9 +6,10 @@
 // Backward, with xhat = (x - mean) rstd, p = mean(w dy), q = mean(w dy xhat):
 //     dx = rstd (w dy - p - xhat q);   dw = sum over rows of dy xhat;   db = sum over rows of dy
 //
-// Both read every value once and write every result once, so HBM bounds them: 16384 x 4096 bf16 takes 48 us forward
-// and 74 us backward, 86 and 83 % of what the copy rate allows (8192 x 4096 f32: 49 and 71; 65536 x 1024 bf16: 51
-// and 72; unaligned 32768 x 1001 bf16: 46 and 80, 43 and 38 %, bound by instructions). A row belongs to one
+// Both read every value once and write every result once, so HBM bounds them: 16384 x 4096 bf16 takes 51 us forward
+// and 80 us backward, 81 and 77 % of what the copy rate allows; calls back to back overlap at their ends and take 47 and 74, 87
+// and 83 % (8192 x 4096 f32: 49 and 71; 65536 x 1024 bf16: 51
+// and 71; unaligned 32768 x 1001 bf16: 46 and 80, 43 and 38 %, bound by instructions). A row belongs to one
 // group of threads: 1 to 32 lanes of a warp for narrow rows, a whole block for wider ones, 8 to 32 values a thread: a
 // row costs a thread some 150 instructions beside its values, which with 8 values were most of them. The mean
 // is taken first and the variance from the differences (the row is on chip, a second pass costs no memory), with
@@ -20,7 +21,8 @@
 // registers instead, 16 KB an SM were in flight and 16384 x 4096 bf16 took 116 us forward
 // and 128 backward.) Rows of any other alignment come in 16-byte units all the same and are read
 // value by value. A spill in the walk is dear, with the SM's memory given to the ring no cache is left
-// for it: the forms are cut, and distances between a thread's values kept opaque, so that there is none.
+// for it: the forms are cut, and distances between a thread's values kept opaque, so that there is none forward and 16 bytes at
+// most backward (sx, loop and the vx of f32).
 //
 // The backward pass walks the rows once for all three results: each thread adds dy
 // and dy xhat of its own columns into registers over all the rows its block sees,
