@@ -18,10 +18,9 @@
 // Precision, by the type of the result:
 //   two planes (f32, f16 results): every operand is hi + lo = fp16(x) + fp16(x - hi), 22
 //     bits, and a product is lo.hi + hi.lo + hi.hi. The tensor core adds with truncation, so a
-//     long sum drifts: K is cut into chunks of 128 (64-tiles: 256), of 64 where the large diagonal of S or Q comes
-//     in, whose sums are added round-to-nearest in registers. What an instruction drops among its own sixteen
-//     products stays: the result's error is 0.3 to 1.0 times that of fp32 products from sides of some 700 on (4096 x 4096
-//     1.6e-6 of the norm), 0.8 to 3 times below (256 x 256 2.5e-6 against 1.5e-6, 300 x 77 4.3e-6 against 1.4e-6).
+//     long sum drifts: K is cut into chunks of 128 (64-tiles: two sums of 128 each), of 64 where the large diagonal of S or Q comes
+//     in, whose sums are added round-to-nearest in registers. The result's error is 0.3 to 1.3 times
+//     that of fp32 products, at sides of about 100 up to 1.6 times (96 x 96 2.0e-6 of the norm, 4096 x 4096 1.6e-6).
 //   one plane (bf16 results): products use the hi parts only, a third of the work. X
 //     still has a lo plane, and Q X adds Q_hi X_lo for the K blocks around the diagonal, where a X
 //     comes from: the iteration multiplies what small singular values lose by up to
@@ -601,8 +600,8 @@ __device__ __forceinline__ void store_result_64(const Product &p, uint32_t tile,
 // the product meet, and a box each for hi and lo.
 constexpr uint32_t OPERAND_BYTES = 196608, OPERAND_BYTES_64 = 163840, QUARTERS_64 = 49152;
 
-// Two planes: where the accumulator is drained, after every `run` K blocks (64-tiles, whose small products have sums of their
-// own: 4; else 2) and after every one on the tile's diagonal.
+// Two planes: where the accumulator is drained, after every `run` K blocks (64-tiles, whose small products and halves of K blocks
+// have sums of their own: 4; else 2) and after every one on the tile's diagonal.
 __device__ __forceinline__ bool chunk_ends(int kb, int run, int diag0, int diag, bool sym)
 {
     return (kb & (run - 1)) == run - 1 || (sym && kb >= diag0 && kb < diag0 + diag);
@@ -625,10 +624,16 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
     constexpr int STAGES = (SIDE == 64 ? OPERAND_BYTES_64 : OPERAND_BYTES) / STAGE;
     constexpr int HALF = SIDE / 2;                                  // columns per epilogue warp
     // Rows and columns of one tensor instruction. 64-tiles in two planes take hi and lo, which lie one below the
-    // other, as one operand of 128: the four quarters of a 128 x 128 product are hi.hi, hi.lo, lo.hi and lo.lo, four
-    // instructions a K block instead of twelve (an instruction takes some 90 clocks however small it is).
+    // other, as one operand of 128: the four quarters of a 128 x 128 product are hi.hi, hi.lo, lo.hi and lo.lo (which
+    // costs nothing here and is taken along), four instructions a K block instead of twelve (an instruction takes some 90 clocks however small it is).
     constexpr int MMA = SIDE == 64 ? 64 * PLANES : SIDE;
-    constexpr uint32_t TMEM_COLS = 2 * MMA;                         // two accumulators
+    // 64-tiles in two planes have two sums, one of the first and one of the second half of each K block: an instruction drops of
+    // each of its products what lies 25 bits below the sum it adds to, and half as many instructions make half the sum. Small
+    // matrices need that, they have no long sums in which such losses would even out: 128 x 128 was 2.4 times as far off as with fp32
+    // products and is 1.2 times, 256 x 256 1.5 and is 0.8, for 1 to 2 us a call. (A sum drained after every half block was no
+    // more exact and took 12 to 27 us.)
+    constexpr bool FINE = SIDE == 64 && PLANES == 2;
+    constexpr uint32_t TMEM_COLS = (FINE ? 4 : 2) * MMA;            // two accumulators
     const WaitCtl status = { p.status, p.wait_ns };
 
     extern __shared__ uint8_t smem_orth[];
@@ -748,7 +753,7 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         if (!ok) break;
                         g++;
                     }
-                    const uint32_t tacc = tmem + buf * (uint32_t)MMA;
+                    const uint32_t tacc = tmem + buf * (TMEM_COLS / 2);
                     ok = warp_wait(full, ph, status, 2);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -773,7 +778,8 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         }
 #pragma unroll
                         for (int kk = 0; kk < BK / 16; kk++)
-                            umma<PAIR>(tacc, desc(ah + kk * ak), desc(bh + kk * bk), idesc, (PLANES == 2 && SIDE != 64) || kk ? 1u : acc);
+                            umma<PAIR>(FINE ? tacc + (uint32_t)(kk / 2 * MMA) : tacc, desc(ah + kk * ak), desc(bh + kk * bk), idesc,
+                                       (PLANES == 2 && SIDE != 64) || (FINE ? kk & 1 : kk) ? 1u : acc);
                         commit<PAIR>(empty, first);
                         if (ends) commit<PAIR>(acc_full0 + 8 * buf, first);
                     }
@@ -818,8 +824,9 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                     if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
                     if (lane < 16) put_quarter(quarters, x, q * 16 + lane, h * 8);
                 } else {
-                    // rows of hi (q 0, 1) or lo, columns of hi (h 0) or lo; the quarter lo.lo is left out
-                    const bool used = q < 2 || h == 0;
+                    // Rows of hi (q 0, 1) or lo, columns of hi or lo. Warps of hi rows have the columns of one of them (h); of the
+                    // lo rows each has half the columns of both, lo.hi and the small lo.lo, which it adds up.
+                    const uint32_t mine = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(q < 2 ? h * 64 : h * 32), more = q < 2 ? 32u : 64u;
                     float acc[64];
 #pragma unroll
                     for (int c = 0; c < 64; c++) acc[c] = 0.f;
@@ -830,26 +837,31 @@ __device__ __forceinline__ void product(const CUtensorMap &a_hi, const CUtensorM
                         if (!ok) break;
                         g++;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        if (used) {
 #pragma unroll
-                            for (int cc = 0; cc < 2; cc++) {
-                                uint32_t x[32];
-                                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * (uint32_t)MMA + (uint32_t)(h * 64 + cc * 32), x);
-                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        for (int half = 0; half < 2; half++) {
+                            uint32_t x[2][32];
+                            tmem_ld32(mine + buf * (TMEM_COLS / 2) + (uint32_t)(half * MMA), x[0]);
+                            tmem_ld32(mine + buf * (TMEM_COLS / 2) + (uint32_t)(half * MMA) + more, x[1]);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                                for (int c = 0; c < 32; c++) acc[cc * 32 + c] = __fadd_rn(acc[cc * 32 + c], __uint_as_float(x[c]));
+                            for (int c = 0; c < 32; c++) acc[c] = __fadd_rn(acc[c], __uint_as_float(x[0][c]));
+                            if (q < 2) {
+#pragma unroll
+                                for (int c = 0; c < 32; c++) acc[32 + c] = __fadd_rn(acc[32 + c], __uint_as_float(x[1][c]));
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < 32; c++) acc[c] = __fadd_rn(acc[c], __uint_as_float(x[1][c]));
                             }
                         }
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * buf);
                     }
-                    if (used) {
-                        uint32_t x[64];
+                    uint32_t x[2][32];
 #pragma unroll
-                        for (int c = 0; c < 64; c++) x[c] = __float_as_uint(acc[c]);
-                        put_quarter(quarters + (q < 2 ? h : 2) * 16384u, x, (q & 1) * 32 + lane, 0);
-                    }
+                    for (int c = 0; c < 32; c++) { x[0][c] = __float_as_uint(acc[c]); x[1][c] = __float_as_uint(acc[32 + c]); }
+                    put_quarter(quarters + (q < 2 ? h : 2) * 16384u, x[0], (q & 1) * 32 + lane, q < 2 ? 0 : h * 8);
+                    if (q < 2) put_quarter(quarters + h * 16384u, x[1], (q & 1) * 32 + lane, 8);
                 }
                 const int stop = gave_up(p);
                 ok = all_ok<256>(1, ok);

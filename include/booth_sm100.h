@@ -323,8 +323,8 @@ typedef struct booth_newton_schulz {
 /* out = the iteration's result for each of `batch` matrices [rows, cols]; element (r, c)
  * of matrix k lies k * stride + r * ld + c elements from the operand's address (strides
  * are not looked at when batch is 1). dtype (SM100_F32, SM100_BF16, SM100_F16) is the type
- * of both. f32 and f16 results are computed from 22-bit operands: before the last rounding they are off by 0.3 to 1.0
- * times what fp32 products are for sides from some 700 on, by up to 3 times below (some 4e-6 of the result's norm).
+ * of both. f32 and f16 results are computed from 22-bit operands: before the last rounding they are off by 0.3 to 1.3
+ * times what fp32 products are, at sides of about 100 by up to 1.6 times (some 2e-6 of the result's norm).
  * bf16 results come from 11-bit operands and a 22-bit X: off by 0.2 to 0.4 percent of the norm, 0.17 of which is
  * bf16's own rounding, where the usual bf16 iteration is off by 0.8 to 50 percent. A matrix of zeros
  * gives zeros; one that holds an infinity or NaN gives no finite result, without
